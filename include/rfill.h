@@ -575,6 +575,82 @@ int rf_window_mass(const uint16_t* q, int64_t ldq, int w, int64_t pos0, int hq, 
                    int hkv, int64_t head_stride, int64_t row_stride, float scale, double* mass, void* workspace,
                    size_t ws_bytes, hipStream_t stream);
 
+/* ---- a paged K / V cache of several sequences: appending, attending, reading back. No counterpart in the reference
+ * (its serving engines keep caches of their own); rows and rotation are those of rf_rope_kv_write and rf_norm_q. ---- */
+
+#define RF_PAGES_BF16 0
+#define RF_PAGES_MX4 1
+
+/* The pages of one layer. A page holds `page` tokens (16, 32, 64, 128, 256, 512 or 1024) of all hkv heads (head_dim d:
+ * 64, 128 or 256); slot s is token s % page of page s / page.
+ * RF_PAGES_BF16: k, v [n_pages, hkv, page, d] bf16; ks, vs NULL.
+ * RF_PAGES_MX4: 4-bit codes (E2M1: sign, two exponent bits, one mantissa bit; 0 .5 1 1.5 2 3 4 6) with one scale a
+ * block of 32 values along d (a byte e, 2^(e - 127); 255: the block reads as NaN):
+ *   k [n_pages, hkv, page, d / 2]: two codes a byte, the lower d in the low half;
+ *   v [n_pages, hkv, page / 8, 16, 8, d / 32]: of 8 tokens, 16 runs of d / 16 values, token by token within a run (what a
+ *     lane of the attention reads for its 8 tokens lies together);
+ *   ks, vs [n_pages, hkv, page / 8, d / 32, 8]: the scales of 8 tokens side by side.
+ * page_stride: bytes from a page to the next, of k and of v (at least a page's own bytes, a multiple of 16);
+ * scale_stride: the same of ks and vs (a multiple of 8). k, v 16-byte and ks, vs 8-byte aligned. */
+typedef struct rf_pages {
+  void* k;
+  void* v;
+  uint8_t* ks;
+  uint8_t* vs;
+  int64_t n_pages, page_stride, scale_stride;
+  int kind, hkv, d, page;
+} rf_pages;
+
+/* Slots and positions of T new rows of n_seq sequences: sequence b's rows are [cu[b], cu[b + 1]) of the T (cu int32
+ * [n_seq + 1], rising from 0), its last ones after this call: positions lens[b] - rows ..  lens[b] - 1 (lens int32, the
+ * tokens with the new ones). table int32 [n_seq, table_width] (row stride ld_table): the pages of each sequence in
+ * order. slots[t] = the row's slot, or -1 for rows of no sequence (t >= cu[n_seq]), positions before 0 or past the
+ * table, and pages outside [0, n_pages); pos[t] = its position, 0 where there is none. slots, pos int64 [T]. */
+int rf_paged_slots(const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu,
+                   int n_seq, int64_t n_pages, int page, int64_t T, int64_t* slots, int64_t* pos, hipStream_t stream);
+
+/* K / V of T new rows into slots[t] of the pages (int64, device; a row whose slot lies outside [0, n_pages page) is
+ * skipped; two rows of one call must not share a slot), with the norm and the rotation on the way, and the same rows'
+ * queries, normed and rotated, to q_out:
+ *   k, v: row t, head h at k + t ld_k + h head_k (elements; multiples of 8, a head's d values contiguous);
+ *   cs [T, rot] bf16 (rf_rope_table of the rows' positions) or NULL: nothing is rotated (rot is then ignored);
+ *   q [T, hq d] (row stride ld_q) or NULL with hq 0: no queries; q_out [T, hq d] (row stride ld_qo), may be q itself;
+ *     the queries of skipped rows are written too;
+ *   qnorm, knorm [d] bf16 or NULL: per-head RMSNorm gains (norm_kind 0: gain, 1: 1 + gain; epsilon eps).
+ * A head vector x becomes x r g (r = 1 / sqrt(mean(x^2) + eps), the mean in fp64), then its first rot dims are rotated
+ * by halves, in fp32, and it is rounded once: to bf16, or to its 4-bit codes. A block's scale is the least power of two
+ * at which its largest value rounds to at most 6; codes round to nearest, halfway to the even one; a block with a NaN or
+ * an infinity reads as NaN. Needs rot <= d, rot / 2 a multiple of 8 or equal to 4. */
+int rf_paged_append(const uint16_t* k, int64_t ld_k, int64_t head_k, const uint16_t* v, int64_t ld_v, int64_t head_v,
+                    int64_t T, const int64_t* slots, const rf_pages* pages, const uint16_t* cs, int rot,
+                    const uint16_t* q, int64_t ld_q, int hq, uint16_t* q_out, int64_t ld_qo, const uint16_t* qnorm,
+                    const uint16_t* knorm, int norm_kind, float eps, hipStream_t stream);
+
+/* Rows of the pages as bf16: k_out, v_out [T, hkv, d] (row strides ld_k, ld_v) = the K / V at slots[t] (int64, device);
+ * zeros for a slot outside [0, n_pages page). */
+int rf_paged_read(const rf_pages* pages, const int64_t* slots, int64_t T, uint16_t* k_out, int64_t ld_k,
+                  uint16_t* v_out, int64_t ld_v, hipStream_t stream);
+
+/* Causal attention of the T new rows of n_seq sequences over their pages. Sequence b's queries are rows
+ * [cu[b], cu[b + 1]) of q [T, hq d] (row stride ldq), its last tokens: with n of them, query i is at position
+ * p = lens[b] - n + i and sees keys 0 .. p of the sequence's pages (table as rf_paged_slots). out row (row stride ldo) =
+ * sum_j softmax_j(scale q . k_j) v_j, scores and softmax in fp32, the probabilities rounded to bf16 for the second
+ * product; zeros for a query that sees no key (position before 0, or every page outside [0, n_pages)). Keys outside a
+ * query's sight never touch its output, whatever they hold; rows of no sequence are left as they were.
+ * lens, cu and table are read on the device, so a captured call follows them: max_rows bounds the rows of a sequence and
+ * max_keys its tokens (host values; a sequence with more rows than max_rows or more tokens than max_keys, or than its
+ * table, is taken as that much; they also choose the kernel). Any hq / hkv up to 64. The workspace (device memory, 16-byte
+ * aligned) of rf_attend_paged_workspace_bytes lets the keys of a sequence be split over blocks, whose parts are merged in
+ * a fixed order; with a smaller one or NULL they are not split. */
+int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages, const int32_t* table,
+                    int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu, int n_seq,
+                    int64_t max_rows, int64_t max_keys, float scale, uint16_t* out, int64_t ldo, void* workspace,
+                    size_t ws_bytes, hipStream_t stream);
+
+/* Bytes of rf_attend_paged's workspace for these sizes (0: the keys are not split). Host only. */
+int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows,
+                                    int64_t max_keys, size_t* bytes);
+
 /* ---- map formats ---- */
 
 /* int8 map rows with per-row group scales -> bf16 maps: out[i][j] = bf16(codes[i][j] * scale[i][j / group]),

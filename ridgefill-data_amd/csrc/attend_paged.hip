@@ -1,0 +1,717 @@
+// Attention of new tokens of many sequences over a paged K / V cache (bf16 or 4-bit codes), gfx950.
+//
+// k_paged_few: a few query rows a sequence (one token of each, or some drafted ones). The keys are read once from HBM and
+// that read is the bound, so a wave streams them from memory straight into the registers of its products, with no LDS on
+// the way: a block takes one K / V head and up to 16 MT query rows (queries x the query heads of the K / V head, query by
+// query) of one sequence, its four waves take turns at the key tiles (32 keys) of the block's split. Per tile and wave:
+//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16. A's row m of key half kb is key 8 (m / 4) + 4 kb + m % 4 of the tile, so that
+//       lane (n, g) (n = lane % 16, g = lane / 16) holds, for query row n, the scores of keys 8 g .. 8 g + 7: the order in
+//       which A of the second product wants them. The contraction's order over d is free, too: a lane takes its share of d
+//       as memory gives it (bf16: 16-byte chunk 4 s + g in step s; 4 bits: codes of d / 4 consecutive values).
+//   Softmax in fp32 base 2, the running maximum raised only when a score exceeds it by 2^8 (lazily: O is rescaled rarely).
+//   O += P V on the same MFMA: B's column n of product nb is d = n (D / 16) + nb, so a lane reads D / 16 consecutive values
+//       of each of its 8 keys and transposes 2 x 2 with v_perm (half an instruction a value); O's columns of a lane are
+//       consecutive in memory again.
+// 4-bit codes become bf16 by v_cvt_scalef32_pk_bf16_fp4, scale included, exactly: the arithmetic after it is that of bf16
+// pages. The waves' parts are merged through LDS in wave order.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "paged.h"
+
+namespace rf {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ bf16x8 as_frag(const uint4& u) { return __builtin_bit_cast(bf16x8, u); }
+
+constexpr int KT = 32;                     // keys a tile
+constexpr float RESCALE_LOG2 = 8.0f;       // headroom of the lazy rescale: probabilities stay below 2^8
+constexpr int NW = 4;                      // waves a block
+
+struct PagedArgs {
+  const uint16_t* q;
+  int64_t ldq, T;
+  PagesDev pg;
+  const int32_t* table;
+  int64_t ld_table;
+  int width;                               // pages of a sequence at most
+  const int32_t* lens;
+  const int32_t* cu;
+  int n_seq, hq, hkv, rep, qb;             // qb: queries a block
+  int max_rows, max_keys;
+  float c;                                 // scale log2(e)
+  uint16_t* out;
+  int64_t ldo;
+  float* part;                             // partials of the splits, or null
+  int target;                              // blocks that the splits aim at (0: no splits)
+  int64_t units;                           // units that the workspace holds partials of
+};
+
+struct Seq {
+  int rows, keys, first;                   // new rows, tokens with them, the first row of q
+};
+
+// Sequence b, its sizes brought into what the caller's bounds, the table and q hold.
+__device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
+  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1];
+  const int64_t held = min(static_cast<int64_t>(a.width) << a.pg.shift, static_cast<int64_t>(a.max_keys));
+  Seq s;
+  s.first = static_cast<int>(max<int64_t>(c0, 0));
+  s.rows = static_cast<int>(max<int64_t>(0, min(min(c1, a.T) - s.first, static_cast<int64_t>(a.max_rows))));
+  s.keys = static_cast<int>(max<int64_t>(0, min<int64_t>(a.lens[b], held)));
+  return s;
+}
+
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + KT - 1) / KT); }
+
+struct Unit {
+  int b, rb, sp, ns;                       // sequence (-1: none), row block, split, splits of the sequence
+  int W;                                   // key tiles a split
+  int64_t part;                            // index of the row block's first split's partial; the next ones are nrb apart
+  int nrb;
+  Seq s;
+};
+
+__device__ __forceinline__ int wave_sum_below(int v, int lane, int& total) {     // exclusive prefix sum over 64 lanes
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(s, o, 64);
+    if (lane >= o) s += u;
+  }
+  total = __shfl(s, 63, 64);
+  return s - v;
+}
+
+// Unit `want` of the call: units are the (sequence, split, row block)s in that order, row blocks fastest; with rows_only
+// the (sequence, row block)s. The split length W comes from the work of the whole call (key tiles x row blocks x heads over
+// `target`), read from the sequences' sizes here: every block does the same integer arithmetic, so no launch before this one
+// has to plan and a captured graph follows its lens. (A wave looks at 64 sequences at once.)
+__device__ Unit find_unit(const PagedArgs& a, int want, bool rows_only) {
+  const int lane = threadIdx.x & 63;
+  int W = 1 << 30;
+  if (a.target) {
+    float work = 0.f;                      // (only the split length depends on it; the same sum in every block)
+    for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
+      float w = 0.f;
+      if (b0 + lane < a.n_seq) {
+        const Seq s = seq_of(a, b0 + lane);
+        w = static_cast<float>((s.rows + a.qb - 1) / a.qb) * static_cast<float>(tiles_of(s.keys));
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) w += __shfl_xor(w, o, 64);
+      work += w;
+    }
+    W = max(2 * NW, static_cast<int>(ceilf(work * static_cast<float>(a.hkv) / static_cast<float>(a.target))));
+  }
+  Unit u;
+  u.b = -1;
+  int before = 0, parts = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
+    Seq s{0, 0, 0};
+    int nrb = 0, ns = 1;
+    if (b0 + lane < a.n_seq) {
+      s = seq_of(a, b0 + lane);
+      nrb = (s.rows + a.qb - 1) / a.qb;
+      ns = (tiles_of(s.keys) + W - 1) / W;
+    }
+    const int n = rows_only ? nrb : nrb * ns;
+    int total, ptotal;
+    const int pre = wave_sum_below(n, lane, total);
+    const int ppre = rows_only ? wave_sum_below(nrb * ns, lane, ptotal) : pre;
+    if (!rows_only) ptotal = total;
+    if (want < before + total) {
+      const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
+      const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      const int at = want - before - __shfl(pre, l, 64);
+      u.b = b0 + l;
+      u.nrb = __shfl(nrb, l, 64);
+      u.ns = __shfl(ns, l, 64);
+      u.s = Seq{__shfl(s.rows, l, 64), __shfl(s.keys, l, 64), __shfl(s.first, l, 64)};
+      u.rb = at % u.nrb;
+      u.sp = at / u.nrb;
+      u.W = W;
+      u.part = parts + __shfl(ppre, l, 64) + u.rb;
+      return u;
+    }
+    before += total;
+    parts += ptotal;
+  }
+  return u;
+}
+
+// Key half kb's registers of a tile: the lane's share of d of its key.
+template <int D, bool MX>
+struct KTile {
+  static constexpr int NS = D / 32;                          // 32-deep steps over d
+  uint4 x[MX ? 1 : 2][MX ? 1 : NS];                          // bf16
+  uint32_t c[MX ? 2 : 1][MX ? D / 32 : 1];                   // codes of D / 4 values
+  uint2 sc[MX ? (D == 256 ? 2 : 1) : 1];                     // scales of the 8 keys that the lane's two keys are among
+};
+
+template <int D, bool MX>
+struct VTile {
+  static constexpr int VL = D / 16;                          // consecutive values a lane takes of a key
+  uint32_t x[MX ? 1 : 8][MX ? 1 : VL / 2];                   // bf16 pairs of 8 keys
+  uint32_t c[MX ? 8 * VL / 8 : 1];                           // codes of 8 keys, key by key
+  uint2 sc;
+};
+
+template <int D, bool MX>
+__device__ __forceinline__ void load_k(KTile<D, MX>& kt, const PagesDev& pg, int64_t id, int head, int tok0, int m, int g) {
+  // tok0: the page's token of the 16-key half of the tile that key row m lies in
+  const int key = 8 * ((m >> 2) & 1) + (m & 3);              // of that half, for kb = 0
+  const char* base = pg.k + id * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
+  if constexpr (!MX) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const char* row = base + (tok0 + key + 4 * kb) * (D * 2) + g * 16;
+#pragma unroll
+      for (int s = 0; s < KTile<D, MX>::NS; ++s) kt.x[kb][s] = *reinterpret_cast<const uint4*>(row + s * 64);
+    }
+  } else {
+    constexpr int LB = D / 8;                                // bytes a lane takes of a key
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const char* row = base + (tok0 + key + 4 * kb) * (D / 2) + g * LB;
+      if constexpr (D == 64) {
+        const uint2 w = *reinterpret_cast<const uint2*>(row);
+        kt.c[kb][0] = w.x;
+        kt.c[kb][1] = w.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < LB / 16; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * i);
+          kt.c[kb][4 * i] = w.x;
+          kt.c[kb][4 * i + 1] = w.y;
+          kt.c[kb][4 * i + 2] = w.z;
+          kt.c[kb][4 * i + 3] = w.w;
+        }
+      }
+    }
+    const uint8_t* sc = pg.ks + id * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales +
+                        ((tok0 + 8 * ((m >> 2) & 1)) >> 3) * (D / 4);
+    if constexpr (D == 256) {
+      kt.sc[0] = *reinterpret_cast<const uint2*>(sc + (2 * g) * 8);
+      kt.sc[1] = *reinterpret_cast<const uint2*>(sc + (2 * g + 1) * 8);
+    } else {
+      kt.sc[0] = *reinterpret_cast<const uint2*>(sc + (D == 128 ? g : g >> 1) * 8);
+    }
+  }
+}
+
+template <int D, bool MX>
+__device__ __forceinline__ void load_v(VTile<D, MX>& vt, const PagesDev& pg, int64_t id, int head, int tok0, int n, int g) {
+  const int key = 8 * (g & 1);                               // first of the lane's 8 keys within the 16-key half
+  const char* base = pg.v + id * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
+  constexpr int VL = D / 16;
+  if constexpr (!MX) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const char* row = base + (tok0 + key + e) * (D * 2) + n * (VL * 2);
+      if constexpr (VL == 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(row);
+        vt.x[e][0] = w.x;
+        vt.x[e][1] = w.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VL / 8; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * i);
+          vt.x[e][4 * i] = w.x;
+          vt.x[e][4 * i + 1] = w.y;
+          vt.x[e][4 * i + 2] = w.z;
+          vt.x[e][4 * i + 3] = w.w;
+        }
+      }
+    }
+  } else {
+    const char* run = base + ((tok0 + key) >> 3) * (4 * D) + n * (VL * 4);    // 8 keys x VL / 2 bytes
+#pragma unroll
+    for (int i = 0; i < VL / 4; ++i) {
+      const uint4 w = *reinterpret_cast<const uint4*>(run + 16 * i);
+      vt.c[4 * i] = w.x;
+      vt.c[4 * i + 1] = w.y;
+      vt.c[4 * i + 2] = w.z;
+      vt.c[4 * i + 3] = w.w;
+    }
+    const uint8_t* sc = pg.vs + id * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales +
+                        ((tok0 + key) >> 3) * (D / 4) + (n * VL / 32) * 8;
+    vt.sc = *reinterpret_cast<const uint2*>(sc);
+  }
+}
+
+// The 32-deep step s of key half kb as an MFMA operand.
+template <int D, bool MX>
+__device__ __forceinline__ bf16x8 k_frag(const KTile<D, MX>& kt, const float (&scale)[2][2], int kb, int s) {
+  if constexpr (!MX) return as_frag(kt.x[kb][s]);
+  const uint32_t w = kt.c[kb][s];
+  const float f = scale[kb][D == 256 ? s / 4 : 0];
+  return as_frag(make_uint4(fp4_pair<0>(w, f), fp4_pair<1>(w, f), fp4_pair<2>(w, f), fp4_pair<3>(w, f)));
+}
+
+__device__ __forceinline__ float byte_scale(const uint2& w, int i) {       // i in 0 .. 7, known when inlined or not
+  const uint32_t v = i < 4 ? w.x : w.y;
+  return __uint_as_float(((v >> (8 * (i & 3))) & 255u) << 23);
+}
+
+// V's bf16 pairs of the lane's 8 keys at pair j (d = n VL + 2 j, 2 j + 1), one dword a key.
+template <int D, bool MX>
+__device__ __forceinline__ void v_pairs(const VTile<D, MX>& vt, const float (&vs)[8], int j, uint32_t (&p)[8]) {
+  if constexpr (!MX) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = vt.x[e][j];
+  } else {
+    constexpr int VB = D / 32;                               // bytes a key
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int byte = e * VB + j;
+      const uint32_t w = vt.c[byte / 4];
+      switch (byte & 3) {
+        case 0: p[e] = fp4_pair<0>(w, vs[e]); break;
+        case 1: p[e] = fp4_pair<1>(w, vs[e]); break;
+        case 2: p[e] = fp4_pair<2>(w, vs[e]); break;
+        default: p[e] = fp4_pair<3>(w, vs[e]); break;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t both_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t both_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+__device__ __forceinline__ bool not_finite(uint32_t pair) {  // either bf16 half is NaN or infinite
+  return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+
+template <int D, int MT>
+constexpr int merge_floats() { return NW * 16 * (D + 4) + 2 * NW * 16; }
+
+// The row r of a row block is query r / rep, query head r % rep of the K / V head.
+template <int D, bool MX, int MT>
+__global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
+  constexpr int NS = D / 32, NB = D / 16;
+  __shared__ float lds[merge_floats<D, MT>()];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % a.hkv;
+  const Unit u = find_unit(a, blockIdx.x / a.hkv, false);
+  if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
+  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0); // the block's queries
+  const int p0 = u.s.keys - u.s.rows + q0;                   // position of the first of them (may lie before 0)
+  const int plast = p0 + nq - 1;                             // keys 0 .. plast are read
+  const int ntiles = plast < 0 ? 0 : plast / KT + 1;
+  const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);  // (it0 < 2^31: ns W is below tiles + W)
+
+  // queries: row 16 mt + n
+  bf16x8 qf[MT][NS];
+  int pos[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = 16 * mt + n, qi = r / a.rep;
+    const bool live = qi < nq;
+    pos[mt] = live ? p0 + qi : -1;
+    const uint16_t* row = a.q + static_cast<int64_t>(u.s.first + q0 + (live ? qi : 0)) * a.ldq +
+                          (head * a.rep + (live ? r - qi * a.rep : 0)) * D;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      qf[mt][s] = as_frag(*reinterpret_cast<const uint4*>(row + (MX ? g * (D / 4) + 8 * s : 32 * s + 8 * g)));
+  }
+
+  f32x4 o[MT][NB];
+  float m[MT], l[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -INFINITY;
+    l[mt] = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[mt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The wave's tiles are it0 + w + NW i. Lane l holds the page of 16-key half l % 2 of tile i0 + l / 2 (32 tiles at once;
+  // 0 for pages that are none, whose keys `bad` then hides).
+  const int mine = it0 + w < it1 ? (it1 - it0 - w + NW - 1) / NW : 0;
+  int ids = 0;
+  uint64_t bad = 0;
+  auto fetch_ids = [&](int i0) {
+    const int it = it0 + w + NW * (i0 + (lane >> 1));
+    const int at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
+    int id = -1;
+    if (it < it1 && at < a.width) id = a.table[static_cast<int64_t>(u.b) * a.ld_table + at];
+    const bool out = id < 0 || id >= a.pg.n_pages;
+    ids = out ? 0 : id;
+    bad = __ballot(out);
+  };
+  const int mask = (1 << a.pg.shift) - 1;
+  KTile<D, MX> kt;
+  VTile<D, MX> vt;
+  auto get_k = [&](int i) {
+    const int it = it0 + w + NW * i;
+    const int id0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31)), id1 = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + 1);
+    const bool up = n >= 8;
+    load_k<D, MX>(kt, a.pg, up ? id1 : id0, head, (it * KT + (up ? 16 : 0)) & mask, n, g);
+  };
+  auto get_v = [&](int i) {
+    const int it = it0 + w + NW * i;
+    const int id0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31)), id1 = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + 1);
+    const bool up = g >= 2;
+    load_v<D, MX>(vt, a.pg, up ? id1 : id0, head, (it * KT + (up ? 16 : 0)) & mask, n, g);
+  };
+
+  for (int i = 0; i < mine; ++i) {
+    if ((i & 31) == 0) fetch_ids(i);
+    get_k(i);
+    get_v(i);
+    const int k0 = (it0 + w + NW * i) * KT;
+    const uint32_t bad2 = static_cast<uint32_t>(bad >> (2 * (i & 31))) & 3u;
+    // scores: lane (n, g) gets keys k0 + 8 g + 4 kb + j of query row 16 mt + n
+    float ks[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    if constexpr (MX) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
+          ks[kb][x] = __uint_as_float((((kb ? kt.sc[x].y : kt.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
+    }
+    f32x4 sc[MT][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const bf16x8 kf = k_frag<D, MX>(kt, ks, kb, s);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[mt][s], sc[mt][kb], 0, 0, 0);
+      }
+    }
+    const bool edge = k0 + KT - 1 > p0 || bad2;              // some row does not see some key of the tile
+    const bool hidden = (bad2 >> (g >> 1)) & 1u;             // the lane's 8 keys lie on a page that is none
+    uint32_t pk[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if (edge) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
+      }
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, sc[mt][kb][j]);
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      if (__any(tmax > m[mt] + RESCALE_LOG2 / a.c)) {
+        const float top = fmaxf(m[mt], tmax);
+        const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[mt] - top) * a.c);
+        m[mt] = top;
+        l[mt] *= alpha;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float al = __shfl(alpha, 4 * g + j, 64);     // O's rows of a lane are 4 g + j
+#pragma unroll
+          for (int b = 0; b < NB; ++b) o[mt][b][j] *= al;
+        }
+      }
+      const float mc = m[mt] == -INFINITY ? 0.f : m[mt] * a.c;
+      float psum = 0.f;
+      float p[8];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[4 * kb + j] = __builtin_amdgcn_exp2f(fmaf(sc[mt][kb][j], a.c, -mc));
+          psum += p[4 * kb + j];
+        }
+      l[mt] += psum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pk[mt][j] = bf16_pair(p[2 * j], p[2 * j + 1]);
+    }
+    // O += P V
+    float vs[8];
+    if constexpr (MX) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vs[e] = byte_scale(vt.sc, e);
+    }
+    bool apart = false;                                      // a value that some row must not meet is not finite
+    if (edge) {
+      const int last = hidden ? -1 : plast - k0 - 8 * g;     // of the lane's keys, the last that any row sees
+#pragma unroll
+      for (int j = 0; j < NB / 2; ++j) {
+        uint32_t p[8];
+        v_pairs<D, MX>(vt, vs, j, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) apart |= e <= last && not_finite(p[e]);
+      }
+      apart = __any(apart);
+      if constexpr (!MX) {                                   // keys that no row sees may hold anything
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int j = 0; j < NB / 2; ++j) vt.x[e][j] = e <= last ? vt.x[e][j] : 0u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vs[e] = e <= last ? vs[e] : 0.f;       // (2^-127: the codes' values stay finite, p is 0)
+      }
+    }
+    if (!apart) {
+#pragma unroll
+      for (int j = 0; j < NB / 2; ++j) {
+        uint32_t p[8];
+        v_pairs<D, MX>(vt, vs, j, p);
+        const bf16x8 f0 = as_frag(make_uint4(both_low(p[0], p[1]), both_low(p[2], p[3]), both_low(p[4], p[5]), both_low(p[6], p[7])));
+        const bf16x8 f1 = as_frag(make_uint4(both_high(p[0], p[1]), both_high(p[2], p[3]), both_high(p[4], p[5]), both_high(p[6], p[7])));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const bf16x8 pf = as_frag(make_uint4(pk[mt][0], pk[mt][1], pk[mt][2], pk[mt][3]));
+          o[mt][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, o[mt][2 * j], 0, 0, 0);
+          o[mt][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, o[mt][2 * j + 1], 0, 0, 0);
+        }
+      }
+    } else {
+      // 0 x infinity must not reach a row that does not see the key: query by query with the keys past it zeroed, each
+      // product kept for that query's rows only
+      for (int qi = 0; qi < nq; ++qi) {
+        const int last = hidden ? -1 : p0 + qi - k0 - 8 * g;
+        for (int j = 0; j < NB / 2; ++j) {
+#pragma unroll
+          for (int jj = 0; jj < NB / 2; ++jj) {              // (static register indexes)
+            if (jj != j) continue;
+            uint32_t p[8];
+            v_pairs<D, MX>(vt, vs, jj, p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = e <= last ? p[e] : 0u;
+            const bf16x8 f0 = as_frag(make_uint4(both_low(p[0], p[1]), both_low(p[2], p[3]), both_low(p[4], p[5]), both_low(p[6], p[7])));
+            const bf16x8 f1 = as_frag(make_uint4(both_high(p[0], p[1]), both_high(p[2], p[3]), both_high(p[4], p[5]), both_high(p[6], p[7])));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const bf16x8 pf = as_frag(make_uint4(pk[mt][0], pk[mt][1], pk[mt][2], pk[mt][3]));
+              const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+              const f32x4 t0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, z, 0, 0, 0);
+              const f32x4 t1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, z, 0, 0, 0);
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if ((16 * mt + 4 * g + x) / a.rep == qi) {
+                  o[mt][2 * jj][x] += t0[x];
+                  o[mt][2 * jj + 1][x] += t1[x];
+                }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // merge the waves: thread t takes row t / 16 of each 16 rows and D / 16 columns
+  const int64_t part = (u.part + static_cast<int64_t>(u.sp) * u.nrb) * a.hkv + head;
+  float* ml = lds + NW * 16 * (D + 4);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    if (mt) __syncthreads();
+    float ls = l[mt];
+    ls += __shfl_xor(ls, 16, 64);
+    ls += __shfl_xor(ls, 32, 64);
+    if (g == 0) {
+      ml[w * 16 + n] = m[mt] == -INFINITY ? m[mt] : m[mt] * a.c;           // base 2
+      ml[(NW + w) * 16 + n] = ls;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int b = 0; b < NB; b += 4)
+        *reinterpret_cast<float4*>(lds + (w * 16 + 4 * g + j) * (D + 4) + n * NB + b) =
+            make_float4(o[mt][b][j], o[mt][b + 1][j], o[mt][b + 2][j], o[mt][b + 3][j]);
+    __syncthreads();
+    const int row = t >> 4, d0 = (t & 15) * NB;
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) top = fmaxf(top, ml[x * 16 + row]);
+    float sum = 0.f, acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float mx = ml[x * 16 + row];
+      const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
+      sum += ml[(NW + x) * 16 + row] * f;
+#pragma unroll
+      for (int b = 0; b < NB; b += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(lds + (x * 16 + row) * (D + 4) + d0 + b);
+        if (f != 0.f) {                                      // (a wave without keys of this row holds zeros or nothing)
+          acc[b] += v.x * f;
+          acc[b + 1] += v.y * f;
+          acc[b + 2] += v.z * f;
+          acc[b + 3] += v.w * f;
+        }
+      }
+    }
+    const int r = 16 * mt + row, qi = r / a.rep;
+    if (qi >= nq) continue;
+    if (u.ns > 1) {
+      float* p = a.part + part * (16 * MT * (D + 2));
+#pragma unroll
+      for (int b = 0; b < NB; b += 4)
+        *reinterpret_cast<float4*>(p + r * D + d0 + b) = make_float4(acc[b], acc[b + 1], acc[b + 2], acc[b + 3]);
+      if ((t & 15) == 0) {
+        p[16 * MT * D + r] = top;
+        p[16 * MT * (D + 1) + r] = sum;
+      }
+      continue;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;          // no key: zeros (a NaN stays one)
+    uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+#pragma unroll
+    for (int b = 0; b < NB; b += 4)
+      *reinterpret_cast<uint2*>(dst + b) =
+          make_uint2(bf16_pair(acc[b] * inv, acc[b + 1] * inv), bf16_pair(acc[b + 2] * inv, acc[b + 3] * inv));
+  }
+}
+
+// Merges the splits of one row block and head in split order: a thread takes D / 16 columns of one row.
+template <int D, int MT>
+__global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
+  constexpr int NB = D / 16;
+  const int t = threadIdx.x, head = blockIdx.x % a.hkv;
+  const Unit u = find_unit(a, blockIdx.x / a.hkv, true);
+  // (partials past the last unit: only with a cu that does not rise, whose units the launch does not hold)
+  if (u.b < 0 || u.ns == 1 || u.part + static_cast<int64_t>(u.ns - 1) * u.nrb >= a.units) return;
+  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0);
+  const int d0 = (t & 15) * NB, r = blockIdx.y * 16 + (t >> 4), qi = r / a.rep;
+  if (qi >= nq) return;
+  const float* p0 = a.part + (u.part * a.hkv + head) * (16 * MT * (D + 2));
+  const int64_t step = static_cast<int64_t>(u.nrb) * a.hkv * (16 * MT * (D + 2));
+  float top = -INFINITY;
+  for (int s = 0; s < u.ns; ++s) top = fmaxf(top, p0[s * step + 16 * MT * D + r]);
+  float sum = 0.f, acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = 0.f;
+  for (int s = 0; s < u.ns; ++s) {
+    const float* p = p0 + s * step;
+    const float ms = p[16 * MT * D + r];
+    if (ms == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(ms - top);
+    sum += p[16 * MT * (D + 1) + r] * f;
+#pragma unroll
+    for (int b = 0; b < NB; b += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + r * D + d0 + b);
+      acc[b] += v.x * f;
+      acc[b + 1] += v.y * f;
+      acc[b + 2] += v.z * f;
+      acc[b + 3] += v.w * f;
+    }
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+#pragma unroll
+  for (int b = 0; b < NB; b += 4)
+    *reinterpret_cast<uint2*>(dst + b) =
+        make_uint2(bf16_pair(acc[b] * inv, acc[b + 1] * inv), bf16_pair(acc[b + 2] * inv, acc[b + 3] * inv));
+}
+
+// 16-row blocks a wave takes: as few as hold a sequence's rows.
+int row_tiles(int rep, int64_t max_rows) {
+  const int64_t rows = std::min<int64_t>(max_rows, 64) * rep;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+
+struct Plan {
+  int mt, qb, target;
+  int64_t blocks, units;                   // (sequence, row block)s at most, and with their splits
+  size_t bytes;
+};
+
+// The launch for these sizes. Row blocks: sum of ceil(rows / qb) <= T / qb + n_seq. Splits: sum of nrb ceil(tiles / W) <=
+// sum of nrb tiles / W + row blocks, and W >= work hkv / target, so they are at most target / hkv + row blocks.
+Plan plan_of(int64_t T, int hq, int hkv, int d, int n_seq, int64_t max_rows, int64_t max_keys) {
+  Plan p{};
+  const int rep = hq / hkv;
+  p.mt = row_tiles(rep, max_rows);
+  p.qb = 16 * p.mt / rep;
+  p.blocks = std::min<int64_t>(T, T / p.qb + n_seq);
+  p.target = max_keys > 16 * NW * KT ? 1024 : 0;
+  p.units = p.target ? p.target / hkv + 1 + p.blocks : p.blocks;
+  p.bytes = p.target ? static_cast<size_t>(p.units) * hkv * (16 * p.mt * (d + 2)) * 4 : 0;
+  return p;
+}
+
+int attend_sizes(const char* fn, int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows, int64_t max_keys) {
+  if (d != 64 && d != 128 && d != 256) return fail(RF_EUNSUPPORTED, "%s: head_dim %d (the kernels take 64, 128, 256)", fn, d);
+  if (hq <= 0 || hkv <= 0 || hkv > 4096 || hq % hkv || hq / hkv > 64)
+    return fail(RF_EUNSUPPORTED, "%s: %d query heads over %d K / V heads (groups of up to 64)", fn, hq, hkv);
+  if (kind != RF_PAGES_BF16 && kind != RF_PAGES_MX4) return fail(RF_EINVAL_ARG, "%s: kind of pages %d", fn, kind);
+  if (T < 0 || T > (1 << 24) || n_seq < 0 || n_seq > (1 << 20) || max_rows < 0 || max_keys < 0 || max_keys > (1 << 30))
+    return fail(RF_EINVAL_SHAPE, "%s: %lld rows of %d sequences, at most %lld rows and %lld keys each", fn, (long long)T, n_seq,
+                (long long)max_rows, (long long)max_keys);
+  return RF_OK;
+}
+
+}  // namespace
+}  // namespace rf
+
+using namespace rf;
+
+extern "C" int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows,
+                                               int64_t max_keys, size_t* bytes) {
+  const char* fn = "rf_attend_paged_workspace_bytes";
+  if (!bytes) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (int rc = attend_sizes(fn, T, hq, hkv, d, kind, n_seq, max_rows, max_keys)) return rc;
+  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, n_seq, max_rows, max_keys).bytes : 0;
+  return RF_OK;
+}
+
+extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages,
+                               const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens,
+                               const int32_t* cu, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out,
+                               int64_t ldo, void* workspace, size_t ws_bytes, hipStream_t stream) {
+  const char* fn = "rf_attend_paged";
+  PagesDev pg;
+  if (int rc = check_pages(fn, pages, &pg)) return rc;
+  const int d = pages->d, hkv = pages->hkv;
+  if (!q || !table || !lens || !cu || !out) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (int rc = attend_sizes(fn, T, hq, hkv, d, pages->kind, n_seq, max_rows, max_keys)) return rc;
+  if (ldq < static_cast<int64_t>(hq) * d || ldo < static_cast<int64_t>(hq) * d || ldq % 8 || ldo % 4 || table_width < 0 ||
+      table_width > (1 << 26) || ld_table < table_width)
+    return fail(RF_EINVAL_SHAPE, "%s: strides (q %lld, out %lld) or a table %lld wide (row stride %lld)", fn, (long long)ldq,
+                (long long)ldo, (long long)table_width, (long long)ld_table);
+  if (!aligned16(q) || (reinterpret_cast<uintptr_t>(out) & 7u) || (workspace && !aligned16(workspace)))
+    return fail(RF_EINVAL_SHAPE, "%s: alignment", fn);
+  if (!(scale > 0.f) || !(scale < 1e30f))
+    return fail(RF_EINVAL_ARG, "%s: scale %g (must be positive)", fn, static_cast<double>(scale));
+  if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
+  Plan p = plan_of(T, hq, hkv, d, n_seq, max_rows, max_keys);
+  if (p.target && (!workspace || ws_bytes < p.bytes)) {
+    p.target = 0;
+    p.units = p.blocks;
+  }
+  const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.qb,
+                    static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
+                    scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace), p.target, p.units};
+  const dim3 grid(static_cast<unsigned>(p.units * hkv)), grid2(static_cast<unsigned>(p.blocks * hkv), p.mt);
+  const bool mx = pages->kind == RF_PAGES_MX4;
+#define RF_FEW(D, MT)                                                                                    \
+  do {                                                                                                   \
+    if (mx) hipLaunchKernelGGL((k_paged_few<D, true, MT>), grid, dim3(64 * NW), 0, stream, a);           \
+    else hipLaunchKernelGGL((k_paged_few<D, false, MT>), grid, dim3(64 * NW), 0, stream, a);             \
+    if (p.target) {                                                                                      \
+      if (int rc = check_launch(fn)) return rc;                                                          \
+      hipLaunchKernelGGL((k_paged_merge<D, MT>), grid2, dim3(256), 0, stream, a);                        \
+    }                                                                                                    \
+  } while (0)
+#define RF_FEW_D(D)                    \
+  do {                                 \
+    if (p.mt == 1) RF_FEW(D, 1);       \
+    else if (p.mt == 2) RF_FEW(D, 2);  \
+    else RF_FEW(D, 4);                 \
+  } while (0)
+  if (d == 64) RF_FEW_D(64);
+  else if (d == 128) RF_FEW_D(128);
+  else RF_FEW_D(256);
+#undef RF_FEW_D
+#undef RF_FEW
+  return check_launch(fn);
+}

@@ -5,6 +5,7 @@ explicit caches) on PyTorch-ROCm tensors, with the arithmetic in librfill.so's h
 kernels (the C ABI in include/rfill.h). Submodules:
   rfill.ops    tensor front end of the C ABI
   rfill.model  FillModel: packed per-layer weights and the fill / fill_kv API
+  rfill.paged  Pages: a paged cache of several sequences, bfloat16 or 4 bits
   rfill.kva    Arm, Projector, fill_late (finish()'s late-layer fill loop)
   rfill.synth  seeded synthetic workloads
 Importing rfill does not load the library; the first kernel call does, and raises ImportError if

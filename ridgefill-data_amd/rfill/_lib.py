@@ -28,6 +28,13 @@ _SZ, _PSZ = ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
 _PP = ctypes.POINTER(ctypes.c_void_p)       # a host array of device pointers
 _PI64 = ctypes.POINTER(ctypes.c_int64)      # a host array of counts
 
+
+class RfPages(ctypes.Structure):
+    """rf_pages of include/rfill.h."""
+    _fields_ = [("k", _P), ("v", _P), ("ks", _P), ("vs", _P), ("n_pages", _I64), ("page_stride", _I64),
+                ("scale_stride", _I64), ("kind", _I32), ("hkv", _I32), ("d", _I32), ("page", _I32)]
+
+
 # name -> argument types (every function returns int status)
 SIGNATURES = {
     "rf_map_apply": [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _SZ, _P],
@@ -97,6 +104,12 @@ SIGNATURES = {
     "rf_dequant_gguf_rows": [_I32, _P, _I64, _I64, _I64, _P, _I64, _P],
     "rf_dequant_i8_rows": [_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _P],
     "rf_read_cosine": [_P, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P, _I32, _F64, _P, _P, _SZ, _P],
+    "rf_paged_slots": [_P, _I64, _I64, _P, _P, _I32, _I64, _I32, _I64, _P, _P, _P],
+    "rf_paged_append": [_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _I64, _I32, _P, _I64, _P, _P, _I32,
+                        _F32, _P],
+    "rf_paged_read": [_P, _P, _I64, _P, _I64, _P, _I64, _P],
+    "rf_attend_paged": [_P, _I64, _I64, _I32, _P, _P, _I64, _I64, _P, _P, _I32, _I64, _I64, _F32, _P, _I64, _P, _SZ, _P],
+    "rf_attend_paged_workspace_bytes": [_I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _PSZ],
     "rf_window_mass_workspace_bytes": [_I32, _I32, _I32, _I32, _I64, _PSZ],
     "rf_window_mass": [_P, _I64, _I32, _I64, _I32, _I32, _P, _I32, _I64, _I64, _F32, _P, _P, _SZ, _P],
 }

@@ -995,3 +995,155 @@ def inv_freq_llama3(theta, dim, factor, low_freq_factor, high_freq_factor, origi
     mixed = (1 - smooth) * scaled / factor + smooth * scaled
     mid = (wavelen >= hi_wl) & (wavelen <= lo_wl)
     return torch.where(mid, mixed, scaled)
+
+
+# ------------------------------------------------------------------------------------------ the paged cache
+# Checks as above, and two more: every tensor on the pages' device, and the launch made with that device current (a
+# serving process may hold several).
+
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: on {t.device}, the pages are on {dev}")
+
+
+def _call_on(t, name, *args):
+    if t.get_device() == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args)
+
+
+def _sequences(table, lens, cu):
+    _need(table, "table", torch.int32, 2)
+    _need(lens, "lens", torch.int32, 1)
+    _need(cu, "cu", torch.int32, 1)
+    n = lens.shape[0]
+    if table.shape[0] != n or cu.shape[0] != n + 1:
+        raise ValueError(f"table {tuple(table.shape)}, lens {tuple(lens.shape)}, cu {tuple(cu.shape)}: one row of pages and "
+                         f"one length a sequence, one more offset")
+    return n
+
+
+def paged_slots(table, lens, cu, rows, pages):
+    """Slots and positions (int64 [rows] each, on the device) of the new rows of several sequences: sequence b's rows are
+    [cu[b], cu[b + 1]) and become its last tokens, positions lens[b] - count .. lens[b] - 1, in the pages table[b] lists in
+    order. A row of no sequence, before position 0, past the table or on a page outside the pool gets slot -1."""
+    n = _sequences(table, lens, cu)
+    _same_device(pages.k.device, table=table, lens=lens, cu=cu)
+    slots = torch.empty(rows, dtype=torch.int64, device=table.device)
+    pos = torch.empty_like(slots)
+    _call_on(table, "rf_paged_slots", _ptr(table) or _ptr(lens), max(table.stride(0), table.shape[1]), table.shape[1],
+             _ptr(lens) or _ptr(cu), _ptr(cu), n, pages.n_pages, pages.page, rows, _ptr(slots) or _ptr(cu),
+             _ptr(pos) or _ptr(cu), _stream(cu))
+    return slots, pos
+
+
+def paged_append(k, v, slots, pages, cs=None, q=None, out=None, qnorm=None, knorm=None, norm_kind=0, eps=0.0):
+    """Write K / V of new rows k, v [rows, hkv, d] bf16 (any row and head stride) into slots [rows] of the pages
+    (rfill.paged.Pages; a slot outside the pool is skipped; no slot twice), normed by knorm [d] and rotated by the table cs
+    [rows, rot] (rope_table of the rows' positions) where given, and return the rows' queries q [rows, hq d] normed by qnorm
+    and rotated (None without q; out may be q). norm_kind: 0 gain, 1 (1 + gain). fp32 arithmetic, one rounding."""
+    for name, t in (("k", k), ("v", v)):
+        _need(t, name, torch.bfloat16, 3)
+        if tuple(t.shape[1:]) != (pages.hkv, pages.d):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [rows, {pages.hkv}, {pages.d}]")
+    rows, d = k.shape[0], pages.d
+    _need(slots, "slots", torch.int64, 1)
+    if v.shape[0] != rows or slots.shape[0] != rows:
+        raise ValueError(f"paged_append: {rows} rows of K, {v.shape[0]} of V, {slots.shape[0]} slots")
+    hq = rot = 0
+    if cs is not None:
+        _need(cs, "cs", torch.bfloat16, 2)
+        rot = cs.shape[1]
+        if cs.shape[0] != rows or not cs.is_contiguous():
+            raise ValueError("paged_append: cs rows")
+    if q is not None:
+        _need(q, "q", torch.bfloat16, 2)
+        if q.shape[0] != rows or q.shape[1] % d:
+            raise ValueError(f"paged_append: q {tuple(q.shape)}, expected [{rows}, heads x {d}]")
+        hq = q.shape[1] // d
+        out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device) if out is None else out
+        _need(out, "out", torch.bfloat16, 2)
+        if out.shape != q.shape:
+            raise ValueError(f"paged_append: out {tuple(out.shape)}, expected {tuple(q.shape)}")
+    elif out is not None or qnorm is not None:
+        raise ValueError("paged_append: out and qnorm go with q")
+    for name, t in (("qnorm", qnorm), ("knorm", knorm)):
+        if t is not None:
+            _need(t, name, torch.bfloat16, 1)
+            if t.shape[0] != d:
+                raise ValueError(f"paged_append: {name} width")
+    dev = pages.k.device
+    if not (k.device == v.device == slots.device == dev):
+        _same_device(dev, k=k, v=v, slots=slots)
+    _same_device(dev, cs=cs, q=q, out=out, qnorm=qnorm, knorm=knorm)
+    if rows == 0:
+        return out
+    _call_on(k, "rf_paged_append", _ptr(k), k.stride(0) if rows > 1 else max(k.stride(0), d), k.stride(1) if pages.hkv > 1
+             else d, _ptr(v), v.stride(0) if rows > 1 else max(v.stride(0), d), v.stride(1) if pages.hkv > 1 else d, rows,
+             _ptr(slots), pages.handle, _ptr(cs), rot, _ptr(q), 0 if q is None else max(q.stride(0), hq * d), hq, _ptr(out),
+             0 if q is None else max(out.stride(0), hq * d), _ptr(qnorm), _ptr(knorm), int(norm_kind), float(eps),
+             _stream(k))
+    return out
+
+
+def paged_read(pages, slots, k_out=None, v_out=None):
+    """K, V [rows, hkv, d] bf16 at the pages' slots [rows] (zeros for slots outside the pool)."""
+    _need(slots, "slots", torch.int64, 1)
+    shape = (slots.shape[0], pages.hkv, pages.d)
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        t = torch.empty(shape, dtype=torch.bfloat16, device=slots.device) if t is None else t
+        _need(t, name, torch.bfloat16, 3)
+        if tuple(t.shape) != shape or (shape[1] > 1 and t.stride(1) != pages.d):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape} with its heads side by side")
+        outs.append(t)
+    _same_device(pages.k.device, slots=slots, k_out=outs[0], v_out=outs[1])
+    if shape[0]:
+        lds = [max(t.stride(0), shape[1] * shape[2]) for t in outs]
+        _call_on(slots, "rf_paged_read", pages.handle, _ptr(slots), shape[0], _ptr(outs[0]), lds[0], _ptr(outs[1]), lds[1],
+                 _stream(slots))
+    return outs[0], outs[1]
+
+
+@_size_rule
+def attend_paged_workspace_bytes(rows, hq, hkv, d, kind, n_seq, max_rows, max_keys):
+    """Device bytes attend_paged uses to split the keys of a sequence over more blocks (0: no split)."""
+    b = ctypes.c_size_t(0)
+    _lib.call("rf_attend_paged_workspace_bytes", rows, hq, hkv, d, kind, n_seq, max_rows, max_keys, ctypes.byref(b))
+    return b.value
+
+
+def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=None, workspace="auto"):
+    """Causal attention of the new rows q [rows, hq d] of several sequences over their pages (rfill.paged.Pages): sequence
+    b's rows [cu[b], cu[b + 1]) are its last tokens of lens[b], in the pages table[b] lists in order (table int32 [n, width],
+    lens int32 [n], cu int32 [n + 1], all on the device). max_rows / max_keys: host bounds on a sequence's rows and tokens
+    (more of either is not looked at). Returns [rows, hq d] bf16; a row that sees no key gets zeros, a row of no sequence is
+    left as it was. workspace: uint8 device memory for splits of the keys ("auto": allocated here; None: no split)."""
+    _need(q, "q", torch.bfloat16, 2)
+    n = _sequences(table, lens, cu)
+    rows, d = q.shape[0], pages.d
+    if q.shape[1] < hq * d:
+        raise ValueError(f"attend_paged: q {tuple(q.shape)} for {hq} heads of {d}")
+    out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device) if out is None else out
+    _need(out, "out", torch.bfloat16, 2)
+    if out.shape[0] != rows or out.shape[1] < hq * d:
+        raise ValueError(f"attend_paged: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
+    need = attend_paged_workspace_bytes(rows, hq, pages.hkv, d, pages.kind, n, max_rows, max_keys)
+    if isinstance(workspace, str):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    if workspace is not None:
+        _need(workspace, "workspace", torch.uint8, 1)
+    dev = pages.k.device
+    if not (q.device == table.device == lens.device == cu.device == out.device == dev):
+        _same_device(dev, q=q, table=table, lens=lens, cu=cu, out=out)
+    _same_device(dev, workspace=workspace)
+    if rows == 0 or n == 0:
+        return out
+    _call_on(q, "rf_attend_paged", _ptr(q), max(q.stride(0), hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),
+             max(table.stride(0), table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), n, max_rows, max_keys, float(scale),
+             _ptr(out), max(out.stride(0), hq * d), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+             _stream(q))
+    return out
