@@ -287,15 +287,208 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {  // either bf16 half
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
 
-template <int D, int MT>
+__device__ __forceinline__ float inverse_sum(float sum) {    // no key seen: zeros (a NaN stays one)
+  return sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+}
+
+// N columns from d0 of row r of a row block (query q0 + r / rep): the output, or the partial of a split.
+template <int D, int N>
+__device__ __forceinline__ void finish_row(const PagedArgs& a, const Unit& u, int64_t part, int rpb, int r, int head, int q0,
+                                           int d0, const float (&acc)[N], float top, float sum) {
+  if (u.ns > 1) {
+    float* p = a.part + part * (static_cast<int64_t>(rpb) * (D + 2));
+#pragma unroll
+    for (int b = 0; b < N; b += 4)
+      *reinterpret_cast<float4*>(p + r * D + d0 + b) = make_float4(acc[b], acc[b + 1], acc[b + 2], acc[b + 3]);
+    if (d0 == 0) {
+      p[rpb * D + r] = top;
+      p[rpb * (D + 1) + r] = sum;
+    }
+    return;
+  }
+  const float inv = inverse_sum(sum);
+  const int qi = r / a.rep;
+  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+#pragma unroll
+  for (int b = 0; b < N; b += 4)
+    *reinterpret_cast<uint2*>(dst + b) =
+        make_uint2(bf16_pair(acc[b] * inv, acc[b + 1] * inv), bf16_pair(acc[b + 2] * inv, acc[b + 3] * inv));
+}
+
+template <int D>
 constexpr int merge_floats() { return NW * 16 * (D + 4) + 2 * NW * 16; }
 
-// The row r of a row block is query r / rep, query head r % rep of the K / V head.
-template <int D, bool MX, int MT>
-__global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
+// One tile's registers and what its pages are.
+template <int D, bool MX>
+struct Tile {
+  KTile<D, MX> k;
+  VTile<D, MX> v;
+  int k0;                                  // first key
+  uint32_t bad;                            // bits: a 16-key half on a page that is none
+};
+
+// The wave's running state: O [rows 16 mt + 4 g + j][d = n NB + b], and of row 16 mt + n the reference maximum m (raw
+// scores; the same in the four lanes of a row) and the lane's share of the row sum.
+template <int D, int MT>
+struct Rows {
+  f32x4 o[MT][D / 16];
+  float m[MT], l[MT];
+};
+
+__device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // with zeros for the halves that are NaN or infinite
+  p = (p & 0x7f80u) == 0x7f80u ? p & 0xffff0000u : p;
+  return (p & 0x7f800000u) == 0x7f800000u ? p & 0xffffu : p;
+}
+
+// V's fragments of pair j; CUT: with zeros for the lane's keys past `last` and for what is not finite.
+template <int D, bool MX, bool CUT>
+__device__ __forceinline__ void v_frags(const VTile<D, MX>& vt, const float (&vs)[8], int j, int last, bf16x8& f0, bf16x8& f1) {
+  uint32_t p[8];
+  v_pairs<D, MX>(vt, vs, j, p);
+  if constexpr (CUT) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = e <= last ? finite_pair(p[e]) : 0u;
+  }
+  f0 = as_frag(make_uint4(both_low(p[0], p[1]), both_low(p[2], p[3]), both_low(p[4], p[5]), both_low(p[6], p[7])));
+  f1 = as_frag(make_uint4(both_high(p[0], p[1]), both_high(p[2], p[3]), both_high(p[4], p[5]), both_high(p[6], p[7])));
+}
+
+// What a row meets of V that is not finite, kept apart from the products (there, 0 x infinity would reach rows that do not
+// see the key): marks of (row, column), one byte each (1 infinity, 2 -infinity, 4 NaN).
+__device__ __forceinline__ uint32_t mark_of(uint32_t half) {
+  return (half & 0x7f80u) != 0x7f80u ? 0u : (half & 0x7fu) ? 4u : (half & 0x8000u) ? 2u : 1u;
+}
+
+__device__ __forceinline__ float marked(uint32_t m) {
+  return (m & 4u) || (m & 3u) == 3u ? NAN : (m & 1u) ? INFINITY : (m & 2u) ? -INFINITY : 0.f;
+}
+
+// One tile: scores, softmax, O += P V. next_k / next_v load the following tile's registers where this one's are done with.
+// EDGE: some row does not see some key of it. Keys are hidden from rows by their scores (-infinity); of V, what no row sees
+// and what is not finite enters the product as zero, and the latter leaves its marks in the rows that see it.
+template <int D, bool MX, int MT, bool EDGE, class NK, class NV>
+__device__ __forceinline__ void tile_step(Tile<D, MX>& tl, const bf16x8 (&qf)[MT][D / 32], const int (&pos)[MT],
+                                          Rows<D, MT>& st, float c, int p0, int plast, int rep, int lane, uint32_t* marks,
+                                          NK&& next_k, NV&& next_v) {
   constexpr int NS = D / 32, NB = D / 16;
-  __shared__ float lds[merge_floats<D, MT>()];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = lane & 15, g = lane >> 4;
+  const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
+  const uint32_t bad = tl.bad;
+  float ks[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  if constexpr (MX) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
+        ks[kb][x] = __uint_as_float((((kb ? tl.k.sc[x].y : tl.k.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
+  }
+  f32x4 sc[MT][2];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const bf16x8 kf = k_frag<D, MX>(tl.k, ks, kb, s);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[mt][s], sc[mt][kb], 0, 0, 0);
+    }
+  }
+  next_k();
+  const bool hidden = EDGE && ((bad >> (g >> 1)) & 1u);      // the lane's 8 keys lie on a page that is none
+  bf16x8 pf[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
+    }
+    float tmax = -INFINITY;                                  // of the lane's keys; the row's only where the maximum rises
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, sc[mt][kb][j]);
+    if (__any(tmax > st.m[mt] + RESCALE_LOG2 / c)) {
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      const float top = fmaxf(st.m[mt], tmax);
+      const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[mt] - top) * c);
+      st.m[mt] = top;
+      st.l[mt] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float al = __shfl(alpha, 4 * g + j, 64);       // O's rows of a lane are 4 g + j
+#pragma unroll
+        for (int b = 0; b < NB; ++b) st.o[mt][b][j] *= al;
+      }
+    }
+    const float mc = st.m[mt] == -INFINITY ? 0.f : st.m[mt] * c;
+    float p[8];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[4 * kb + j] = __builtin_amdgcn_exp2f(fmaf(sc[mt][kb][j], c, -mc));
+    st.l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    pf[mt] = as_frag(make_uint4(bf16_pair(p[0], p[1]), bf16_pair(p[2], p[3]), bf16_pair(p[4], p[5]), bf16_pair(p[6], p[7])));
+  }
+  float vs[8];
+  if constexpr (MX) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vs[e] = byte_scale(tl.v.sc, e);
+  }
+  const int last = !EDGE ? 8 : hidden ? -1 : plast - k0 - 8 * g;        // of the lane's keys, the last that any row sees
+  if constexpr (EDGE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+      for (int j = 0; j < NB / 2; ++j) {
+        uint32_t two;
+        if constexpr (MX) {                                  // 4 bits: only a scale can make values NaN
+          if (j) continue;
+          two = (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
+        } else {
+          two = tl.v.x[e][j];
+        }
+        if (e <= last && not_finite(two)) {
+          const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 8;
+          const int first = max(0, k0 + 8 * g + e - p0) * rep;          // rows from the key's own query on
+          for (int r = first; r < min(16 * MT, (plast - p0 + 1) * rep); ++r) {
+            if constexpr (MX) {
+#pragma unroll
+              for (int x = 0; x < NB / 4; ++x) atomicOr(marks + (r * D + n * NB) / 4 + x, 0x04040404u);
+            } else {
+              atomicOr(marks + (r * D + n * NB + 2 * j) / 4, m2 << (j & 1 ? 16 : 0));
+            }
+          }
+          marks[16 * MT * D / 4] = 1u;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NB / 2; ++j) {
+    bf16x8 f0, f1;
+    v_frags<D, MX, EDGE>(tl.v, vs, j, last, f0, f1);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      st.o[mt][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f0, st.o[mt][2 * j], 0, 0, 0);
+      st.o[mt][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f1, st.o[mt][2 * j + 1], 0, 0, 0);
+    }
+  }
+  next_v();
+}
+
+// The row r of a row block is query r / rep, query head r % rep of the K / V head.
+template <int D, int MT>
+constexpr int few_waves() { return D == 64 ? (MT <= 3 ? 2 : 1) : D == 128 && MT <= 2 ? 2 : 1; }
+
+template <int D, bool MX, int MT>
+__global__ __launch_bounds__(64 * NW, (few_waves<D, MT>())) void k_paged_few(PagedArgs a) {
+  constexpr int NS = D / 32, NB = D / 16;
+  __shared__ float lds[merge_floats<D>() + 4 * MT * D + 1];
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % a.hkv;
   const Unit u = find_unit(a, blockIdx.x / a.hkv, false);
   if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
@@ -305,6 +498,51 @@ __global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
   const int ntiles = plast < 0 ? 0 : plast / KT + 1;
   const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);  // (it0 < 2^31: ns W is below tiles + W)
 
+  // The wave's tiles are it0 + w + NW i, i < mine. Lane l holds the page of 16-key half l % 2 of tile i0 + l / 2 of a window
+  // of 32 tiles (0 for pages that are none, whose keys `bad` then hides), and the next window's entry on its way.
+  const int mine = it0 + w < it1 ? (it1 - it0 - w + NW - 1) / NW : 0;
+  const int32_t* row = a.table + static_cast<int64_t>(u.b) * a.ld_table;
+  auto entry = [&](int i0) {
+    const int it = it0 + w + NW * (i0 + (lane >> 1));
+    const int at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
+    return it < it1 && at < a.width ? row[at] : -1;
+  };
+  int ids = entry(0), coming = entry(32);
+  uint64_t bad;
+  auto settle = [&]() {
+    const bool out = ids < 0 || ids >= a.pg.n_pages;
+    ids = out ? 0 : ids;
+    bad = __ballot(out);
+  };
+  settle();
+  const int mask = (1 << a.pg.shift) - 1;
+  auto window = [&](int i) {                                 // before the loads of tile i
+    if ((i & 31) == 0) {
+      ids = coming;
+      settle();
+      coming = entry(i + 32);
+    }
+  };
+  auto get_k = [&](Tile<D, MX>& tl, int i) {                 // i < mine; windows in order
+    const int x = 2 * (i & 31), id0 = __builtin_amdgcn_readlane(ids, x), id1 = __builtin_amdgcn_readlane(ids, x + 1);
+    const int k0 = (it0 + w + NW * i) * KT;
+    load_k<D, MX>(tl.k, a.pg, n >= 8 ? id1 : id0, head, (k0 + (n >= 8 ? 16 : 0)) & mask, n, g);
+  };
+  auto get_v = [&](Tile<D, MX>& tl, int i) {
+    const int x = 2 * (i & 31), id0 = __builtin_amdgcn_readlane(ids, x), id1 = __builtin_amdgcn_readlane(ids, x + 1);
+    tl.k0 = (it0 + w + NW * i) * KT;
+    tl.bad = static_cast<uint32_t>(bad >> x) & 3u;
+    load_v<D, MX>(tl.v, a.pg, g >= 2 ? id1 : id0, head, (tl.k0 + (g >= 2 ? 16 : 0)) & mask, n, g);
+  };
+
+  Tile<D, MX> ta, tb;
+  if (mine) {
+    get_k(ta, 0);
+    get_v(ta, 0);
+  }
+  uint32_t* marks = reinterpret_cast<uint32_t*>(lds + merge_floats<D>());
+  for (int x = t; x <= 4 * MT * D; x += 64 * NW) marks[x] = 0u;
+  __syncthreads();
   // queries: row 16 mt + n
   bf16x8 qf[MT][NS];
   int pos[MT];
@@ -313,197 +551,54 @@ __global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
     const int r = 16 * mt + n, qi = r / a.rep;
     const bool live = qi < nq;
     pos[mt] = live ? p0 + qi : -1;
-    const uint16_t* row = a.q + static_cast<int64_t>(u.s.first + q0 + (live ? qi : 0)) * a.ldq +
-                          (head * a.rep + (live ? r - qi * a.rep : 0)) * D;
+    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + q0 + (live ? qi : 0)) * a.ldq +
+                           (head * a.rep + (live ? r - qi * a.rep : 0)) * D;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
-      qf[mt][s] = as_frag(*reinterpret_cast<const uint4*>(row + (MX ? g * (D / 4) + 8 * s : 32 * s + 8 * g)));
+      qf[mt][s] = as_frag(*reinterpret_cast<const uint4*>(qrow + (MX ? g * (D / 4) + 8 * s : 32 * s + 8 * g)));
   }
-
-  f32x4 o[MT][NB];
-  float m[MT], l[MT];
+  Rows<D, MT> st;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -INFINITY;
-    l[mt] = 0.f;
+    st.m[mt] = -INFINITY;
+    st.l[mt] = 0.f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) o[mt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < NB; ++b) st.o[mt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  // The wave's tiles are it0 + w + NW i. Lane l holds the page of 16-key half l % 2 of tile i0 + l / 2 (32 tiles at once;
-  // 0 for pages that are none, whose keys `bad` then hides).
-  const int mine = it0 + w < it1 ? (it1 - it0 - w + NW - 1) / NW : 0;
-  int ids = 0;
-  uint64_t bad = 0;
-  auto fetch_ids = [&](int i0) {
-    const int it = it0 + w + NW * (i0 + (lane >> 1));
-    const int at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
-    int id = -1;
-    if (it < it1 && at < a.width) id = a.table[static_cast<int64_t>(u.b) * a.ld_table + at];
-    const bool out = id < 0 || id >= a.pg.n_pages;
-    ids = out ? 0 : id;
-    bad = __ballot(out);
-  };
-  const int mask = (1 << a.pg.shift) - 1;
-  KTile<D, MX> kt;
-  VTile<D, MX> vt;
-  auto get_k = [&](int i) {
-    const int it = it0 + w + NW * i;
-    const int id0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31)), id1 = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + 1);
-    const bool up = n >= 8;
-    load_k<D, MX>(kt, a.pg, up ? id1 : id0, head, (it * KT + (up ? 16 : 0)) & mask, n, g);
-  };
-  auto get_v = [&](int i) {
-    const int it = it0 + w + NW * i;
-    const int id0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31)), id1 = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + 1);
-    const bool up = g >= 2;
-    load_v<D, MX>(vt, a.pg, up ? id1 : id0, head, (it * KT + (up ? 16 : 0)) & mask, n, g);
-  };
-
-  for (int i = 0; i < mine; ++i) {
-    if ((i & 31) == 0) fetch_ids(i);
-    get_k(i);
-    get_v(i);
-    const int k0 = (it0 + w + NW * i) * KT;
-    const uint32_t bad2 = static_cast<uint32_t>(bad >> (2 * (i & 31))) & 3u;
-    // scores: lane (n, g) gets keys k0 + 8 g + 4 kb + j of query row 16 mt + n
-    float ks[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    if constexpr (MX) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
-          ks[kb][x] = __uint_as_float((((kb ? kt.sc[x].y : kt.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
+  // Whole tiles first, then the tiles that some row sees in part; from the first page that is none on all of them are taken
+  // as such. 4 bits: two tiles' registers in turn, each tile's loads in flight while the one before it computes. bf16, where
+  // a tile takes D / 2 registers: one, its keys reloaded behind the scores and its values behind the product. (The last load
+  // may repeat the last tile: no load of these loops is conditional.)
+  const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
+  int i = 0;
+  if constexpr (MX) {
+    for (; i + 1 < whole; i += 2) {
+      window(i + 1);
+      get_k(tb, i + 1);
+      get_v(tb, i + 1);
+      if (ta.bad | tb.bad) break;
+      tile_step<D, MX, MT, false>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
+      const int i2 = min(i + 2, mine - 1);
+      if (i2 > i + 1) window(i2);
+      get_k(ta, i2);
+      get_v(ta, i2);
+      tile_step<D, MX, MT, false>(tb, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
     }
-    f32x4 sc[MT][2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const bf16x8 kf = k_frag<D, MX>(kt, ks, kb, s);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[mt][s], sc[mt][kb], 0, 0, 0);
-      }
+  } else {
+    for (; i < whole; ++i) {
+      if (ta.bad) break;
+      const int i1 = min(i + 1, mine - 1);
+      if (i1 > i) window(i1);
+      tile_step<D, MX, MT, false>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [&] { get_k(ta, i1); },
+                                  [&] { get_v(ta, i1); });
     }
-    const bool edge = k0 + KT - 1 > p0 || bad2;              // some row does not see some key of the tile
-    const bool hidden = (bad2 >> (g >> 1)) & 1u;             // the lane's 8 keys lie on a page that is none
-    uint32_t pk[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if (edge) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
-      }
-      float tmax = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, sc[mt][kb][j]);
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-      if (__any(tmax > m[mt] + RESCALE_LOG2 / a.c)) {
-        const float top = fmaxf(m[mt], tmax);
-        const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[mt] - top) * a.c);
-        m[mt] = top;
-        l[mt] *= alpha;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float al = __shfl(alpha, 4 * g + j, 64);     // O's rows of a lane are 4 g + j
-#pragma unroll
-          for (int b = 0; b < NB; ++b) o[mt][b][j] *= al;
-        }
-      }
-      const float mc = m[mt] == -INFINITY ? 0.f : m[mt] * a.c;
-      float psum = 0.f;
-      float p[8];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[4 * kb + j] = __builtin_amdgcn_exp2f(fmaf(sc[mt][kb][j], a.c, -mc));
-          psum += p[4 * kb + j];
-        }
-      l[mt] += psum;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) pk[mt][j] = bf16_pair(p[2 * j], p[2 * j + 1]);
-    }
-    // O += P V
-    float vs[8];
-    if constexpr (MX) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) vs[e] = byte_scale(vt.sc, e);
-    }
-    bool apart = false;                                      // a value that some row must not meet is not finite
-    if (edge) {
-      const int last = hidden ? -1 : plast - k0 - 8 * g;     // of the lane's keys, the last that any row sees
-#pragma unroll
-      for (int j = 0; j < NB / 2; ++j) {
-        uint32_t p[8];
-        v_pairs<D, MX>(vt, vs, j, p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) apart |= e <= last && not_finite(p[e]);
-      }
-      apart = __any(apart);
-      if constexpr (!MX) {                                   // keys that no row sees may hold anything
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int j = 0; j < NB / 2; ++j) vt.x[e][j] = e <= last ? vt.x[e][j] : 0u;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vs[e] = e <= last ? vs[e] : 0.f;       // (2^-127: the codes' values stay finite, p is 0)
-      }
-    }
-    if (!apart) {
-#pragma unroll
-      for (int j = 0; j < NB / 2; ++j) {
-        uint32_t p[8];
-        v_pairs<D, MX>(vt, vs, j, p);
-        const bf16x8 f0 = as_frag(make_uint4(both_low(p[0], p[1]), both_low(p[2], p[3]), both_low(p[4], p[5]), both_low(p[6], p[7])));
-        const bf16x8 f1 = as_frag(make_uint4(both_high(p[0], p[1]), both_high(p[2], p[3]), both_high(p[4], p[5]), both_high(p[6], p[7])));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const bf16x8 pf = as_frag(make_uint4(pk[mt][0], pk[mt][1], pk[mt][2], pk[mt][3]));
-          o[mt][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, o[mt][2 * j], 0, 0, 0);
-          o[mt][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, o[mt][2 * j + 1], 0, 0, 0);
-        }
-      }
-    } else {
-      // 0 x infinity must not reach a row that does not see the key: query by query with the keys past it zeroed, each
-      // product kept for that query's rows only
-      for (int qi = 0; qi < nq; ++qi) {
-        const int last = hidden ? -1 : p0 + qi - k0 - 8 * g;
-        for (int j = 0; j < NB / 2; ++j) {
-#pragma unroll
-          for (int jj = 0; jj < NB / 2; ++jj) {              // (static register indexes)
-            if (jj != j) continue;
-            uint32_t p[8];
-            v_pairs<D, MX>(vt, vs, jj, p);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = e <= last ? p[e] : 0u;
-            const bf16x8 f0 = as_frag(make_uint4(both_low(p[0], p[1]), both_low(p[2], p[3]), both_low(p[4], p[5]), both_low(p[6], p[7])));
-            const bf16x8 f1 = as_frag(make_uint4(both_high(p[0], p[1]), both_high(p[2], p[3]), both_high(p[4], p[5]), both_high(p[6], p[7])));
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              const bf16x8 pf = as_frag(make_uint4(pk[mt][0], pk[mt][1], pk[mt][2], pk[mt][3]));
-              const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-              const f32x4 t0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, z, 0, 0, 0);
-              const f32x4 t1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, z, 0, 0, 0);
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                if ((16 * mt + 4 * g + x) / a.rep == qi) {
-                  o[mt][2 * jj][x] += t0[x];
-                  o[mt][2 * jj + 1][x] += t1[x];
-                }
-            }
-          }
-        }
-      }
+  }
+  for (; i < mine; ++i) {
+    tile_step<D, MX, MT, true>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
+    if (i + 1 < mine) {
+      window(i + 1);
+      get_k(ta, i + 1);
+      get_v(ta, i + 1);
     }
   }
 
@@ -513,11 +608,11 @@ __global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     if (mt) __syncthreads();
-    float ls = l[mt];
+    float ls = st.l[mt];
     ls += __shfl_xor(ls, 16, 64);
     ls += __shfl_xor(ls, 32, 64);
     if (g == 0) {
-      ml[w * 16 + n] = m[mt] == -INFINITY ? m[mt] : m[mt] * a.c;           // base 2
+      ml[w * 16 + n] = st.m[mt] == -INFINITY ? st.m[mt] : st.m[mt] * a.c;  // base 2
       ml[(NW + w) * 16 + n] = ls;
     }
 #pragma unroll
@@ -525,98 +620,113 @@ __global__ __launch_bounds__(64 * NW) void k_paged_few(PagedArgs a) {
 #pragma unroll
       for (int b = 0; b < NB; b += 4)
         *reinterpret_cast<float4*>(lds + (w * 16 + 4 * g + j) * (D + 4) + n * NB + b) =
-            make_float4(o[mt][b][j], o[mt][b + 1][j], o[mt][b + 2][j], o[mt][b + 3][j]);
+            make_float4(st.o[mt][b][j], st.o[mt][b + 1][j], st.o[mt][b + 2][j], st.o[mt][b + 3][j]);
     __syncthreads();
-    const int row = t >> 4, d0 = (t & 15) * NB;
+    const int rw = t >> 4, d0 = (t & 15) * NB;
     float top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < NW; ++x) top = fmaxf(top, ml[x * 16 + row]);
+    for (int x = 0; x < NW; ++x) top = fmaxf(top, ml[x * 16 + rw]);
     float sum = 0.f, acc[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = 0.f;
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
-      const float mx = ml[x * 16 + row];
+      const float mx = ml[x * 16 + rw];
       const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
-      sum += ml[(NW + x) * 16 + row] * f;
+      sum += ml[(NW + x) * 16 + rw] * f;
 #pragma unroll
       for (int b = 0; b < NB; b += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(lds + (x * 16 + row) * (D + 4) + d0 + b);
-        if (f != 0.f) {                                      // (a wave without keys of this row holds zeros or nothing)
-          acc[b] += v.x * f;
-          acc[b + 1] += v.y * f;
-          acc[b + 2] += v.z * f;
-          acc[b + 3] += v.w * f;
-        }
+        const float4 v = *reinterpret_cast<const float4*>(lds + (x * 16 + rw) * (D + 4) + d0 + b);
+        acc[b] += v.x * f;
+        acc[b + 1] += v.y * f;
+        acc[b + 2] += v.z * f;
+        acc[b + 3] += v.w * f;
       }
     }
-    const int r = 16 * mt + row, qi = r / a.rep;
-    if (qi >= nq) continue;
-    if (u.ns > 1) {
-      float* p = a.part + part * (16 * MT * (D + 2));
+    const int r = 16 * mt + rw, qi = r / a.rep;
+    if (marks[4 * MT * D]) {
 #pragma unroll
-      for (int b = 0; b < NB; b += 4)
-        *reinterpret_cast<float4*>(p + r * D + d0 + b) = make_float4(acc[b], acc[b + 1], acc[b + 2], acc[b + 3]);
-      if ((t & 15) == 0) {
-        p[16 * MT * D + r] = top;
-        p[16 * MT * (D + 1) + r] = sum;
-      }
-      continue;
+      for (int b = 0; b < NB; ++b) acc[b] += marked((marks[(r * D + d0 + b) / 4] >> (8 * (b & 3))) & 255u);
     }
-    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;          // no key: zeros (a NaN stays one)
-    uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
-#pragma unroll
-    for (int b = 0; b < NB; b += 4)
-      *reinterpret_cast<uint2*>(dst + b) =
-          make_uint2(bf16_pair(acc[b] * inv, acc[b + 1] * inv), bf16_pair(acc[b + 2] * inv, acc[b + 3] * inv));
+    if (qi < nq) finish_row<D, NB>(a, u, part, 16 * MT, r, head, q0, d0, acc, top, sum);
   }
 }
 
-// Merges the splits of one row block and head in split order: a thread takes D / 16 columns of one row.
-template <int D, int MT>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
-  constexpr int NB = D / 16;
-  const int t = threadIdx.x, head = blockIdx.x % a.hkv;
+// Merges the splits of a row block and head in split order: of 16 / G rows and 64 columns a block, G groups of 16 lanes a row
+// take every G-th split (4 columns a lane, four splits' loads in flight), then the groups' sums are added in order. G is
+// large where few rows have many splits.
+template <int D, int G>
+__global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int rpb) {
+  __shared__ float4 ls[256];
+  __shared__ float lm[16], ll[16];
+  const int t = threadIdx.x, head = blockIdx.x % a.hkv, ln = t & 15, grp = (t >> 4) % G, rr = (t >> 4) / G;
   const Unit u = find_unit(a, blockIdx.x / a.hkv, true);
   // (partials past the last unit: only with a cu that does not rise, whose units the launch does not hold)
   if (u.b < 0 || u.ns == 1 || u.part + static_cast<int64_t>(u.ns - 1) * u.nrb >= a.units) return;
   const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0);
-  const int d0 = (t & 15) * NB, r = blockIdx.y * 16 + (t >> 4), qi = r / a.rep;
-  if (qi >= nq) return;
-  const float* p0 = a.part + (u.part * a.hkv + head) * (16 * MT * (D + 2));
-  const int64_t step = static_cast<int64_t>(u.nrb) * a.hkv * (16 * MT * (D + 2));
+  const int r = blockIdx.y * (16 / G) + rr, qi = r / a.rep, d0 = blockIdx.z * 64 + 4 * ln;
+  const int last_row = min(nq * a.rep, rpb) - 1, rc = min(r, last_row);
+  if (static_cast<int>(blockIdx.y) * (16 / G) > last_row) return;
+  const float* p0 = a.part + (u.part * a.hkv + head) * (static_cast<int64_t>(rpb) * (D + 2));
+  const int64_t step = static_cast<int64_t>(u.nrb) * a.hkv * (static_cast<int64_t>(rpb) * (D + 2));
+  const float* ms = p0 + static_cast<int64_t>(rpb) * D + rc;
+  // the row's maximum: each lane of the row's groups takes splits
   float top = -INFINITY;
-  for (int s = 0; s < u.ns; ++s) top = fmaxf(top, p0[s * step + 16 * MT * D + r]);
-  float sum = 0.f, acc[NB];
+  for (int s = grp * 16 + ln; s < u.ns; s += 16 * G) top = fmaxf(top, ms[s * step]);
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = 0.f;
-  for (int s = 0; s < u.ns; ++s) {
-    const float* p = p0 + s * step;
-    const float ms = p[16 * MT * D + r];
-    if (ms == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ms - top);
-    sum += p[16 * MT * (D + 1) + r] * f;
+  for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (ln == 0) lm[t >> 4] = top;
+  __syncthreads();
 #pragma unroll
-    for (int b = 0; b < NB; b += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + r * D + d0 + b);
-      acc[b] += v.x * f;
-      acc[b + 1] += v.y * f;
-      acc[b + 2] += v.z * f;
-      acc[b + 3] += v.w * f;
+  for (int x = 0; x < G; ++x) top = fmaxf(top, lm[rr * G + x]);
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = grp; s0 < u.ns; s0 += 4 * G) {
+    float4 v[4];
+    float m4[4], l4[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int64_t s = min(s0 + x * G, u.ns - 1);
+      m4[x] = ms[s * step];
+      l4[x] = ms[s * step + rpb];
+      v[x] = *reinterpret_cast<const float4*>(p0 + s * step + static_cast<int64_t>(rc) * D + d0);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = s0 + x * G >= u.ns || m4[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m4[x] - top);
+      if (f == 0.f) continue;
+      sum += l4[x] * f;
+      acc.x += v[x].x * f;
+      acc.y += v[x].y * f;
+      acc.z += v[x].z * f;
+      acc.w += v[x].w * f;
     }
   }
-  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+  ls[t] = acc;
+  if (ln == 0) ll[t >> 4] = sum;
+  __syncthreads();
+  if (grp || r > last_row) return;
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int b = 0; b < NB; b += 4)
-    *reinterpret_cast<uint2*>(dst + b) =
-        make_uint2(bf16_pair(acc[b] * inv, acc[b + 1] * inv), bf16_pair(acc[b + 2] * inv, acc[b + 3] * inv));
+  for (int x = 0; x < G; ++x) {
+    const float4 v = ls[(rr * G + x) * 16 + ln];
+    sum += ll[rr * G + x];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  }
+  const float inv = inverse_sum(sum);
+  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
 }
 
-// 16-row blocks a wave takes: as few as hold a sequence's rows.
-int row_tiles(int rep, int64_t max_rows) {
+// 16-row blocks a wave takes: as few as hold a sequence's rows (their state and queries live in registers: up to 4, 3 at
+// head_dim 256).
+int row_tiles(int rep, int d, int64_t max_rows) {
   const int64_t rows = std::min<int64_t>(max_rows, 64) * rep;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return static_cast<int>(std::min<int64_t>(d == 256 && rep <= 48 ? 3 : 4, (rows + 15) / 16));
 }
 
 struct Plan {
@@ -630,7 +740,7 @@ struct Plan {
 Plan plan_of(int64_t T, int hq, int hkv, int d, int n_seq, int64_t max_rows, int64_t max_keys) {
   Plan p{};
   const int rep = hq / hkv;
-  p.mt = row_tiles(rep, max_rows);
+  p.mt = row_tiles(rep, d, max_rows);
   p.qb = 16 * p.mt / rep;
   p.blocks = std::min<int64_t>(T, T / p.qb + n_seq);
   p.target = max_keys > 16 * NW * KT ? 1024 : 0;
@@ -691,7 +801,7 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.qb,
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
                     scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace), p.target, p.units};
-  const dim3 grid(static_cast<unsigned>(p.units * hkv)), grid2(static_cast<unsigned>(p.blocks * hkv), p.mt);
+  const dim3 grid(static_cast<unsigned>(p.units * hkv)), grid2(static_cast<unsigned>(p.blocks * hkv), 16 * p.mt, d / 64);
   const bool mx = pages->kind == RF_PAGES_MX4;
 #define RF_FEW(D, MT)                                                                                    \
   do {                                                                                                   \
@@ -699,13 +809,14 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
     else hipLaunchKernelGGL((k_paged_few<D, false, MT>), grid, dim3(64 * NW), 0, stream, a);             \
     if (p.target) {                                                                                      \
       if (int rc = check_launch(fn)) return rc;                                                          \
-      hipLaunchKernelGGL((k_paged_merge<D, MT>), grid2, dim3(256), 0, stream, a);                        \
+      hipLaunchKernelGGL((k_paged_merge<D, 16>), grid2, dim3(256), 0, stream, a, 16 * MT);               \
     }                                                                                                    \
   } while (0)
 #define RF_FEW_D(D)                    \
   do {                                 \
     if (p.mt == 1) RF_FEW(D, 1);       \
     else if (p.mt == 2) RF_FEW(D, 2);  \
+    else if (p.mt == 3) RF_FEW(D, 3);  \
     else RF_FEW(D, 4);                 \
   } while (0)
   if (d == 64) RF_FEW_D(64);
