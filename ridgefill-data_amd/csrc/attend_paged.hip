@@ -83,7 +83,7 @@ __device__ __forceinline__ int wave_sum_below(int v, int lane, int& total) {    
     const int u = __shfl_up(s, o, 64);
     if (lane >= o) s += u;
   }
-  total = __shfl(s, 63, 64);
+  total = __builtin_amdgcn_readlane(s, 63);
   return s - v;
 }
 
@@ -106,7 +106,8 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool rows_only) {
       for (int o = 32; o >= 1; o >>= 1) w += __shfl_xor(w, o, 64);
       work += w;
     }
-    W = max(2 * NW, static_cast<int>(ceilf(work * static_cast<float>(a.hkv) / static_cast<float>(a.target))));
+    W = __builtin_amdgcn_readfirstlane(
+        max(2 * NW, static_cast<int>(ceilf(work * static_cast<float>(a.hkv) / static_cast<float>(a.target)))));
   }
   Unit u;
   u.b = -1;
@@ -125,17 +126,18 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool rows_only) {
     const int ppre = rows_only ? wave_sum_below(nrb * ns, lane, ptotal) : pre;
     if (!rows_only) ptotal = total;
     if (want < before + total) {
+      // (scalar from here on: what follows from a unit is uniform over its block)
       const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
-      const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      const int at = want - before - __shfl(pre, l, 64);
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+      const int at = want - before - __builtin_amdgcn_readlane(pre, l);
       u.b = b0 + l;
-      u.nrb = __shfl(nrb, l, 64);
-      u.ns = __shfl(ns, l, 64);
-      u.s = Seq{__shfl(s.rows, l, 64), __shfl(s.keys, l, 64), __shfl(s.first, l, 64)};
-      u.rb = at % u.nrb;
+      u.nrb = __builtin_amdgcn_readlane(nrb, l);
+      u.ns = __builtin_amdgcn_readlane(ns, l);
+      u.s = Seq{__builtin_amdgcn_readlane(s.rows, l), __builtin_amdgcn_readlane(s.keys, l), __builtin_amdgcn_readlane(s.first, l)};
       u.sp = at / u.nrb;
+      u.rb = at - u.sp * u.nrb;
       u.W = W;
-      u.part = parts + __shfl(ppre, l, 64) + u.rb;
+      u.part = parts + __builtin_amdgcn_readlane(ppre, l) + u.rb;
       return u;
     }
     before += total;
@@ -363,129 +365,143 @@ __device__ __forceinline__ float marked(uint32_t m) {
   return (m & 4u) || (m & 3u) == 3u ? NAN : (m & 1u) ? INFINITY : (m & 2u) ? -INFINITY : 0.f;
 }
 
-// One tile: scores, softmax, O += P V. next_k / next_v load the following tile's registers where this one's are done with.
-// EDGE: some row does not see some key of it. Keys are hidden from rows by their scores (-infinity); of V, what no row sees
-// and what is not finite enters the product as zero, and the latter leaves its marks in the rows that see it.
-template <int D, bool MX, int MT, bool EDGE, class NK, class NV>
-__device__ __forceinline__ void tile_step(Tile<D, MX>& tl, const bf16x8 (&qf)[MT][D / 32], const int (&pos)[MT],
-                                          Rows<D, MT>& st, float c, int p0, int plast, int rep, int lane, uint32_t* marks,
-                                          NK&& next_k, NV&& next_v) {
-  constexpr int NS = D / 32, NB = D / 16;
-  const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
-  const uint32_t bad = tl.bad;
+// S^T of a tile: sc[mt][kb][j] = the raw score of key 8 g + 4 kb + j for query row 16 mt + n.
+template <int D, bool MX, int MT>
+__device__ __forceinline__ void scores(const KTile<D, MX>& kt, const bf16x8 (&qf)[MT][D / 32], f32x4 (&sc)[MT][2], int n) {
+  constexpr int NS = D / 32;
   float ks[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
   if constexpr (MX) {
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
-        ks[kb][x] = __uint_as_float((((kb ? tl.k.sc[x].y : tl.k.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
+        ks[kb][x] = __uint_as_float((((kb ? kt.sc[x].y : kt.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
   }
-  f32x4 sc[MT][2];
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const bf16x8 kf = k_frag<D, MX>(tl.k, ks, kb, s);
+      const bf16x8 kf = k_frag<D, MX>(kt, ks, kb, s);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[mt][s], sc[mt][kb], 0, 0, 0);
     }
   }
-  next_k();
-  const bool hidden = EDGE && ((bad >> (g >> 1)) & 1u);      // the lane's 8 keys lie on a page that is none
-  bf16x8 pf[MT];
+}
+
+__device__ __forceinline__ float lane_max(const f32x4 (&s)[2]) {
+  return fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+}
+
+// Raise row block mt's reference maxima to what its rows' four lanes have seen (tmax), and rescale their sums and O.
+template <int D, int MT>
+__device__ __forceinline__ void raise(Rows<D, MT>& st, int mt, float tmax, float c, int g) {
+  tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+  tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+  const float top = fmaxf(st.m[mt], tmax);
+  const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[mt] - top) * c);
+  st.m[mt] = top;
+  st.l[mt] *= alpha;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    if constexpr (EDGE) {
+  for (int j = 0; j < 4; ++j) {
+    const float al = __shfl(alpha, 4 * g + j, 64);           // O's rows of a lane are 4 g + j
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
-    }
-    float tmax = -INFINITY;                                  // of the lane's keys; the row's only where the maximum rises
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, sc[mt][kb][j]);
-    if (__any(tmax > st.m[mt] + RESCALE_LOG2 / c)) {
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-      const float top = fmaxf(st.m[mt], tmax);
-      const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[mt] - top) * c);
-      st.m[mt] = top;
-      st.l[mt] *= alpha;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float al = __shfl(alpha, 4 * g + j, 64);       // O's rows of a lane are 4 g + j
-#pragma unroll
-        for (int b = 0; b < NB; ++b) st.o[mt][b][j] *= al;
-      }
-    }
-    const float mc = st.m[mt] == -INFINITY ? 0.f : st.m[mt] * c;
-    float p[8];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[4 * kb + j] = __builtin_amdgcn_exp2f(fmaf(sc[mt][kb][j], c, -mc));
-    st.l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    pf[mt] = as_frag(make_uint4(bf16_pair(p[0], p[1]), bf16_pair(p[2], p[3]), bf16_pair(p[4], p[5]), bf16_pair(p[6], p[7])));
+    for (int b = 0; b < D / 16; ++b) st.o[mt][b][j] *= al;
   }
+}
+
+// The probabilities of a tile as the product's operand; their sum goes to l.
+__device__ __forceinline__ bf16x8 probabilities(const f32x4 (&s)[2], float m, float c, float& l) {
+  const float mc = m == -INFINITY ? 0.f : m * c;             // (no key seen yet)
+  float p[8];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[4 * kb + j] = __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -mc));
+  l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+  return as_frag(make_uint4(bf16_pair(p[0], p[1]), bf16_pair(p[2], p[3]), bf16_pair(p[4], p[5]), bf16_pair(p[6], p[7])));
+}
+
+// O += P V. CUT: as v_frags.
+template <int D, bool MX, int MT, bool CUT>
+__device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 (&pf)[MT], int last, Rows<D, MT>& st) {
   float vs[8];
   if constexpr (MX) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vs[e] = byte_scale(tl.v.sc, e);
-  }
-  const int last = !EDGE ? 8 : hidden ? -1 : plast - k0 - 8 * g;        // of the lane's keys, the last that any row sees
-  if constexpr (EDGE) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-#pragma unroll
-      for (int j = 0; j < NB / 2; ++j) {
-        uint32_t two;
-        if constexpr (MX) {                                  // 4 bits: only a scale can make values NaN
-          if (j) continue;
-          two = (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
-        } else {
-          two = tl.v.x[e][j];
-        }
-        if (e <= last && not_finite(two)) {
-          const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 8;
-          const int first = max(0, k0 + 8 * g + e - p0) * rep;          // rows from the key's own query on
-          for (int r = first; r < min(16 * MT, (plast - p0 + 1) * rep); ++r) {
-            if constexpr (MX) {
-#pragma unroll
-              for (int x = 0; x < NB / 4; ++x) atomicOr(marks + (r * D + n * NB) / 4 + x, 0x04040404u);
-            } else {
-              atomicOr(marks + (r * D + n * NB + 2 * j) / 4, m2 << (j & 1 ? 16 : 0));
-            }
-          }
-          marks[16 * MT * D / 4] = 1u;
-        }
-      }
-    }
+    for (int e = 0; e < 8; ++e) vs[e] = byte_scale(vt.sc, e);
   }
 #pragma unroll
-  for (int j = 0; j < NB / 2; ++j) {
+  for (int j = 0; j < D / 32; ++j) {
     bf16x8 f0, f1;
-    v_frags<D, MX, EDGE>(tl.v, vs, j, last, f0, f1);
+    v_frags<D, MX, CUT>(vt, vs, j, last, f0, f1);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       st.o[mt][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f0, st.o[mt][2 * j], 0, 0, 0);
       st.o[mt][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f1, st.o[mt][2 * j + 1], 0, 0, 0);
     }
   }
-  next_v();
 }
 
-// The row r of a row block is query r / rep, query head r % rep of the K / V head.
-template <int D, int MT>
-constexpr int few_waves() { return D == 64 ? (MT <= 3 ? 2 : 1) : D == 128 && MT <= 2 ? 2 : 1; }
+// A tile of which some row does not see some key. Keys are hidden from rows by their scores (-infinity); of V, what no row
+// sees and what is not finite enters the product as zero, and the latter leaves its marks in the rows that see it.
+template <int D, bool MX, int MT>
+__device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const bf16x8 (&qf)[MT][D / 32], const int (&pos)[MT],
+                                          Rows<D, MT>& st, float c, int p0, int plast, int rep, int lane, uint32_t* marks) {
+  constexpr int NB = D / 16;
+  const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
+  f32x4 sc[MT][2];
+  scores<D, MX, MT>(tl.k, qf, sc, n);
+  const bool hidden = (tl.bad >> (g >> 1)) & 1u;             // the lane's 8 keys lie on a page that is none
+  bf16x8 pf[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
+    const float tmax = lane_max(sc[mt]);
+    if (__any(tmax > st.m[mt] + RESCALE_LOG2 / c)) raise<D, MT>(st, mt, tmax, c, g);
+    pf[mt] = probabilities(sc[mt], st.m[mt], c, st.l[mt]);
+  }
+  const int last = hidden ? -1 : plast - k0 - 8 * g;         // of the lane's keys, the last that any row sees
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int j = 0; j < NB / 2; ++j) {
+      uint32_t two;
+      if constexpr (MX) {                                    // 4 bits: only a scale can make values NaN
+        if (j) continue;
+        two = (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
+      } else {
+        two = tl.v.x[e][j];
+      }
+      if (e <= last && not_finite(two)) {
+        const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 8;
+        const int first = max(0, k0 + 8 * g + e - p0) * rep;            // rows from the key's own query on
+        for (int r = first; r < min(16 * MT, (plast - p0 + 1) * rep); ++r) {
+          if constexpr (MX) {
+#pragma unroll
+            for (int x = 0; x < NB / 4; ++x) atomicOr(marks + (r * D + n * NB) / 4 + x, 0x04040404u);
+          } else {
+            atomicOr(marks + (r * D + n * NB + 2 * j) / 4, m2 << (j & 1 ? 16 : 0));
+          }
+        }
+        marks[4 * MT * D] = 1u;
+      }
+    }
+  }
+  product<D, MX, MT, true>(tl.v, pf, last, st);
+}
+
+// Blocks a CU that the registers of a kernel hold.
+constexpr int few_blocks(int d, bool mx, int mt) {
+  return d == 64 ? (mt <= 2 ? 3 : mt == 3 ? 2 : 1) : d == 128 ? (mt == 1 && mx ? 3 : mt <= 2 ? 2 : 1) : 1;
+}
 
 template <int D, bool MX, int MT>
-__global__ __launch_bounds__(64 * NW, (few_waves<D, MT>())) void k_paged_few(PagedArgs a) {
+__global__ __launch_bounds__(64 * NW, (few_blocks(D, MX, MT))) void k_paged_few(PagedArgs a) {
   constexpr int NS = D / 32, NB = D / 16;
   __shared__ float lds[merge_floats<D>() + 4 * MT * D + 1];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 15, g = lane >> 4;
@@ -535,10 +551,14 @@ __global__ __launch_bounds__(64 * NW, (few_waves<D, MT>())) void k_paged_few(Pag
     load_v<D, MX>(tl.v, a.pg, g >= 2 ? id1 : id0, head, (tl.k0 + (g >= 2 ? 16 : 0)) & mask, n, g);
   };
 
-  Tile<D, MX> ta, tb;
+  constexpr int NT = MX || D == 64 ? 2 : 1;                  // tiles at once
+  Tile<D, MX> tl[NT];
   if (mine) {
-    get_k(ta, 0);
-    get_v(ta, 0);
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      get_k(tl[x], min(x, mine - 1));
+      get_v(tl[x], min(x, mine - 1));
+    }
   }
   uint32_t* marks = reinterpret_cast<uint32_t*>(lds + merge_floats<D>());
   for (int x = t; x <= 4 * MT * D; x += 64 * NW) marks[x] = 0u;
@@ -565,40 +585,58 @@ __global__ __launch_bounds__(64 * NW, (few_waves<D, MT>())) void k_paged_few(Pag
 #pragma unroll
     for (int b = 0; b < NB; ++b) st.o[mt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // Whole tiles first, then the tiles that some row sees in part; from the first page that is none on all of them are taken
-  // as such. 4 bits: two tiles' registers in turn, each tile's loads in flight while the one before it computes. bf16, where
-  // a tile takes D / 2 registers: one, its keys reloaded behind the scores and its values behind the product. (The last load
-  // may repeat the last tile: no load of these loops is conditional.)
+  // Whole tiles first (NT at once; the keys' registers are reloaded behind the scores, the values' behind the product, so
+  // that loads are always in flight), then the tiles that some row sees in part; from the first page that is none on all of
+  // them are taken as such. A maximum that has to rise leaves the inner loop: with the rescale inside it the compiler moves
+  // all of O at every tile (16 to 48 rows of head_dim 256 in 4 bits). Tiles past the last are loaded as the last one again:
+  // no load of the loop is conditional.
   const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
   int i = 0;
-  if constexpr (MX) {
-    for (; i + 1 < whole; i += 2) {
-      window(i + 1);
-      get_k(tb, i + 1);
-      get_v(tb, i + 1);
-      if (ta.bad | tb.bad) break;
-      tile_step<D, MX, MT, false>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
-      const int i2 = min(i + 2, mine - 1);
-      if (i2 > i + 1) window(i2);
-      get_k(ta, i2);
-      get_v(ta, i2);
-      tile_step<D, MX, MT, false>(tb, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
+  bool none = false;
+  while (!none && i + NT <= whole) {
+    f32x4 sc[NT][MT][2];
+    float tmax[MT];
+    for (; i + NT <= whole; i += NT) {
+      uint32_t bads = 0;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) bads |= tl[x].bad;
+      none = bads != 0;
+      if (none) break;
+      bool up = false;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) scores<D, MX, MT>(tl[x].k, qf, sc[x], n);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        tmax[mt] = lane_max(sc[0][mt]);
+        if constexpr (NT > 1) tmax[mt] = fmaxf(tmax[mt], lane_max(sc[NT - 1][mt]));
+        up |= tmax[mt] > st.m[mt] + RESCALE_LOG2 / a.c;
+      }
+      if (__any(up)) break;
+      const int i1 = min(i + NT, mine - 1);
+      if (i1 == i + NT) window(i1);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) get_k(tl[x], min(i1 + x, mine - 1));
+      bf16x8 pf[NT][MT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) pf[x][mt] = probabilities(sc[x][mt], st.m[mt], a.c, st.l[mt]);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) product<D, MX, MT, false>(tl[x].v, pf[x], 8, st);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) get_v(tl[x], min(i1 + x, mine - 1));
     }
-  } else {
-    for (; i < whole; ++i) {
-      if (ta.bad) break;
-      const int i1 = min(i + 1, mine - 1);
-      if (i1 > i) window(i1);
-      tile_step<D, MX, MT, false>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [&] { get_k(ta, i1); },
-                                  [&] { get_v(ta, i1); });
+    if (!none && i + NT <= whole) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) raise<D, MT>(st, mt, tmax[mt], a.c, g);
     }
   }
   for (; i < mine; ++i) {
-    tile_step<D, MX, MT, true>(ta, qf, pos, st, a.c, p0, plast, a.rep, lane, marks, [] {}, [] {});
+    edge_step<D, MX, MT>(tl[0], qf, pos, st, a.c, p0, plast, a.rep, lane, marks);
     if (i + 1 < mine) {
       window(i + 1);
-      get_k(ta, i + 1);
-      get_v(ta, i + 1);
+      get_k(tl[0], i + 1);
+      get_v(tl[0], i + 1);
     }
   }
 
@@ -652,74 +690,93 @@ __global__ __launch_bounds__(64 * NW, (few_waves<D, MT>())) void k_paged_few(Pag
   }
 }
 
-// Merges the splits of a row block and head in split order: of 16 / G rows and 64 columns a block, G groups of 16 lanes a row
-// take every G-th split (4 columns a lane, four splits' loads in flight), then the groups' sums are added in order. G is
-// large where few rows have many splits.
-template <int D, int G>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int rpb) {
-  __shared__ float4 ls[256];
-  __shared__ float lm[16], ll[16];
-  const int t = threadIdx.x, head = blockIdx.x % a.hkv, ln = t & 15, grp = (t >> 4) % G, rr = (t >> 4) / G;
+// Merges the splits of a row block and head: D / 4 lanes a row (4 columns each); the block's lanes beyond its rows make G
+// groups a row, group i takes splits i, i + G, .. (eight in flight) with a running maximum, and the groups are joined in
+// order through LDS. The order depends on the sizes alone. blockIdx.y takes a share of the rows where few row blocks leave
+// CUs idle.
+constexpr int MERGE_THREADS = 1024;
+template <int D>
+__global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a, int rpb) {
+  constexpr int LPR = D / 4, U = 8;
+  __shared__ float4 ls[MERGE_THREADS];
+  __shared__ float lm[MERGE_THREADS / LPR], ll[MERGE_THREADS / LPR];
+  const int t = threadIdx.x, head = blockIdx.x % a.hkv, slots = blockDim.x / LPR, slot = t / LPR, col = 4 * (t % LPR);
   const Unit u = find_unit(a, blockIdx.x / a.hkv, true);
   // (partials past the last unit: only with a cu that does not rise, whose units the launch does not hold)
   if (u.b < 0 || u.ns == 1 || u.part + static_cast<int64_t>(u.ns - 1) * u.nrb >= a.units) return;
-  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0);
-  const int r = blockIdx.y * (16 / G) + rr, qi = r / a.rep, d0 = blockIdx.z * 64 + 4 * ln;
-  const int last_row = min(nq * a.rep, rpb) - 1, rc = min(r, last_row);
-  if (static_cast<int>(blockIdx.y) * (16 / G) > last_row) return;
+  const int q0 = u.rb * a.qb, rows = min(a.qb, u.s.rows - q0) * a.rep;
+  const int per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
+  if (r0 >= r1) return;
+  int G = 1;
+  while (2 * G * (r1 - r0) <= slots && 2 * G <= u.ns) G *= 2;
+  const int grp = slot % G;
   const float* p0 = a.part + (u.part * a.hkv + head) * (static_cast<int64_t>(rpb) * (D + 2));
   const int64_t step = static_cast<int64_t>(u.nrb) * a.hkv * (static_cast<int64_t>(rpb) * (D + 2));
-  const float* ms = p0 + static_cast<int64_t>(rpb) * D + rc;
-  // the row's maximum: each lane of the row's groups takes splits
-  float top = -INFINITY;
-  for (int s = grp * 16 + ln; s < u.ns; s += 16 * G) top = fmaxf(top, ms[s * step]);
+  for (int rb = r0; rb < r1; rb += slots / G) {              // (uniform)
+    const int r = rb + slot / G, rc = min(r, r1 - 1);
+    const float* pv = p0 + static_cast<int64_t>(rc) * D + col;
+    const float* ms = p0 + static_cast<int64_t>(rpb) * D + rc;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = grp; s0 < u.ns; s0 += U * G) {
+      float4 v[U];
+      float m[U], l[U];
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  if (ln == 0) lm[t >> 4] = top;
-  __syncthreads();
+      for (int x = 0; x < U; ++x) {
+        const int64_t s = min(s0 + x * G, u.ns - 1);
+        m[x] = ms[s * step];
+        l[x] = ms[s * step + rpb];
+        v[x] = *reinterpret_cast<const float4*>(pv + s * step);
+      }
+      float now = top;
 #pragma unroll
-  for (int x = 0; x < G; ++x) top = fmaxf(top, lm[rr * G + x]);
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = grp; s0 < u.ns; s0 += 4 * G) {
-    float4 v[4];
-    float m4[4], l4[4];
+      for (int x = 0; x < U; ++x) now = fmaxf(now, s0 + x * G < u.ns ? m[x] : -INFINITY);
+      const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= f0;
+      acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int64_t s = min(s0 + x * G, u.ns - 1);
-      m4[x] = ms[s * step];
-      l4[x] = ms[s * step + rpb];
-      v[x] = *reinterpret_cast<const float4*>(p0 + s * step + static_cast<int64_t>(rc) * D + d0);
+      for (int x = 0; x < U; ++x) {
+        if (s0 + x * G >= u.ns) break;                       // (uniform over a group)
+        const float f = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - top);
+        sum += l[x] * f;
+        acc.x += v[x].x * f;
+        acc.y += v[x].y * f;
+        acc.z += v[x].z * f;
+        acc.w += v[x].w * f;
+      }
     }
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float f = s0 + x * G >= u.ns || m4[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m4[x] - top);
-      if (f == 0.f) continue;
-      sum += l4[x] * f;
-      acc.x += v[x].x * f;
-      acc.y += v[x].y * f;
-      acc.z += v[x].z * f;
-      acc.w += v[x].w * f;
+    if (G > 1) {
+      __syncthreads();                                       // the last rows' groups were read
+      ls[t] = acc;
+      if (col == 0) {
+        lm[slot] = top;
+        ll[slot] = sum;
+      }
+      __syncthreads();
+      if (grp == 0) {
+        const int first = slot;
+        for (int x = 0; x < G; ++x) top = fmaxf(top, lm[first + x]);
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = 0; x < G; ++x) {
+          const float m = lm[first + x], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          const float4 v = ls[t + x * LPR];
+          sum += ll[first + x] * f;
+          acc.x += v.x * f;
+          acc.y += v.y * f;
+          acc.z += v.z * f;
+          acc.w += v.w * f;
+        }
+      }
+    }
+    if (grp == 0 && r < r1) {
+      const float inv = inverse_sum(sum);
+      const int qi = r / a.rep;
+      uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + col;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
     }
   }
-  ls[t] = acc;
-  if (ln == 0) ll[t >> 4] = sum;
-  __syncthreads();
-  if (grp || r > last_row) return;
-  sum = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int x = 0; x < G; ++x) {
-    const float4 v = ls[(rr * G + x) * 16 + ln];
-    sum += ll[rr * G + x];
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
-  }
-  const float inv = inverse_sum(sum);
-  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
 }
 
 // 16-row blocks a wave takes: as few as hold a sequence's rows (their state and queries live in registers: up to 4, 3 at
@@ -737,13 +794,13 @@ struct Plan {
 
 // The launch for these sizes. Row blocks: sum of ceil(rows / qb) <= T / qb + n_seq. Splits: sum of nrb ceil(tiles / W) <=
 // sum of nrb tiles / W + row blocks, and W >= work hkv / target, so they are at most target / hkv + row blocks.
-Plan plan_of(int64_t T, int hq, int hkv, int d, int n_seq, int64_t max_rows, int64_t max_keys) {
+Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys) {
   Plan p{};
   const int rep = hq / hkv;
   p.mt = row_tiles(rep, d, max_rows);
   p.qb = 16 * p.mt / rep;
   p.blocks = std::min<int64_t>(T, T / p.qb + n_seq);
-  p.target = max_keys > 16 * NW * KT ? 1024 : 0;
+  p.target = max_keys > 16 * NW * KT ? 256 * few_blocks(d, mx, p.mt) : 0;
   p.units = p.target ? p.target / hkv + 1 + p.blocks : p.blocks;
   p.bytes = p.target ? static_cast<size_t>(p.units) * hkv * (16 * p.mt * (d + 2)) * 4 : 0;
   return p;
@@ -770,7 +827,7 @@ extern "C" int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d
   const char* fn = "rf_attend_paged_workspace_bytes";
   if (!bytes) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
   if (int rc = attend_sizes(fn, T, hq, hkv, d, kind, n_seq, max_rows, max_keys)) return rc;
-  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, n_seq, max_rows, max_keys).bytes : 0;
+  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, kind == RF_PAGES_MX4, n_seq, max_rows, max_keys).bytes : 0;
   return RF_OK;
 }
 
@@ -793,7 +850,7 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   if (!(scale > 0.f) || !(scale < 1e30f))
     return fail(RF_EINVAL_ARG, "%s: scale %g (must be positive)", fn, static_cast<double>(scale));
   if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
-  Plan p = plan_of(T, hq, hkv, d, n_seq, max_rows, max_keys);
+  Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys);
   if (p.target && (!workspace || ws_bytes < p.bytes)) {
     p.target = 0;
     p.units = p.blocks;
@@ -801,7 +858,11 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.qb,
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
                     scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace), p.target, p.units};
-  const dim3 grid(static_cast<unsigned>(p.units * hkv)), grid2(static_cast<unsigned>(p.blocks * hkv), 16 * p.mt, d / 64);
+  const dim3 grid(static_cast<unsigned>(p.units * hkv));
+  // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
+  const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, 16 * p.mt);
+  const dim3 grid2(static_cast<unsigned>(pairs), static_cast<unsigned>(std::min<int64_t>(rows, (511 + pairs) / pairs)));
+  const dim3 merge(grid2.x * grid2.y <= 256 ? MERGE_THREADS : 256);
   const bool mx = pages->kind == RF_PAGES_MX4;
 #define RF_FEW(D, MT)                                                                                    \
   do {                                                                                                   \
@@ -809,7 +870,7 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
     else hipLaunchKernelGGL((k_paged_few<D, false, MT>), grid, dim3(64 * NW), 0, stream, a);             \
     if (p.target) {                                                                                      \
       if (int rc = check_launch(fn)) return rc;                                                          \
-      hipLaunchKernelGGL((k_paged_merge<D, 16>), grid2, dim3(256), 0, stream, a, 16 * MT);               \
+      hipLaunchKernelGGL(k_paged_merge<D>, grid2, merge, 0, stream, a, 16 * MT);                         \
     }                                                                                                    \
   } while (0)
 #define RF_FEW_D(D)                    \
