@@ -18,19 +18,16 @@
 
 #include <algorithm>
 
+#include "attend_tile.h"
 #include "paged.h"
 
 namespace rf {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ bf16x8 as_frag(const uint4& u) { return __builtin_bit_cast(bf16x8, u); }
-
-constexpr int KT = 32;                     // keys a tile
-constexpr float RESCALE_LOG2 = 8.0f;       // headroom of the lazy rescale: probabilities stay below 2^8
-constexpr int NW = 4;                      // waves a block
+constexpr int KT = 32;                     // keys a tile of k_paged_few
+constexpr int NW = 4;                      // its waves a block
 
 struct PagedArgs {
   const uint16_t* q;
@@ -46,9 +43,13 @@ struct PagedArgs {
   float c;                                 // scale log2(e)
   uint16_t* out;
   int64_t ldo;
-  float* part;                             // partials of the splits, or null
-  int target;                              // blocks that the splits aim at (0: no splits)
-  int64_t units;                           // units that the workspace holds partials of
+  float* part;                             // partials of the splits
+  int* length;                             // behind them: the split length, from the splits' launch to the merge
+  int fit;                                 // units a head that one round of blocks holds (0: no splits)
+  bool once;                               // as many as that at most
+  float ov;                                // what a unit costs besides its tiles, in tiles
+  int64_t units;                           // units a head that the launch has blocks and the workspace partials for
+  int kt, wmin;                            // keys a tile, key tiles a split at least
 };
 
 struct Seq {
@@ -66,7 +67,7 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
   return s;
 }
 
-__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + KT - 1) / KT); }
+__device__ __forceinline__ int tiles_of(int keys, int kt) { return max(1, (keys + kt - 1) / kt); }
 
 struct Unit {
   int b, rb, sp, ns;                       // sequence (-1: none), row block, split, splits of the sequence
@@ -76,55 +77,98 @@ struct Unit {
   Seq s;
 };
 
-__device__ __forceinline__ int wave_sum_below(int v, int lane, int& total) {     // exclusive prefix sum over 64 lanes
-  int s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(s, o, 64);
-    if (lane >= o) s += u;
-  }
+// Inclusive scan of a wave by data-parallel moves (within rows of 16 lanes, then across them); lane 63 has the total.
+template <class F>
+__device__ __forceinline__ int wave_scan(int v, int none, F&& f) {
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));      // row_shr:1, 2, 4, 8
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));      // row_bcast:15, 31
+  return f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));
+}
+
+__device__ __forceinline__ int wave_sum_below(int v, int& total) {              // exclusive prefix sum over 64 lanes
+  const int s = wave_scan(v, 0, [](int x, int y) { return x + y; });
   total = __builtin_amdgcn_readlane(s, 63);
   return s - v;
 }
 
-// Unit `want` of the call: units are the (sequence, split, row block)s in that order, row blocks fastest; with rows_only
-// the (sequence, row block)s. The split length W comes from the work of the whole call (key tiles x row blocks x heads over
-// `target`), read from the sequences' sizes here: every block does the same integer arithmetic, so no launch before this one
-// has to plan and a captured graph follows its lens. (A wave looks at 64 sequences at once.)
-__device__ Unit find_unit(const PagedArgs& a, int want, bool rows_only) {
+__device__ __forceinline__ float wave_sum(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(
+      wave_scan(__float_as_uint(v), 0, [](int x, int y) { return static_cast<int>(__float_as_uint(__uint_as_float(x) + __uint_as_float(y))); }), 63));
+}
+
+__device__ __forceinline__ int wave_max(int v) {                                // v >= 0
+  return __builtin_amdgcn_readlane(wave_scan(v, 0, [](int x, int y) { return max(x, y); }), 63);
+}
+
+// The key tiles of a split. Blocks of one length that fill the GPU once are best; a few more than fill it wait for a second
+// round, so splits are as short as one round of blocks allows (fit: its units a head). Where the row blocks alone nearly fill
+// it, the length of the least estimated time: all tiles and what each unit costs besides (ov) over the round's blocks, and a
+// third of a split for the end (or one round's longest split). 32 sequences of 500 to 8000 keys (bf16, 8 heads): 80 us
+// as one round, 85 at 1.25; 48 of 1500 to 24000 in 4 bits 98 against 107; 1499-row chunks of three prompts 521 at three
+// rounds, 599 at 1.6. Up to 64 sequences the lanes try 64 lengths each; more of them take a length that
+// surely fits. Every block does the same arithmetic on the same sizes: no launch has to plan before this one, and a captured
+// graph follows its lens.
+__device__ int split_length(const PagedArgs& a, float work, float blocks, int tmax, int nrb0, int tiles0, int lane) {
+  const float fit = static_cast<float>(a.fit);
+  const bool once = a.once;
+  if (a.n_seq > 64) {
+    const float W = once ? work / fmaxf(fit - blocks, 1.f) : work / (2.f * fit);
+    return max(a.wmin, static_cast<int>(ceilf(W)));
+  }
+  const float lo = fmaxf(static_cast<float>(a.wmin), ceilf(work / (once ? fit : 3.f * fit)));
+  const float hi = fmaxf(static_cast<float>(tmax), lo);
+  const float W = ceilf(lo * __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(hi / lo) * (static_cast<float>(lane) / 63.f)));
+  const float inv = 1.f / W;
+  float units = 0.f;
+  for (int b = 0; b < a.n_seq; ++b)
+    units += static_cast<float>(__builtin_amdgcn_readlane(nrb0, b)) *
+             ceilf(static_cast<float>(__builtin_amdgcn_readlane(tiles0, b)) * inv);
+  const float longest = fminf(W, static_cast<float>(tmax));
+  float cost = units <= fit ? fmaxf(longest, work / fit) : (work + a.ov * units) / fit + 0.35f * longest;
+  // (lane 63's length is every tile: one unit a row block, which always fits)
+  if (once && units > fit + 0.5f && lane != 63) cost = 3e38f;
+  // the least cost, the shorter length among equals (the bits of positive floats are in order)
+  const int bits = static_cast<int>(__float_as_uint(cost)), least = 0x7f800000 - wave_max(0x7f800000 - bits);
+  const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(__ballot(bits == least))) - 1);
+  return __builtin_amdgcn_readlane(static_cast<int>(W), l);
+}
+
+// Unit `want` of the call: units are the (sequence, split, row block)s in that order, row blocks fastest; merging:
+// the (sequence, row block)s. (A wave looks at 64 sequences at once.)
+__device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
   const int lane = threadIdx.x & 63;
   int W = 1 << 30;
-  if (a.target) {
-    float work = 0.f;                      // (only the split length depends on it; the same sum in every block)
+  Seq s0{0, 0, 0};
+  if (lane < a.n_seq) s0 = seq_of(a, lane);
+  if (a.fit && merging) {
+    W = *a.length;                         // as the launch before this one found it
+  } else if (a.fit) {
+    float work = 0.f, blocks = 0.f;        // (only the split length depends on them; the same sums in every block)
+    int tmax = 1;
     for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
-      float w = 0.f;
-      if (b0 + lane < a.n_seq) {
-        const Seq s = seq_of(a, b0 + lane);
-        w = static_cast<float>((s.rows + a.qb - 1) / a.qb) * static_cast<float>(tiles_of(s.keys));
-      }
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) w += __shfl_xor(w, o, 64);
-      work += w;
+      const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
+      const float r = static_cast<float>((s.rows + a.qb - 1) / a.qb);
+      work += wave_sum(r * static_cast<float>(tiles_of(s.keys, a.kt)));
+      blocks += wave_sum(r);
+      tmax = max(tmax, wave_max(s.rows ? tiles_of(s.keys, a.kt) : 1));
     }
-    W = __builtin_amdgcn_readfirstlane(
-        max(2 * NW, static_cast<int>(ceilf(work * static_cast<float>(a.hkv) / static_cast<float>(a.target)))));
+    W = split_length(a, work, blocks, tmax, (s0.rows + a.qb - 1) / a.qb, tiles_of(s0.keys, a.kt), lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.length = W;
   }
   Unit u;
   u.b = -1;
   int before = 0, parts = 0;
   for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
-    Seq s{0, 0, 0};
-    int nrb = 0, ns = 1;
-    if (b0 + lane < a.n_seq) {
-      s = seq_of(a, b0 + lane);
-      nrb = (s.rows + a.qb - 1) / a.qb;
-      ns = (tiles_of(s.keys) + W - 1) / W;
-    }
-    const int n = rows_only ? nrb : nrb * ns;
+    const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
+    const int nrb = (s.rows + a.qb - 1) / a.qb, ns = nrb ? (tiles_of(s.keys, a.kt) + W - 1) / W : 0;
+    const int n = merging ? nrb : nrb * ns;
     int total, ptotal;
-    const int pre = wave_sum_below(n, lane, total);
-    const int ppre = rows_only ? wave_sum_below(nrb * ns, lane, ptotal) : pre;
-    if (!rows_only) ptotal = total;
+    const int pre = wave_sum_below(n, total);
+    const int ppre = merging ? wave_sum_below(nrb * ns, ptotal) : pre;
+    if (!merging) ptotal = total;
     if (want < before + total) {
       // (scalar from here on: what follows from a unit is uniform over its block)
       const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
@@ -690,6 +734,350 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX, MT))) void k_paged_few(
   }
 }
 
+// k_paged_many: many query rows a sequence (a chunk of a prompt). A block takes 256 query rows (queries x the query heads of
+// a K / V head) of one sequence, 32 a wave, and the key tiles of its split through LDS, each read by all eight waves:
+// attend_causal.hip's tile (S^T = K Q^T, P^T straight from the score registers, V^T by transpose reads), with rows of any
+// query and head side by side in a wave, so that any group size fills it. Tiles come from pages: bf16 by direct loads, three
+// tiles in flight, the page of each load's rows (never more than 16) read off a lane; 4 bits through registers, a tile's
+// codes loaded while the one before it is converted into LDS, once for all eight waves (160 of a tile's 2000 cycles).
+// Bound by the products and the softmax beside them (64 keys: 1024 cycles of MFMA a wave, two waves a SIMD).
+template <int AD, bool MX>
+struct ManyCodes {
+  uint2 k, v;                              // codes of 16 values (8 at head_dim 64)
+  uint32_t ks, vs;                         // their scale bytes
+};
+
+// The wave's 16-key half of a tile that it loads: rows of one page.
+template <int AD>
+__device__ __forceinline__ int half_of_wave(int w) { return AD == 256 ? w >> 2 : w >> 1; }
+
+// A thread's codes of a tile whose half lies at token tok0 of page id.
+template <int AD>
+__device__ __forceinline__ void load_codes(ManyCodes<AD, true>& c, const PagesDev& pg, int id, int head, int tok0, int w, int lane) {
+  const int64_t at = static_cast<int64_t>(id) * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
+  const int64_t sat = static_cast<int64_t>(id) * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales;
+  constexpr int TPR = AD == 256 ? 16 : 8;                    // threads a key row (8 bytes each; 4 at head_dim 64)
+  const int row = (AD == 256 ? 4 * (w & 3) : 8 * (w & 1)) + lane / TPR, part = lane % TPR;
+  const char* kp = pg.k + at + (tok0 + row) * (AD / 2) + part * (AD / 2 / TPR);
+  if constexpr (AD == 64) c.k.x = *reinterpret_cast<const uint32_t*>(kp);
+  else c.k = *reinterpret_cast<const uint2*>(kp);
+  c.ks = pg.ks[sat + ((tok0 + row) >> 3) * (AD / 4) + (part * (AD / TPR) / 32) * 8 + (row & 7)];
+  // values: 8 tokens' runs; d 128: two tokens of a run of 8 values, 256: one of 16, 64: one of two runs of 4
+  const int grp = AD == 256 ? (w >> 1) & 1 : w & 1;
+  const char* vp = pg.v + at + ((tok0 >> 3) + grp) * (4 * AD);
+  const uint8_t* sp = pg.vs + sat + ((tok0 >> 3) + grp) * (AD / 4);
+  if constexpr (AD == 128) {
+    c.v = *reinterpret_cast<const uint2*>(vp + lane * 8);
+    c.vs = *reinterpret_cast<const uint16_t*>(sp + ((lane >> 2) / 4) * 8 + 2 * (lane & 3));
+  } else if constexpr (AD == 256) {
+    const int x = 64 * (w & 1) + lane;
+    c.v = *reinterpret_cast<const uint2*>(vp + x * 8);
+    c.vs = sp[((x >> 3) / 2) * 8 + (x & 7)];
+  } else {
+    const int cc = lane >> 3, key = lane & 7;
+    c.v.x = *reinterpret_cast<const uint16_t*>(vp + (2 * cc) * 16 + 2 * key) |
+            static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vp + (2 * cc + 1) * 16 + 2 * key)) << 16;
+    c.vs = sp[(cc / 4) * 8 + key];
+  }
+}
+
+__device__ __forceinline__ uint4 eight_values(uint32_t w, float s) {
+  return make_uint4(fp4_pair<0>(w, s), fp4_pair<1>(w, s), fp4_pair<2>(w, s), fp4_pair<3>(w, s));
+}
+
+// ... as bf16 into a stage.
+template <int AD>
+__device__ __forceinline__ void store_codes(const ManyCodes<AD, true>& c, char* st, int w, int lane) {
+  using L = Layout<AD>;
+  constexpr int TPR = AD == 256 ? 16 : 8;
+  const int row = (AD == 256 ? 4 : 8) * w + lane / TPR, part = lane % TPR;
+  uint4* s4 = reinterpret_cast<uint4*>(st);
+  const float ks = scale_of<0>(c.ks), vs = scale_of<0>(c.vs);
+  if constexpr (AD == 64) {
+    s4[L::kslot(row, part)] = eight_values(c.k.x, ks);
+    s4[L::vslot(8 * w + (lane & 7), lane >> 3)] = eight_values(c.v.x, vs);
+  } else {
+    s4[L::kslot(row, 2 * part)] = eight_values(c.k.x, ks);
+    s4[L::kslot(row, 2 * part + 1)] = eight_values(c.k.y, ks);
+    if constexpr (AD == 128) {
+      const int r = 8 * w + 2 * (lane & 3);
+      s4[L::vslot(r, lane >> 2)] = eight_values(c.v.x, vs);
+      s4[L::vslot(r + 1, lane >> 2)] = eight_values(c.v.y, scale_of<1>(c.vs));
+    } else {
+      const int x = 64 * (w & 1) + lane, r = 8 * (w >> 1) + (x & 7);
+      s4[L::vslot(r, 2 * (x >> 3))] = eight_values(c.v.x, vs);
+      s4[L::vslot(r, 2 * (x >> 3) + 1)] = eight_values(c.v.y, vs);
+    }
+  }
+}
+
+// tile_step for a tile of which some row does not see some key, without the next tile's scores: bad has a bit a 16-key half
+// on a page that is none. Of V, what is not finite enters the product as zero; a row that sees such a value takes it
+// from LDS afterwards (0 x infinity must not reach the rows that do not).
+template <int AD>
+__device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&sc)[Cfg<AD>::KB], f32x16 (&o)[AD / 32],
+                                          float& mref, float& lsum, int k0, uint32_t bad, int mypos, int hh, float c,
+                                          const FragOffsets<AD>& fo) {
+  using L = Layout<AD>;
+  constexpr int NB = AD / 32, KB = Cfg<AD>::KB, KTL = Cfg<AD>::KT, NP = 8 * KB;
+  const int rel = min(max(mypos - k0, -1), KTL) - 4 * hh;
+  float tmax = -INFINITY;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const bool gone = (bad >> (2 * kb + (j >> 3))) & 1u;   // keys 32 kb + 8 (j / 4) + ..
+      if (gone || 32 * kb + 8 * (j >> 2) + (j & 3) > rel) sc[kb][j] = -INFINITY;
+      tmax = fmaxf(tmax, sc[kb][j]);
+    }
+  float lo, hi;
+  lane_pair(tmax, lo, hi);
+  tmax = fmaxf(lo, hi);
+  if (tmax > mref + RESCALE_LOG2 / c) {
+    const float alpha = __builtin_amdgcn_exp2f((mref - tmax) * c);
+    mref = tmax;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+    lsum *= alpha;
+  }
+  const float mc = mref == -INFINITY ? 0.f : mref * c;
+  float psum = 0.f;
+  uint32_t pk[NP];
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+    const float q0 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8)], c, -mc));
+    const float q1 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8) + 1], c, -mc));
+    psum += q0 + q1;
+    pk[e] = bf16_pair(q0, q1);
+  }
+  lsum += psum;
+  bool odd = false;
+#pragma unroll
+  for (int stp = 0; stp < KTL / 16; ++stp) {
+    const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const char* vp = st + fo.v(b) + 16 * stp * L::KCPR * 16;
+      uint2 vl = read_tr(vp), vh = read_tr(vp + 8 * L::KCPR * 16);
+      odd |= not_finite(vl.x) || not_finite(vl.y) || not_finite(vh.x) || not_finite(vh.y);
+      vl = make_uint2(finite_pair(vl.x), finite_pair(vl.y));
+      vh = make_uint2(finite_pair(vh.x), finite_pair(vh.y));
+      o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(make_uint4(vl.x, vl.y, vh.x, vh.y)), pf, o[b], 0, 0, 0);
+    }
+  }
+  if (!__any(odd)) return;
+  for (int kk = 0; kk < KTL; ++kk) {
+    if (((bad >> (kk >> 4)) & 1u) || k0 + kk > mypos) continue;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {                          // d = 32 b + 8 g + 4 hh + 0 .. 3
+        const uint2 v = *reinterpret_cast<const uint2*>(st + L::vslot(kk, 4 * b + g) * 16 + 8 * hh);
+        o[b][4 * g] += marked(mark_of(v.x & 0xffffu));
+        o[b][4 * g + 1] += marked(mark_of(v.x >> 16));
+        o[b][4 * g + 2] += marked(mark_of(v.y & 0xffffu));
+        o[b][4 * g + 3] += marked(mark_of(v.y >> 16));
+      }
+  }
+}
+
+template <int AD, bool MX>
+__global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
+  using L = Layout<AD>;
+  constexpr int NS = AD / 16, NB = AD / 32, KTL = Cfg<AD>::KT, QROWS = Cfg<AD>::QROWS, KB = Cfg<AD>::KB;
+  constexpr int HPT = KTL / 16, WIN = 64 / HPT;              // 16-key halves a tile, tiles a window of table entries
+  __shared__ uint4 lds[NSTAGE * L::STAGE_U4];
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 31, hh = lane >> 5;
+  // heads fastest within a unit's row blocks: a head's row blocks of one split lie hkv blocks apart
+  const int head = blockIdx.x % a.hkv;
+  const Unit u = find_unit(a, blockIdx.x / a.hkv, false);
+  if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
+  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0), rows = nq * a.rep;
+  const int p0 = u.s.keys - u.s.rows + q0, plast = p0 + nq - 1;
+  const int ntiles = plast < 0 ? 0 : plast / KTL + 1;
+  const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);
+
+  // row 32 w + n: query r / rep, head r % rep; lanes past the last row repeat it and write nothing
+  const int r = min(32 * w + n, rows - 1), qi = r / a.rep;
+  const bool live = 32 * w + n < rows;
+  const int mypos = p0 + qi;
+  const int wave_last = 32 * w < rows ? p0 + min(32 * w + 31, rows - 1) / a.rep : -1;
+  bf16x8 qf[NS];
+  {
+    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldq + (head * a.rep + r - qi * a.rep) * AD + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = as_frag(*reinterpret_cast<const uint4*>(qrow + 16 * s));
+  }
+
+  // pages: lane l holds the entry of half l % HPT of tile l / HPT of a window of WIN tiles (0 for none, with its bit of bad)
+  const int32_t* row = a.table + static_cast<int64_t>(u.b) * a.ld_table;
+  auto entry = [&](int win) {
+    const int it = it0 + win * WIN + lane / HPT;
+    const int at = (it * HPT + lane % HPT) >> (a.pg.shift - 4);
+    return it < it1 && at < a.width ? row[at] : -1;
+  };
+  int ids = entry(0), coming = entry(1), window = 0;
+  uint64_t bad = 0, bad_before = 0;
+  auto settle = [&]() {
+    const bool out = ids < 0 || ids >= a.pg.n_pages;
+    ids = out ? 0 : ids;
+    bad_before = bad;
+    bad = __ballot(out);
+  };
+  settle();
+  wait_vm_lgkm0<0>();        // queries and entries are in registers before any tile load is in flight
+  auto advance = [&](int it) {                               // before tile it is loaded; tiles in order
+    if ((it - it0) / WIN != window) {
+      ++window;
+      ids = coming;
+      settle();
+      coming = entry(window + 1);
+    }
+  };
+  auto bad_of = [&](int it) {
+    const int win = (it - it0) / WIN, x = ((it - it0) % WIN) * HPT;
+    return static_cast<uint32_t>((win == window ? bad : bad_before) >> x) & ((1u << HPT) - 1u);
+  };
+  const int mask = (1 << a.pg.shift) - 1;
+  char* base = reinterpret_cast<char*>(lds);
+  auto stage = [&](int it) { return base + ((it - it0) % NSTAGE) * L::STAGE_U4 * 16; };
+  auto id_of = [&](int it, int half) { return __builtin_amdgcn_readlane(ids, ((it - it0) % WIN) * HPT + half); };
+
+  // bf16: instruction i of wave w fills 64 consecutive 16-byte slots, rows row0 .. of one half; the lane's slot gives the row
+  // and the chunk it fetches
+  [[maybe_unused]] auto issue = [&](int it) {
+    advance(it);
+    char* st = stage(it);
+#pragma unroll
+    for (int i = 0; i < L::KLOADS; ++i) {
+      constexpr int RPI = 64 / L::KCPR;
+      const int row0 = (w * L::KLOADS + i) * RPI, half = row0 >> 4;
+      const int tok = (it * KTL + row0) & mask;
+      const int64_t at = static_cast<int64_t>(id_of(it, half)) * a.pg.page_stride + static_cast<int64_t>(head) * a.pg.head_bytes +
+                         static_cast<int64_t>(tok) * (AD * 2);
+      const int rl = lane / L::KCPR, pc = lane % L::KCPR;
+      const uint32_t ko = static_cast<uint32_t>(rl * (AD * 2) + (pc ^ ((row0 + rl) & (L::KCPR - 1))) * 16);
+      const uint32_t vo = static_cast<uint32_t>(rl * (AD * 2) + (pc ^ (4 * L::vsw(row0 + rl))) * 16);
+      const __amdgpu_buffer_rsrc_t rk = buffer_rsrc(a.pg.k + at, 1024u), rv = buffer_rsrc(a.pg.v + at, 1024u);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(st + (w * L::KLOADS + i) * 1024), 16, ko, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(st + (L::K_U4 + (w * L::VLOADS + i) * 64) * 16), 16, vo, 0, 0, 0);
+    }
+  };
+  // 4 bits: the tile's codes into registers
+  [[maybe_unused]] ManyCodes<AD, true> codes;
+  [[maybe_unused]] auto fetch = [&](int it) {
+    advance(it);
+    const int half = half_of_wave<AD>(w);
+    load_codes<AD>(codes, a.pg, id_of(it, half), head, (it * KTL + 16 * half) & mask, w, lane);
+  };
+
+  f32x16 o[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[b][x] = 0.f;
+  float m = -INFINITY, lsum = 0.f;
+  const float c = a.c;
+  const FragOffsets<AD> fo(lane);
+  f32x16 sc[KB], sn[KB];
+  // Turn it, then softmax and product of tile it, with the scores of tile it + 1 in the same block. bf16: tile it + 3 is
+  // loaded into the stage of tile it - 1, whose last reads ended before this iteration's barrier. 4 bits: the codes of tile
+  // it + 2 go to its stage (tile it - 2's) and those of tile it + 3 to registers; the next barrier makes the stage visible.
+  if constexpr (MX) {
+    for (int i = 0; i < 2; ++i)
+      if (it0 + i < it1) {
+        fetch(it0 + i);
+        store_codes<AD>(codes, stage(it0 + i), w, lane);
+      }
+    if (it0 + 2 < it1) fetch(it0 + 2);
+    __syncthreads();
+  } else {
+    for (int i = 0; i < 3; ++i)
+      if (it0 + i < it1) issue(it0 + i);
+    if (it0 + 2 < it1) wait_vm_lgkm0<2 * L::LOADS>();        // tile it0 landed
+    else if (it0 + 1 < it1) wait_vm_lgkm0<L::LOADS>();
+    else wait_vm_lgkm0<0>();
+    __builtin_amdgcn_s_barrier();
+  }
+  if (it0 < it1) tile_scores<AD>(stage(it0), qf, sc, fo);
+  auto turn = [&](int it) {
+    if constexpr (MX) {
+      __syncthreads();
+      if (it + 2 < it1) store_codes<AD>(codes, stage(it + 2), w, lane);
+      if (it + 3 < it1) fetch(it + 3);
+    } else {
+      if (it + 2 < it1) wait_vm_lgkm0<L::LOADS>();           // tile it + 1 landed, tile it + 2 may fly
+      else wait_vm_lgkm0<0>();
+      __builtin_amdgcn_s_barrier();                          // every wave's share of it has landed and every
+      if (it + 3 < it1) issue(it + 3);                       // wave is done with the stage reloaded here
+    }
+  };
+  // Tiles that every row of the block sees whole, in pairs (the scores' buffers swap roles), up to the first page that is
+  // none (uniform over the block, as the barriers need); then the others, whose code stays out of this loop's registers.
+  if (32 * w >= rows) {                                      // a wave without rows: its share of the loads and the barriers
+    for (int it = it0; it < it1; ++it) turn(it);
+    return;
+  }
+  const int full = p0 >= KTL - 1 ? min(it1, (p0 + 1) / KTL) : it0;
+  int it = it0;
+  if constexpr (AD == 256) {                                 // (one buffer's copy each: in pairs it spills)
+    for (; it < full; ++it) {
+      if (bad_of(it)) break;
+      turn(it);
+      tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) sc[kb] = sn[kb];
+    }
+  } else {
+    for (; it + 1 < full; it += 2) {
+      if (bad_of(it) | bad_of(it + 1)) break;
+      turn(it);
+      tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
+      turn(it + 1);
+      tile_step<AD>(stage(it + 1), stage(it + 2), qf, sn, sc, o, m, lsum, it * KTL + KTL, false, mypos, hh, c, fo);
+    }
+  }
+  for (; it < it1; ++it) {
+    turn(it);
+    if (it * KTL > wave_last) continue;                      // this and every later tile lie past the wave's rows
+    edge_tile<AD>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), mypos, hh, c, fo);
+    tile_scores<AD>(stage(it + 1), qf, sc, fo);
+  }
+  wait_vm_lgkm0<0>();
+
+  // lane holds O[row n][d = 32 b + 8 (j / 4) + 4 hh + j % 4]
+  float llo, lhi;
+  lane_pair(lsum, llo, lhi);
+  const float ltot = llo + lhi;
+  if (!live) return;
+  if (u.ns > 1) {
+    const int64_t part = (u.part + static_cast<int64_t>(u.sp) * u.nrb) * a.hkv + head;
+    float* pb = a.part + part * (static_cast<int64_t>(QROWS) * (AD + 2));
+    float* orow = pb + r * AD + 4 * hh;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(orow + 32 * b + 8 * g) = make_float4(o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2],
+                                                                        o[b][4 * g + 3]);
+    if (hh == 0) {
+      pb[QROWS * AD + r] = m == -INFINITY ? m : m * c;
+      pb[QROWS * (AD + 1) + r] = ltot;
+    }
+    return;
+  }
+  const float inv = inverse_sum(ltot);
+  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * AD + 4 * hh;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(dst + 32 * b + 8 * g) =
+          make_uint2(bf16_pair(o[b][4 * g] * inv, o[b][4 * g + 1] * inv), bf16_pair(o[b][4 * g + 2] * inv, o[b][4 * g + 3] * inv));
+}
+
 // Merges the splits of a row block and head: D / 4 lanes a row (4 columns each); the block's lanes beyond its rows make G
 // groups a row, group i takes splits i, i + G, .. (eight in flight) with a running maximum, and the groups are joined in
 // order through LDS. The order depends on the sizes alone. blockIdx.y takes a share of the rows where few row blocks leave
@@ -782,27 +1170,33 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a, int 
 // 16-row blocks a wave takes: as few as hold a sequence's rows (their state and queries live in registers: up to 4, 3 at
 // head_dim 256).
 int row_tiles(int rep, int d, int64_t max_rows) {
-  const int64_t rows = std::min<int64_t>(max_rows, 64) * rep;
-  return static_cast<int>(std::min<int64_t>(d == 256 && rep <= 48 ? 3 : 4, (rows + 15) / 16));
+  return static_cast<int>(std::min<int64_t>(d == 256 ? 3 : 4, (max_rows * rep + 15) / 16));
 }
 
 struct Plan {
-  int mt, qb, target;
+  bool many, once;
+  int mt, qb, fit, kt;                     // mt: 16-row blocks of k_paged_few
   int64_t blocks, units;                   // (sequence, row block)s at most, and with their splits
   size_t bytes;
+  int rows() const { return many ? Cfg<128>::QROWS : 16 * mt; }
 };
 
-// The launch for these sizes. Row blocks: sum of ceil(rows / qb) <= T / qb + n_seq. Splits: sum of nrb ceil(tiles / W) <=
-// sum of nrb tiles / W + row blocks, and W >= work hkv / target, so they are at most target / hkv + row blocks.
+// The launch for these sizes: a sequence's rows in the registers of k_paged_few's waves, or more of them through
+// k_paged_many. Row blocks: sum of ceil(rows / qb) <= T / qb + n_seq. With splits of W tiles at most work / W units more
+// (split_length: one round of blocks, or W >= work / 3 fit).
 Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys) {
   Plan p{};
   const int rep = hq / hkv;
-  p.mt = row_tiles(rep, d, max_rows);
-  p.qb = 16 * p.mt / rep;
+  p.many = std::min<int64_t>(max_rows, T) * rep > (d == 256 ? 48 : 64);
+  p.mt = p.many ? 0 : row_tiles(rep, d, std::min<int64_t>(max_rows, T));
+  p.qb = p.rows() / rep;
+  p.kt = p.many ? (d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
   p.blocks = std::min<int64_t>(T, T / p.qb + n_seq);
-  p.target = max_keys > 16 * NW * KT ? 256 * few_blocks(d, mx, p.mt) : 0;
-  p.units = p.target ? p.target / hkv + 1 + p.blocks : p.blocks;
-  p.bytes = p.target ? static_cast<size_t>(p.units) * hkv * (16 * p.mt * (d + 2)) * 4 : 0;
+  const int round = p.many ? 256 : 256 * few_blocks(d, mx, p.mt);
+  p.fit = max_keys <= 16 * NW * KT ? 0 : std::max(1, round / hkv);
+  p.once = p.blocks * 4 <= static_cast<int64_t>(p.fit) * 3;
+  p.units = !p.fit ? p.blocks : p.once ? p.fit : 3 * p.fit + 1 + p.blocks;
+  p.bytes = p.fit ? static_cast<size_t>(p.units) * hkv * (p.rows() * (d + 2)) * 4 + 16 : 0;
   return p;
 }
 
@@ -811,7 +1205,7 @@ int attend_sizes(const char* fn, int64_t T, int hq, int hkv, int d, int kind, in
   if (hq <= 0 || hkv <= 0 || hkv > 4096 || hq % hkv || hq / hkv > 64)
     return fail(RF_EUNSUPPORTED, "%s: %d query heads over %d K / V heads (groups of up to 64)", fn, hq, hkv);
   if (kind != RF_PAGES_BF16 && kind != RF_PAGES_MX4) return fail(RF_EINVAL_ARG, "%s: kind of pages %d", fn, kind);
-  if (T < 0 || T > (1 << 24) || n_seq < 0 || n_seq > (1 << 20) || max_rows < 0 || max_keys < 0 || max_keys > (1 << 30))
+  if (T < 0 || T > (1 << 24) || n_seq < 0 || n_seq > (1 << 20) || max_rows < 0 || max_keys < 0 || max_keys > (1 << 27))
     return fail(RF_EINVAL_SHAPE, "%s: %lld rows of %d sequences, at most %lld rows and %lld keys each", fn, (long long)T, n_seq,
                 (long long)max_rows, (long long)max_keys);
   return RF_OK;
@@ -851,39 +1245,43 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
     return fail(RF_EINVAL_ARG, "%s: scale %g (must be positive)", fn, static_cast<double>(scale));
   if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
   Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys);
-  if (p.target && (!workspace || ws_bytes < p.bytes)) {
-    p.target = 0;
+  if (p.fit && (!workspace || ws_bytes < p.bytes)) {
+    p.fit = 0;
     p.units = p.blocks;
   }
   const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.qb,
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
-                    scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace), p.target, p.units};
+                    scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace),
+                    p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.many ? 3.f : 1.f, p.units, p.kt,
+                    p.many ? 4 : 2 * NW};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
-  const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, 16 * p.mt);
-  const dim3 grid2(static_cast<unsigned>(pairs), static_cast<unsigned>(std::min<int64_t>(rows, (511 + pairs) / pairs)));
+  const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, p.rows());
+  const dim3 grid2(static_cast<unsigned>(pairs), static_cast<unsigned>(std::min<int64_t>(p.many ? (rows + 15) / 16 : rows, ((p.many ? 2047 : 511) + pairs) / pairs)));
   const dim3 merge(grid2.x * grid2.y <= 256 ? MERGE_THREADS : 256);
   const bool mx = pages->kind == RF_PAGES_MX4;
 #define RF_FEW(D, MT)                                                                                    \
   do {                                                                                                   \
     if (mx) hipLaunchKernelGGL((k_paged_few<D, true, MT>), grid, dim3(64 * NW), 0, stream, a);           \
     else hipLaunchKernelGGL((k_paged_few<D, false, MT>), grid, dim3(64 * NW), 0, stream, a);             \
-    if (p.target) {                                                                                      \
+  } while (0)
+#define RF_ATTEND(D)                                                                                     \
+  do {                                                                                                   \
+    if (p.many && mx) hipLaunchKernelGGL((k_paged_many<D, true>), grid, dim3(Cfg<D>::NTHR), 0, stream, a); \
+    else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false>), grid, dim3(Cfg<D>::NTHR), 0, stream, a); \
+    else if (p.mt == 1) RF_FEW(D, 1);                                                                    \
+    else if (p.mt == 2) RF_FEW(D, 2);                                                                    \
+    else if (p.mt == 3) RF_FEW(D, 3);                                                                    \
+    else if constexpr (D != 256) RF_FEW(D, 4);                                                           \
+    if (p.fit) {                                                                                         \
       if (int rc = check_launch(fn)) return rc;                                                          \
-      hipLaunchKernelGGL(k_paged_merge<D>, grid2, merge, 0, stream, a, 16 * MT);                         \
+      hipLaunchKernelGGL(k_paged_merge<D>, grid2, merge, 0, stream, a, p.rows());                        \
     }                                                                                                    \
   } while (0)
-#define RF_FEW_D(D)                    \
-  do {                                 \
-    if (p.mt == 1) RF_FEW(D, 1);       \
-    else if (p.mt == 2) RF_FEW(D, 2);  \
-    else if (p.mt == 3) RF_FEW(D, 3);  \
-    else RF_FEW(D, 4);                 \
-  } while (0)
-  if (d == 64) RF_FEW_D(64);
-  else if (d == 128) RF_FEW_D(128);
-  else RF_FEW_D(256);
-#undef RF_FEW_D
+  if (d == 64) RF_ATTEND(64);
+  else if (d == 128) RF_ATTEND(128);
+  else RF_ATTEND(256);
+#undef RF_ATTEND
 #undef RF_FEW
   return check_launch(fn);
 }

@@ -72,7 +72,7 @@ def test_bad_attention_is_refused():
     _attend(_pages())
     for bad in (dict(q=None), dict(lens=None), dict(cu=None), dict(table=None), dict(out=None), dict(T=-1), dict(ldq=252),
                 dict(ldq=248), dict(ldo=255), dict(width=-1), dict(ldt=3), dict(n=-1), dict(rows=-1), dict(keys=-1),
-                dict(keys=1 << 31), dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=(1 << 20) + 8),
+                dict(keys=(1 << 27) + 1), dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=(1 << 20) + 8),
                 dict(out=(1 << 20) + 4), dict(ws=(1 << 20) + 8)):
         with pytest.raises(ValueError):
             _attend(_pages(), **bad)
