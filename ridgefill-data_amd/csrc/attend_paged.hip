@@ -1,19 +1,23 @@
 // Attention of new tokens of many sequences over a paged K / V cache (bf16 or 4-bit codes), gfx950.
 //
 // k_paged_few: a few query rows a sequence (one token of each, or some drafted ones). The keys are read once from HBM and
-// that read is the bound, so a wave streams them from memory straight into the registers of its products, with no LDS on
-// the way: a block takes one K / V head and up to 16 MT query rows (queries x the query heads of the K / V head, query by
-// query) of one sequence, its four waves take turns at the key tiles (32 keys) of the block's split. Per tile and wave:
-//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16. A's row m of key half kb is key 8 (m / 4) + 4 kb + m % 4 of the tile, so that
-//       lane (n, g) (n = lane % 16, g = lane / 16) holds, for query row n, the scores of keys 8 g .. 8 g + 7: the order in
-//       which A of the second product wants them. The contraction's order over d is free, too: a lane takes its share of d
-//       as memory gives it (bf16: 16-byte chunk 4 s + g in step s; 4 bits: codes of d / 4 consecutive values).
+// that read is the bound: a block takes one K / V head and 16 query rows (queries x the query heads of the K / V head, query
+// by query) of one sequence, its four waves take turns at the key tiles (32 keys) of the block's run, with no barrier until
+// they join. bf16 tiles go straight from memory into the registers of the products; 4-bit ones, half the bytes a product,
+// through a ring of four tiles in LDS a wave, which keeps enough of them in flight. Per tile and wave:
+//   S^T = K Q^T. A's row m of key half kb is key 8 (m / 4) + 4 kb + m % 4 of the tile, so that lane (n, g) (n = lane % 16,
+//       g = lane / 16) holds, for query row n, the scores of keys 8 g .. 8 g + 7: the order in which A of the second product
+//       wants them. bf16: v_mfma_f32_16x16x32_bf16, the contraction's order over d as memory gives it (16-byte chunk 4 s + g
+//       in step s). 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4, which takes codes and scales as they are; the queries as two
+//       E4M3 terms (load_queries).
 //   Softmax in fp32 base 2, the running maximum raised only when a score exceeds it by 2^8 (lazily: O is rescaled rarely).
-//   O += P V on the same MFMA: B's column n of product nb is d = n (D / 16) + nb, so a lane reads D / 16 consecutive values
-//       of each of its 8 keys and transposes 2 x 2 with v_perm (half an instruction a value); O's columns of a lane are
-//       consecutive in memory again.
-// 4-bit codes become bf16 by v_cvt_scalef32_pk_bf16_fp4, scale included, exactly: the arithmetic after it is that of bf16
-// pages. The waves' parts are merged through LDS in wave order.
+//   O += P V on v_mfma_f32_16x16x32_bf16: B's column n of product nb is d = n (D / 16) + nb, so a lane reads D / 16 consecutive
+//       values of each of its 8 keys and transposes 2 x 2 with v_perm (half an instruction a value); O's columns of a lane are
+//       consecutive in memory again. 4-bit values become bf16 by v_cvt_scalef32_pk_bf16_fp4, scale included, exactly. (P in
+//       8 bits or less would round the probabilities by 2^-4 and more; they keep bf16's 2^-8.)
+// The waves' parts are merged through LDS in wave order. Measured, merge included: 32 sequences of 500 to 8111 keys, 8 heads of
+// 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 95 us for 405 MB; one of 122880 keys in 4
+// bits, 2 heads of 256, 31 us for 67 MB: of that 7 are the merge and 10 the launch, the first tiles' way and the end.
 #include <stdint.h>
 
 #include <algorithm>
@@ -25,6 +29,7 @@ namespace rf {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int KT = 32;                     // keys a tile of k_paged_few
 constexpr int NW = 4;                      // its waves a block
@@ -38,15 +43,15 @@ struct PagedArgs {
   int width;                               // pages of a sequence at most
   const int32_t* lens;
   const int32_t* cu;
-  int n_seq, hq, hkv, rep, qb;             // qb: queries a block
+  int n_seq, hq, hkv, rep, rpb;            // rpb: query rows a block
   int max_rows, max_keys;
   float c;                                 // scale log2(e)
   uint16_t* out;
   int64_t ldo;
   float* part;                             // partials of the splits
   int* length;                             // behind them: the split length, from the splits' launch to the merge
-  int fit;                                 // units a head that one round of blocks holds (0: no splits)
-  bool once;                               // as many as that at most
+  int fit;                                 // blocks a head that one round holds (0: no splits)
+  bool once;                               // k_paged_many: as many units as that at most
   float ov;                                // what a unit costs besides its tiles, in tiles
   int64_t units;                           // units a head that the launch has blocks and the workspace partials for
   int kt, wmin;                            // keys a tile, key tiles a split at least
@@ -66,6 +71,19 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
   s.keys = static_cast<int>(max<int64_t>(0, min<int64_t>(a.lens[b], held)));
   return s;
 }
+
+// Query rows are a sequence's (query, head of the K / V head)s, query by query; row blocks take rpb of them.
+__device__ __forceinline__ int row_blocks(const PagedArgs& a, const Seq& s) { return (s.rows * a.rep + a.rpb - 1) / a.rpb; }
+
+struct RowBlock {
+  int q0, off, rows;                       // query and head of its first row, its rows
+  __device__ RowBlock(const PagedArgs& a, const Seq& s, int rb) {
+    const int r0 = rb * a.rpb;
+    q0 = r0 / a.rep;
+    off = r0 - q0 * a.rep;
+    rows = min(a.rpb, s.rows * a.rep - r0);
+  }
+};
 
 __device__ __forceinline__ int tiles_of(int keys, int kt) { return max(1, (keys + kt - 1) / kt); }
 
@@ -150,12 +168,12 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
     int tmax = 1;
     for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
       const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
-      const float r = static_cast<float>((s.rows + a.qb - 1) / a.qb);
+      const float r = static_cast<float>(row_blocks(a, s));
       work += wave_sum(r * static_cast<float>(tiles_of(s.keys, a.kt)));
       blocks += wave_sum(r);
       tmax = max(tmax, wave_max(s.rows ? tiles_of(s.keys, a.kt) : 1));
     }
-    W = split_length(a, work, blocks, tmax, (s0.rows + a.qb - 1) / a.qb, tiles_of(s0.keys, a.kt), lane);
+    W = split_length(a, work, blocks, tmax, row_blocks(a, s0), tiles_of(s0.keys, a.kt), lane);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.length = W;
   }
   Unit u;
@@ -163,7 +181,7 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
   int before = 0, parts = 0;
   for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
     const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
-    const int nrb = (s.rows + a.qb - 1) / a.qb, ns = nrb ? (tiles_of(s.keys, a.kt) + W - 1) / W : 0;
+    const int nrb = row_blocks(a, s), ns = nrb ? (tiles_of(s.keys, a.kt) + W - 1) / W : 0;
     const int n = merging ? nrb : nrb * ns;
     int total, ptotal;
     const int pre = wave_sum_below(n, total);
@@ -190,12 +208,62 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
   return u;
 }
 
+// k_paged_few's shares: the key tiles of all (sequence, row block)s in a row, cut into equal runs, one a block of a round
+// (a run may end inside a row block and begin the next one's: its parts are then two pieces or more). 48 sequences of 1500
+// to 24000 keys in 96 splits of one length at most were a quarter empty; equal runs take 97 us where those took 107.
+struct Piece {
+  int b, rb, t0, nt;                       // sequence (-1: none), row block, tile that the position falls on, its tiles
+  int begin;                               // position of its first tile
+  Seq s;
+};
+
+// The piece at position `want` of the tiles in a row; by_block: the want-th (sequence, row block), from its first tile.
+__device__ __forceinline__ Piece piece_at(const PagedArgs& a, const Seq& s0, int want, bool by_block, int lane) {
+  Piece pc;
+  pc.b = -1;
+  int before = 0, tiles_before = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
+    const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
+    const int nrb = row_blocks(a, s), nt = tiles_of(s.keys, a.kt);
+    int total, tiles;
+    const int tpre = wave_sum_below(nrb * nt, tiles), pre = by_block ? wave_sum_below(nrb, total) : tpre, n = by_block ? nrb : nrb * nt;
+    if (!by_block) total = tiles;
+    if (want < before + total) {
+      const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+      const int off = want - before - __builtin_amdgcn_readlane(pre, l);
+      pc.b = b0 + l;
+      pc.nt = __builtin_amdgcn_readlane(nt, l);
+      pc.rb = by_block ? off : off / pc.nt;
+      pc.t0 = by_block ? 0 : off - pc.rb * pc.nt;
+      pc.begin = tiles_before + __builtin_amdgcn_readlane(tpre, l) + pc.rb * pc.nt;
+      pc.s = Seq{__builtin_amdgcn_readlane(s.rows, l), __builtin_amdgcn_readlane(s.keys, l), __builtin_amdgcn_readlane(s.first, l)};
+      return pc;
+    }
+    before += total;
+    tiles_before += tiles;
+  }
+  return pc;
+}
+
+// The length of a run: every block's own sum of the tiles.
+__device__ __forceinline__ int run_length(const PagedArgs& a, const Seq& s0, int lane, int& total) {
+  total = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
+    const Seq s = b0 == 0 ? s0 : b0 + lane < a.n_seq ? seq_of(a, b0 + lane) : Seq{0, 0, 0};
+    int n;
+    wave_sum_below(row_blocks(a, s) * tiles_of(s.keys, a.kt), n);
+    total += n;
+  }
+  return max(a.wmin, (total + a.fit - 1) / a.fit);
+}
+
 // Key half kb's registers of a tile: the lane's share of d of its key.
 template <int D, bool MX>
 struct KTile {
   static constexpr int NS = D / 32;                          // 32-deep steps over d
   uint4 x[MX ? 1 : 2][MX ? 1 : NS];                          // bf16
-  uint32_t c[MX ? 2 : 1][MX ? D / 32 : 1];                   // codes of D / 4 values
+  uint32_t c[MX ? 2 : 1][MX ? (D == 256 ? 8 : 4) : 1];       // codes: of 32 values from d = 128 s + 32 g on, 4 dwords each
   uint2 sc[MX ? (D == 256 ? 2 : 1) : 1];                     // scales of the 8 keys that the lane's two keys are among
 };
 
@@ -207,96 +275,193 @@ struct VTile {
   uint2 sc;
 };
 
-template <int D, bool MX>
-__device__ __forceinline__ void load_k(KTile<D, MX>& kt, const PagesDev& pg, int64_t id, int head, int tok0, int m, int g) {
-  // tok0: the page's token of the 16-key half of the tile that key row m lies in
+// bf16: a tile's registers from memory. tok0: the page's token of the 16-key half of the tile that key row m (load_k), or
+// lane group g's 8 keys (load_v), lie in.
+template <int D>
+__device__ __forceinline__ void load_k(KTile<D, false>& kt, const PagesDev& pg, int64_t id, int head, int tok0, int m, int g) {
   const int key = 8 * ((m >> 2) & 1) + (m & 3);              // of that half, for kb = 0
   const char* base = pg.k + id * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
-  if constexpr (!MX) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const char* row = base + (tok0 + key + 4 * kb) * (D * 2) + g * 16;
+  for (int kb = 0; kb < 2; ++kb) {
+    const char* row = base + (tok0 + key + 4 * kb) * (D * 2) + g * 16;
 #pragma unroll
-      for (int s = 0; s < KTile<D, MX>::NS; ++s) kt.x[kb][s] = *reinterpret_cast<const uint4*>(row + s * 64);
-    }
-  } else {
-    constexpr int LB = D / 8;                                // bytes a lane takes of a key
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const char* row = base + (tok0 + key + 4 * kb) * (D / 2) + g * LB;
-      if constexpr (D == 64) {
-        const uint2 w = *reinterpret_cast<const uint2*>(row);
-        kt.c[kb][0] = w.x;
-        kt.c[kb][1] = w.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < LB / 16; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * i);
-          kt.c[kb][4 * i] = w.x;
-          kt.c[kb][4 * i + 1] = w.y;
-          kt.c[kb][4 * i + 2] = w.z;
-          kt.c[kb][4 * i + 3] = w.w;
-        }
-      }
-    }
-    const uint8_t* sc = pg.ks + id * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales +
-                        ((tok0 + 8 * ((m >> 2) & 1)) >> 3) * (D / 4);
-    if constexpr (D == 256) {
-      kt.sc[0] = *reinterpret_cast<const uint2*>(sc + (2 * g) * 8);
-      kt.sc[1] = *reinterpret_cast<const uint2*>(sc + (2 * g + 1) * 8);
-    } else {
-      kt.sc[0] = *reinterpret_cast<const uint2*>(sc + (D == 128 ? g : g >> 1) * 8);
-    }
+    for (int s = 0; s < D / 32; ++s) kt.x[kb][s] = *reinterpret_cast<const uint4*>(row + s * 64);
   }
 }
 
-template <int D, bool MX>
-__device__ __forceinline__ void load_v(VTile<D, MX>& vt, const PagesDev& pg, int64_t id, int head, int tok0, int n, int g) {
-  const int key = 8 * (g & 1);                               // first of the lane's 8 keys within the 16-key half
-  const char* base = pg.v + id * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
+template <int D>
+__device__ __forceinline__ void load_v(VTile<D, false>& vt, const PagesDev& pg, int64_t id, int head, int tok0, int n, int g) {
   constexpr int VL = D / 16;
-  if constexpr (!MX) {
+  const char* base = pg.v + id * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const char* row = base + (tok0 + key + e) * (D * 2) + n * (VL * 2);
-      if constexpr (VL == 4) {
-        const uint2 w = *reinterpret_cast<const uint2*>(row);
-        vt.x[e][0] = w.x;
-        vt.x[e][1] = w.y;
-      } else {
+  for (int e = 0; e < 8; ++e) {
+    const char* row = base + (tok0 + 8 * (g & 1) + e) * (D * 2) + n * (VL * 2);
+    if constexpr (VL == 4) {
+      const uint2 w = *reinterpret_cast<const uint2*>(row);
+      vt.x[e][0] = w.x;
+      vt.x[e][1] = w.y;
+    } else {
 #pragma unroll
-        for (int i = 0; i < VL / 8; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * i);
-          vt.x[e][4 * i] = w.x;
-          vt.x[e][4 * i + 1] = w.y;
-          vt.x[e][4 * i + 2] = w.z;
-          vt.x[e][4 * i + 3] = w.w;
-        }
+      for (int i = 0; i < VL / 8; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * i);
+        vt.x[e][4 * i] = w.x;
+        vt.x[e][4 * i + 1] = w.y;
+        vt.x[e][4 * i + 2] = w.z;
+        vt.x[e][4 * i + 3] = w.w;
       }
     }
-  } else {
-    const char* run = base + ((tok0 + key) >> 3) * (4 * D) + n * (VL * 4);    // 8 keys x VL / 2 bytes
-#pragma unroll
-    for (int i = 0; i < VL / 4; ++i) {
-      const uint4 w = *reinterpret_cast<const uint4*>(run + 16 * i);
-      vt.c[4 * i] = w.x;
-      vt.c[4 * i + 1] = w.y;
-      vt.c[4 * i + 2] = w.z;
-      vt.c[4 * i + 3] = w.w;
-    }
-    const uint8_t* sc = pg.vs + id * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales +
-                        ((tok0 + key) >> 3) * (D / 4) + (n * VL / 32) * 8;
-    vt.sc = *reinterpret_cast<const uint2*>(sc);
   }
 }
 
-// The 32-deep step s of key half kb as an MFMA operand.
+// 4 bits: a wave's ring of tiles in LDS, as they lie in memory: 32 keys' codes (16 D bytes), their values' (16 D), the keys'
+// scales (D) and the values' (D; 256 bytes for both at least, as their loads write).
+template <int D>
+struct Ring {
+  static constexpr int R = 4;                                // tiles
+  static constexpr int SLOT = 32 * D + (D < 128 ? 256 : 2 * D);
+  static constexpr int L = D == 64 ? 3 : D == 128 ? 5 : 10;  // load instructions a tile
+  static constexpr int BYTES = R * SLOT + 256;               // and the coming window's table entries
+};
+
+template <int D>
+__device__ __forceinline__ void read_k(KTile<D, true>& kt, const char* slot, int n, int g) {
+  const int gd = D == 64 ? g & 1 : g;                        // (head_dim 64: lanes of d past 64 repeat; their queries are zero)
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int s = 0; s < (D == 256 ? 2 : 1); ++s) {
+      const uint4 w = *reinterpret_cast<const uint4*>(slot + (8 * (n >> 2) + 4 * kb + (n & 3)) * (D / 2) + s * 64 + gd * 16);
+      kt.c[kb][4 * s] = w.x;
+      kt.c[kb][4 * s + 1] = w.y;
+      kt.c[kb][4 * s + 2] = w.z;
+      kt.c[kb][4 * s + 3] = w.w;
+    }
+#pragma unroll
+  for (int s = 0; s < (D == 256 ? 2 : 1); ++s)
+    kt.sc[s] = *reinterpret_cast<const uint2*>(slot + 32 * D + (n >> 2) * (D / 4) + (4 * s + gd) * 8);
+}
+
+template <int D>
+__device__ __forceinline__ void read_v(VTile<D, true>& vt, const char* slot, int n, int g) {
+  constexpr int VL = D / 16;
+  const char* run = slot + 16 * D + g * (4 * D) + n * (VL * 4);         // 8 keys x VL / 2 bytes
+#pragma unroll
+  for (int i = 0; i < VL / 4; ++i) {
+    const uint4 w = *reinterpret_cast<const uint4*>(run + 16 * i);
+    vt.c[4 * i] = w.x;
+    vt.c[4 * i + 1] = w.y;
+    vt.c[4 * i + 2] = w.z;
+    vt.c[4 * i + 3] = w.w;
+  }
+  vt.sc = *reinterpret_cast<const uint2*>(slot + 33 * D + g * (D / 4) + (n * VL / 32) * 8);
+}
+
+// Loads from memory into LDS (64 lanes side by side from lds on), without destination registers: the kernel's own waits
+// order them. (As builtins the compiler makes every LDS read wait for all of them. M0 has no other use in this kernel.)
+__device__ __forceinline__ void to_lds16(uint32_t lds, const char* base, uint32_t off) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint64_t s = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)))) << 32 |
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(off), "s"(s) : "memory");
+}
+__device__ __forceinline__ void to_lds16(uint32_t lds, const char* at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(at) : "memory");
+}
+__device__ __forceinline__ void to_lds4(uint32_t lds, const void* at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(at) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// A tile into the slot at lds: its 16-key halves' codes lie o0, o1 bytes into the pools (keys' rows and values' runs alike), their
+// scales s0, s1.
+template <int D>
+__device__ __forceinline__ void issue_tile(uint32_t lds, const PagesDev& pg, int64_t o0, int64_t o1, int64_t s0, int64_t s1, int lane) {
+  if constexpr (D == 64) {                                   // 512 bytes a half: lanes 0 .. 31 and 32 .. 63
+    const int64_t o = (lane < 32 ? o0 : o1) + (lane & 31) * 16;
+    to_lds16(lds, pg.k + o);
+    to_lds16(lds + 1024, pg.v + o);
+  } else {
+    constexpr int I = D / 128;                               // 1 KB instructions a half
+    const uint32_t off = 16 * lane;
+#pragma unroll
+    for (int x = 0; x < I; ++x) {
+      to_lds16(lds + 1024 * x, pg.k + o0 + 1024 * x, off);
+      to_lds16(lds + 1024 * (I + x), pg.k + o1 + 1024 * x, off);
+      to_lds16(lds + 1024 * (2 * I + x), pg.v + o0 + 1024 * x, off);
+      to_lds16(lds + 1024 * (3 * I + x), pg.v + o1 + 1024 * x, off);
+    }
+  }
+  constexpr int H = D / 8;                                   // dwords of a half's scales
+  if constexpr (D == 256) {
+    const int64_t s = (lane < 32 ? s0 : s1) + (lane & 31) * 4;
+    to_lds4(lds + 32 * D, pg.ks + s);
+    to_lds4(lds + 33 * D, pg.vs + s);
+  } else {                                                   // keys' halves, values' halves; past them they are repeated
+    const int part = (lane / H) & 3;
+    const int64_t s = ((part & 1) ? s1 : s0) + (lane % H) * 4;
+    to_lds4(lds + 32 * D, (part & 2) ? pg.vs + s : pg.ks + s);
+  }
+}
+
+// A row block's queries as the products' operands. bf16: 32-deep steps. 4 bits: the matrix instruction takes codes and scales
+// as they are when the other side has 8 bits, so a query's 32 values are split as q = 2^e (hi + lo / 16) with hi, lo in E4M3
+// (4 significant bits each, a bf16 value has 8) and 128 <= max |q| / 2^e < 256: exact for values down to 2^-14 of
+// the largest of their 32, and off by less than 2^-22 of that below. An operand holds d 128 s + 16 g .. + 15 and 64 more
+// on in its two halves.
 template <int D, bool MX>
-__device__ __forceinline__ bf16x8 k_frag(const KTile<D, MX>& kt, const float (&scale)[2][2], int kb, int s) {
-  if constexpr (!MX) return as_frag(kt.x[kb][s]);
-  const uint32_t w = kt.c[kb][s];
-  const float f = scale[kb][D == 256 ? s / 4 : 0];
-  return as_frag(make_uint4(fp4_pair<0>(w, f), fp4_pair<1>(w, f), fp4_pair<2>(w, f), fp4_pair<3>(w, f)));
+struct Queries {
+  bf16x8 x[MX ? 1 : D / 32];
+  i32x8 hi[MX ? (D == 256 ? 2 : 1) : 1], lo[MX ? (D == 256 ? 2 : 1) : 1];
+  int eh[MX ? (D == 256 ? 2 : 1) : 1], el[MX ? (D == 256 ? 2 : 1) : 1];       // scale bytes of block 4 s + g
+};
+
+__device__ __forceinline__ uint32_t fp8x4(float a, float b, float c, float d) {
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+
+template <int D>
+__device__ __forceinline__ void load_queries(Queries<D, true>& q, const uint16_t* row, int g, int lane) {
+#pragma unroll
+  for (int s = 0; s < (D == 256 ? 2 : 1); ++s) {
+    int e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};              // 16 values
+      if (D > 64 || h == 0) {
+        const uint4 a = *reinterpret_cast<const uint4*>(row + 128 * s + 64 * h + 16 * g);
+        const uint4 b = *reinterpret_cast<const uint4*>(row + 128 * s + 64 * h + 16 * g + 8);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+      }
+      int top = 0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) top = max(top, max(static_cast<int>(w[x] & 0x7fffu), static_cast<int>((w[x] >> 16) & 0x7fffu)));
+      top = max(top, __shfl_xor(top, 16, 64));               // of the block of 32
+      const bool odd = top >= 0x7f80;                        // a NaN or an infinity: the block is NaN
+      e[h] = min(max(top >> 7, 20), 254) - 7;                // biased; tiny values keep a scale in range
+      const float up = __uint_as_float(static_cast<uint32_t>(254 - e[h]) << 23);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float v0 = bf_lo(w[2 * x]) * up, v1 = bf_hi(w[2 * x]) * up, v2 = bf_lo(w[2 * x + 1]) * up, v3 = bf_hi(w[2 * x + 1]) * up;
+        const uint32_t hi = fp8x4(v0, v1, v2, v3);
+        const auto h01 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), h23 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+        const uint32_t lo = fp8x4((v0 - h01[0]) * 16.f, (v1 - h01[1]) * 16.f, (v2 - h23[0]) * 16.f, (v3 - h23[1]) * 16.f);
+        q.hi[s][4 * h + x] = odd ? 0x7f7f7f7f : hi;
+        q.lo[s][4 * h + x] = odd ? 0x7f7f7f7f : lo;
+      }
+    }
+    // block 4 s + g's scale: d 32 g .. are the first halves of lanes 2 g, 2 g + 1 for g < 2, else second halves
+    const int from = (lane & 15) + 32 * (g & 1), e0 = __shfl(e[0], from, 64), e1 = __shfl(e[1], from, 64);
+    q.eh[s] = g < 2 ? e0 : e1;
+    q.el[s] = q.eh[s] - 4;
+  }
 }
 
 __device__ __forceinline__ float byte_scale(const uint2& w, int i) {       // i in 0 .. 7, known when inlined or not
@@ -337,24 +502,24 @@ __device__ __forceinline__ float inverse_sum(float sum) {    // no key seen: zer
   return sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
 }
 
-// N columns from d0 of row r of a row block (query q0 + r / rep): the output, or the partial of a split.
+// N columns from d0 of row r of a 16-row block that begins at head off of row `first` of q: the output, or a part's partial.
 template <int D, int N>
-__device__ __forceinline__ void finish_row(const PagedArgs& a, const Unit& u, int64_t part, int rpb, int r, int head, int q0,
+__device__ __forceinline__ void finish_row(const PagedArgs& a, int first, int off, bool whole, int64_t part, int r, int head,
                                            int d0, const float (&acc)[N], float top, float sum) {
-  if (u.ns > 1) {
-    float* p = a.part + part * (static_cast<int64_t>(rpb) * (D + 2));
+  if (!whole) {
+    float* p = a.part + part * (16 * (D + 2));
 #pragma unroll
     for (int b = 0; b < N; b += 4)
       *reinterpret_cast<float4*>(p + r * D + d0 + b) = make_float4(acc[b], acc[b + 1], acc[b + 2], acc[b + 3]);
     if (d0 == 0) {
-      p[rpb * D + r] = top;
-      p[rpb * (D + 1) + r] = sum;
+      p[16 * D + r] = top;
+      p[16 * (D + 1) + r] = sum;
     }
     return;
   }
   const float inv = inverse_sum(sum);
-  const int qi = r / a.rep;
-  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + d0;
+  const int qi = (off + r) / a.rep;
+  uint16_t* dst = a.out + static_cast<int64_t>(first + qi) * a.ldo + (head * a.rep + off + r - qi * a.rep) * D + d0;
 #pragma unroll
   for (int b = 0; b < N; b += 4)
     *reinterpret_cast<uint2*>(dst + b) =
@@ -373,12 +538,12 @@ struct Tile {
   uint32_t bad;                            // bits: a 16-key half on a page that is none
 };
 
-// The wave's running state: O [rows 16 mt + 4 g + j][d = n NB + b], and of row 16 mt + n the reference maximum m (raw
+// The wave's running state: O [rows 4 g + j][d = n NB + b], and of row n the reference maximum m (raw
 // scores; the same in the four lanes of a row) and the lane's share of the row sum.
-template <int D, int MT>
+template <int D>
 struct Rows {
-  f32x4 o[MT][D / 16];
-  float m[MT], l[MT];
+  f32x4 o[D / 16];
+  float m, l;
 };
 
 __device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // with zeros for the halves that are NaN or infinite
@@ -400,36 +565,32 @@ __device__ __forceinline__ void v_frags(const VTile<D, MX>& vt, const float (&vs
 }
 
 // What a row meets of V that is not finite, kept apart from the products (there, 0 x infinity would reach rows that do not
-// see the key): marks of (row, column), one byte each (1 infinity, 2 -infinity, 4 NaN).
+// see the key): marks of (row, column), two bits each (1 infinity, 2 -infinity, 3 NaN, also of both).
 __device__ __forceinline__ uint32_t mark_of(uint32_t half) {
-  return (half & 0x7f80u) != 0x7f80u ? 0u : (half & 0x7fu) ? 4u : (half & 0x8000u) ? 2u : 1u;
+  return (half & 0x7f80u) != 0x7f80u ? 0u : (half & 0x7fu) ? 3u : (half & 0x8000u) ? 2u : 1u;
 }
 
-__device__ __forceinline__ float marked(uint32_t m) {
-  return (m & 4u) || (m & 3u) == 3u ? NAN : (m & 1u) ? INFINITY : (m & 2u) ? -INFINITY : 0.f;
-}
+__device__ __forceinline__ float marked(uint32_t m) { return m == 3u ? NAN : m == 1u ? INFINITY : m == 2u ? -INFINITY : 0.f; }
 
-// S^T of a tile: sc[mt][kb][j] = the raw score of key 8 g + 4 kb + j for query row 16 mt + n.
-template <int D, bool MX, int MT>
-__device__ __forceinline__ void scores(const KTile<D, MX>& kt, const bf16x8 (&qf)[MT][D / 32], f32x4 (&sc)[MT][2], int n) {
-  constexpr int NS = D / 32;
-  float ks[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  if constexpr (MX) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
-        ks[kb][x] = __uint_as_float((((kb ? kt.sc[x].y : kt.sc[x].x) >> (8 * (n & 3))) & 255u) << 23);
-  }
+// S^T of a tile: sc[kb][j] = the raw score of key 8 g + 4 kb + j for query row n.
+template <int D, bool MX>
+__device__ __forceinline__ void scores(const KTile<D, MX>& kt, const Queries<D, MX> &qf, f32x4 (&sc)[2], int n) {
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
+    sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (MX) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < (D == 256 ? 2 : 1); ++s) {
+        const i32x8 k = {static_cast<int>(kt.c[kb][4 * s]), static_cast<int>(kt.c[kb][4 * s + 1]), static_cast<int>(kt.c[kb][4 * s + 2]),
+                         static_cast<int>(kt.c[kb][4 * s + 3]), 0, 0, 0, 0};
+        const int e = static_cast<int>((kb ? kt.sc[s].y : kt.sc[s].x) >> (8 * (n & 3)));        // (its low byte counts)
+        sc[kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qf.lo[s], sc[kb], 4, 0, 0, e, 0, qf.el[s]);
+        sc[kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qf.hi[s], sc[kb], 4, 0, 0, e, 0, qf.eh[s]);
+      }
+    } else {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const bf16x8 kf = k_frag<D, MX>(kt, ks, kb, s);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sc[mt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[mt][s], sc[mt][kb], 0, 0, 0);
+      for (int s = 0; s < D / 32; ++s)
+        sc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_frag(kt.x[kb][s]), qf.x[s], sc[kb], 0, 0, 0);
     }
   }
 }
@@ -438,20 +599,20 @@ __device__ __forceinline__ float lane_max(const f32x4 (&s)[2]) {
   return fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
 }
 
-// Raise row block mt's reference maxima to what its rows' four lanes have seen (tmax), and rescale their sums and O.
-template <int D, int MT>
-__device__ __forceinline__ void raise(Rows<D, MT>& st, int mt, float tmax, float c, int g) {
+// Raise the reference maxima to what the rows' four lanes have seen (tmax), and rescale their sums and O.
+template <int D>
+__device__ __forceinline__ void raise(Rows<D>& st, float tmax, float c, int g) {
   tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
   tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-  const float top = fmaxf(st.m[mt], tmax);
-  const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[mt] - top) * c);
-  st.m[mt] = top;
-  st.l[mt] *= alpha;
+  const float top = fmaxf(st.m, tmax);
+  const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m - top) * c);
+  st.m = top;
+  st.l *= alpha;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float al = __shfl(alpha, 4 * g + j, 64);           // O's rows of a lane are 4 g + j
 #pragma unroll
-    for (int b = 0; b < D / 16; ++b) st.o[mt][b][j] *= al;
+    for (int b = 0; b < D / 16; ++b) st.o[b][j] *= al;
   }
 }
 
@@ -468,8 +629,8 @@ __device__ __forceinline__ bf16x8 probabilities(const f32x4 (&s)[2], float m, fl
 }
 
 // O += P V. CUT: as v_frags.
-template <int D, bool MX, int MT, bool CUT>
-__device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 (&pf)[MT], int last, Rows<D, MT>& st) {
+template <int D, bool MX, bool CUT>
+__device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf, int last, Rows<D>& st) {
   float vs[8];
   if constexpr (MX) {
 #pragma unroll
@@ -478,37 +639,31 @@ __device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 (&p
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
     bf16x8 f0, f1;
+    if constexpr (CUT) __builtin_amdgcn_sched_barrier(0);    // (all pairs at once would not fit the registers)
     v_frags<D, MX, CUT>(vt, vs, j, last, f0, f1);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      st.o[mt][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f0, st.o[mt][2 * j], 0, 0, 0);
-      st.o[mt][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[mt], f1, st.o[mt][2 * j + 1], 0, 0, 0);
-    }
+    st.o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, st.o[2 * j], 0, 0, 0);
+    st.o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, st.o[2 * j + 1], 0, 0, 0);
   }
 }
 
 // A tile of which some row does not see some key. Keys are hidden from rows by their scores (-infinity); of V, what no row
 // sees and what is not finite enters the product as zero, and the latter leaves its marks in the rows that see it.
-template <int D, bool MX, int MT>
-__device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const bf16x8 (&qf)[MT][D / 32], const int (&pos)[MT],
-                                          Rows<D, MT>& st, float c, int p0, int plast, int rep, int lane, uint32_t* marks) {
+template <int D, bool MX>
+__device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D, MX> &qf, int pos,
+                                          Rows<D>& st, float c, int p0, int plast, const RowBlock& rows, int rep, int lane, uint32_t* marks) {
   constexpr int NB = D / 16;
   const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
-  f32x4 sc[MT][2];
-  scores<D, MX, MT>(tl.k, qf, sc, n);
+  f32x4 sc[2];
+  scores<D, MX>(tl.k, qf, sc, n);
   const bool hidden = (tl.bad >> (g >> 1)) & 1u;             // the lane's 8 keys lie on a page that is none
-  bf16x8 pf[MT];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (hidden || k0 + 8 * g + 4 * kb + j > pos[mt]) sc[mt][kb][j] = -INFINITY;
-    const float tmax = lane_max(sc[mt]);
-    if (__any(tmax > st.m[mt] + RESCALE_LOG2 / c)) raise<D, MT>(st, mt, tmax, c, g);
-    pf[mt] = probabilities(sc[mt], st.m[mt], c, st.l[mt]);
-  }
+    for (int j = 0; j < 4; ++j)
+      if (hidden || k0 + 8 * g + 4 * kb + j > pos) sc[kb][j] = -INFINITY;
+  const float tmax = lane_max(sc);
+  if (__any(tmax > st.m + RESCALE_LOG2 / c)) raise<D>(st, tmax, c, g);
+  const bf16x8 pf = probabilities(sc, st.m, c, st.l);
   const int last = hidden ? -1 : plast - k0 - 8 * g;         // of the lane's keys, the last that any row sees
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -522,179 +677,282 @@ __device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const bf16x8 (&
         two = tl.v.x[e][j];
       }
       if (e <= last && not_finite(two)) {
-        const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 8;
-        const int first = max(0, k0 + 8 * g + e - p0) * rep;            // rows from the key's own query on
-        for (int r = first; r < min(16 * MT, (plast - p0 + 1) * rep); ++r) {
-          if constexpr (MX) {
-#pragma unroll
-            for (int x = 0; x < NB / 4; ++x) atomicOr(marks + (r * D + n * NB) / 4 + x, 0x04040404u);
-          } else {
-            atomicOr(marks + (r * D + n * NB + 2 * j) / 4, m2 << (j & 1 ? 16 : 0));
-          }
+        const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 2;
+        const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);          // rows from the key's own query on
+        for (int r = first; r < rows.rows; ++r) {
+          const int at = r * D + n * NB + 2 * j;             // 16 columns a word; the lane's NB lie in one
+          atomicOr(marks + at / 16, (MX ? static_cast<uint32_t>((1ull << (2 * NB)) - 1) : m2) << (2 * (at % 16)));
         }
-        marks[4 * MT * D] = 1u;
+        marks[D] = 1u;
       }
     }
   }
-  product<D, MX, MT, true>(tl.v, pf, last, st);
+  product<D, MX, true>(tl.v, pf, last, st);
 }
 
-// Blocks a CU that the registers of a kernel hold.
-constexpr int few_blocks(int d, bool mx, int mt) {
-  return d == 64 ? (mt <= 2 ? 3 : mt == 3 ? 2 : 1) : d == 128 ? (mt == 1 && mx ? 3 : mt <= 2 ? 2 : 1) : 1;
-}
+// Blocks a CU that the registers of a kernel hold (4 bits: and its rings the LDS).
+constexpr int few_blocks(int d) { return d == 256 ? 1 : 2; }
 
-template <int D, bool MX, int MT>
-__global__ __launch_bounds__(64 * NW, (few_blocks(D, MX, MT))) void k_paged_few(PagedArgs a) {
-  constexpr int NS = D / 32, NB = D / 16;
-  __shared__ float lds[merge_floats<D>() + 4 * MT * D + 1];
+template <int D, bool MX>
+struct FewLds {
+  static constexpr int RINGS = MX ? NW * Ring<D>::BYTES : 0;
+  static constexpr int MARKS = RINGS > merge_floats<D>() * 4 ? RINGS : merge_floats<D>() * 4;   // (the merge takes the rings' place)
+  static constexpr int BYTES = MARKS + 4 * D + 16;
+};
+
+template <int D, bool MX>
+__global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArgs a) {
+  constexpr int NB = D / 16;
+  using F = FewLds<D, MX>;
+  __shared__ uint4 lds4[F::BYTES / 16];
+  float* lds = reinterpret_cast<float*>(lds4);
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 15, g = lane >> 4;
-  const int head = blockIdx.x % a.hkv;
-  const Unit u = find_unit(a, blockIdx.x / a.hkv, false);
-  if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
-  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0); // the block's queries
-  const int p0 = u.s.keys - u.s.rows + q0;                   // position of the first of them (may lie before 0)
-  const int plast = p0 + nq - 1;                             // keys 0 .. plast are read
-  const int ntiles = plast < 0 ? 0 : plast / KT + 1;
-  const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);  // (it0 < 2^31: ns W is below tiles + W)
-
-  // The wave's tiles are it0 + w + NW i, i < mine. Lane l holds the page of 16-key half l % 2 of tile i0 + l / 2 of a window
-  // of 32 tiles (0 for pages that are none, whose keys `bad` then hides), and the next window's entry on its way.
-  const int mine = it0 + w < it1 ? (it1 - it0 - w + NW - 1) / NW : 0;
-  const int32_t* row = a.table + static_cast<int64_t>(u.b) * a.ld_table;
-  auto entry = [&](int i0) {
-    const int it = it0 + w + NW * (i0 + (lane >> 1));
-    const int at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
-    return it < it1 && at < a.width ? row[at] : -1;
-  };
-  int ids = entry(0), coming = entry(32);
-  uint64_t bad;
-  auto settle = [&]() {
-    const bool out = ids < 0 || ids >= a.pg.n_pages;
-    ids = out ? 0 : ids;
-    bad = __ballot(out);
-  };
-  settle();
-  const int mask = (1 << a.pg.shift) - 1;
-  auto window = [&](int i) {                                 // before the loads of tile i
-    if ((i & 31) == 0) {
-      ids = coming;
-      settle();
-      coming = entry(i + 32);
-    }
-  };
-  auto get_k = [&](Tile<D, MX>& tl, int i) {                 // i < mine; windows in order
-    const int x = 2 * (i & 31), id0 = __builtin_amdgcn_readlane(ids, x), id1 = __builtin_amdgcn_readlane(ids, x + 1);
-    const int k0 = (it0 + w + NW * i) * KT;
-    load_k<D, MX>(tl.k, a.pg, n >= 8 ? id1 : id0, head, (k0 + (n >= 8 ? 16 : 0)) & mask, n, g);
-  };
-  auto get_v = [&](Tile<D, MX>& tl, int i) {
-    const int x = 2 * (i & 31), id0 = __builtin_amdgcn_readlane(ids, x), id1 = __builtin_amdgcn_readlane(ids, x + 1);
-    tl.k0 = (it0 + w + NW * i) * KT;
-    tl.bad = static_cast<uint32_t>(bad >> x) & 3u;
-    load_v<D, MX>(tl.v, a.pg, g >= 2 ? id1 : id0, head, (tl.k0 + (g >= 2 ? 16 : 0)) & mask, n, g);
-  };
-
-  constexpr int NT = MX || D == 64 ? 2 : 1;                  // tiles at once
-  Tile<D, MX> tl[NT];
-  if (mine) {
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      get_k(tl[x], min(x, mine - 1));
-      get_v(tl[x], min(x, mine - 1));
-    }
-  }
-  uint32_t* marks = reinterpret_cast<uint32_t*>(lds + merge_floats<D>());
-  for (int x = t; x <= 4 * MT * D; x += 64 * NW) marks[x] = 0u;
+  // (heads slowest: the blocks of an XCD then read all heads' parts of the pages. With heads fastest and 8 of them each XCD
+  // reads one head's, which all lie at the same offset of a page, and in 4 bits, 4 KB of 32, 4 % slower)
+  const int blocks = gridDim.x / a.hkv, head = blockIdx.x / blocks, mask = (1 << a.pg.shift) - 1;
+  uint32_t* marks = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(lds4) + F::MARKS);
+  for (int x = t; x <= D; x += 64 * NW) marks[x] = 0u;
   __syncthreads();
-  // queries: row 16 mt + n
-  bf16x8 qf[MT][NS];
-  int pos[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = 16 * mt + n, qi = r / a.rep;
-    const bool live = qi < nq;
-    pos[mt] = live ? p0 + qi : -1;
-    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + q0 + (live ? qi : 0)) * a.ldq +
-                           (head * a.rep + (live ? r - qi * a.rep : 0)) * D;
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-      qf[mt][s] = as_frag(*reinterpret_cast<const uint4*>(qrow + (MX ? g * (D / 4) + 8 * s : 32 * s + 8 * g)));
+  Seq s0{0, 0, 0};
+  if (lane < a.n_seq) s0 = seq_of(a, lane);
+  // the block's run of tiles [at, end), or (unsplit) its row block
+  const int x0 = blockIdx.x - head * blocks;
+  int at = 0, end = 1, run = 0;
+  if (a.fit) {
+    int total;
+    run = run_length(a, s0, lane, total);
+    at = x0 * run;
+    end = min(total, at + run);
+    if (blockIdx.x == 0 && t == 0) *a.length = run;          // for the merge
   }
-  Rows<D, MT> st;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    st.m[mt] = -INFINITY;
-    st.l[mt] = 0.f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) st.o[mt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  // Whole tiles first (NT at once; the keys' registers are reloaded behind the scores, the values' behind the product, so
-  // that loads are always in flight), then the tiles that some row sees in part; from the first page that is none on all of
-  // them are taken as such. A maximum that has to rise leaves the inner loop: with the rescale inside it the compiler moves
-  // all of O at every tile (16 to 48 rows of head_dim 256 in 4 bits). Tiles past the last are loaded as the last one again:
-  // no load of the loop is conditional.
-  const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
-  int i = 0;
-  bool none = false;
-  while (!none && i + NT <= whole) {
-    f32x4 sc[NT][MT][2];
-    float tmax[MT];
-    for (; i + NT <= whole; i += NT) {
-      uint32_t bads = 0;
-#pragma unroll
-      for (int x = 0; x < NT; ++x) bads |= tl[x].bad;
-      none = bads != 0;
-      if (none) break;
-      bool up = false;
-#pragma unroll
-      for (int x = 0; x < NT; ++x) scores<D, MX, MT>(tl[x].k, qf, sc[x], n);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        tmax[mt] = lane_max(sc[0][mt]);
-        if constexpr (NT > 1) tmax[mt] = fmaxf(tmax[mt], lane_max(sc[NT - 1][mt]));
-        up |= tmax[mt] > st.m[mt] + RESCALE_LOG2 / a.c;
-      }
-      if (__any(up)) break;
-      const int i1 = min(i + NT, mine - 1);
-      if (i1 == i + NT) window(i1);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) get_k(tl[x], min(i1 + x, mine - 1));
-      bf16x8 pf[NT][MT];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) pf[x][mt] = probabilities(sc[x][mt], st.m[mt], a.c, st.l[mt]);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) product<D, MX, MT, false>(tl[x].v, pf[x], 8, st);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) get_v(tl[x], min(i1 + x, mine - 1));
-    }
-    if (!none && i + NT <= whole) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) raise<D, MT>(st, mt, tmax[mt], a.c, g);
-    }
-  }
-  for (; i < mine; ++i) {
-    edge_step<D, MX, MT>(tl[0], qf, pos, st, a.c, p0, plast, a.rep, lane, marks);
-    if (i + 1 < mine) {
-      window(i + 1);
-      get_k(tl[0], i + 1);
-      get_v(tl[0], i + 1);
-    }
-  }
+  for (bool once = true; at < end; once = false) {           // (uniform over the block)
+    const Piece u = a.fit ? piece_at(a, s0, at, false, lane) : piece_at(a, s0, x0, true, lane);
+    if (u.b < 0) return;
+    const int it0 = u.t0, itn = a.fit ? min(u.nt, it0 + end - at) : u.nt;
+    const bool whole_block = it0 == 0 && itn == u.nt;
+    const int64_t part = static_cast<int64_t>(2 * x0 + (once ? 0 : 1)) * a.hkv + head;    // (only the first and last pieces are parts)
+    at += a.fit ? itn - it0 : 1;
+    const RowBlock r(a, u.s, u.rb);
+    const int p0 = u.s.keys - u.s.rows + r.q0;                 // position of its first query (may lie before 0)
+    const int plast = p0 + (r.off + r.rows - 1) / a.rep;       // keys 0 .. plast are read
+    const int it1 = min(itn, plast < 0 ? 0 : plast / KT + 1);
 
-  // merge the waves: thread t takes row t / 16 of each 16 rows and D / 16 columns
-  const int64_t part = (u.part + static_cast<int64_t>(u.sp) * u.nrb) * a.hkv + head;
-  float* ml = lds + NW * 16 * (D + 4);
+    // The wave's tiles are it0 + w + NW i, i < mine. Lane l holds the page of 16-key half l % 2 of tile i0 + l / 2 of a window
+    // of 32 tiles (0 for pages that are none, whose keys `bad` then hides), and the next window's entry on its way.
+    const int mine = it0 + w < it1 ? (it1 - it0 - w + NW - 1) / NW : 0;
+    const int32_t* row = a.table + static_cast<int64_t>(u.b) * a.ld_table;
+    auto entry = [&](int i0) {
+      const int it = it0 + w + NW * (i0 + (lane >> 1));
+      const int at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
+      return it < it1 && at < a.width ? row[at] : -1;
+    };
+    int ids = entry(0);
+    [[maybe_unused]] int coming = MX ? 0 : entry(32);
+    uint64_t bad;
+    auto settle = [&]() {
+      const bool out = ids < 0 || ids >= a.pg.n_pages;
+      ids = out ? 0 : ids;
+      bad = __ballot(out);
+    };
+    settle();
+    // queries: row n
+    Queries<D, MX> qf;
+    int pos;
+    auto queries = [&]() {
+      const int x = r.off + min(n, r.rows - 1), qi = x / a.rep;            // (rows past the last repeat it, and see nothing)
+      pos = n < r.rows ? p0 + qi : -1;
+      const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + r.q0 + qi) * a.ldq + (head * a.rep + x - qi * a.rep) * D;
+      if constexpr (MX) {
+        load_queries<D>(qf, qrow, g, lane);
+      } else {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    if (mt) __syncthreads();
-    float ls = st.l[mt];
+        for (int s = 0; s < D / 32; ++s) qf.x[s] = as_frag(*reinterpret_cast<const uint4*>(qrow + 32 * s + 8 * g));
+      }
+    };
+    Rows<D> st;
+    st.m = -INFINITY;
+    st.l = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Whole tiles first, then the tiles that some row sees in part; from the first page that is none on all of them are taken as
+    // such. A maximum that has to rise leaves the inner loop: with the rescale inside it the compiler moves all of O at every tile.
+    const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
+    int i = 0;
+    bool none = false;
+    if constexpr (MX) {
+      // Tiles come through the wave's ring, two a turn. (A wave that loaded its next two tiles into
+      // registers behind their last use had one product's time for a latency of 2 us: 8500 cycles a turn at head_dim 256 for 3000
+      // of work; one 122880-key sequence took 23 us.)
+      using G = Ring<D>;
+      char* ring = reinterpret_cast<char*>(lds4) + w * G::BYTES;
+      const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring));
+      uint32_t bads = 0;                                       // two bits a slot
+      // a lane's entry as byte offsets of its half's codes and scales, once a window
+      int64_t code_at = 0, scale_at = 0;
+      auto place = [&](int i0) {
+        const int tok = ((it0 + w + NW * (i0 + (lane >> 1))) * KT + 16 * (lane & 1)) & mask;
+        code_at = ids * a.pg.page_stride + static_cast<int64_t>(head) * a.pg.head_bytes + tok * (D / 2);
+        scale_at = ids * a.pg.scale_stride + static_cast<int64_t>(head) * a.pg.head_scales + (tok >> 3) * (D / 4);
+      };
+      auto lane64 = [](int64_t v, int l) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+      };
+      place(0);
+      auto fetch_entries = [&](int i0) {                       // table entries of the window that begins at tile i0
+        const int at = ((it0 + w + NW * (i0 + (lane >> 1))) * 2 + (lane & 1)) >> (a.pg.shift - 4);
+        to_lds4(ring_at + G::R * G::SLOT, row + min(at, a.width - 1));
+      };
+      int slot_in = 0, slot_out = 0;                           // of the tile issued next, and of tile i
+      auto issue = [&](int x) {                                // tile x < mine, in order; its slot's reads have returned
+        if ((x & 31) == 0 && x) {
+          const int it = it0 + w + NW * (x + (lane >> 1)), at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
+          ids = reinterpret_cast<const int32_t*>(ring + G::R * G::SLOT)[lane];     // landed 28 tiles ago
+          wait_lds_reads();
+          ids = it < it1 && at < a.width ? ids : -1;
+          settle();
+          place(x);
+          fetch_entries(x + 32);
+        }
+        const int y = 2 * (x & 31);
+        bads = (bads & ~(3u << (2 * slot_in))) | (static_cast<uint32_t>(bad >> y) & 3u) << (2 * slot_in);
+        issue_tile<D>(ring_at + slot_in * G::SLOT, a.pg, lane64(code_at, y), lane64(code_at, y + 1), lane64(scale_at, y),
+                      lane64(scale_at, y + 1), lane);
+        slot_in = slot_in + 1 == G::R ? 0 : slot_in + 1;
+      };
+      if (mine) {
+        fetch_entries(32);
+        for (int x = 0; x < min(mine, G::R); ++x) issue(x);
+      }
+      queries();                                               // (behind the tiles: they land in order)
+      // tiles up to x + 1 (x) have landed: the newer ones are those issued after them
+      auto landed = [&](int x, bool two) {
+        if (x + G::R > mine) wait_loads<0>();
+        else if (two) wait_loads<G::L * (G::R - 2)>();
+        else wait_loads<G::L * (G::R - 1)>();
+      };
+      while (!none && i + 2 <= whole) {
+        f32x4 sc[2][2];
+        float tmax;
+        for (; i + 2 <= whole; i += 2) {
+          const int slot_next = slot_out + 1 == G::R ? 0 : slot_out + 1;
+          const char* const slots[2] = {ring + slot_out * G::SLOT, ring + slot_next * G::SLOT};
+          none = (((bads >> (2 * slot_out)) | (bads >> (2 * slot_next))) & 3u) != 0;
+          if (none) break;
+          landed(i, true);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            KTile<D, true> kt;
+            read_k<D>(kt, slots[x], n, g);
+            scores<D, true>(kt, qf, sc[x], n);
+          }
+          tmax = fmaxf(lane_max(sc[0]), lane_max(sc[1]));
+          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const bf16x8 pf = probabilities(sc[x], st.m, a.c, st.l);
+            VTile<D, true> vt;
+            read_v<D>(vt, slots[x], n, g);
+            product<D, true, false>(vt, pf, 8, st);
+          }
+          wait_lds_reads();
+          slot_out = slot_next + 1 == G::R ? 0 : slot_next + 1;
+          if (i + G::R < mine) issue(i + G::R);
+          if (i + G::R + 1 < mine) issue(i + G::R + 1);
+        }
+        if (!none && i + 2 <= whole) raise<D>(st, tmax, a.c, g);
+      }
+      for (; i < mine; ++i) {
+        landed(i, false);
+        const char* slot = ring + slot_out * G::SLOT;
+        Tile<D, true> tl;
+        read_k<D>(tl.k, slot, n, g);
+        read_v<D>(tl.v, slot, n, g);
+        tl.k0 = (it0 + w + NW * i) * KT;
+        tl.bad = (bads >> (2 * slot_out)) & 3u;
+        edge_step<D, true>(tl, qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
+        wait_lds_reads();
+        slot_out = slot_out + 1 == G::R ? 0 : slot_out + 1;
+        if (i + G::R < mine) issue(i + G::R);
+      }
+      wait_loads<0>();                                         // nothing in flight into the rings:
+      __syncthreads();                                         // the merge takes their place
+    } else {
+      // A tile takes D / 2 registers: one (two at head_dim 64), the keys' reloaded behind the scores and the values' behind the
+      // product. Tiles past the last are loaded as the last one again: no load of the loop is conditional.
+      constexpr int NT = D == 64 ? 2 : 1;
+      auto window = [&](int x) {                               // before the loads of tile x
+        if ((x & 31) == 0) {
+          ids = coming;
+          settle();
+          coming = entry(x + 32);
+        }
+      };
+      auto get_k = [&](Tile<D, false>& tl, int x) {            // x < mine; windows in order
+        const int y = 2 * (x & 31), id0 = __builtin_amdgcn_readlane(ids, y), id1 = __builtin_amdgcn_readlane(ids, y + 1);
+        const int k0 = (it0 + w + NW * x) * KT;
+        load_k<D>(tl.k, a.pg, n >= 8 ? id1 : id0, head, (k0 + (n >= 8 ? 16 : 0)) & mask, n, g);
+      };
+      auto get_v = [&](Tile<D, false>& tl, int x) {
+        const int y = 2 * (x & 31), id0 = __builtin_amdgcn_readlane(ids, y), id1 = __builtin_amdgcn_readlane(ids, y + 1);
+        tl.k0 = (it0 + w + NW * x) * KT;
+        tl.bad = static_cast<uint32_t>(bad >> y) & 3u;
+        load_v<D>(tl.v, a.pg, g >= 2 ? id1 : id0, head, (tl.k0 + (g >= 2 ? 16 : 0)) & mask, n, g);
+      };
+      Tile<D, false> tl[NT];
+      if (mine) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          get_k(tl[x], min(x, mine - 1));
+          get_v(tl[x], min(x, mine - 1));
+        }
+      }
+      queries();
+      while (!none && i + NT <= whole) {
+        f32x4 sc[NT][2];
+        float tmax;
+        for (; i + NT <= whole; i += NT) {
+          uint32_t bads = 0;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) bads |= tl[x].bad;
+          none = bads != 0;
+          if (none) break;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) scores<D, false>(tl[x].k, qf, sc[x], n);
+          tmax = lane_max(sc[0]);
+          if constexpr (NT > 1) tmax = fmaxf(tmax, lane_max(sc[NT - 1]));
+          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
+          const int i1 = min(i + NT, mine - 1);
+          if (i1 == i + NT) window(i1);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) get_k(tl[x], min(i1 + x, mine - 1));
+          bf16x8 pf[NT];
+#pragma unroll
+          for (int x = 0; x < NT; ++x) pf[x] = probabilities(sc[x], st.m, a.c, st.l);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) product<D, false, false>(tl[x].v, pf[x], 8, st);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) get_v(tl[x], min(i1 + x, mine - 1));
+        }
+        if (!none && i + NT <= whole) raise<D>(st, tmax, a.c, g);
+      }
+      for (; i < mine; ++i) {
+        edge_step<D, false>(tl[0], qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
+        if (i + 1 < mine) {
+          window(i + 1);
+          get_k(tl[0], i + 1);
+          get_v(tl[0], i + 1);
+        }
+      }
+    }
+
+    // merge the waves: thread t takes row t / 16 and D / 16 columns
+    float* ml = lds + NW * 16 * (D + 4);
+    float ls = st.l;
     ls += __shfl_xor(ls, 16, 64);
     ls += __shfl_xor(ls, 32, 64);
     if (g == 0) {
-      ml[w * 16 + n] = st.m[mt] == -INFINITY ? st.m[mt] : st.m[mt] * a.c;  // base 2
+      ml[w * 16 + n] = st.m == -INFINITY ? st.m : st.m * a.c;  // base 2
       ml[(NW + w) * 16 + n] = ls;
     }
 #pragma unroll
@@ -702,7 +960,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX, MT))) void k_paged_few(
 #pragma unroll
       for (int b = 0; b < NB; b += 4)
         *reinterpret_cast<float4*>(lds + (w * 16 + 4 * g + j) * (D + 4) + n * NB + b) =
-            make_float4(st.o[mt][b][j], st.o[mt][b + 1][j], st.o[mt][b + 2][j], st.o[mt][b + 3][j]);
+            make_float4(st.o[b][j], st.o[b + 1][j], st.o[b + 2][j], st.o[b + 3][j]);
     __syncthreads();
     const int rw = t >> 4, d0 = (t & 15) * NB;
     float top = -INFINITY;
@@ -725,12 +983,17 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX, MT))) void k_paged_few(
         acc[b + 3] += v.w * f;
       }
     }
-    const int r = 16 * mt + rw, qi = r / a.rep;
-    if (marks[4 * MT * D]) {
+    if (marks[D]) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b] += marked((marks[(r * D + d0 + b) / 4] >> (8 * (b & 3))) & 255u);
+      for (int b = 0; b < NB; ++b) acc[b] += marked((marks[(rw * D + d0 + b) / 16] >> (2 * ((d0 + b) % 16))) & 3u);
     }
-    if (qi < nq) finish_row<D, NB>(a, u, part, 16 * MT, r, head, q0, d0, acc, top, sum);
+    if (rw < r.rows) finish_row<D, NB>(a, u.s.first + r.q0, r.off, whole_block, part, rw, head, d0, acc, top, sum);
+    __syncthreads();                                           // the next piece takes the LDS
+    if (marks[D]) {
+      __syncthreads();
+      for (int x = t; x <= D; x += 64 * NW) marks[x] = 0u;
+      __syncthreads();
+    }
   }
 }
 
@@ -748,31 +1011,24 @@ struct ManyCodes {
 };
 
 // The wave's 16-key half of a tile that it loads: rows of one page.
-template <int AD>
-__device__ __forceinline__ int half_of_wave(int w) { return AD == 256 ? w >> 2 : w >> 1; }
+__device__ __forceinline__ int half_of_wave(int w) { return w >> 1; }
 
 // A thread's codes of a tile whose half lies at token tok0 of page id.
 template <int AD>
 __device__ __forceinline__ void load_codes(ManyCodes<AD, true>& c, const PagesDev& pg, int id, int head, int tok0, int w, int lane) {
   const int64_t at = static_cast<int64_t>(id) * pg.page_stride + static_cast<int64_t>(head) * pg.head_bytes;
   const int64_t sat = static_cast<int64_t>(id) * pg.scale_stride + static_cast<int64_t>(head) * pg.head_scales;
-  constexpr int TPR = AD == 256 ? 16 : 8;                    // threads a key row (8 bytes each; 4 at head_dim 64)
-  const int row = (AD == 256 ? 4 * (w & 3) : 8 * (w & 1)) + lane / TPR, part = lane % TPR;
-  const char* kp = pg.k + at + (tok0 + row) * (AD / 2) + part * (AD / 2 / TPR);
+  const int row = 8 * (w & 1) + lane / 8, part = lane % 8;   // eight threads a key row
+  const char* kp = pg.k + at + (tok0 + row) * (AD / 2) + part * (AD / 16);
   if constexpr (AD == 64) c.k.x = *reinterpret_cast<const uint32_t*>(kp);
   else c.k = *reinterpret_cast<const uint2*>(kp);
-  c.ks = pg.ks[sat + ((tok0 + row) >> 3) * (AD / 4) + (part * (AD / TPR) / 32) * 8 + (row & 7)];
-  // values: 8 tokens' runs; d 128: two tokens of a run of 8 values, 256: one of 16, 64: one of two runs of 4
-  const int grp = AD == 256 ? (w >> 1) & 1 : w & 1;
-  const char* vp = pg.v + at + ((tok0 >> 3) + grp) * (4 * AD);
-  const uint8_t* sp = pg.vs + sat + ((tok0 >> 3) + grp) * (AD / 4);
+  c.ks = pg.ks[sat + ((tok0 + row) >> 3) * (AD / 4) + (part * (AD / 8) / 32) * 8 + (row & 7)];
+  // values: 8 tokens' runs; d 128: two tokens of a run of 8 values, 64: one of two runs of 4
+  const char* vp = pg.v + at + ((tok0 >> 3) + (w & 1)) * (4 * AD);
+  const uint8_t* sp = pg.vs + sat + ((tok0 >> 3) + (w & 1)) * (AD / 4);
   if constexpr (AD == 128) {
     c.v = *reinterpret_cast<const uint2*>(vp + lane * 8);
     c.vs = *reinterpret_cast<const uint16_t*>(sp + ((lane >> 2) / 4) * 8 + 2 * (lane & 3));
-  } else if constexpr (AD == 256) {
-    const int x = 64 * (w & 1) + lane;
-    c.v = *reinterpret_cast<const uint2*>(vp + x * 8);
-    c.vs = sp[((x >> 3) / 2) * 8 + (x & 7)];
   } else {
     const int cc = lane >> 3, key = lane & 7;
     c.v.x = *reinterpret_cast<const uint16_t*>(vp + (2 * cc) * 16 + 2 * key) |
@@ -789,8 +1045,7 @@ __device__ __forceinline__ uint4 eight_values(uint32_t w, float s) {
 template <int AD>
 __device__ __forceinline__ void store_codes(const ManyCodes<AD, true>& c, char* st, int w, int lane) {
   using L = Layout<AD>;
-  constexpr int TPR = AD == 256 ? 16 : 8;
-  const int row = (AD == 256 ? 4 : 8) * w + lane / TPR, part = lane % TPR;
+  const int row = 8 * w + lane / 8, part = lane % 8;
   uint4* s4 = reinterpret_cast<uint4*>(st);
   const float ks = scale_of<0>(c.ks), vs = scale_of<0>(c.vs);
   if constexpr (AD == 64) {
@@ -799,16 +1054,50 @@ __device__ __forceinline__ void store_codes(const ManyCodes<AD, true>& c, char* 
   } else {
     s4[L::kslot(row, 2 * part)] = eight_values(c.k.x, ks);
     s4[L::kslot(row, 2 * part + 1)] = eight_values(c.k.y, ks);
-    if constexpr (AD == 128) {
-      const int r = 8 * w + 2 * (lane & 3);
-      s4[L::vslot(r, lane >> 2)] = eight_values(c.v.x, vs);
-      s4[L::vslot(r + 1, lane >> 2)] = eight_values(c.v.y, scale_of<1>(c.vs));
-    } else {
-      const int x = 64 * (w & 1) + lane, r = 8 * (w >> 1) + (x & 7);
-      s4[L::vslot(r, 2 * (x >> 3))] = eight_values(c.v.x, vs);
-      s4[L::vslot(r, 2 * (x >> 3) + 1)] = eight_values(c.v.y, vs);
-    }
+    const int r = 8 * w + 2 * (lane & 3);
+    s4[L::vslot(r, lane >> 2)] = eight_values(c.v.x, vs);
+    s4[L::vslot(r + 1, lane >> 2)] = eight_values(c.v.y, scale_of<1>(c.vs));
   }
+}
+
+// The largest of a row's scores of a tile.
+template <int AD>
+__device__ __forceinline__ float top_score(const f32x16 (&sc)[Cfg<AD>::KB]) {
+  float tmax = -INFINITY, lo, hi;
+#pragma unroll
+  for (int kb = 0; kb < Cfg<AD>::KB; ++kb)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) tmax = fmaxf(tmax, sc[kb][j]);
+  lane_pair(tmax, lo, hi);
+  return fmaxf(lo, hi);
+}
+
+template <int AD>
+__device__ __forceinline__ void raise_tile(f32x16 (&o)[AD / 32], float& mref, float& lsum, float tmax, float c) {
+  const float top = fmaxf(mref, tmax);
+  const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mref - top) * c);
+  mref = top;
+#pragma unroll
+  for (int b = 0; b < AD / 32; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+  lsum *= alpha;
+}
+
+// The probabilities of a tile, in pairs as the product takes them; their sum goes to lsum.
+template <int AD>
+__device__ __forceinline__ void tile_probabilities(const f32x16 (&sc)[Cfg<AD>::KB], uint32_t (&pk)[8 * Cfg<AD>::KB], float mref,
+                                                   float& lsum, float c) {
+  const float mc = mref == -INFINITY ? 0.f : mref * c;
+  float psum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8 * Cfg<AD>::KB; ++e) {
+    const float q0 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8)], c, -mc));
+    const float q1 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8) + 1], c, -mc));
+    psum += q0 + q1;
+    pk[e] = bf16_pair(q0, q1);
+  }
+  lsum += psum;
 }
 
 // tile_step for a tile of which some row does not see some key, without the next tile's scores: bad has a bit a 16-key half
@@ -819,40 +1108,19 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
                                           float& mref, float& lsum, int k0, uint32_t bad, int mypos, int hh, float c,
                                           const FragOffsets<AD>& fo) {
   using L = Layout<AD>;
-  constexpr int NB = AD / 32, KB = Cfg<AD>::KB, KTL = Cfg<AD>::KT, NP = 8 * KB;
+  constexpr int NB = AD / 32, KB = Cfg<AD>::KB, KTL = Cfg<AD>::KT;
   const int rel = min(max(mypos - k0, -1), KTL) - 4 * hh;
-  float tmax = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const bool gone = (bad >> (2 * kb + (j >> 3))) & 1u;   // keys 32 kb + 8 (j / 4) + ..
       if (gone || 32 * kb + 8 * (j >> 2) + (j & 3) > rel) sc[kb][j] = -INFINITY;
-      tmax = fmaxf(tmax, sc[kb][j]);
     }
-  float lo, hi;
-  lane_pair(tmax, lo, hi);
-  tmax = fmaxf(lo, hi);
-  if (tmax > mref + RESCALE_LOG2 / c) {
-    const float alpha = __builtin_amdgcn_exp2f((mref - tmax) * c);
-    mref = tmax;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
-    lsum *= alpha;
-  }
-  const float mc = mref == -INFINITY ? 0.f : mref * c;
-  float psum = 0.f;
-  uint32_t pk[NP];
-#pragma unroll
-  for (int e = 0; e < NP; ++e) {
-    const float q0 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8)], c, -mc));
-    const float q1 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8) + 1], c, -mc));
-    psum += q0 + q1;
-    pk[e] = bf16_pair(q0, q1);
-  }
-  lsum += psum;
+  const float tmax = top_score<AD>(sc);
+  if (__any(tmax > mref + RESCALE_LOG2 / c)) raise_tile<AD>(o, mref, lsum, tmax, c);
+  uint32_t pk[8 * KB];
+  tile_probabilities<AD>(sc, pk, mref, lsum, c);
   bool odd = false;
 #pragma unroll
   for (int stp = 0; stp < KTL / 16; ++stp) {
@@ -883,10 +1151,17 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
   }
 }
 
+// Its waves (32 rows each): 8, two a SIMD. head_dim 256: 4, with the 512 registers that O^T (128), the queries (64), two tiles'
+// scores and the edge tiles' code want (8 waves of 256 spilled 360 registers, and 350 us of 13 sequences of 256 rows were 157).
+constexpr int many_waves(int d) { return d == 256 ? 4 : 8; }
+constexpr int many_rows(int d) { return 32 * many_waves(d); }
+
 template <int AD, bool MX>
-__global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
+__global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs a) {
   using L = Layout<AD>;
-  constexpr int NS = AD / 16, NB = AD / 32, KTL = Cfg<AD>::KT, QROWS = Cfg<AD>::QROWS, KB = Cfg<AD>::KB;
+  constexpr int NS = AD / 16, NB = AD / 32, KTL = Cfg<AD>::KT, QROWS = many_rows(AD), KB = Cfg<AD>::KB;
+  constexpr int NWM = many_waves(AD), SHARES = Cfg<AD>::NW / NWM;      // shares of a tile's loads a wave takes
+  constexpr int KLOADS = L::KLOADS * SHARES, LOADS = L::LOADS * SHARES;
   constexpr int HPT = KTL / 16, WIN = 64 / HPT;              // 16-key halves a tile, tiles a window of table entries
   __shared__ uint4 lds[NSTAGE * L::STAGE_U4];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 31, hh = lane >> 5;
@@ -894,19 +1169,20 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
   const int head = blockIdx.x % a.hkv;
   const Unit u = find_unit(a, blockIdx.x / a.hkv, false);
   if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
-  const int q0 = u.rb * a.qb, nq = min(a.qb, u.s.rows - q0), rows = nq * a.rep;
-  const int p0 = u.s.keys - u.s.rows + q0, plast = p0 + nq - 1;
+  const RowBlock rb(a, u.s, u.rb);
+  const int q0 = rb.q0, rows = rb.rows;
+  const int p0 = u.s.keys - u.s.rows + q0, plast = p0 + (rb.off + rows - 1) / a.rep;
   const int ntiles = plast < 0 ? 0 : plast / KTL + 1;
   const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);
 
-  // row 32 w + n: query r / rep, head r % rep; lanes past the last row repeat it and write nothing
-  const int r = min(32 * w + n, rows - 1), qi = r / a.rep;
+  // row 32 w + n of the block; lanes past the last row repeat it and write nothing
+  const int r = min(32 * w + n, rows - 1), qi = (rb.off + r) / a.rep, hd = head * a.rep + rb.off + r - qi * a.rep;
   const bool live = 32 * w + n < rows;
   const int mypos = p0 + qi;
-  const int wave_last = 32 * w < rows ? p0 + min(32 * w + 31, rows - 1) / a.rep : -1;
+  const int wave_last = 32 * w < rows ? p0 + (rb.off + min(32 * w + 31, rows - 1)) / a.rep : -1;
   bf16x8 qf[NS];
   {
-    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldq + (head * a.rep + r - qi * a.rep) * AD + 8 * hh;
+    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldq + hd * AD + 8 * hh;
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = as_frag(*reinterpret_cast<const uint4*>(qrow + 16 * s));
   }
@@ -951,9 +1227,9 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
     advance(it);
     char* st = stage(it);
 #pragma unroll
-    for (int i = 0; i < L::KLOADS; ++i) {
+    for (int i = 0; i < KLOADS; ++i) {
       constexpr int RPI = 64 / L::KCPR;
-      const int row0 = (w * L::KLOADS + i) * RPI, half = row0 >> 4;
+      const int row0 = (w * KLOADS + i) * RPI, half = row0 >> 4;
       const int tok = (it * KTL + row0) & mask;
       const int64_t at = static_cast<int64_t>(id_of(it, half)) * a.pg.page_stride + static_cast<int64_t>(head) * a.pg.head_bytes +
                          static_cast<int64_t>(tok) * (AD * 2);
@@ -961,15 +1237,15 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
       const uint32_t ko = static_cast<uint32_t>(rl * (AD * 2) + (pc ^ ((row0 + rl) & (L::KCPR - 1))) * 16);
       const uint32_t vo = static_cast<uint32_t>(rl * (AD * 2) + (pc ^ (4 * L::vsw(row0 + rl))) * 16);
       const __amdgpu_buffer_rsrc_t rk = buffer_rsrc(a.pg.k + at, 1024u), rv = buffer_rsrc(a.pg.v + at, 1024u);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(st + (w * L::KLOADS + i) * 1024), 16, ko, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(st + (L::K_U4 + (w * L::VLOADS + i) * 64) * 16), 16, vo, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(st + (w * KLOADS + i) * 1024), 16, ko, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(st + (L::K_U4 + (w * KLOADS + i) * 64) * 16), 16, vo, 0, 0, 0);
     }
   };
   // 4 bits: the tile's codes into registers
   [[maybe_unused]] ManyCodes<AD, true> codes;
   [[maybe_unused]] auto fetch = [&](int it) {
     advance(it);
-    const int half = half_of_wave<AD>(w);
+    const int half = half_of_wave(w);
     load_codes<AD>(codes, a.pg, id_of(it, half), head, (it * KTL + 16 * half) & mask, w, lane);
   };
 
@@ -996,8 +1272,8 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
   } else {
     for (int i = 0; i < 3; ++i)
       if (it0 + i < it1) issue(it0 + i);
-    if (it0 + 2 < it1) wait_vm_lgkm0<2 * L::LOADS>();        // tile it0 landed
-    else if (it0 + 1 < it1) wait_vm_lgkm0<L::LOADS>();
+    if (it0 + 2 < it1) wait_vm_lgkm0<2 * LOADS>();        // tile it0 landed
+    else if (it0 + 1 < it1) wait_vm_lgkm0<LOADS>();
     else wait_vm_lgkm0<0>();
     __builtin_amdgcn_s_barrier();
   }
@@ -1008,7 +1284,7 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
       if (it + 2 < it1) store_codes<AD>(codes, stage(it + 2), w, lane);
       if (it + 3 < it1) fetch(it + 3);
     } else {
-      if (it + 2 < it1) wait_vm_lgkm0<L::LOADS>();           // tile it + 1 landed, tile it + 2 may fly
+      if (it + 2 < it1) wait_vm_lgkm0<LOADS>();           // tile it + 1 landed, tile it + 2 may fly
       else wait_vm_lgkm0<0>();
       __builtin_amdgcn_s_barrier();                          // every wave's share of it has landed and every
       if (it + 3 < it1) issue(it + 3);                       // wave is done with the stage reloaded here
@@ -1022,22 +1298,12 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
   }
   const int full = p0 >= KTL - 1 ? min(it1, (p0 + 1) / KTL) : it0;
   int it = it0;
-  if constexpr (AD == 256) {                                 // (one buffer's copy each: in pairs it spills)
-    for (; it < full; ++it) {
-      if (bad_of(it)) break;
-      turn(it);
-      tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) sc[kb] = sn[kb];
-    }
-  } else {
-    for (; it + 1 < full; it += 2) {
-      if (bad_of(it) | bad_of(it + 1)) break;
-      turn(it);
-      tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
-      turn(it + 1);
-      tile_step<AD>(stage(it + 1), stage(it + 2), qf, sn, sc, o, m, lsum, it * KTL + KTL, false, mypos, hh, c, fo);
-    }
+  for (; it + 1 < full; it += 2) {
+    if (bad_of(it) | bad_of(it + 1)) break;
+    turn(it);
+    tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
+    turn(it + 1);
+    tile_step<AD>(stage(it + 1), stage(it + 2), qf, sn, sc, o, m, lsum, it * KTL + KTL, false, mypos, hh, c, fo);
   }
   for (; it < it1; ++it) {
     turn(it);
@@ -1069,7 +1335,7 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
     return;
   }
   const float inv = inverse_sum(ltot);
-  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * AD + 4 * hh;
+  uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + hd * AD + 4 * hh;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1083,49 +1349,76 @@ __global__ __launch_bounds__(Cfg<AD>::NTHR, 1) void k_paged_many(PagedArgs a) {
 // order through LDS. The order depends on the sizes alone. blockIdx.y takes a share of the rows where few row blocks leave
 // CUs idle.
 constexpr int MERGE_THREADS = 1024;
-template <int D>
-__global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a, int rpb) {
+template <int D, bool RUNS>
+__global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a) {
+  const int rpb = a.rpb;
   constexpr int LPR = D / 4, U = 8;
   __shared__ float4 ls[MERGE_THREADS];
   __shared__ float lm[MERGE_THREADS / LPR], ll[MERGE_THREADS / LPR];
   const int t = threadIdx.x, head = blockIdx.x % a.hkv, slots = blockDim.x / LPR, slot = t / LPR, col = 4 * (t % LPR);
-  const Unit u = find_unit(a, blockIdx.x / a.hkv, true);
-  // (partials past the last unit: only with a cu that does not rise, whose units the launch does not hold)
-  if (u.b < 0 || u.ns == 1 || u.part + static_cast<int64_t>(u.ns - 1) * u.nrb >= a.units) return;
-  const int q0 = u.rb * a.qb, rows = min(a.qb, u.s.rows - q0) * a.rep;
+  const int64_t size = static_cast<int64_t>(rpb) * (D + 2);
+  // the parts: ns of them, the first at `first`, part s > 0 at rest + s step
+  int ns, rows, row0, off;
+  const float *first, *rest;
+  int64_t step;
+  if constexpr (RUNS) {                                      // runs of tiles: its own run's last piece (or first), then first pieces
+    Seq s0{0, 0, 0};
+    if ((t & 63) < a.n_seq) s0 = seq_of(a, t & 63);
+    const Piece u = piece_at(a, s0, blockIdx.x / a.hkv, true, t & 63);
+    if (u.b < 0) return;
+    const int run = *a.length, x0 = u.begin / run;
+    ns = (u.begin + u.nt - 1) / run - x0 + 1;
+    if (u.begin < 0 || x0 + ns > a.fit) return;              // (only with a cu that does not rise: more tiles than 31 bits count)
+    const RowBlock r(a, u.s, u.rb);
+    off = r.off;
+    rows = r.rows;
+    row0 = u.s.first + r.q0;
+    step = 2 * a.hkv * size;
+    rest = a.part + (2 * static_cast<int64_t>(x0) * a.hkv + head) * size;
+    first = u.begin == x0 * run ? rest : rest + a.hkv * size;
+  } else {
+    const Unit u = find_unit(a, blockIdx.x / a.hkv, true);
+    // (partials past the last unit: only with a cu that does not rise, whose units the launch does not hold)
+    if (u.b < 0 || u.part + static_cast<int64_t>(u.ns - 1) * u.nrb >= a.units) return;
+    ns = u.ns;
+    const RowBlock r(a, u.s, u.rb);
+    off = r.off;
+    rows = r.rows;
+    row0 = u.s.first + r.q0;
+    step = static_cast<int64_t>(u.nrb) * a.hkv * size;
+    first = rest = a.part + (u.part * a.hkv + head) * size;
+  }
+  if (ns == 1) return;
   const int per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
   if (r0 >= r1) return;
   int G = 1;
-  while (2 * G * (r1 - r0) <= slots && 2 * G <= u.ns) G *= 2;
+  while (2 * G * (r1 - r0) <= slots && 2 * G <= ns) G *= 2;
   const int grp = slot % G;
-  const float* p0 = a.part + (u.part * a.hkv + head) * (static_cast<int64_t>(rpb) * (D + 2));
-  const int64_t step = static_cast<int64_t>(u.nrb) * a.hkv * (static_cast<int64_t>(rpb) * (D + 2));
   for (int rb = r0; rb < r1; rb += slots / G) {              // (uniform)
     const int r = rb + slot / G, rc = min(r, r1 - 1);
-    const float* pv = p0 + static_cast<int64_t>(rc) * D + col;
-    const float* ms = p0 + static_cast<int64_t>(rpb) * D + rc;
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = grp; s0 < u.ns; s0 += U * G) {
+    for (int s0 = grp; s0 < ns; s0 += U * G) {
       float4 v[U];
       float m[U], l[U];
 #pragma unroll
       for (int x = 0; x < U; ++x) {
-        const int64_t s = min(s0 + x * G, u.ns - 1);
-        m[x] = ms[s * step];
-        l[x] = ms[s * step + rpb];
-        v[x] = *reinterpret_cast<const float4*>(pv + s * step);
+        const int s = min(s0 + x * G, ns - 1);
+        const float* p = s ? rest + s * step : first;
+        m[x] = p[static_cast<int64_t>(rpb) * D + rc];
+        l[x] = p[static_cast<int64_t>(rpb) * (D + 1) + rc];
+        v[x] = *reinterpret_cast<const float4*>(p + static_cast<int64_t>(rc) * D + col);
       }
       float now = top;
 #pragma unroll
-      for (int x = 0; x < U; ++x) now = fmaxf(now, s0 + x * G < u.ns ? m[x] : -INFINITY);
+      for (int x = 0; x < U; ++x) now = fmaxf(now, s0 + x * G < ns ? m[x] : -INFINITY);
       const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= f0;
       acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
 #pragma unroll
       for (int x = 0; x < U; ++x) {
-        if (s0 + x * G >= u.ns) break;                       // (uniform over a group)
+        if (s0 + x * G >= ns) break;                       // (uniform over a group)
         const float f = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - top);
         sum += l[x] * f;
         acc.x += v[x].x * f;
@@ -1143,14 +1436,13 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a, int 
       }
       __syncthreads();
       if (grp == 0) {
-        const int first = slot;
-        for (int x = 0; x < G; ++x) top = fmaxf(top, lm[first + x]);
+        for (int x = 0; x < G; ++x) top = fmaxf(top, lm[slot + x]);
         sum = 0.f;
         acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int x = 0; x < G; ++x) {
-          const float m = lm[first + x], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          const float m = lm[slot + x], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
           const float4 v = ls[t + x * LPR];
-          sum += ll[first + x] * f;
+          sum += ll[slot + x] * f;
           acc.x += v.x * f;
           acc.y += v.y * f;
           acc.z += v.z * f;
@@ -1160,43 +1452,45 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a, int 
     }
     if (grp == 0 && r < r1) {
       const float inv = inverse_sum(sum);
-      const int qi = r / a.rep;
-      uint16_t* dst = a.out + static_cast<int64_t>(u.s.first + q0 + qi) * a.ldo + (head * a.rep + r - qi * a.rep) * D + col;
+      const int qi = (off + r) / a.rep;
+      uint16_t* dst = a.out + static_cast<int64_t>(row0 + qi) * a.ldo + (head * a.rep + off + r - qi * a.rep) * D + col;
       *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_pair(acc.x * inv, acc.y * inv), bf16_pair(acc.z * inv, acc.w * inv));
     }
   }
 }
 
-// 16-row blocks a wave takes: as few as hold a sequence's rows (their state and queries live in registers: up to 4, 3 at
-// head_dim 256).
-int row_tiles(int rep, int d, int64_t max_rows) {
-  return static_cast<int>(std::min<int64_t>(d == 256 ? 3 : 4, (max_rows * rep + 15) / 16));
-}
-
 struct Plan {
   bool many, once;
-  int mt, qb, fit, kt;                     // mt: 16-row blocks of k_paged_few
+  int fit, kt;
   int64_t blocks, units;                   // (sequence, row block)s at most, and with their splits
   size_t bytes;
-  int rows() const { return many ? Cfg<128>::QROWS : 16 * mt; }
+  int d;
+  int rows() const { return many ? many_rows(d) : 16; }
 };
 
-// The launch for these sizes: a sequence's rows in the registers of k_paged_few's waves, or more of them through
-// k_paged_many. Row blocks: sum of ceil(rows / qb) <= T / qb + n_seq. With splits of W tiles at most work / W units more
-// (split_length: one round of blocks, or W >= work / 3 fit).
+// The most rows a sequence that k_paged_few takes in blocks of 16. 13 sequences of 2000 to 8000 keys, few against many (us):
+// bf16, d 128, 12 rows 52 / 55, 28 64 / 58, 64 108 / 63; d 64, 16 rows 22 / 22, 64 28 / 22; d 256, 64 rows 66 / 96, 128
+// 105 / 110, 256 185 / 157. 4 bits, d 128, 64 rows 45 / 65, 128 71 / 67, 256 121 / 92; d 64, 64 rows 23 / 23, 128 26 / 25;
+// d 256, 256 rows 81 / 146, 512 138 / 239: there k_paged_many is not built (its products take bf16, those of k_paged_few the
+// keys' codes at four times the rate, and a wave's 256 columns leave no registers to convert the codes beside them).
+constexpr int64_t few_rows(int d, bool mx) { return d == 256 ? (mx ? INT64_MAX : 128) : mx ? 96 : 16; }
+
+// The launch for these sizes: k_paged_few or k_paged_many. Row blocks: sum of ceil(rows rep / rpb) <= T rep / rpb + n_seq. k_paged_few: `fit` runs a head, two parts each;
+// k_paged_many: with splits of W tiles at most work / W units more (split_length: one round of blocks, or W >= work / 3 fit).
 Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys) {
   Plan p{};
+  p.d = d;
   const int rep = hq / hkv;
-  p.many = std::min<int64_t>(max_rows, T) * rep > (d == 256 ? 48 : 64);
-  p.mt = p.many ? 0 : row_tiles(rep, d, std::min<int64_t>(max_rows, T));
-  p.qb = p.rows() / rep;
+  p.many = std::min<int64_t>(max_rows, T) * rep > few_rows(d, mx);
   p.kt = p.many ? (d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
-  p.blocks = std::min<int64_t>(T, T / p.qb + n_seq);
-  const int round = p.many ? 256 : 256 * few_blocks(d, mx, p.mt);
-  p.fit = max_keys <= 16 * NW * KT ? 0 : std::max(1, round / hkv);
+  p.blocks = std::min<int64_t>(T * rep, T * rep / p.rows() + n_seq);
+  const int round = p.many ? 256 : 256 * few_blocks(d);
+  // (no splits either where the tiles would not count in 31 bits)
+  const bool split = max_keys > 16 * NW * KT && static_cast<double>(p.blocks) * static_cast<double>(max_keys / p.kt + 1) < 1e9;
+  p.fit = split ? std::max(1, round / hkv) : 0;
   p.once = p.blocks * 4 <= static_cast<int64_t>(p.fit) * 3;
-  p.units = !p.fit ? p.blocks : p.once ? p.fit : 3 * p.fit + 1 + p.blocks;
-  p.bytes = p.fit ? static_cast<size_t>(p.units) * hkv * (p.rows() * (d + 2)) * 4 + 16 : 0;
+  p.units = !p.fit ? p.blocks : !p.many || p.once ? p.fit : 3 * p.fit + 1 + p.blocks;
+  p.bytes = p.fit ? static_cast<size_t>(p.many ? p.units : 2 * p.units) * hkv * (p.rows() * (d + 2)) * 4 + 16 : 0;
   return p;
 }
 
@@ -1245,11 +1539,13 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
     return fail(RF_EINVAL_ARG, "%s: scale %g (must be positive)", fn, static_cast<double>(scale));
   if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
   Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys);
+  if (std::max(p.units, p.blocks) * hkv > INT32_MAX)
+    return fail(RF_EINVAL_SHAPE, "%s: %lld blocks of query rows over %d K / V heads", fn, (long long)p.blocks, hkv);
   if (p.fit && (!workspace || ws_bytes < p.bytes)) {
     p.fit = 0;
     p.units = p.blocks;
   }
-  const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.qb,
+  const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.rows(),
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
                     scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace),
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.many ? 3.f : 1.f, p.units, p.kt,
@@ -1260,28 +1556,22 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   const dim3 grid2(static_cast<unsigned>(pairs), static_cast<unsigned>(std::min<int64_t>(p.many ? (rows + 15) / 16 : rows, ((p.many ? 2047 : 511) + pairs) / pairs)));
   const dim3 merge(grid2.x * grid2.y <= 256 ? MERGE_THREADS : 256);
   const bool mx = pages->kind == RF_PAGES_MX4;
-#define RF_FEW(D, MT)                                                                                    \
-  do {                                                                                                   \
-    if (mx) hipLaunchKernelGGL((k_paged_few<D, true, MT>), grid, dim3(64 * NW), 0, stream, a);           \
-    else hipLaunchKernelGGL((k_paged_few<D, false, MT>), grid, dim3(64 * NW), 0, stream, a);             \
-  } while (0)
 #define RF_ATTEND(D)                                                                                     \
   do {                                                                                                   \
-    if (p.many && mx) hipLaunchKernelGGL((k_paged_many<D, true>), grid, dim3(Cfg<D>::NTHR), 0, stream, a); \
-    else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false>), grid, dim3(Cfg<D>::NTHR), 0, stream, a); \
-    else if (p.mt == 1) RF_FEW(D, 1);                                                                    \
-    else if (p.mt == 2) RF_FEW(D, 2);                                                                    \
-    else if (p.mt == 3) RF_FEW(D, 3);                                                                    \
-    else if constexpr (D != 256) RF_FEW(D, 4);                                                           \
+    if (p.many && mx) {                                                                                  \
+      if constexpr (D != 256) hipLaunchKernelGGL((k_paged_many<D, true>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    } else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    else if (mx) hipLaunchKernelGGL((k_paged_few<D, true>), grid, dim3(64 * NW), 0, stream, a);          \
+    else hipLaunchKernelGGL((k_paged_few<D, false>), grid, dim3(64 * NW), 0, stream, a);                 \
     if (p.fit) {                                                                                         \
       if (int rc = check_launch(fn)) return rc;                                                          \
-      hipLaunchKernelGGL(k_paged_merge<D>, grid2, merge, 0, stream, a, p.rows());                        \
+      if (p.many) hipLaunchKernelGGL((k_paged_merge<D, false>), grid2, merge, 0, stream, a);   \
+      else hipLaunchKernelGGL((k_paged_merge<D, true>), grid2, merge, 0, stream, a);           \
     }                                                                                                    \
   } while (0)
   if (d == 64) RF_ATTEND(64);
   else if (d == 128) RF_ATTEND(128);
   else RF_ATTEND(256);
 #undef RF_ATTEND
-#undef RF_FEW
   return check_launch(fn);
 }

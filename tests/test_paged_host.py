@@ -104,12 +104,14 @@ def test_bad_slots_and_reads_are_refused():
 
 
 def test_workspace_rule():
-    """Nothing for short sequences; otherwise room for every split's part, growing with the rows and sequences."""
+    """Nothing for short sequences; room for one round of parts for few rows a sequence, whatever their number; for chunks it
+    grows with the rows."""
     from rfill import ops
     f = ops.attend_paged_workspace_bytes
     assert f(1, 32, 8, 128, 0, 1, 1, 500) == 0
     one, many = f(1, 32, 8, 128, 0, 1, 1, 100000), f(64, 32, 8, 128, 0, 64, 1, 100000)
-    assert 0 < one < many < (1 << 28)
+    assert 0 < one == many < (1 << 28)
+    assert many < f(2048, 32, 8, 128, 0, 1, 2048, 100000) < f(16384, 32, 8, 128, 0, 8, 2048, 100000) < (1 << 32)
     assert f(0, 32, 8, 128, 0, 4, 1, 100000) == 0
     with pytest.raises(ValueError):
         f(1, 32, 7, 128, 0, 1, 1, 500)
