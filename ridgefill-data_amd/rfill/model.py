@@ -8,6 +8,9 @@ arithmetic in librfill's HIP kernels.
   forward_exact(ids, hook)      exact forward of one document, hook(i, h) on every layer input
                                 (code/kva/model.py:167-181)
   new_cache()                   one dict per layer (code/kva/model.py:105-106)
+  layer_paged(i, h, step, cache), forward_paged(cache, seqs, ids)
+                                exact layers and forward of new tokens of several sequences over a
+                                paged cache (rfill.paged.PagedCache)
 
 Cache layout (code/kva/model.py:139-159): attention layers hold kbuf / vbuf [Hkv, cap, d] bf16 with
 cap = rows + KV_RESERVE, 'n' and the views k / v = buf[:, :n]; appended row j lands in slot n + j.
@@ -551,6 +554,74 @@ class FillModel:
             o = ops.attend_rows(q, torch.arange(slot, slot + T, device=h.device), c["kbuf"], c["vbuf"], c["n"],
                                 self.n_heads, self.scale, workspace=self._attn_workspace(T, c["n"], h.device))
         return self._out_mlp(w, h, self._gate(w, h, ssq, o, gate))
+
+    def layer_paged(self, i, h, step, cache, ssq=None):
+        """Exact layer i for the new rows h [rows, H] bf16 of several sequences over a paged cache (rfill.paged.PagedCache;
+        step: its plan() of these rows), as layer() of each sequence alone: queries, gate, K and V of all rows from one
+        product, K and V normed and rotated into the pages, attention over them, then o_proj, the residual and the MLP. GDN
+        layers continue each sequence's states. Returns (layer output [rows, H] bf16, its row sum-of-squares partials)."""
+        if h.shape[0] != step.rows:
+            raise ValueError(f"layer_paged: {h.shape[0]} rows, the step has {step.rows}")
+        if ssq is None:
+            ssq = ops.row_ssq(h)
+        w = self._pack_rows(i)
+        R, H = h.shape
+        if w["kind"] != "attn":
+            return self._gdn_paged(i, w, h, ssq, step, cache)
+        pages = cache.pools[i]
+        hq, hkv, d = self.n_heads, self.n_kv, self.head_dim
+        N = w["wattn"].shape[0]
+        x = ops.norm_linear(h, ssq, self.eps, w["wattn"], workspace=self.gemm_workspace(R, N, H, h.device))
+        q, g = x[:, :hq * d], x[:, hq * d:N - 2 * hkv * d] if "wgate" in w else None
+        k, v = (x[:, N - j * hkv * d:N - (j - 1) * hkv * d].unflatten(1, (hkv, d)) for j in (2, 1))
+        ops.paged_append(k, v, step.slots, pages, cs=step.cs, q=q, out=q, qnorm=w.get("q_norm"), knorm=w.get("k_norm"),
+                         norm_kind=self.knorm_kind, eps=self.eps)
+        o = ops.attend_paged(q, pages, step.table, step.lens, step.cu, hq, self.scale, step.max_rows, step.max_keys,
+                             workspace=self._paged_workspace(R, pages, step, h.device))
+        return self._out_mlp(w, h, self._gate(w, h, ssq, o, g))
+
+    def _paged_workspace(self, rows, pages, step, device):
+        """attend_paged's workspace, shared by every layer (stream-ordered reuse)."""
+        need = ops.attend_paged_workspace_bytes(rows, self.n_heads, self.n_kv, self.head_dim, pages.kind, len(step.counts),
+                                                step.max_rows, step.max_keys)
+        ws = getattr(self, "_paged_ws", None)
+        if need and (ws is None or ws.numel() < need or ws.device != device):
+            self._paged_ws = ws = None                  # (the old one back before the larger one is taken)
+            self._paged_ws = ws = torch.empty(need, dtype=torch.uint8, device=device)
+        return ws if need else None
+
+    def _gdn_paged(self, i, w, h, ssq, step, cache):
+        """_gdn_layer for the new rows of several sequences: the products over all rows, the delta rule of each sequence
+        from its own states (updated in place)."""
+        R, H = h.shape
+        gws = self.gemm_workspace
+        pre = ops.norm_linear(h, ssq, self.eps, w["w_in"], workspace=gws(R, w["w_in"].shape[0], H, h.device))
+        out = torch.empty(R, self.nv * self.dv, dtype=torch.bfloat16, device=h.device)
+        ws = self._gdn_forward_workspace(step.max_rows, h.device)
+        r = 0
+        for seq, n in zip(step.seqs, step.counts):
+            st = cache.states(seq, i)
+            if st["rec"] is None:
+                st["rec"] = torch.zeros(self.nv, self.dk, self.dv, dtype=torch.float32, device=h.device)
+            _, st["conv"] = ops.gdn_forward(pre[r:r + n], self.nk, self.nv, self.dk, self.dv, w["conv"], st["conv"],
+                                            w["a_log"], w["dt_bias"], st["rec"], out=out[r:r + n], workspace=ws)
+            r += n
+        z = ops.norm_linear(h, ssq, self.eps, w["wz"], workspace=gws(R, w["wz"].shape[0], H, h.device))
+        return self._out_mlp(w, h, ops.gated_rms_norm(out, z, w["gnorm"], self.nv, self.dv, self.eps))
+
+    def forward_paged(self, cache, seqs, ids):
+        """Exact forward of new tokens of several sequences of a paged cache (a token of each, or a chunk of a prompt):
+        ids[b], the token ids that sequence seqs[b] gets next. Returns the logits of each sequence's last row
+        [len(seqs), V] fp32."""
+        ids = [torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in ids]
+        if len(cache.layers) != self.n_layers or cache.model is not self:
+            raise ValueError("forward_paged: a cache of this model, with every layer packed")
+        h, ssq = self.embed(torch.cat(ids) if ids else torch.empty(0, dtype=torch.int64))
+        step = cache.plan(seqs, [x.numel() for x in ids])
+        for i in range(self.n_layers):
+            h, ssq = self.layer_paged(i, h, step, cache, ssq=ssq)
+        last = step.cu[1:].long() - 1
+        return self.logits(*ops.row_gather(h, last))
 
     def embed(self, ids):
         """Embedding rows of token ids [T] (code/kva/model.py:108-109): a bit-exact row gather from the bf16

@@ -2,12 +2,16 @@
 
 Pages: the pools of one layer as the kernels read them (ops.paged_append, paged_read, attend_paged), in bfloat16 or in 4
 bits (17 / 32 byte a value: E2M1 codes with a power-of-two scale for each 32 values; include/rfill.h has the layout).
+PagedCache: the pages of every attention layer of a FillModel and the states of its GDN layers, for sequences that come
+(empty, or with a cache that finish() or forward_exact() filled), grow (plan(), then FillModel.layer_paged of each layer;
+FillModel.forward_paged does both) and go.
 """
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 BF16, MX4 = 0, 1                        # kinds of pages (RF_PAGES_BF16, RF_PAGES_MX4)
 KINDS = {"bf16": BF16, "mx4": MX4}
@@ -74,3 +78,161 @@ class Pages:
 
     def nbytes(self):
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.ks, self.vs) if t is not None)
+
+
+@dataclass
+class Step:
+    """New tokens of several sequences (PagedCache.plan): sequence b's rows are [cu[b], cu[b + 1]) and become its last
+    tokens. On the device: table (its pages), lens (its tokens with them), cu, and of each row the slot, the position and
+    the RoPE table row."""
+    seqs: list
+    counts: list
+    table: torch.Tensor
+    lens: torch.Tensor
+    cu: torch.Tensor
+    slots: torch.Tensor
+    pos: torch.Tensor
+    cs: torch.Tensor
+    max_rows: int
+    max_keys: int
+
+    @property
+    def rows(self):
+        return sum(self.counts)
+
+
+class _Sequence:
+    def __init__(self):
+        self.tokens = 0
+        self.pages = []
+        self.states = {}                    # GDN layers: conv, rec (own tensors, updated in place)
+
+
+class PagedCache:
+    """n_pages pages of `page` tokens (kind "bf16" or "mx4") in every packed attention layer of model; a page number means
+    the same tokens in each of them. Sequences are named by the integers that add() returns."""
+
+    def __init__(self, model, n_pages, page=64, kind="bf16"):
+        self.model, self.page, self.kind = model, page, kind
+        self.layers = [i for i in range(model.n_layers) if model.W[i] is not None]
+        self.pools = {i: Pages.empty(n_pages, model.n_kv, page, model.head_dim, kind, model.device)
+                      for i in self.layers if model.layer_types[i] == "attn"}
+        self.n_pages = n_pages
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._seqs = {}
+        self._next = 0
+
+    def __contains__(self, seq):
+        return seq in self._seqs
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def nbytes(self):
+        return sum(p.nbytes() for p in self.pools.values())
+
+    def _of(self, seq):
+        if seq not in self._seqs:
+            raise KeyError(f"no sequence {seq!r} in this cache")
+        return self._seqs[seq]
+
+    def tokens(self, seq):
+        return self._of(seq).tokens
+
+    def states(self, seq, i):
+        """GDN layer i's states of the sequence (conv and rec; None before its first token)."""
+        return self._of(seq).states.setdefault(i, dict(conv=None, rec=None))
+
+    def add(self, cache=None):
+        """A new sequence, empty or with the tokens of `cache` (one dict a layer, as FillModel.new_cache: every packed
+        layer filled with as many tokens): K and V are copied into pages, in 4 bits rounded. Returns its name."""
+        s = _Sequence()
+        n = 0
+        if cache is not None:
+            counts = {i: cache[i].get("n" if self.model.layer_types[i] == "attn" else "len", 0) for i in self.layers}
+            n = max(counts.values(), default=0)
+            if any(c != n for c in counts.values()):
+                raise ValueError(f"add: the cache's layers hold {sorted(set(counts.values()))} tokens")
+        self._grow([(s, n)])
+        if n:
+            try:
+                step = self._step([s], [n])
+                for i in self.layers:
+                    c = cache[i]
+                    if i in self.pools:
+                        ops.paged_append(c["kbuf"][:, :n].transpose(0, 1), c["vbuf"][:, :n].transpose(0, 1), step.slots,
+                                         self.pools[i])
+                    else:
+                        s.states[i] = dict(conv=c["conv"].clone(), rec=c["rec"].float().contiguous().clone())
+            except Exception:
+                self._free += reversed(s.pages)
+                raise
+        name = self._next
+        self._next += 1
+        self._seqs[name] = s
+        return name
+
+    def remove(self, seq):
+        """Forget a sequence; its pages are free for the next plan() or add(). (Work that reads them must have been queued
+        on the stream that writes them next.)"""
+        s = self._of(seq)
+        del self._seqs[seq]
+        self._free += reversed(s.pages)
+
+    def plan(self, seqs, counts):
+        """Room for counts[b] new tokens of each sequence seqs[b]: the Step that layer_paged of every layer takes. The
+        sequences count the tokens from now on. Raises MemoryError, with nothing changed, when the pages do not suffice."""
+        if len(seqs) != len(counts) or not len(seqs):
+            raise ValueError(f"plan: {len(seqs)} sequences, {len(counts)} counts")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("plan: a sequence is named twice")
+        if any(int(c) < 1 for c in counts):
+            raise ValueError(f"plan: counts {list(counts)} (at least one token each)")
+        ss, counts = [self._of(q) for q in seqs], [int(c) for c in counts]
+        self._grow(list(zip(ss, counts)))
+        return self._step(ss, counts, list(seqs))
+
+    def _grow(self, wants):
+        need = [-(-(s.tokens + n) // self.page) - len(s.pages) for s, n in wants]
+        if sum(need) > len(self._free):
+            raise MemoryError(f"{sum(need)} pages wanted, {len(self._free)} of {self.n_pages} free")
+        for (s, n), m in zip(wants, need):
+            s.pages += [self._free.pop() for _ in range(m)]
+            s.tokens += n
+
+    def _step(self, ss, counts, seqs=None):
+        dev = self.model.device
+        width = max(1, max(len(s.pages) for s in ss))
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+        table = i32([s.pages + [-1] * (width - len(s.pages)) for s in ss])
+        lens, cu = i32([s.tokens for s in ss]), i32(cu)
+        if not self.pools:                  # GDN layers alone: no slots
+            slots = pos = cs = None
+        else:
+            slots, pos = ops.paged_slots(table, lens, cu, sum(counts), next(iter(self.pools.values())))
+            cs = self.model.rope_table(pos)
+        return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(s.tokens for s in ss))
+
+    def read(self, seq):
+        """The sequence's cache as FillModel.new_cache lays it out (bf16 buffers of its own; of 4-bit pages what they hold)."""
+        s = self._of(seq)
+        out = self.model.new_cache()
+        step = self._step([s], [s.tokens]) if s.tokens else None
+        for i in self.layers:
+            if step is None:
+                continue
+            if i in self.pools:
+                c, n = out[i], s.tokens
+                self.model.reserve(c, n, self.model.n_kv, self.model.head_dim, self.model.device)
+                k, v = ops.paged_read(self.pools[i], step.slots)
+                c["kbuf"][:, :n].copy_(k.transpose(0, 1))
+                c["vbuf"][:, :n].copy_(v.transpose(0, 1))
+                self.model.commit(c, n)
+            else:
+                st = self.states(seq, i)
+                out[i].update(conv=st["conv"].clone(), rec=st["rec"].clone(), len=s.tokens)
+        return out

@@ -130,3 +130,46 @@ def test_oracle_four_bit_values():
     x[0, 3] = float("inf")
     c, b = OP.mx4_encode(x)
     assert int(b) == 255 and bool(OP.mx4_decode(c, b).isnan().all())
+
+
+class _Stub:
+    """What PagedCache asks of a model; GDN layers alone need no pools on a GPU."""
+    n_layers, n_kv, head_dim, layer_types, device = 2, 1, 64, ["gdn", "gdn"], torch.device("cpu")
+    W = [dict(kind="gdn"), dict(kind="gdn")]
+
+    def new_cache(self):
+        return [dict() for _ in range(self.n_layers)]
+
+
+def test_page_accounting():
+    """Pages come and go with the sequences; a plan that cannot be met or is malformed changes nothing."""
+    from rfill.paged import PagedCache
+    c = PagedCache(_Stub(), 10, page=16)
+    a, b = c.add(), c.add()
+    step = c.plan([a, b], [17, 16])
+    assert c.free_pages == 7 and c.tokens(a) == 17 and step.rows == 33 and step.max_rows == 17 and step.max_keys == 17
+    assert step.cu.tolist() == [0, 17, 33] and step.lens.tolist() == [17, 16]
+    assert step.table.tolist() == [[0, 1], [2, -1]]
+    step = c.plan([b], [1])
+    assert step.table.tolist() == [[2, 3]] and step.lens.tolist() == [17] and step.max_rows == 1
+    for seqs, counts, error in (([a, b], [100, 100], MemoryError), ([a, a], [1, 1], ValueError), ([a], [0], ValueError),
+                                ([a], [1, 1], ValueError), ([], [], ValueError), ([a, 99], [1, 1], KeyError)):
+        with pytest.raises(error):
+            c.plan(seqs, counts)
+        assert c.free_pages == 6 and c.tokens(a) == c.tokens(b) == 17
+    c.remove(a)
+    assert c.free_pages == 8 and a not in c and b in c
+    with pytest.raises(KeyError):
+        c.tokens(a)
+    state = dict(conv=torch.zeros(3, 8), rec=torch.ones(1, 4, 4), len=20)
+    d = c.add([dict(state), dict(state)])
+    assert c.tokens(d) == 20 and c.free_pages == 6 and d not in (a, b)
+    c.states(d, 0)["rec"].zero_()
+    assert float(state["rec"].sum()) == 16                    # the sequence has states of its own
+    with pytest.raises(ValueError):
+        c.add([dict(state), dict(state, len=21)])
+    with pytest.raises(MemoryError):
+        c.add([dict(state, len=200), dict(state, len=200)])
+    with pytest.raises(KeyError):
+        c.add([dict(len=20), dict(len=20)])                    # no states: its pages are given back
+    assert c.free_pages == 6
