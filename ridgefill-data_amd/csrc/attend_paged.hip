@@ -938,7 +938,14 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
       }
       for (; i < mine; ++i) {
         edge_step<D, false>(tl[0], qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
-        if (i + 1 < mine) {
+        if constexpr (NT > 1) {                                // the next one is here, the one after it on its way
+          tl[0] = tl[1];
+          if (i + 2 < mine) {
+            window(i + 2);
+            get_k(tl[1], i + 2);
+            get_v(tl[1], i + 2);
+          }
+        } else if (i + 1 < mine) {
           window(i + 1);
           get_k(tl[0], i + 1);
           get_v(tl[0], i + 1);
@@ -1362,11 +1369,12 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a) {
   const float *first, *rest;
   int64_t step;
   if constexpr (RUNS) {                                      // runs of tiles: its own run's last piece (or first), then first pieces
+    const int run = *a.length;
     Seq s0{0, 0, 0};
     if ((t & 63) < a.n_seq) s0 = seq_of(a, t & 63);
     const Piece u = piece_at(a, s0, blockIdx.x / a.hkv, true, t & 63);
     if (u.b < 0) return;
-    const int run = *a.length, x0 = u.begin / run;
+    const int x0 = u.begin / run;
     ns = (u.begin + u.nt - 1) / run - x0 + 1;
     if (u.begin < 0 || x0 + ns > a.fit) return;              // (only with a cu that does not rise: more tiles than 31 bits count)
     const RowBlock r(a, u.s, u.rb);
