@@ -190,6 +190,7 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
     if (want < before + total) {
       // (scalar from here on: what follows from a unit is uniform over its block)
       const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
+      if (!hit) return u;                 // (sums past 31 bits: only with a cu that does not rise)
       const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
       const int at = want - before - __builtin_amdgcn_readlane(pre, l);
       u.b = b0 + l;
@@ -230,6 +231,7 @@ __device__ __forceinline__ Piece piece_at(const PagedArgs& a, const Seq& s0, int
     if (!by_block) total = tiles;
     if (want < before + total) {
       const uint64_t hit = __ballot(n > 0 && before + pre <= want && want < before + pre + n);
+      if (!hit) return pc;                 // (sums past 31 bits: only with a cu that does not rise)
       const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
       const int off = want - before - __builtin_amdgcn_readlane(pre, l);
       pc.b = b0 + l;
@@ -970,6 +972,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
             make_float4(st.o[b][j], st.o[b + 1][j], st.o[b + 2][j], st.o[b + 3][j]);
     __syncthreads();
     const int rw = t >> 4, d0 = (t & 15) * NB;
+    const bool odd = marks[D] != 0;                            // (read between barriers: a wave ahead may mark the next piece)
     float top = -INFINITY;
 #pragma unroll
     for (int x = 0; x < NW; ++x) top = fmaxf(top, ml[x * 16 + rw]);
@@ -990,14 +993,13 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
         acc[b + 3] += v.w * f;
       }
     }
-    if (marks[D]) {
+    if (odd) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) acc[b] += marked((marks[(rw * D + d0 + b) / 16] >> (2 * ((d0 + b) % 16))) & 3u);
     }
     if (rw < r.rows) finish_row<D, NB>(a, u.s.first + r.q0, r.off, whole_block, part, rw, head, d0, acc, top, sum);
     __syncthreads();                                           // the next piece takes the LDS
-    if (marks[D]) {
-      __syncthreads();
+    if (odd) {
       for (int x = t; x <= D; x += 64 * NW) marks[x] = 0u;
       __syncthreads();
     }

@@ -474,6 +474,95 @@ def test_pages_past_32_bit_offsets(dev):
     check(got, want.flatten(1), size.flatten(1), "far pages")
 
 
+def test_far_four_bit_pages(dev):
+    """The same of 4-bit pages, codes and scales, with one row and with a chunk."""
+    from rfill import ops
+    from rfill.paged import Pages
+    hq, hkv, d, page, n_pages = 4, 2, 64, 16, 3
+    far = lambda: torch.empty(2 * (3 << 30) + 4096, dtype=torch.uint8, device=dev)   # noqa: E731  3 GiB from page to page
+    view = lambda *s: far().as_strided((n_pages, *s), (3 << 30, *torch.empty(s, device="meta").stride()))   # noqa: E731
+    pages = Pages(view(hkv, page, d // 2), view(hkv, page // 8, 16, 8, d // 32), view(hkv, page // 8, d // 32, 8),
+                  view(hkv, page // 8, d // 32, 8))
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(40, hkv, d, generator=g).to(torch.bfloat16) for _ in "kv")
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    at = torch.arange(40)
+    slots = (table[0, at // page].long() * page + at % page).to(dev)
+    ops.paged_append(k.to(dev), v.to(dev), slots, pages)
+    rk, rv = (x.cpu().double() for x in ops.paged_read(pages, slots))
+    for x, y in ((k, rk), (v, rv)):
+        code, scale = OP.mx4_encode(x.float())
+        assert torch.equal(OP.mx4_decode(code, scale).double(), y)
+    for rows in (1, 40):
+        q = torch.randn(rows, hq * d, generator=g).to(torch.bfloat16)
+        want, size = OP.attend(q.view(rows, hq, d), rk, rv, torch.ones(40, dtype=torch.bool), d ** -0.5)
+        got = ops.attend_paged(q.to(dev), pages, table.to(dev), torch.tensor([40], dtype=torch.int32, device=dev),
+                               torch.tensor([0, rows], dtype=torch.int32, device=dev), hq, d ** -0.5, rows, 40)
+        check(got, want.flatten(1), size.flatten(1), rows)
+
+
+@pytest.mark.parametrize("hq,hkv,d,mx", [(6, 2, 256, False), (12, 1, 256, True), (20, 1, 256, False), (7, 1, 64, False),
+                                         (40, 2, 128, True), (64, 2, 64, True), (5, 1, 128, False)])
+def test_row_blocks_within_a_query(dev, hq, hkv, d, mx):
+    """Groups that do not divide a block of 16, 128 or 256 query rows: blocks begin and end among a query's heads."""
+    for rows, lens in (([3, 1, 7, 11], [300, 5, 1000, 64]), ([1, 1], [2100, 31]), ([60, 33], [60, 150])):
+        pools, table, n_pages, q = batch(hq, hkv, d, 16, mx, rows, lens, d + hq)
+        want, size = oracle_attend(pools, table, n_pages, q, rows, lens, hq, d ** -0.5)
+        for kw in (dict(), dict(max_keys=1 << 20), dict(max_rows=1 << 20)):
+            check(run(dev, pools, table, q, rows, lens, hq, d ** -0.5, **kw), want, size, (rows, kw))
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_runs_over_sequences(dev, mx):
+    """Runs of tiles that hold the end of one sequence, all of some and the beginning of another; a value that is NaN in one
+    of them reaches that sequence's column alone."""
+    hq = hkv = 32
+    d, page = 64, 16
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(1, 700, (40,), generator=g).tolist()
+    lens[11], lens[12], lens[20] = 5000, 1, 0
+    rows = [min(n, 1) for n in lens]
+    pools, table, n_pages, q = batch(hq, hkv, d, page, mx, rows, lens, 4)
+    want, size = oracle_attend(pools, table, n_pages, q, rows, lens, hq, d ** -0.5)
+    check(run(dev, pools, table, q, rows, lens, hq, d ** -0.5, max_keys=1 << 20), want, size, "runs")
+    at = (lens[5] - 1) % page                                  # the last token of sequence 5, head 0
+    last = int(table[5, (lens[5] - 1) // page])
+    if mx:
+        pools.vs[last, 0, at // 8, 1, at % 8] = 255            # its second block of 32 columns
+        hit = slice(32, 64)
+    else:
+        pools.v[last, 0, at, 7] = float("nan")
+        hit = slice(7, 8)
+    got = run(dev, pools, table, q, rows, lens, hq, d ** -0.5, max_keys=1 << 20).cpu()
+    row = sum(rows[:5])
+    assert bool(got[row, hit].isnan().all())
+    got[row, hit], want[row, hit] = 0, 0
+    check(got, want, size, "with a NaN")
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("max_rows", [3, 200])
+def test_sizes_that_contradict_each_other(dev, mx, max_rows):
+    """Offsets that fall, lengths below zero and past the table, pages that are none: rows of sound sequences stay right."""
+    from rfill import ops
+    hq, hkv, d, page = 8, 2, 128, 16
+    pools, table, n_pages, q = batch(hq, hkv, d, page, mx, [3, 1, 1], [50, 20, 33], 9)
+    want, size = oracle_attend(pools, table, n_pages, q[:3], [3], [50], hq, d ** -0.5)
+    t = torch.cat((table, table.flip(0)))[:5].contiguous()
+    t[3:] = torch.tensor(1 << 30)
+    pages = pages_on(pools, dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    for keys in (64, 1 << 20):
+        lens, cu = i32([50, -4, 1 << 30, 7, -(1 << 31)]), i32([0, 3, 3, -5, (1 << 31) - 1, 4])
+        ops.attend_paged(q.to(dev), pages, t.to(dev), lens, cu, hq, d ** -0.5, max_rows, keys)
+        torch.cuda.synchronize()
+        slots, pos = ops.paged_slots(t.to(dev), lens, cu, 5, pages)
+        assert bool(((slots >= -1) & (slots < n_pages * page)).all())
+        cu = i32([0, 3, 3, 3, 3, 3])
+        got = ops.attend_paged(q.to(dev), pages, t.to(dev), lens, cu, hq, d ** -0.5, max_rows, keys)
+        check(got[:3], want, size, keys)
+
+
 def test_many_sequences(dev):
     """More sequences than a wave looks at at once, most of them empty."""
     hq, hkv, d, page = 4, 2, 64, 16
