@@ -635,13 +635,15 @@ int rf_paged_read(const rf_pages* pages, const int64_t* slots, int64_t T, uint16
  * [cu[b], cu[b + 1]) of q [T, hq d] (row stride ldq), its last tokens: with n of them, query i is at position
  * p = lens[b] - n + i and sees keys 0 .. p of the sequence's pages (table as rf_paged_slots). out row (row stride ldo) =
  * sum_j softmax_j(scale q . k_j) v_j, scores and softmax in fp32, the probabilities rounded to bf16 for the second
- * product; zeros for a query that sees no key (position before 0, or every page outside [0, n_pages)). Keys outside a
+ * product (4-bit pages: a query's values below 2^-14 of the largest of their 32 are taken to 2^-22 of it); zeros for a
+ * query that sees no key (position before 0, or every page outside [0, n_pages)). Keys outside a
  * query's sight never touch its output, whatever they hold; rows of no sequence are left as they were.
  * lens, cu and table are read on the device, so a captured call follows them: max_rows bounds the rows of a sequence and
  * max_keys its tokens (host values; a sequence with more rows than max_rows or more tokens than max_keys, or than its
  * table, is taken as that much; they also choose the kernel). Any hq / hkv up to 64. The workspace (device memory, 16-byte
  * aligned) of rf_attend_paged_workspace_bytes lets the keys of a sequence be split over blocks, whose parts are merged in
- * a fixed order; with a smaller one or NULL they are not split. */
+ * a fixed order; with a smaller one or NULL they are not split. Its content need not be kept or cleared between calls;
+ * calls that may run at once need one each. */
 int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages, const int32_t* table,
                     int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu, int n_seq,
                     int64_t max_rows, int64_t max_keys, float scale, uint16_t* out, int64_t ldo, void* workspace,

@@ -88,9 +88,41 @@ __device__ __forceinline__ uint32_t encode8(const float (&f)[8], uint32_t& byte)
   return byte == 255u ? 0u : c;
 }
 
+// Sum over the D / 8 lanes of a head vector, by data-parallel moves within rows of 16 (a sum's two sides in either order).
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xf, 0xf, true);
+  return __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+
+template <int D>
+__device__ __forceinline__ double vector_sum(double s) {
+  s += moved<0xb1>(s);                                       // lanes ^ 1, ^ 2, mirrored in 8, in 16
+  s += moved<0x4e>(s);
+  s += moved<0x141>(s);
+  if constexpr (D > 64) s += moved<0x140>(s);
+  if constexpr (D > 128) s += __shfl_xor(s, 16, 64);
+  return s;
+}
+
+// 1 / sqrt(mean of squares + eps) from the lane's 8 values: the squares of bf16 values and nearly always their sum are exact
+// in fp64; the instruction's root gets one step of Newton's. (With the library's root and quotient, sums through LDS and every
+// partner normed twice, 6200 rows of 32 query and 8 K / V heads into 4 bits took 38 us, now 35; their 134 MB take 26.)
+template <int D>
+__device__ __forceinline__ float inverse_rms(const float (&f)[8], float eps) {
+  double s = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), s);
+  const double m = vector_sum<D>(s) * (1.0 / D) + static_cast<double>(eps), y = __builtin_amdgcn_rsq(m);
+  return static_cast<float>(m < 1e300 ? y * fma(-0.5 * m * y, y, 1.5) : y);       // (an infinity's root is 0)
+}
+
 // D / 8 lanes a head vector, 8 values a lane; blockIdx.y is the head of [queries | keys | values], blockIdx.x a run of
 // rows: the rows of one head lie side by side in a block, so that the codes of a page's tokens, side by side in memory, are
-// written together. A lane loads its 16 bytes and those of its rotation partner (d / 2 apart or less, in L1).
+// written together. Heads that stay bf16: a lane takes 4 values and their rotation partners. Keys that become codes: 8 values
+// side by side, for a block's scale comes from 4 lanes, and their partners once more (d / 2 apart or less, in L1).
 template <int D, bool MX>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;
@@ -104,29 +136,61 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   const uint16_t* src = is_q ? a.q + rr * a.ld_q + h * D
                              : is_v ? a.v + rr * a.ld_v + h * a.head_v : a.k + rr * a.ld_k + h * a.head_k;
   const int64_t slot = is_q ? 0 : a.slots[rr];
+  const uint16_t* gain = is_q ? a.qnorm : a.knorm;
+  const int half = a.cs ? a.rot >> 1 : 0;
+  const bool turn = j0 < 2 * half;
   float f[8];
-  uint4 raw = *reinterpret_cast<const uint4*>(src + j0);
-  bool same = is_v;                                          // values that are written as they came
-  if (!is_v) {
-    const uint16_t* gain = is_q ? a.qnorm : a.knorm;
-    const int half = a.cs ? a.rot >> 1 : 0;
-    const bool turn = j0 < 2 * half, low = j0 < half;
+  if (is_q || (!MX && !is_v)) {
+    const int ja = turn ? 4 * c : j0, jb = turn ? half + 4 * c : j0 + 4;
+    const uint2 xa = *reinterpret_cast<const uint2*>(src + ja), xb = *reinterpret_cast<const uint2*>(src + jb);
+    uint4 raw = make_uint4(xa.x, xa.y, xb.x, xb.y);
+    unpack8(f, raw);
+    if (gain) {
+      const uint2 ga = *reinterpret_cast<const uint2*>(gain + ja), gb = *reinterpret_cast<const uint2*>(gain + jb);
+      normed(f, make_uint4(ga.x, ga.y, gb.x, gb.y), a.norm_kind, inverse_rms<D>(f, a.eps));
+    }
+    if (turn) {
+#pragma clang fp contract(off)
+      const uint16_t* tab = a.cs + rr * a.rot + 4 * c;
+      const uint2 cv = *reinterpret_cast<const uint2*>(tab), sv = *reinterpret_cast<const uint2*>(tab + half);
+      const uint4 cs = make_uint4(cv.x, cv.y, sv.x, sv.y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float co = bf2f(lane_of(cs, e)), si = bf2f(lane_of(cs, e + 4)), x = f[e], y = f[e + 4];
+        const float xc = x * co, ys = y * si, yc = y * co, xs = x * si;
+        f[e] = xc - ys;
+        f[e + 4] = yc + xs;
+      }
+    }
+    if (gain || turn)
+      raw = make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+    const int64_t page = slot >> a.pg.shift;
+    if (!in || slot < 0 || page >= a.pg.n_pages) return;     // (queries: slot 0)
+    uint16_t* dst;
+    if (is_q) {
+      dst = a.q_out + row * a.ld_qo + h * D;
+    } else {
+      const int tok = static_cast<int>(slot) & ((1 << a.pg.shift) - 1);
+      dst = reinterpret_cast<uint16_t*>(a.pg.k + page * a.pg.page_stride + static_cast<int64_t>(h) * a.pg.head_bytes) + tok * D;
+    }
+    *reinterpret_cast<uint2*>(dst + ja) = make_uint2(raw.x, raw.y);
+    *reinterpret_cast<uint2*>(dst + jb) = make_uint2(raw.z, raw.w);
+    return;
+  }
+  const uint4 raw = *reinterpret_cast<const uint4*>(src + j0);
+  if (MX && !is_v) {
+    const bool low = j0 < half;
     const int jp = half == 4 || !turn ? j0 : low ? j0 + half : j0 - half;
-    const uint4 rawp = *reinterpret_cast<const uint4*>(src + jp);
+    uint4 rawp = raw;
+    if (turn) rawp = *reinterpret_cast<const uint4*>(src + jp);
     float p[8];
     unpack8(f, raw);
     unpack8(p, rawp);
     if (gain) {
-      double s = 0;                                          // squares of bf16 values: exact, and nearly always their sum
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), s);
-#pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o, 64);
-      const float r = static_cast<float>(1.0 / sqrt(s * (1.0 / D) + static_cast<double>(a.eps)));
+      const float r = inverse_rms<D>(f, a.eps);
       normed(f, *reinterpret_cast<const uint4*>(gain + j0), a.norm_kind, r);
       normed(p, *reinterpret_cast<const uint4*>(gain + jp), a.norm_kind, r);
     }
-    same = !gain && !turn;
     if (turn) {
 #pragma clang fp contract(off)
       const uint16_t* tab = a.cs + rr * a.rot;
@@ -147,20 +211,11 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
       }
     }
   }
-  if (!MX || is_q) {
-    if (!same)
-      raw = make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
-    if (!in) return;
-    if (is_q) {
-      *reinterpret_cast<uint4*>(a.q_out + row * a.ld_qo + h * D + j0) = raw;
-      return;
-    }
+  if (!MX) {                                                 // values as they came
     const int64_t page = slot >> a.pg.shift;
-    if (slot < 0 || page >= a.pg.n_pages) return;
+    if (!in || slot < 0 || page >= a.pg.n_pages) return;
     const int tok = static_cast<int>(slot) & ((1 << a.pg.shift) - 1);
-    char* dst = (is_v ? a.pg.v : a.pg.k) + page * a.pg.page_stride + static_cast<int64_t>(h) * a.pg.head_bytes +
-                (tok * D + j0) * 2;
-    *reinterpret_cast<uint4*>(dst) = raw;
+    *reinterpret_cast<uint4*>(a.pg.v + page * a.pg.page_stride + static_cast<int64_t>(h) * a.pg.head_bytes + (tok * D + j0) * 2) = raw;
     return;
   }
   if (is_v) unpack8(f, raw);

@@ -1121,7 +1121,8 @@ def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=N
     b's rows [cu[b], cu[b + 1]) are its last tokens of lens[b], in the pages table[b] lists in order (table int32 [n, width],
     lens int32 [n], cu int32 [n + 1], all on the device). max_rows / max_keys: host bounds on a sequence's rows and tokens
     (more of either is not looked at). Returns [rows, hq d] bf16; a row that sees no key gets zeros, a row of no sequence is
-    left as it was. workspace: uint8 device memory for splits of the keys ("auto": allocated here; None: no split)."""
+    left as it was. workspace: uint8 device memory for splits of the keys ("auto": allocated here; None: no split; calls that
+    may run at once need one each)."""
     _need(q, "q", torch.bfloat16, 2)
     n = _sequences(table, lens, cu)
     rows, d = q.shape[0], pages.d
