@@ -3,21 +3,21 @@
 // k_paged_few: a few query rows a sequence (one token of each, or some drafted ones). The keys are read once from HBM and
 // that read is the bound: a block takes one K / V head and 16 query rows (queries x the query heads of the K / V head, query
 // by query) of one sequence, its four waves take turns at the key tiles (32 keys) of the block's run, with no barrier until
-// they join. bf16 tiles go straight from memory into the registers of the products; 4-bit ones, half the bytes a product,
-// through a ring of four tiles in LDS a wave, which keeps enough of them in flight. Per tile and wave:
+// they join. bf16 tiles go straight from memory into the registers of the products; 4-bit ones, a quarter of the bytes a
+// product, through a ring in LDS a wave, which keeps enough of them in flight. Per tile and wave:
 //   S^T = K Q^T. A's row m of key half kb is key 8 (m / 4) + 4 kb + m % 4 of the tile, so that lane (n, g) (n = lane % 16,
 //       g = lane / 16) holds, for query row n, the scores of keys 8 g .. 8 g + 7: the order in which A of the second product
 //       wants them. bf16: v_mfma_f32_16x16x32_bf16, the contraction's order over d as memory gives it (16-byte chunk 4 s + g
 //       in step s). 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4, which takes codes and scales as they are; the queries as two
-//       E4M3 terms (load_queries).
+//       E4M3 terms (split_queries).
 //   Softmax in fp32 base 2, the running maximum raised only when a score exceeds it by 2^8 (lazily: O is rescaled rarely).
 //   O += P V on v_mfma_f32_16x16x32_bf16: B's column n of product nb is d = n (D / 16) + nb, so a lane reads D / 16 consecutive
 //       values of each of its 8 keys and transposes 2 x 2 with v_perm (half an instruction a value); O's columns of a lane are
 //       consecutive in memory again. 4-bit values become bf16 by v_cvt_scalef32_pk_bf16_fp4, scale included, exactly. (P in
 //       8 bits or less would round the probabilities by 2^-4 and more; they keep bf16's 2^-8.)
 // The waves' parts are merged through LDS in wave order. Measured, merge included: 32 sequences of 500 to 8111 keys, 8 heads of
-// 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 95 us for 405 MB; one of 122880 keys in 4
-// bits, 2 heads of 256, 31 us for 67 MB: of that 7 are the merge and 10 the launch, the first tiles' way and the end.
+// 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 94 us for 405 MB; one of 122880 keys in 4
+// bits, 2 heads of 256, 30 us for 67 MB: of that 7 are the merge and 10 the launch, the first tiles' way and the end.
 #include <stdint.h>
 
 #include <algorithm>
@@ -315,13 +315,17 @@ __device__ __forceinline__ void load_v(VTile<D, false>& vt, const PagesDev& pg, 
   }
 }
 
-// 4 bits: a wave's ring of tiles in LDS, as they lie in memory: 32 keys' codes (16 D bytes), their values' (16 D), the keys'
-// scales (D) and the values' (D; 256 bytes for both at least, as their loads write).
+// 4 bits: a wave's ring of tiles in LDS, as they lie in memory, keys and values apart: 32 keys' codes (16 D bytes) and their
+// scales (D; 256 bytes at least, as their load writes). Two turns of T tiles: while one is computed the other is on its way,
+// and each half is loaded again as soon as it has been read. (head_dim 256: with two tiles a turn the LDS holds four waves, one
+// a SIMD; with one tile two a SIMD: 9 sequences of 5 new tokens and up to 30011 keys 49 -> 43 us, 1024 rows of 8007 keys 285 ->
+// 232. An order of its 16-byte chunks that spreads every read over all banks changed nothing: the conversion of the values
+// bounds it, 64 v_cvt_scalef32_pk_bf16_fp4 and as many v_perm a tile.)
 template <int D>
 struct Ring {
-  static constexpr int R = 4;                                // tiles
-  static constexpr int SLOT = 32 * D + (D < 128 ? 256 : 2 * D);
-  static constexpr int L = D == 64 ? 3 : D == 128 ? 5 : 10;  // load instructions a tile
+  static constexpr int T = D == 256 ? 1 : 2, R = 2 * T;      // tiles a turn, tiles
+  static constexpr int HALF = 16 * D + (D < 256 ? 256 : D), SLOT = 2 * HALF;
+  static constexpr int L = (D == 64 ? 1 : D / 64) + 1;       // load instructions a half
   static constexpr int BYTES = R * SLOT + 256;               // and the coming window's table entries
 };
 
@@ -340,22 +344,22 @@ __device__ __forceinline__ void read_k(KTile<D, true>& kt, const char* slot, int
     }
 #pragma unroll
   for (int s = 0; s < (D == 256 ? 2 : 1); ++s)
-    kt.sc[s] = *reinterpret_cast<const uint2*>(slot + 32 * D + (n >> 2) * (D / 4) + (4 * s + gd) * 8);
+    kt.sc[s] = *reinterpret_cast<const uint2*>(slot + 16 * D + (n >> 2) * (D / 4) + (4 * s + gd) * 8);
 }
 
 template <int D>
 __device__ __forceinline__ void read_v(VTile<D, true>& vt, const char* slot, int n, int g) {
   constexpr int VL = D / 16;
-  const char* run = slot + 16 * D + g * (4 * D) + n * (VL * 4);         // 8 keys x VL / 2 bytes
+  slot += Ring<D>::HALF;
 #pragma unroll
   for (int i = 0; i < VL / 4; ++i) {
-    const uint4 w = *reinterpret_cast<const uint4*>(run + 16 * i);
+    const uint4 w = *reinterpret_cast<const uint4*>(slot + g * (4 * D) + n * (VL * 4) + 16 * i);       // 8 keys x VL / 2 bytes
     vt.c[4 * i] = w.x;
     vt.c[4 * i + 1] = w.y;
     vt.c[4 * i + 2] = w.z;
     vt.c[4 * i + 3] = w.w;
   }
-  vt.sc = *reinterpret_cast<const uint2*>(slot + 33 * D + g * (D / 4) + (n * VL / 32) * 8);
+  vt.sc = *reinterpret_cast<const uint2*>(slot + 16 * D + g * (D / 4) + (n * VL / 32) * 8);
 }
 
 // Loads from memory into LDS (64 lanes side by side from lds on), without destination registers: the kernel's own waits
@@ -382,35 +386,20 @@ __device__ __forceinline__ void wait_loads() {
 }
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// A tile into the slot at lds: its 16-key halves' codes lie o0, o1 bytes into the pools (keys' rows and values' runs alike), their
-// scales s0, s1.
+// A tile's keys or values into the half slot at lds: its 16-key halves' codes lie o0, o1 bytes into the pool (keys' rows and
+// values' runs alike), their scales s0, s1.
 template <int D>
-__device__ __forceinline__ void issue_tile(uint32_t lds, const PagesDev& pg, int64_t o0, int64_t o1, int64_t s0, int64_t s1, int lane) {
-  if constexpr (D == 64) {                                   // 512 bytes a half: lanes 0 .. 31 and 32 .. 63
-    const int64_t o = (lane < 32 ? o0 : o1) + (lane & 31) * 16;
-    to_lds16(lds, pg.k + o);
-    to_lds16(lds + 1024, pg.v + o);
+__device__ __forceinline__ void issue_half(uint32_t lds, const char* codes, const uint8_t* scales, int64_t o0, int64_t o1, int64_t s0,
+                                           int64_t s1, int lane) {
+  if constexpr (D == 64) {                                   // 512 bytes a 16-key half: lanes 0 .. 31 and 32 .. 63
+    to_lds16(lds, codes + (lane < 32 ? o0 : o1) + (lane & 31) * 16);
   } else {
-    constexpr int I = D / 128;                               // 1 KB instructions a half
-    const uint32_t off = 16 * lane;
+    constexpr int I = D / 128;                               // 1 KB instructions a 16-key half
 #pragma unroll
-    for (int x = 0; x < I; ++x) {
-      to_lds16(lds + 1024 * x, pg.k + o0 + 1024 * x, off);
-      to_lds16(lds + 1024 * (I + x), pg.k + o1 + 1024 * x, off);
-      to_lds16(lds + 1024 * (2 * I + x), pg.v + o0 + 1024 * x, off);
-      to_lds16(lds + 1024 * (3 * I + x), pg.v + o1 + 1024 * x, off);
-    }
+    for (int x = 0; x < 2 * I; ++x) to_lds16(lds + 1024 * x, codes + (x < I ? o0 : o1) + 1024 * (x % I), 16 * lane);
   }
-  constexpr int H = D / 8;                                   // dwords of a half's scales
-  if constexpr (D == 256) {
-    const int64_t s = (lane < 32 ? s0 : s1) + (lane & 31) * 4;
-    to_lds4(lds + 32 * D, pg.ks + s);
-    to_lds4(lds + 33 * D, pg.vs + s);
-  } else {                                                   // keys' halves, values' halves; past them they are repeated
-    const int part = (lane / H) & 3;
-    const int64_t s = ((part & 1) ? s1 : s0) + (lane % H) * 4;
-    to_lds4(lds + 32 * D, (part & 2) ? pg.vs + s : pg.ks + s);
-  }
+  constexpr int H = D / 8;                                   // dwords of a 16-key half's scales; past both they are repeated
+  to_lds4(lds + 16 * D, scales + (((lane / H) & 1) ? s1 : s0) + (lane % H) * 4);
 }
 
 // A row block's queries as the products' operands. bf16: 32-deep steps. 4 bits: the matrix instruction takes codes and scales
@@ -429,8 +418,38 @@ __device__ __forceinline__ uint32_t fp8x4(float a, float b, float c, float d) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
 
+// The values of a lane: 16 of each 128, and 16 more 64 on.
 template <int D>
-__device__ __forceinline__ void load_queries(Queries<D, true>& q, const uint16_t* row, int g, int lane) {
+struct RawQueries {
+  uint4 x[D / 128 + (D == 64)][D > 64 ? 2 : 1][2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_queries(RawQueries<D>& q, const uint16_t* row, int g) {
+#pragma unroll
+  for (int s = 0; s < (D == 256 ? 2 : 1); ++s)
+#pragma unroll
+    for (int h = 0; h < (D > 64 ? 2 : 1); ++h)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) q.x[s][h][x] = *reinterpret_cast<const uint4*>(row + 128 * s + 64 * h + 16 * g + 8 * x);
+}
+
+// (here, and not behind the loads into LDS that follow, which the compiler does not count)
+template <int D>
+__device__ __forceinline__ void arrived(RawQueries<D>& q) {
+#pragma unroll
+  for (int s = 0; s < (D == 256 ? 2 : 1); ++s)
+#pragma unroll
+    for (int h = 0; h < (D > 64 ? 2 : 1); ++h)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint4& v = q.x[s][h][x];
+        asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+      }
+}
+
+template <int D>
+__device__ __forceinline__ void split_queries(Queries<D, true>& q, const RawQueries<D>& raw, int g, int lane) {
 #pragma unroll
   for (int s = 0; s < (D == 256 ? 2 : 1); ++s) {
     int e[2];
@@ -438,8 +457,7 @@ __device__ __forceinline__ void load_queries(Queries<D, true>& q, const uint16_t
     for (int h = 0; h < 2; ++h) {
       uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};              // 16 values
       if (D > 64 || h == 0) {
-        const uint4 a = *reinterpret_cast<const uint4*>(row + 128 * s + 64 * h + 16 * g);
-        const uint4 b = *reinterpret_cast<const uint4*>(row + 128 * s + 64 * h + 16 * g + 8);
+        const uint4 a = raw.x[s][D > 64 ? h : 0][0], b = raw.x[s][D > 64 ? h : 0][1];
         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
       }
       int top = 0;
@@ -693,7 +711,7 @@ __device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D
 }
 
 // Blocks a CU that the registers of a kernel hold (4 bits: and its rings the LDS).
-constexpr int few_blocks(int d) { return d == 256 ? 1 : 2; }
+constexpr int few_blocks(int d, bool mx) { return d == 256 && !mx ? 1 : 2; }
 
 template <int D, bool MX>
 struct FewLds {
@@ -703,7 +721,7 @@ struct FewLds {
 };
 
 template <int D, bool MX>
-__global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArgs a) {
+__global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(PagedArgs a) {
   constexpr int NB = D / 16;
   using F = FewLds<D, MX>;
   __shared__ uint4 lds4[F::BYTES / 16];
@@ -749,6 +767,18 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
       return it < it1 && at < a.width ? row[at] : -1;
     };
     int ids = entry(0);
+    // queries: row n. Their loads go before the tiles', which wait for the table's entries (behind them, 2 us later a piece)
+    Queries<D, MX> qf;
+    [[maybe_unused]] RawQueries<D> raw;
+    const int qx = r.off + min(n, r.rows - 1), qi = qx / a.rep;            // (rows past the last repeat it, and see nothing)
+    const int pos = n < r.rows ? p0 + qi : -1;
+    const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + r.q0 + qi) * a.ldq + (head * a.rep + qx - qi * a.rep) * D;
+    if constexpr (MX) {
+      load_queries<D>(raw, qrow, g);
+    } else {
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) qf.x[s] = as_frag(*reinterpret_cast<const uint4*>(qrow + 32 * s + 8 * g));
+    }
     [[maybe_unused]] int coming = MX ? 0 : entry(32);
     uint64_t bad;
     auto settle = [&]() {
@@ -757,20 +787,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
       bad = __ballot(out);
     };
     settle();
-    // queries: row n
-    Queries<D, MX> qf;
-    int pos;
-    auto queries = [&]() {
-      const int x = r.off + min(n, r.rows - 1), qi = x / a.rep;            // (rows past the last repeat it, and see nothing)
-      pos = n < r.rows ? p0 + qi : -1;
-      const uint16_t* qrow = a.q + static_cast<int64_t>(u.s.first + r.q0 + qi) * a.ldq + (head * a.rep + x - qi * a.rep) * D;
-      if constexpr (MX) {
-        load_queries<D>(qf, qrow, g, lane);
-      } else {
-#pragma unroll
-        for (int s = 0; s < D / 32; ++s) qf.x[s] = as_frag(*reinterpret_cast<const uint4*>(qrow + 32 * s + 8 * g));
-      }
-    };
+    if constexpr (MX) arrived<D>(raw);
     Rows<D> st;
     st.m = -INFINITY;
     st.l = 0.f;
@@ -782,10 +799,11 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
     int i = 0;
     bool none = false;
     if constexpr (MX) {
-      // Tiles come through the wave's ring, two a turn. (A wave that loaded its next two tiles into
-      // registers behind their last use had one product's time for a latency of 2 us: 8500 cycles a turn at head_dim 256 for 3000
-      // of work; one 122880-key sequence took 23 us.)
+      // Tiles come through the wave's ring. (A wave that loaded its next two tiles into registers behind their last use had one
+      // product's time for a latency of 2 us: 8500 cycles a turn at head_dim 256 for 3000 of work; one 122880-key sequence
+      // took 23 us.)
       using G = Ring<D>;
+      constexpr int TT = G::T, LG = G::L * TT;                 // loads of a turn's keys, or values
       char* ring = reinterpret_cast<char*>(lds4) + w * G::BYTES;
       const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring));
       uint32_t bads = 0;                                       // two bits a slot
@@ -805,77 +823,92 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
         const int at = ((it0 + w + NW * (i0 + (lane >> 1))) * 2 + (lane & 1)) >> (a.pg.shift - 4);
         to_lds4(ring_at + G::R * G::SLOT, row + min(at, a.width - 1));
       };
-      int slot_in = 0, slot_out = 0;                           // of the tile issued next, and of tile i
-      auto issue = [&](int x) {                                // tile x < mine, in order; its slot's reads have returned
+      // tile x < mine, a turn's keys before its values, turns in order; the slot's reads have returned
+      auto issue_k = [&](int x) {
         if ((x & 31) == 0 && x) {
           const int it = it0 + w + NW * (x + (lane >> 1)), at = (it * 2 + (lane & 1)) >> (a.pg.shift - 4);
-          ids = reinterpret_cast<const int32_t*>(ring + G::R * G::SLOT)[lane];     // landed 28 tiles ago
+          ids = reinterpret_cast<const int32_t*>(ring + G::R * G::SLOT)[lane];     // landed turns ago
           wait_lds_reads();
           ids = it < it1 && at < a.width ? ids : -1;
           settle();
           place(x);
           fetch_entries(x + 32);
         }
-        const int y = 2 * (x & 31);
-        bads = (bads & ~(3u << (2 * slot_in))) | (static_cast<uint32_t>(bad >> y) & 3u) << (2 * slot_in);
-        issue_tile<D>(ring_at + slot_in * G::SLOT, a.pg, lane64(code_at, y), lane64(code_at, y + 1), lane64(scale_at, y),
+        const int y = 2 * (x & 31), s = x % G::R;
+        bads = (bads & ~(3u << (2 * s))) | (static_cast<uint32_t>(bad >> y) & 3u) << (2 * s);
+        issue_half<D>(ring_at + s * G::SLOT, a.pg.k, a.pg.ks, lane64(code_at, y), lane64(code_at, y + 1), lane64(scale_at, y),
                       lane64(scale_at, y + 1), lane);
-        slot_in = slot_in + 1 == G::R ? 0 : slot_in + 1;
+      };
+      auto issue_v = [&](int x) {
+        const int y = 2 * (x & 31), s = x % G::R;
+        issue_half<D>(ring_at + s * G::SLOT + G::HALF, a.pg.v, a.pg.vs, lane64(code_at, y), lane64(code_at, y + 1),
+                      lane64(scale_at, y), lane64(scale_at, y + 1), lane);
+      };
+      auto issue_turn = [&](auto&& issue, int x) {
+#pragma unroll
+        for (int y = 0; y < TT; ++y)
+          if (x + y < mine) issue(x + y);
       };
       if (mine) {
         fetch_entries(32);
-        for (int x = 0; x < min(mine, G::R); ++x) issue(x);
-      }
-      queries();                                               // (behind the tiles: they land in order)
-      // tiles up to x + 1 (x) have landed: the newer ones are those issued after them
-      auto landed = [&](int x, bool two) {
-        if (x + G::R > mine) wait_loads<0>();
-        else if (two) wait_loads<G::L * (G::R - 2)>();
-        else wait_loads<G::L * (G::R - 1)>();
-      };
-      while (!none && i + 2 <= whole) {
-        f32x4 sc[2][2];
-        float tmax;
-        for (; i + 2 <= whole; i += 2) {
-          const int slot_next = slot_out + 1 == G::R ? 0 : slot_out + 1;
-          const char* const slots[2] = {ring + slot_out * G::SLOT, ring + slot_next * G::SLOT};
-          none = (((bads >> (2 * slot_out)) | (bads >> (2 * slot_next))) & 3u) != 0;
-          if (none) break;
-          landed(i, true);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            KTile<D, true> kt;
-            read_k<D>(kt, slots[x], n, g);
-            scores<D, true>(kt, qf, sc[x], n);
-          }
-          tmax = fmaxf(lane_max(sc[0]), lane_max(sc[1]));
-          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const bf16x8 pf = probabilities(sc[x], st.m, a.c, st.l);
-            VTile<D, true> vt;
-            read_v<D>(vt, slots[x], n, g);
-            product<D, true, false>(vt, pf, 8, st);
-          }
-          wait_lds_reads();
-          slot_out = slot_next + 1 == G::R ? 0 : slot_next + 1;
-          if (i + G::R < mine) issue(i + G::R);
-          if (i + G::R + 1 < mine) issue(i + G::R + 1);
+        for (int x = 0; x < G::R; x += TT) {
+          issue_turn(issue_k, x);
+          issue_turn(issue_v, x);
         }
-        if (!none && i + 2 <= whole) raise<D>(st, tmax, a.c, g);
       }
-      for (; i < mine; ++i) {
-        landed(i, false);
-        const char* slot = ring + slot_out * G::SLOT;
+      split_queries<D>(qf, raw, g, lane);
+      while (!none && i + TT <= whole) {
+        f32x4 sc[TT][2];
+        float tmax;
+        for (; i + TT <= whole; i += TT) {
+          none = ((bads >> (2 * (i % G::R))) & ((1u << (2 * TT)) - 1u)) != 0;       // (a turn's slots lie side by side)
+          if (none) break;
+          // its keys have landed when no more than the loads after them are on their way: its values, the next turn
+          if (i + 2 * TT <= mine) wait_loads<3 * LG>();
+          else wait_loads<LG>();
+          const char* slot = ring + (i % G::R) * G::SLOT;
+          tmax = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < TT; ++x) {
+            KTile<D, true> kt;
+            read_k<D>(kt, slot + x * G::SLOT, n, g);
+            scores<D, true>(kt, qf, sc[x], n);
+            tmax = fmaxf(tmax, lane_max(sc[x]));
+          }
+          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
+          wait_lds_reads();
+          issue_turn(issue_k, i + G::R);
+          bf16x8 pf[TT];
+#pragma unroll
+          for (int x = 0; x < TT; ++x) pf[x] = probabilities(sc[x], st.m, a.c, st.l);
+          // its values: the next turn, and the keys of the one after it
+          if (i + 3 * TT <= mine) wait_loads<3 * LG>();
+          else if (i + 2 * TT <= mine) wait_loads<2 * LG>();
+          else wait_loads<0>();
+          VTile<D, true> vt[TT];
+#pragma unroll
+          for (int x = 0; x < TT; ++x) read_v<D>(vt[x], slot + x * G::SLOT, n, g);
+          wait_lds_reads();
+          issue_turn(issue_v, i + G::R);
+#pragma unroll
+          for (int x = 0; x < TT; ++x) product<D, true, false>(vt[x], pf[x], 8, st);
+        }
+        if (!none && i + TT <= whole) raise<D>(st, tmax, a.c, g);
+      }
+      for (; i < mine; ++i) {                                  // (few: every load is waited for)
+        wait_loads<0>();
+        const char* slot = ring + (i % G::R) * G::SLOT;
         Tile<D, true> tl;
         read_k<D>(tl.k, slot, n, g);
         read_v<D>(tl.v, slot, n, g);
         tl.k0 = (it0 + w + NW * i) * KT;
-        tl.bad = (bads >> (2 * slot_out)) & 3u;
+        tl.bad = (bads >> (2 * (i % G::R))) & 3u;
         edge_step<D, true>(tl, qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
         wait_lds_reads();
-        slot_out = slot_out + 1 == G::R ? 0 : slot_out + 1;
-        if (i + G::R < mine) issue(i + G::R);
+        if (i + G::R < mine) {
+          issue_k(i + G::R);
+          issue_v(i + G::R);
+        }
       }
       wait_loads<0>();                                         // nothing in flight into the rings:
       __syncthreads();                                         // the merge takes their place
@@ -909,7 +942,6 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D))) void k_paged_few(PagedArg
           get_v(tl[x], min(x, mine - 1));
         }
       }
-      queries();
       while (!none && i + NT <= whole) {
         f32x4 sc[NT][2];
         float tmax;
@@ -1494,7 +1526,7 @@ Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_
   p.many = std::min<int64_t>(max_rows, T) * rep > few_rows(d, mx);
   p.kt = p.many ? (d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
   p.blocks = std::min<int64_t>(T * rep, T * rep / p.rows() + n_seq);
-  const int round = p.many ? 256 : 256 * few_blocks(d);
+  const int round = p.many ? 256 : 256 * few_blocks(d, mx);
   // (no splits either where the tiles would not count in 31 bits)
   const bool split = max_keys > 16 * NW * KT && static_cast<double>(p.blocks) * static_cast<double>(max_keys / p.kt + 1) < 1e9;
   p.fit = split ? std::max(1, round / hkv) : 0;
