@@ -1015,6 +1015,12 @@ def _call_on(t, name, *args):
             _lib.call(name, *args)
 
 
+def _rows_apart(t, width):
+    """The row stride of t; of a single row at least its width. (An expanded or overlapping t keeps its own, which the
+    library refuses.)"""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
 def _sequences(table, lens, cu):
     _need(table, "table", torch.int32, 2)
     _need(lens, "lens", torch.int32, 1)
@@ -1034,7 +1040,7 @@ def paged_slots(table, lens, cu, rows, pages):
     _same_device(pages.k.device, table=table, lens=lens, cu=cu)
     slots = torch.empty(rows, dtype=torch.int64, device=table.device)
     pos = torch.empty_like(slots)
-    _call_on(table, "rf_paged_slots", _ptr(table) or _ptr(lens), max(table.stride(0), table.shape[1]), table.shape[1],
+    _call_on(table, "rf_paged_slots", _ptr(table) or _ptr(lens), _rows_apart(table, table.shape[1]), table.shape[1],
              _ptr(lens) or _ptr(cu), _ptr(cu), n, pages.n_pages, pages.page, rows, _ptr(slots) or _ptr(cu),
              _ptr(pos) or _ptr(cu), _stream(cu))
     return slots, pos
@@ -1081,10 +1087,10 @@ def paged_append(k, v, slots, pages, cs=None, q=None, out=None, qnorm=None, knor
     _same_device(dev, cs=cs, q=q, out=out, qnorm=qnorm, knorm=knorm)
     if rows == 0:
         return out
-    _call_on(k, "rf_paged_append", _ptr(k), k.stride(0) if rows > 1 else max(k.stride(0), d), k.stride(1) if pages.hkv > 1
-             else d, _ptr(v), v.stride(0) if rows > 1 else max(v.stride(0), d), v.stride(1) if pages.hkv > 1 else d, rows,
-             _ptr(slots), pages.handle, _ptr(cs), rot, _ptr(q), 0 if q is None else max(q.stride(0), hq * d), hq, _ptr(out),
-             0 if q is None else max(out.stride(0), hq * d), _ptr(qnorm), _ptr(knorm), int(norm_kind), float(eps),
+    _call_on(k, "rf_paged_append", _ptr(k), _rows_apart(k, d), k.stride(1) if pages.hkv > 1
+             else d, _ptr(v), _rows_apart(v, d), v.stride(1) if pages.hkv > 1 else d, rows,
+             _ptr(slots), pages.handle, _ptr(cs), rot, _ptr(q), 0 if q is None else _rows_apart(q, hq * d), hq, _ptr(out),
+             0 if q is None else _rows_apart(out, hq * d), _ptr(qnorm), _ptr(knorm), int(norm_kind), float(eps),
              _stream(k))
     return out
 
@@ -1102,7 +1108,7 @@ def paged_read(pages, slots, k_out=None, v_out=None):
         outs.append(t)
     _same_device(pages.k.device, slots=slots, k_out=outs[0], v_out=outs[1])
     if shape[0]:
-        lds = [max(t.stride(0), shape[1] * shape[2]) for t in outs]
+        lds = [_rows_apart(t, shape[1] * shape[2]) for t in outs]
         _call_on(slots, "rf_paged_read", pages.handle, _ptr(slots), shape[0], _ptr(outs[0]), lds[0], _ptr(outs[1]), lds[1],
                  _stream(slots))
     return outs[0], outs[1]
@@ -1143,8 +1149,8 @@ def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=N
     _same_device(dev, workspace=workspace)
     if rows == 0 or n == 0:
         return out
-    _call_on(q, "rf_attend_paged", _ptr(q), max(q.stride(0), hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),
-             max(table.stride(0), table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), n, max_rows, max_keys, float(scale),
-             _ptr(out), max(out.stride(0), hq * d), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+    _call_on(q, "rf_attend_paged", _ptr(q), _rows_apart(q, hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),
+             _rows_apart(table, table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), n, max_rows, max_keys, float(scale),
+             _ptr(out), _rows_apart(out, hq * d), _ptr(workspace), 0 if workspace is None else workspace.numel(),
              _stream(q))
     return out

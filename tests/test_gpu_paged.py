@@ -632,3 +632,30 @@ def test_refusals(dev):
     assert ops.paged_read(p, slots[:0])[0].shape == (0, 2, 64)
     ops.paged_append(k[:0], k[:0], slots[:0], p)
     torch.cuda.synchronize()
+
+
+def test_expanded_tensors_are_refused(dev):
+    """Rows that share memory (expand): a stride below a row's width is refused, never read past; one row may have any."""
+    from rfill import ops
+    from rfill.paged import Pages
+    p = Pages.empty(4, 2, 16, 64, "bf16", dev)
+    bf = dict(dtype=torch.bfloat16, device=dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    slots, kv = torch.arange(3, device=dev), torch.ones(3, 2, 64, **bf)
+    table, lens, cu = i32([[0], [1], [2]]), i32([4, 4, 4]), i32([0, 1, 2, 3])
+    q = torch.ones(3, 256, **bf)
+    attend = lambda q=q, table=table, **kw: ops.attend_paged(q, p, table, lens, cu, 4, 0.1, 1, 16, **kw)   # noqa: E731
+    append = lambda k=kv, v=kv, **kw: ops.paged_append(k, v, slots, p, **kw)   # noqa: E731
+    append(q=q)
+    attend()
+    for call in (lambda: attend(q=q[:1].expand(3, -1)), lambda: attend(table=table[:1].expand(3, -1)[:, :1].repeat(1, 2)[:1].expand(3, -1)),
+                 lambda: attend(out=torch.empty(1, 256, **bf).expand(3, -1)), lambda: append(k=kv[:1].expand(3, -1, -1)),
+                 lambda: append(v=kv[:, :1].expand(-1, 2, -1)), lambda: append(q=q[:1].expand(3, -1)),
+                 lambda: append(q=q, out=torch.empty(1, 256, **bf).expand(3, -1)),
+                 lambda: ops.paged_read(p, slots, k_out=torch.empty(1, 2, 64, **bf).expand(3, -1, -1)),
+                 lambda: ops.paged_slots(table[:1].expand(3, -1), lens, cu, 3, p)):
+        with pytest.raises(ValueError):
+            call()
+    one = torch.empty(1, 512, **bf)[:, ::2]
+    with pytest.raises(ValueError):
+        ops.attend_paged(one, p, table[:1], lens[:1], cu[:2], 4, 0.1, 1, 16)       # last dim not contiguous
