@@ -659,3 +659,69 @@ def test_expanded_tensors_are_refused(dev):
     one = torch.empty(1, 512, **bf)[:, ::2]
     with pytest.raises(ValueError):
         ops.attend_paged(one, p, table[:1], lens[:1], cu[:2], 4, 0.1, 1, 16)       # last dim not contiguous
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_two_graphs_on_one_workspace(dev, mx):
+    """A step (slots, append, attention) of few rows and one of a chunk, captured apart over the same pages and the same
+    workspace, replayed in turn; then both kinds at once on two streams with a workspace each."""
+    from rfill import ops
+    hq, hkv, d, page = 8, 2, 128, 16
+    lens0 = [3000, 40, 1200]
+    table, n_pages = layout([n + 400 for n in lens0], page, 12)
+    pools, _, _, _ = batch(hq, hkv, d, page, mx, [1, 1, 1], [n + 400 for n in lens0], 13)
+    pages, tb = pages_on(pools, dev), table.to(dev)
+    g = torch.Generator().manual_seed(14)
+    inv = ops.inv_freq_default(1e4, d).to(dev)
+    keys = 1 << 14
+    steps = []
+    for rows in ([1, 1, 1], [90, 40, 130]):
+        T = sum(rows)
+        x = torch.randn(T, (hq + 2 * hkv) * d, generator=g).to(torch.bfloat16).to(dev)
+        lens = torch.tensor([n + r for n, r in zip(lens0, rows)], dtype=torch.int32, device=dev)
+        steps.append(dict(rows=rows, T=T, x=x, lens=lens, cu=offsets(rows).to(dev)))
+    need = max(ops.attend_paged_workspace_bytes(s["T"], hq, hkv, d, pages.kind, 3, max(s["rows"]), keys) for s in steps)
+    shared = torch.empty(need, dtype=torch.uint8, device=dev)
+
+    def step(s, ws):
+        slots, pos = ops.paged_slots(tb, s["lens"], s["cu"], s["T"], pages)
+        k, v = (s["x"][:, (hq + i * hkv) * d:(hq + (i + 1) * hkv) * d].unflatten(1, (hkv, d)) for i in (0, 1))
+        q = ops.paged_append(k, v, slots, pages, cs=ops.rope_table(pos, inv), q=s["x"][:, : hq * d])
+        return q, ops.attend_paged(q, pages, tb, s["lens"], s["cu"], hq, d ** -0.5, max(s["rows"]), keys, workspace=ws)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in steps:
+            step(s, shared)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for s in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, step(s, shared)))
+    for turn in range(3):
+        for s, (graph, (q, out)) in zip(steps, graphs):
+            s["x"].copy_(torch.randn(s["x"].shape, generator=g).to(torch.bfloat16))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = out.clone()
+            for n in ("k", "v", "ks", "vs"):
+                t = getattr(pages, n)
+                setattr(pools, n, None if t is None else t.cpu())
+            lens = s["lens"].tolist()
+            want, size = oracle_attend(pools, table, n_pages, q.cpu(), s["rows"], lens, hq, d ** -0.5)
+            check(got, want, size, (turn, s["rows"]))
+            q2, eager = step(s, torch.full_like(shared, 0xff))
+            assert torch.equal(q2, q) and torch.equal(eager, got)
+    # at once: the pages hold the last step's rows now; both only read them
+    one = [ops.attend_paged(q, pages, tb, s["lens"], s["cu"], hq, d ** -0.5, max(s["rows"]), keys) for s, (_, (q, _)) in
+           zip(steps, graphs)]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in steps], [None, None]
+    for _ in range(3):
+        for i, (s, (_, (q, _))) in enumerate(zip(steps, graphs)):
+            with torch.cuda.stream(streams[i]):
+                outs[i] = ops.attend_paged(q, pages, tb, s["lens"], s["cu"], hq, d ** -0.5, max(s["rows"]), keys)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], one[0]) and torch.equal(outs[1], one[1])
