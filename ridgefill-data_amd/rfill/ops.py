@@ -1001,14 +1001,15 @@ def inv_freq_llama3(theta, dim, factor, low_freq_factor, high_freq_factor, origi
 # Checks as above, and two more: every tensor on the pages' device, and the launch made with that device current (a
 # serving process may hold several).
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: on {t.device}, the pages are on {dev}")
+def _same_device(pages, *tensors):
+    dev = pages.k.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the pages are on {pages.k.device}")
 
 
 def _call_on(t, name, *args):
-    if t.get_device() == torch.cuda.current_device():
+    if t.get_device() == torch._C._cuda_getDevice():
         _lib.call(name, *args)
     else:
         with torch.cuda.device(t.device):
@@ -1025,8 +1026,8 @@ def _sequences(table, lens, cu):
     _need(table, "table", torch.int32, 2)
     _need(lens, "lens", torch.int32, 1)
     _need(cu, "cu", torch.int32, 1)
-    n = lens.shape[0]
-    if table.shape[0] != n or cu.shape[0] != n + 1:
+    n = lens.size(0)
+    if table.size(0) != n or cu.size(0) != n + 1:
         raise ValueError(f"table {tuple(table.shape)}, lens {tuple(lens.shape)}, cu {tuple(cu.shape)}: one row of pages and "
                          f"one length a sequence, one more offset")
     return n
@@ -1037,7 +1038,7 @@ def paged_slots(table, lens, cu, rows, pages):
     [cu[b], cu[b + 1]) and become its last tokens, positions lens[b] - count .. lens[b] - 1, in the pages table[b] lists in
     order. A row of no sequence, before position 0, past the table or on a page outside the pool gets slot -1."""
     n = _sequences(table, lens, cu)
-    _same_device(pages.k.device, table=table, lens=lens, cu=cu)
+    _same_device(pages, table, lens, cu)
     slots = torch.empty(rows, dtype=torch.int64, device=table.device)
     pos = torch.empty_like(slots)
     _call_on(table, "rf_paged_slots", _ptr(table) or _ptr(lens), _rows_apart(table, table.shape[1]), table.shape[1],
@@ -1053,7 +1054,7 @@ def paged_append(k, v, slots, pages, cs=None, q=None, out=None, qnorm=None, knor
     and rotated (None without q; out may be q). norm_kind: 0 gain, 1 (1 + gain). fp32 arithmetic, one rounding."""
     for name, t in (("k", k), ("v", v)):
         _need(t, name, torch.bfloat16, 3)
-        if tuple(t.shape[1:]) != (pages.hkv, pages.d):
+        if t.size(1) != pages.hkv or t.size(2) != pages.d:
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [rows, {pages.hkv}, {pages.d}]")
     rows, d = k.shape[0], pages.d
     _need(slots, "slots", torch.int64, 1)
@@ -1070,10 +1071,12 @@ def paged_append(k, v, slots, pages, cs=None, q=None, out=None, qnorm=None, knor
         if q.shape[0] != rows or q.shape[1] % d:
             raise ValueError(f"paged_append: q {tuple(q.shape)}, expected [{rows}, heads x {d}]")
         hq = q.shape[1] // d
-        out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device) if out is None else out
-        _need(out, "out", torch.bfloat16, 2)
-        if out.shape != q.shape:
-            raise ValueError(f"paged_append: out {tuple(out.shape)}, expected {tuple(q.shape)}")
+        if out is None:
+            out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device)
+        else:
+            _need(out, "out", torch.bfloat16, 2)
+            if out.shape != q.shape:
+                raise ValueError(f"paged_append: out {tuple(out.shape)}, expected {tuple(q.shape)}")
     elif out is not None or qnorm is not None:
         raise ValueError("paged_append: out and qnorm go with q")
     for name, t in (("qnorm", qnorm), ("knorm", knorm)):
@@ -1081,10 +1084,7 @@ def paged_append(k, v, slots, pages, cs=None, q=None, out=None, qnorm=None, knor
             _need(t, name, torch.bfloat16, 1)
             if t.shape[0] != d:
                 raise ValueError(f"paged_append: {name} width")
-    dev = pages.k.device
-    if not (k.device == v.device == slots.device == dev):
-        _same_device(dev, k=k, v=v, slots=slots)
-    _same_device(dev, cs=cs, q=q, out=out, qnorm=qnorm, knorm=knorm)
+    _same_device(pages, k, v, slots, cs, q, out, qnorm, knorm)
     if rows == 0:
         return out
     _call_on(k, "rf_paged_append", _ptr(k), _rows_apart(k, d), k.stride(1) if pages.hkv > 1
@@ -1106,7 +1106,7 @@ def paged_read(pages, slots, k_out=None, v_out=None):
         if tuple(t.shape) != shape or (shape[1] > 1 and t.stride(1) != pages.d):
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape} with its heads side by side")
         outs.append(t)
-    _same_device(pages.k.device, slots=slots, k_out=outs[0], v_out=outs[1])
+    _same_device(pages, slots, *outs)
     if shape[0]:
         lds = [_rows_apart(t, shape[1] * shape[2]) for t in outs]
         _call_on(slots, "rf_paged_read", pages.handle, _ptr(slots), shape[0], _ptr(outs[0]), lds[0], _ptr(outs[1]), lds[1],
@@ -1134,19 +1134,18 @@ def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=N
     rows, d = q.shape[0], pages.d
     if q.shape[1] < hq * d:
         raise ValueError(f"attend_paged: q {tuple(q.shape)} for {hq} heads of {d}")
-    out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device) if out is None else out
-    _need(out, "out", torch.bfloat16, 2)
-    if out.shape[0] != rows or out.shape[1] < hq * d:
-        raise ValueError(f"attend_paged: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
+    if out is None:
+        out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device)
+    else:
+        _need(out, "out", torch.bfloat16, 2)
+        if out.shape[0] != rows or out.shape[1] < hq * d:
+            raise ValueError(f"attend_paged: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
     need = attend_paged_workspace_bytes(rows, hq, pages.hkv, d, pages.kind, n, max_rows, max_keys)
     if isinstance(workspace, str):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     if workspace is not None:
         _need(workspace, "workspace", torch.uint8, 1)
-    dev = pages.k.device
-    if not (q.device == table.device == lens.device == cu.device == out.device == dev):
-        _same_device(dev, q=q, table=table, lens=lens, cu=cu, out=out)
-    _same_device(dev, workspace=workspace)
+    _same_device(pages, q, table, lens, cu, out, workspace)
     if rows == 0 or n == 0:
         return out
     _call_on(q, "rf_attend_paged", _ptr(q), _rows_apart(q, hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),

@@ -45,15 +45,16 @@ class Pages:
             parts = [("k", k), ("v", v), ("ks", ks), ("vs", vs)]
         if self.n_pages == 0:
             raise ValueError("Pages: no pages")
+        want, dev = torch.bfloat16 if self.kind == BF16 else torch.uint8, k.get_device()
         for name, t in parts:
-            want = torch.bfloat16 if self.kind == BF16 else torch.uint8
             if t.dtype != want:
                 raise ValueError(f"Pages: {name} dtype {t.dtype}, expected {want}")
-            if t.device.type != "cuda" or t.device != k.device:
+            if not t.is_cuda or t.get_device() != dev:
                 raise ValueError(f"Pages: {name} must be on k's GPU (got {t.device})")
-            if not t[0].is_contiguous():
+            if not (t.is_contiguous() or t[0].is_contiguous()):
                 raise ValueError(f"Pages: {name} must be contiguous within a page")
-        strides = [(t.stride(0) if self.n_pages > 1 else t[0].numel()) * t.element_size() for _, t in parts]
+        size = 2 if self.kind == BF16 else 1
+        strides = [(t.stride(0) if self.n_pages > 1 else t[0].numel()) * size for _, t in parts]
         if strides[0] != strides[1] or strides[2:3] != strides[3:]:
             raise ValueError(f"Pages: strides between pages {strides} bytes differ")
         self.k, self.v, self.ks, self.vs = k, v, ks, vs
