@@ -52,7 +52,6 @@ struct PagedArgs {
   int* length;                             // behind them: the split length, from the splits' launch to the merge
   int fit;                                 // blocks a head that one round holds (0: no splits)
   bool once;                               // k_paged_many: as many units as that at most
-  float ov;                                // what a unit costs besides its tiles, in tiles
   int64_t units;                           // units a head that the launch has blocks and the workspace partials for
   int kt, wmin;                            // keys a tile, key tiles a split at least
 };
@@ -121,14 +120,14 @@ __device__ __forceinline__ int wave_max(int v) {                                
   return __builtin_amdgcn_readlane(wave_scan(v, 0, [](int x, int y) { return max(x, y); }), 63);
 }
 
-// The key tiles of a split. Blocks of one length that fill the GPU once are best; a few more than fill it wait for a second
-// round, so splits are as short as one round of blocks allows (fit: its units a head). Where the row blocks alone nearly fill
-// it, the length of the least estimated time: all tiles and what each unit costs besides (ov) over the round's blocks, and a
-// third of a split for the end (or one round's longest split). 32 sequences of 500 to 8000 keys (bf16, 8 heads): 80 us
-// as one round, 85 at 1.25; 48 of 1500 to 24000 in 4 bits 98 against 107; 1499-row chunks of three prompts 521 at three
-// rounds, 599 at 1.6. Up to 64 sequences the lanes try 64 lengths each; more of them take a length that
-// surely fits. Every block does the same arithmetic on the same sizes: no launch has to plan before this one, and a captured
-// graph follows its lens.
+// k_paged_many: the key tiles of a split. Where the row blocks leave a quarter of the GPU idle (once), splits are as short as one
+// round of blocks allows (fit: its units a head): a few more than fill it wait for a second round. Otherwise the length of the
+// least estimated time: all tiles and what each unit costs besides over the round's blocks, and a third of a split for the end
+// (or one round's longest split): 1499-row chunks of three prompts 521 us at three rounds, 599 at 1.6; a unit's cost as 6, 10 or
+// 16 tiles instead of 3 changed nothing that stood out. Up to 64 sequences the lanes try 64 lengths each; more of them take a
+// length that surely fits. Every block does the same arithmetic on the same sizes: no launch has to plan before this one, and a
+// captured graph follows its lens.
+constexpr float UNIT_TILES = 3.f;
 __device__ int split_length(const PagedArgs& a, float work, float blocks, int tmax, int nrb0, int tiles0, int lane) {
   const float fit = static_cast<float>(a.fit);
   const bool once = a.once;
@@ -145,7 +144,7 @@ __device__ int split_length(const PagedArgs& a, float work, float blocks, int tm
     units += static_cast<float>(__builtin_amdgcn_readlane(nrb0, b)) *
              ceilf(static_cast<float>(__builtin_amdgcn_readlane(tiles0, b)) * inv);
   const float longest = fminf(W, static_cast<float>(tmax));
-  float cost = units <= fit ? fmaxf(longest, work / fit) : (work + a.ov * units) / fit + 0.35f * longest;
+  float cost = units <= fit ? fmaxf(longest, work / fit) : (work + UNIT_TILES * units) / fit + 0.35f * longest;
   // (lane 63's length is every tile: one unit a row block, which always fits)
   if (once && units > fit + 0.5f && lane != 63) cost = 3e38f;
   // the least cost, the shorter length among equals (the bits of positive floats are in order)
@@ -211,7 +210,7 @@ __device__ Unit find_unit(const PagedArgs& a, int want, bool merging) {
 
 // k_paged_few's shares: the key tiles of all (sequence, row block)s in a row, cut into equal runs, one a block of a round
 // (a run may end inside a row block and begin the next one's: its parts are then two pieces or more). 48 sequences of 1500
-// to 24000 keys in 96 splits of one length at most were a quarter empty; equal runs take 97 us where those took 107.
+// to 24000 keys in 4 bits, in 96 splits of one length at most: a quarter of the blocks idle, 107 us where equal runs took 97.
 struct Piece {
   int b, rb, t0, nt;                       // sequence (-1: none), row block, tile that the position falls on, its tiles
   int begin;                               // position of its first tile
@@ -319,8 +318,9 @@ __device__ __forceinline__ void load_v(VTile<D, false>& vt, const PagesDev& pg, 
 // scales (D; 256 bytes at least, as their load writes). Two turns of T tiles: while one is computed the other is on its way,
 // and each half is loaded again as soon as it has been read. (head_dim 256: with two tiles a turn the LDS holds four waves, one
 // a SIMD; with one tile two a SIMD: 9 sequences of 5 new tokens and up to 30011 keys 49 -> 43 us, 1024 rows of 8007 keys 285 ->
-// 232. An order of its 16-byte chunks that spreads every read over all banks changed nothing: the conversion of the values
-// bounds it, 64 v_cvt_scalef32_pk_bf16_fp4 and as many v_perm a tile.)
+// 232. There the vector pipe is 51 % busy, the matrix pipe 21 %, and a third of the waves' time is waits: two waves a SIMD, all
+// that the LDS and the registers hold, do not cover more. An order of the 16-byte chunks that spreads every read over all banks
+// changed nothing.)
 template <int D>
 struct Ring {
   static constexpr int T = D == 256 ? 1 : 2, R = 2 * T;      // tiles a turn, tiles
@@ -1044,7 +1044,10 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
 // query and head side by side in a wave, so that any group size fills it. Tiles come from pages: bf16 by direct loads, three
 // tiles in flight, the page of each load's rows (never more than 16) read off a lane; 4 bits through registers, a tile's
 // codes loaded while the one before it is converted into LDS, once for all eight waves (160 of a tile's 2000 cycles).
-// Bound by the products and the softmax beside them (64 keys: 1024 cycles of MFMA a wave, two waves a SIMD).
+// Bound by the products and the softmax beside them (64 keys: 1024 cycles of MFMA a wave, two waves a SIMD): 2048 rows of 32768
+// keys, 8 heads of 128 in groups of 4, bf16, 960 to 1040 us (1.0 to 1.1 PFLOP/s), the same heads in 4 bits, 3 x 1499 rows of up
+// to 12011 keys, 510 to 540 us with the merge's 29 (0.9 PFLOP/s). head_dim 256, 1024 rows of 8007 keys: 520 us, LDS reads as long
+// as the products and one wave a SIMD.
 template <int AD, bool MX>
 struct ManyCodes {
   uint2 k, v;                              // codes of 16 values (8 at head_dim 64)
@@ -1517,8 +1520,9 @@ struct Plan {
 // keys' codes at four times the rate, and a wave's 256 columns leave no registers to convert the codes beside them).
 constexpr int64_t few_rows(int d, bool mx) { return d == 256 ? (mx ? INT64_MAX : 128) : mx ? 96 : 16; }
 
-// The launch for these sizes: k_paged_few or k_paged_many. Row blocks: sum of ceil(rows rep / rpb) <= T rep / rpb + n_seq. k_paged_few: `fit` runs a head, two parts each;
-// k_paged_many: with splits of W tiles at most work / W units more (split_length: one round of blocks, or W >= work / 3 fit).
+// The launch for these sizes: k_paged_few or k_paged_many. Row blocks: sum of ceil(rows rep / rpb) <= T rep / rpb + n_seq.
+// k_paged_few: `fit` runs a head, two parts each; k_paged_many: with splits of W tiles at most work / W units more
+// (split_length: one round of blocks, or W >= work / 3 fit).
 Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys) {
   Plan p{};
   p.d = d;
@@ -1590,7 +1594,7 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.rows(),
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
                     scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace),
-                    p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.many ? 3.f : 1.f, p.units, p.kt,
+                    p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
                     p.many ? 4 : 2 * NW};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
