@@ -3,6 +3,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -109,7 +110,7 @@ __device__ __forceinline__ double vector_sum(double s) {
 
 // 1 / sqrt(mean of squares + eps) from the lane's 8 values: the squares of bf16 values and nearly always their sum are exact
 // in fp64; the instruction's root gets one step of Newton's. (With the library's root and quotient, sums through LDS and every
-// partner normed twice, 6200 rows of 32 query and 8 K / V heads into 4 bits took 38 us, now 35; their 134 MB take 26.)
+// partner normed twice, 6200 rows of 32 query and 8 K / V heads into 4 bits took 38 us, then 35; their 134 MB take 26.)
 template <int D>
 __device__ __forceinline__ float inverse_rms(const float (&f)[8], float eps) {
   double s = 0;
@@ -119,10 +120,11 @@ __device__ __forceinline__ float inverse_rms(const float (&f)[8], float eps) {
   return static_cast<float>(m < 1e300 ? y * fma(-0.5 * m * y, y, 1.5) : y);       // (an infinity's root is 0)
 }
 
-// D / 8 lanes a head vector, 8 values a lane; blockIdx.y is the head of [queries | keys | values], blockIdx.x a run of
-// rows: the rows of one head lie side by side in a block, so that the codes of a page's tokens, side by side in memory, are
+// D / 8 lanes a head vector, 8 values a lane; blockIdx.y is the head of [queries | keys | values] (four heads of the queries, whose
+// gains and rotation are then loaded once: 6200 rows of 32 of them 35 -> 29 us, 4.6 TB/s), blockIdx.x a run of rows: the rows of one head lie side by side in a block, so that the codes of a page's tokens, side by side in memory, are
 // written together. Heads that stay bf16: a lane takes 4 values and their rotation partners. Keys that become codes: 8 values
 // side by side, for a block's scale comes from 4 lanes, and their partners once more (d / 2 apart or less, in L1).
+constexpr int HG = 4;
 template <int D, bool MX>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;
@@ -130,9 +132,9 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + t / LPR;
   const bool in = row < a.T;
   const int64_t rr = in ? row : a.T - 1;                     // (lanes past the end follow along: the shuffles take all)
-  const int head = blockIdx.y;
-  const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
-  const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
+  const int groups = (a.hq + HG - 1) / HG, head = static_cast<int>(blockIdx.y) - groups;        // queries: below 0
+  const bool is_q = head < 0, is_v = head >= a.hkv;
+  const int h = is_q ? static_cast<int>(blockIdx.y) * HG : is_v ? head - a.hkv : head;
   const uint16_t* src = is_q ? a.q + rr * a.ld_q + h * D
                              : is_v ? a.v + rr * a.ld_v + h * a.head_v : a.k + rr * a.ld_k + h * a.head_k;
   const int64_t slot = is_q ? 0 : a.slots[rr];
@@ -142,30 +144,8 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   float f[8];
   if (is_q || (!MX && !is_v)) {
     const int ja = turn ? 4 * c : j0, jb = turn ? half + 4 * c : j0 + 4;
-    const uint2 xa = *reinterpret_cast<const uint2*>(src + ja), xb = *reinterpret_cast<const uint2*>(src + jb);
-    uint4 raw = make_uint4(xa.x, xa.y, xb.x, xb.y);
-    unpack8(f, raw);
-    if (gain) {
-      const uint2 ga = *reinterpret_cast<const uint2*>(gain + ja), gb = *reinterpret_cast<const uint2*>(gain + jb);
-      normed(f, make_uint4(ga.x, ga.y, gb.x, gb.y), a.norm_kind, inverse_rms<D>(f, a.eps));
-    }
-    if (turn) {
-#pragma clang fp contract(off)
-      const uint16_t* tab = a.cs + rr * a.rot + 4 * c;
-      const uint2 cv = *reinterpret_cast<const uint2*>(tab), sv = *reinterpret_cast<const uint2*>(tab + half);
-      const uint4 cs = make_uint4(cv.x, cv.y, sv.x, sv.y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float co = bf2f(lane_of(cs, e)), si = bf2f(lane_of(cs, e + 4)), x = f[e], y = f[e + 4];
-        const float xc = x * co, ys = y * si, yc = y * co, xs = x * si;
-        f[e] = xc - ys;
-        f[e + 4] = yc + xs;
-      }
-    }
-    if (gain || turn)
-      raw = make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
     const int64_t page = slot >> a.pg.shift;
-    if (!in || slot < 0 || page >= a.pg.n_pages) return;     // (queries: slot 0)
+    const bool out = !in || slot < 0 || page >= a.pg.n_pages;            // (queries: slot 0)
     uint16_t* dst;
     if (is_q) {
       dst = a.q_out + row * a.ld_qo + h * D;
@@ -173,8 +153,49 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
       const int tok = static_cast<int>(slot) & ((1 << a.pg.shift) - 1);
       dst = reinterpret_cast<uint16_t*>(a.pg.k + page * a.pg.page_stride + static_cast<int64_t>(h) * a.pg.head_bytes) + tok * D;
     }
-    *reinterpret_cast<uint2*>(dst + ja) = make_uint2(raw.x, raw.y);
-    *reinterpret_cast<uint2*>(dst + jb) = make_uint2(raw.z, raw.w);
+    auto heads = [&](auto count, int n) {                    // n <= count heads side by side
+      constexpr int N = decltype(count)::value;
+      uint4 raw[N];
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const uint16_t* from = src + min(x, n - 1) * D;
+        const uint2 xa = *reinterpret_cast<const uint2*>(from + ja), xb = *reinterpret_cast<const uint2*>(from + jb);
+        raw[x] = make_uint4(xa.x, xa.y, xb.x, xb.y);
+      }
+      uint4 gains = make_uint4(0u, 0u, 0u, 0u), cs = gains;
+      if (gain) {
+        const uint2 ga = *reinterpret_cast<const uint2*>(gain + ja), gb = *reinterpret_cast<const uint2*>(gain + jb);
+        gains = make_uint4(ga.x, ga.y, gb.x, gb.y);
+      }
+      if (turn) {
+        const uint16_t* tab = a.cs + rr * a.rot + 4 * c;
+        const uint2 cv = *reinterpret_cast<const uint2*>(tab), sv = *reinterpret_cast<const uint2*>(tab + half);
+        cs = make_uint4(cv.x, cv.y, sv.x, sv.y);
+      }
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        unpack8(f, raw[x]);
+        if (gain) normed(f, gains, a.norm_kind, inverse_rms<D>(f, a.eps));
+        if (turn) {
+#pragma clang fp contract(off)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float co = bf2f(lane_of(cs, e)), si = bf2f(lane_of(cs, e + 4)), y = f[e], z = f[e + 4];
+            const float yc = y * co, zs = z * si, zc = z * co, ys = y * si;
+            f[e] = yc - zs;
+            f[e + 4] = zc + ys;
+          }
+        }
+        if (gain || turn)
+          raw[x] = make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+        if (!out && x < n) {
+          *reinterpret_cast<uint2*>(dst + x * D + ja) = make_uint2(raw[x].x, raw[x].y);
+          *reinterpret_cast<uint2*>(dst + x * D + jb) = make_uint2(raw[x].z, raw[x].w);
+        }
+      }
+    };
+    if (is_q) heads(std::integral_constant<int, HG>{}, min(HG, a.hq - h));
+    else heads(std::integral_constant<int, 1>{}, 1);
     return;
   }
   const uint4 raw = *reinterpret_cast<const uint4*>(src + j0);
@@ -331,8 +352,8 @@ extern "C" int rf_paged_append(const uint16_t* k, int64_t ld_k, int64_t head_k, 
   const AppendArgs a{k, v, q, ld_k, head_k, ld_v, head_v, ld_q, ld_qo, T, slots, pg, cs, cs ? rot : 0, hq, hkv, q_out,
                      qnorm, knorm, norm_kind, eps};
   const int rpb = 256 / (d / 8);
-  const dim3 grid(static_cast<unsigned>((T + rpb - 1) / rpb), static_cast<unsigned>(hq + 2 * hkv));
   const bool mx = pages->kind == RF_PAGES_MX4;
+  const dim3 grid(static_cast<unsigned>((T + rpb - 1) / rpb), static_cast<unsigned>((hq + HG - 1) / HG + 2 * hkv));
 #define RF_APPEND(D)                                                                                     \
   if (mx) hipLaunchKernelGGL((k_paged_append<D, true>), grid, dim3(256), 0, stream, a);                  \
   else hipLaunchKernelGGL((k_paged_append<D, false>), grid, dim3(256), 0, stream, a)
