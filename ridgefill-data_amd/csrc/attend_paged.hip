@@ -16,7 +16,7 @@
 //       consecutive in memory again. 4-bit values become bf16 by v_cvt_scalef32_pk_bf16_fp4, scale included, exactly. (P in
 //       8 bits or less would round the probabilities by 2^-4 and more; they keep bf16's 2^-8.)
 // The waves' parts are merged through LDS in wave order. Measured, merge included: 32 sequences of 500 to 8111 keys, 8 heads of
-// 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 94 us for 405 MB; one of 122880 keys in 4
+// 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 91 us for 405 MB; one of 122880 keys in 4
 // bits, 2 heads of 256, 30 us for 67 MB: of that 7 are the merge and 10 the launch, the first tiles' way and the end.
 #include <stdint.h>
 
@@ -571,12 +571,13 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // with zeros for
   return (p & 0x7f800000u) == 0x7f800000u ? p & 0xffffu : p;
 }
 
-// V's fragments of pair j; CUT: with zeros for the lane's keys past `last` and for what is not finite.
+// V's fragments of pair j; CUT, if cut: with zeros for the lane's keys past `last` and for what is not finite.
 template <int D, bool MX, bool CUT>
-__device__ __forceinline__ void v_frags(const VTile<D, MX>& vt, const float (&vs)[8], int j, int last, bf16x8& f0, bf16x8& f1) {
+__device__ __forceinline__ void v_frags(const VTile<D, MX>& vt, const float (&vs)[8], int j, int last, bool cut,
+                                        bf16x8& f0, bf16x8& f1) {
   uint32_t p[8];
   v_pairs<D, MX>(vt, vs, j, p);
-  if constexpr (CUT) {
+  if (CUT && cut) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = e <= last ? finite_pair(p[e]) : 0u;
   }
@@ -650,7 +651,7 @@ __device__ __forceinline__ bf16x8 probabilities(const f32x4 (&s)[2], float m, fl
 
 // O += P V. CUT: as v_frags.
 template <int D, bool MX, bool CUT>
-__device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf, int last, Rows<D>& st) {
+__device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf, int last, bool cut, Rows<D>& st) {
   float vs[8];
   if constexpr (MX) {
 #pragma unroll
@@ -660,14 +661,15 @@ __device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf
   for (int j = 0; j < D / 32; ++j) {
     bf16x8 f0, f1;
     if constexpr (CUT) __builtin_amdgcn_sched_barrier(0);    // (all pairs at once would not fit the registers)
-    v_frags<D, MX, CUT>(vt, vs, j, last, f0, f1);
+    v_frags<D, MX, CUT>(vt, vs, j, last, cut, f0, f1);
     st.o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f0, st.o[2 * j], 0, 0, 0);
     st.o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, f1, st.o[2 * j + 1], 0, 0, 0);
   }
 }
 
-// A tile of which some row does not see some key. Keys are hidden from rows by their scores (-infinity); of V, what no row
-// sees and what is not finite enters the product as zero, and the latter leaves its marks in the rows that see it.
+// A tile of which some row does not see some key. Keys are hidden from rows by their scores (-infinity). Where the tile's V is not
+// all finite, what no row sees of it and what is not finite enters the product as zero, and the latter leaves its marks in the
+// rows that see it. (Zeros in any case: 8 sequences of up to 2000 keys in 4 bits 20 us for 18, 48 of up to 24001 94 for 91.)
 template <int D, bool MX>
 __device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D, MX> &qf, int pos,
                                           Rows<D>& st, float c, int p0, int plast, const RowBlock& rows, int rep, int lane, uint32_t* marks) {
@@ -684,30 +686,37 @@ __device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D
   const float tmax = lane_max(sc);
   if (__any(tmax > st.m + RESCALE_LOG2 / c)) raise<D>(st, tmax, c, g);
   const bf16x8 pf = probabilities(sc, st.m, c, st.l);
+  // V's pair j of key e; 4 bits: all of them, of which only a scale can make NaN
+  auto pair = [&](int e, int j) {
+    if constexpr (MX) return (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
+    else return tl.v.x[e][j];
+  };
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+#pragma unroll
+    for (int j = 0; j < (MX ? 1 : NB / 2); ++j) odd |= not_finite(pair(e, j));
+  const bool cut = __any(odd);                               // (else what is hidden counts for nothing by its probability)
   const int last = hidden ? -1 : plast - k0 - 8 * g;         // of the lane's keys, the last that any row sees
+  if (cut) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 8; ++e) {
 #pragma unroll
-    for (int j = 0; j < NB / 2; ++j) {
-      uint32_t two;
-      if constexpr (MX) {                                    // 4 bits: only a scale can make values NaN
-        if (j) continue;
-        two = (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
-      } else {
-        two = tl.v.x[e][j];
-      }
-      if (e <= last && not_finite(two)) {
-        const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 2;
-        const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);          // rows from the key's own query on
-        for (int r = first; r < rows.rows; ++r) {
-          const int at = r * D + n * NB + 2 * j;             // 16 columns a word; the lane's NB lie in one
-          atomicOr(marks + at / 16, (MX ? static_cast<uint32_t>((1ull << (2 * NB)) - 1) : m2) << (2 * (at % 16)));
+      for (int j = 0; j < (MX ? 1 : NB / 2); ++j) {
+        const uint32_t two = pair(e, j);
+        if (e <= last && not_finite(two)) {
+          const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 2;
+          const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);          // rows from the key's own query on
+          for (int r = first; r < rows.rows; ++r) {
+            const int at = r * D + n * NB + 2 * j;             // 16 columns a word; the lane's NB lie in one
+            atomicOr(marks + at / 16, (MX ? static_cast<uint32_t>((1ull << (2 * NB)) - 1) : m2) << (2 * (at % 16)));
+          }
+          marks[D] = 1u;
         }
-        marks[D] = 1u;
       }
     }
   }
-  product<D, MX, true>(tl.v, pf, last, st);
+  product<D, MX, true>(tl.v, pf, last, cut, st);
 }
 
 // Blocks a CU that the registers of a kernel hold (4 bits: and its rings the LDS).
@@ -891,7 +900,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
           wait_lds_reads();
           issue_turn(issue_v, i + G::R);
 #pragma unroll
-          for (int x = 0; x < TT; ++x) product<D, true, false>(vt[x], pf[x], 8, st);
+          for (int x = 0; x < TT; ++x) product<D, true, false>(vt[x], pf[x], 8, false, st);
         }
         if (!none && i + TT <= whole) raise<D>(st, tmax, a.c, g);
       }
@@ -964,7 +973,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
 #pragma unroll
           for (int x = 0; x < NT; ++x) pf[x] = probabilities(sc[x], st.m, a.c, st.l);
 #pragma unroll
-          for (int x = 0; x < NT; ++x) product<D, false, false>(tl[x].v, pf[x], 8, st);
+          for (int x = 0; x < NT; ++x) product<D, false, false>(tl[x].v, pf[x], 8, false, st);
 #pragma unroll
           for (int x = 0; x < NT; ++x) get_v(tl[x], min(i1 + x, mine - 1));
         }
