@@ -620,12 +620,15 @@ __device__ __forceinline__ float lane_max(const f32x4 (&s)[2]) {
   return fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
 }
 
+__device__ __forceinline__ float row_max(float v) {          // of a row's four lanes
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
 // Raise the reference maxima to what the rows' four lanes have seen (tmax), and rescale their sums and O.
 template <int D>
 __device__ __forceinline__ void raise(Rows<D>& st, float tmax, float c, int g) {
-  tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-  tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-  const float top = fmaxf(st.m, tmax);
+  const float top = fmaxf(st.m, row_max(tmax));
   const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m - top) * c);
   st.m = top;
   st.l *= alpha;
@@ -804,9 +807,10 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
     for (int b = 0; b < NB; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     // Whole tiles first, then the tiles that some row sees in part; from the first page that is none on all of them are taken as
     // such. A maximum that has to rise leaves the inner loop: with the rescale inside it the compiler moves all of O at every tile.
+    // (Not the first of a piece, which 13 sequences at head_dim 256, two tiles a wave, took 2 us longer for.)
     const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
     int i = 0;
-    bool none = false;
+    bool none = false, fresh = true;                           // fresh: O is zero, nothing to rescale
     if constexpr (MX) {
       // Tiles come through the wave's ring. (A wave that loaded its next two tiles into registers behind their last use had one
       // product's time for a latency of 2 us: 8500 cycles a turn at head_dim 256 for 3000 of work; one 122880-key sequence
@@ -884,7 +888,11 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
             scores<D, true>(kt, qf, sc[x], n);
             tmax = fmaxf(tmax, lane_max(sc[x]));
           }
-          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
+          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) {
+            if (!fresh) break;
+            fresh = false;
+            st.m = row_max(tmax);
+          }
           wait_lds_reads();
           issue_turn(issue_k, i + G::R);
           bf16x8 pf[TT];
@@ -964,7 +972,11 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
           for (int x = 0; x < NT; ++x) scores<D, false>(tl[x].k, qf, sc[x], n);
           tmax = lane_max(sc[0]);
           if constexpr (NT > 1) tmax = fmaxf(tmax, lane_max(sc[NT - 1]));
-          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) break;
+          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) {
+            if (!fresh) break;
+            fresh = false;
+            st.m = row_max(tmax);
+          }
           const int i1 = min(i + NT, mine - 1);
           if (i1 == i + NT) window(i1);
 #pragma unroll
