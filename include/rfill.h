@@ -585,7 +585,8 @@ int rf_window_mass(const uint16_t* q, int64_t ldq, int w, int64_t pos0, int hq, 
  * 64, 128 or 256); slot s is token s % page of page s / page.
  * RF_PAGES_BF16: k, v [n_pages, hkv, page, d] bf16; ks, vs NULL.
  * RF_PAGES_MX4: 4-bit codes (E2M1: sign, two exponent bits, one mantissa bit; 0 .5 1 1.5 2 3 4 6) with one scale a
- * block of 32 values along d (a byte e, 2^(e - 127); 255: the block reads as NaN):
+ * block of 32 values along d (a byte e, 2^(e - 127); 255: the block reads as NaN; codes that a byte of 253 or 254 takes to
+ * 2^128 and more, beyond bf16, read as infinities, and what a row gets that sees a key with such a value is left open):
  *   k [n_pages, hkv, page, d / 2]: two codes a byte, the lower d in the low half;
  *   v [n_pages, hkv, page / 8, 16, 8, d / 32]: of 8 tokens, 16 runs of d / 16 values, token by token within a run (what a
  *     lane of the attention reads for its 8 tokens lies together);
@@ -620,7 +621,7 @@ int rf_paged_slots(const int32_t* table, int64_t ld_table, int64_t table_width, 
  * A head vector x becomes x r g (r = 1 / sqrt(mean(x^2) + eps), the mean in fp64), then its first rot dims are rotated
  * by halves, in fp32, and it is rounded once: to bf16, or to its 4-bit codes. A block's scale is the least power of two
  * at which its largest value rounds to at most 6; codes round to nearest, halfway to the even one; a block with a NaN or
- * an infinity reads as NaN. Needs rot <= d, rot / 2 a multiple of 8 or equal to 4. */
+ * an infinity reads as NaN, a magnitude above 1.75 2^127 as an infinity. Needs rot <= d, rot / 2 a multiple of 8 or equal to 4. */
 int rf_paged_append(const uint16_t* k, int64_t ld_k, int64_t head_k, const uint16_t* v, int64_t ld_v, int64_t head_v,
                     int64_t T, const int64_t* slots, const rf_pages* pages, const uint16_t* cs, int rot,
                     const uint16_t* q, int64_t ld_q, int hq, uint16_t* q_out, int64_t ld_qo, const uint16_t* qnorm,

@@ -672,10 +672,12 @@ __device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf
 
 // A tile of which some row does not see some key. Keys are hidden from rows by their scores (-infinity). Where the tile's V is not
 // all finite, what no row sees of it and what is not finite enters the product as zero, and the latter leaves its marks in the
-// rows that see it. (Zeros in any case: 8 sequences of up to 2000 keys in 4 bits 20 us for 18, 48 of up to 24001 94 for 91.)
+// rows that see it. slot: the tile in LDS (4 bits). (Zeros in any case: 8 sequences of up to 2000 keys in 4 bits 20 us for 18, 48
+// of up to 24001 94 for 91.)
 template <int D, bool MX>
-__device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D, MX> &qf, int pos,
-                                          Rows<D>& st, float c, int p0, int plast, const RowBlock& rows, int rep, int lane, uint32_t* marks) {
+__device__ __forceinline__ void edge_step(Tile<D, MX>& tl, const Queries<D, MX> &qf, int pos,
+                                          Rows<D>& st, float c, int p0, int plast, const RowBlock& rows, int rep, int lane,
+                                          uint32_t* marks, [[maybe_unused]] const char* slot) {
   constexpr int NB = D / 16;
   const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
   f32x4 sc[2];
@@ -689,37 +691,63 @@ __device__ __forceinline__ void edge_step(const Tile<D, MX>& tl, const Queries<D
   const float tmax = lane_max(sc);
   if (__any(tmax > st.m + RESCALE_LOG2 / c)) raise<D>(st, tmax, c, g);
   const bf16x8 pf = probabilities(sc, st.m, c, st.l);
-  // V's pair j of key e; 4 bits: all of them, of which only a scale can make NaN
-  auto pair = [&](int e, int j) {
-    if constexpr (MX) return (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) == 255u ? 0x7fff7fffu : 0u;
-    else return tl.v.x[e][j];
-  };
+  if constexpr (MX) read_v<D>(tl.v, slot, n, g);
+  // (4 bits: the scales 253 and 254 take some codes past bf16, 255 makes NaN of all)
   bool odd = false;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (MX) {
+      odd |= (((e < 4 ? tl.v.sc.x : tl.v.sc.y) >> (8 * (e & 3))) & 255u) >= 253u;
+    } else {
 #pragma unroll
-    for (int j = 0; j < (MX ? 1 : NB / 2); ++j) odd |= not_finite(pair(e, j));
+      for (int j = 0; j < NB / 2; ++j) odd |= not_finite(tl.v.x[e][j]);
+    }
+  }
   const bool cut = __any(odd);                               // (else what is hidden counts for nothing by its probability)
   const int last = hidden ? -1 : plast - k0 - 8 * g;         // of the lane's keys, the last that any row sees
-  if (cut) {
+  // marks of key e's columns from `from` on, which lie in one word of a row's, in the rows from the key's own query on
+  auto mark = [&](int e, int g, int from, uint32_t m) {
+    const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);
+    for (int r = first; r < rows.rows; ++r) {
+      const int at = r * D + from;
+      atomicOr(marks + at / 16, m << (2 * (at % 16)));
+    }
+    marks[D] = 1u;
+  };
+  if constexpr (!MX) {
+    if (cut) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 8; ++e) {
 #pragma unroll
-      for (int j = 0; j < (MX ? 1 : NB / 2); ++j) {
-        const uint32_t two = pair(e, j);
-        if (e <= last && not_finite(two)) {
-          const uint32_t m2 = mark_of(two & 0xffffu) | mark_of(two >> 16) << 2;
-          const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);          // rows from the key's own query on
-          for (int r = first; r < rows.rows; ++r) {
-            const int at = r * D + n * NB + 2 * j;             // 16 columns a word; the lane's NB lie in one
-            atomicOr(marks + at / 16, (MX ? static_cast<uint32_t>((1ull << (2 * NB)) - 1) : m2) << (2 * (at % 16)));
-          }
-          marks[D] = 1u;
+        for (int j = 0; j < NB / 2; ++j) {
+          const uint32_t two = tl.v.x[e][j];
+          if (e <= last && not_finite(two)) mark(e, g, n * NB + 2 * j, mark_of(two & 0xffffu) | mark_of(two >> 16) << 2);
         }
       }
     }
   }
   product<D, MX, true>(tl.v, pf, last, cut, st);
+  if constexpr (MX) {
+    if (cut) {                                               // (a value at a time from LDS: the registers hold no more)
+      int here = lane;                                       // (nor what follows from it, kept through the tiles)
+      asm volatile("" : "+v"(here));
+      const int m = here & 15, h = here >> 4;
+      const char* values = slot + Ring<D>::HALF + h * (4 * D) + m * (4 * NB);
+      const char* scales = slot + Ring<D>::HALF + 16 * D + h * (D / 4) + (m * NB / 32) * 8;
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        if (e > last) continue;
+        const float s = scale_of<0>(*reinterpret_cast<const uint8_t*>(scales + e));
+        uint32_t all = 0;
+#pragma unroll 1
+        for (int j = 0; j < NB / 2; ++j) {
+          const uint32_t two = fp4_pair<0>(*reinterpret_cast<const uint8_t*>(values + e * (NB / 2) + j), s);
+          all |= (mark_of(two & 0xffffu) | mark_of(two >> 16) << 2) << (4 * j);
+        }
+        if (all) mark(e, h, m * NB, all);
+      }
+    }
+  }
 }
 
 // Blocks a CU that the registers of a kernel hold (4 bits: and its rings the LDS).
@@ -917,10 +945,9 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
         const char* slot = ring + (i % G::R) * G::SLOT;
         Tile<D, true> tl;
         read_k<D>(tl.k, slot, n, g);
-        read_v<D>(tl.v, slot, n, g);
         tl.k0 = (it0 + w + NW * i) * KT;
         tl.bad = (bads >> (2 * (i % G::R))) & 3u;
-        edge_step<D, true>(tl, qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
+        edge_step<D, true>(tl, qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks, slot);
         wait_lds_reads();
         if (i + G::R < mine) {
           issue_k(i + G::R);
@@ -992,7 +1019,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
         if (!none && i + NT <= whole) raise<D>(st, tmax, a.c, g);
       }
       for (; i < mine; ++i) {
-        edge_step<D, false>(tl[0], qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks);
+        edge_step<D, false>(tl[0], qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks, nullptr);
         if constexpr (NT > 1) {                                // the next one is here, the one after it on its way
           tl[0] = tl[1];
           if (i + 2 < mine) {
