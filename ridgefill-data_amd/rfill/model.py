@@ -603,6 +603,7 @@ class FillModel:
             st = cache.states(seq, i)
             if st["rec"] is None:
                 st["rec"] = torch.zeros(self.nv, self.dk, self.dv, dtype=torch.float32, device=h.device)
+            step.moved.add(seq)                         # (PagedCache.undo: from here on it cannot go back)
             _, st["conv"] = ops.gdn_forward(pre[r:r + n], self.nk, self.nv, self.dk, self.dv, w["conv"], st["conv"],
                                             w["a_log"], w["dt_bias"], st["rec"], out=out[r:r + n], workspace=ws)
             r += n
@@ -612,16 +613,21 @@ class FillModel:
     def forward_paged(self, cache, seqs, ids):
         """Exact forward of new tokens of several sequences of a paged cache (a token of each, or a chunk of a prompt):
         ids[b], the token ids that sequence seqs[b] gets next. Returns the logits of each sequence's last row
-        [len(seqs), V] fp32."""
+        [len(seqs), V] fp32. If it raises, the sequences are as they were (but for those whose GDN states had moved, which
+        are lost: PagedCache.undo)."""
         ids = [torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in ids]
         if len(cache.layers) != self.n_layers or cache.model is not self:
             raise ValueError("forward_paged: a cache of this model, with every layer packed")
         h, ssq = self.embed(torch.cat(ids) if ids else torch.empty(0, dtype=torch.int64))
         step = cache.plan(seqs, [x.numel() for x in ids])
-        for i in range(self.n_layers):
-            h, ssq = self.layer_paged(i, h, step, cache, ssq=ssq)
-        last = step.cu[1:].long() - 1
-        return self.logits(*ops.row_gather(h, last))
+        try:
+            for i in range(self.n_layers):
+                h, ssq = self.layer_paged(i, h, step, cache, ssq=ssq)
+            last = step.cu[1:].long() - 1
+            return self.logits(*ops.row_gather(h, last))
+        except BaseException:
+            cache.undo(step)
+            raise
 
     def embed(self, ids):
         """Embedding rows of token ids [T] (code/kva/model.py:108-109): a bit-exact row gather from the bf16

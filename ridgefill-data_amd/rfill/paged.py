@@ -7,7 +7,7 @@ PagedCache: the pages of every attention layer of a FillModel and the states of 
 FillModel.forward_paged does both) and go.
 """
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -85,7 +85,7 @@ class Pages:
 class Step:
     """New tokens of several sequences (PagedCache.plan): sequence b's rows are [cu[b], cu[b + 1]) and become its last
     tokens. On the device: table (its pages), lens (its tokens with them), cu, and of each row the slot, the position and
-    the RoPE table row."""
+    the RoPE table row. moved: the sequences whose GDN states have taken rows of it."""
     seqs: list
     counts: list
     table: torch.Tensor
@@ -96,6 +96,8 @@ class Step:
     cs: torch.Tensor
     max_rows: int
     max_keys: int
+    ends: list = None                       # tokens of each sequence with the new ones
+    moved: set = field(default_factory=set)
 
     @property
     def rows(self):
@@ -107,6 +109,7 @@ class _Sequence:
         self.tokens = 0
         self.pages = []
         self.states = {}                    # GDN layers: conv, rec (own tensors, updated in place)
+        self.lost = False                   # a step failed after its GDN states had moved (undo)
 
 
 class PagedCache:
@@ -136,6 +139,8 @@ class PagedCache:
     def _of(self, seq):
         if seq not in self._seqs:
             raise KeyError(f"no sequence {seq!r} in this cache")
+        if self._seqs[seq].lost:
+            raise RuntimeError(f"sequence {seq!r} was lost in a step that failed: remove() it")
         return self._seqs[seq]
 
     def tokens(self, seq):
@@ -177,13 +182,14 @@ class PagedCache:
     def remove(self, seq):
         """Forget a sequence; its pages are free for the next plan() or add(). (Work that reads them must have been queued
         on the stream that writes them next.)"""
-        s = self._of(seq)
+        s = self._seqs[seq] if seq in self._seqs else self._of(seq)
         del self._seqs[seq]
         self._free += reversed(s.pages)
 
     def plan(self, seqs, counts):
         """Room for counts[b] new tokens of each sequence seqs[b]: the Step that layer_paged of every layer takes. The
-        sequences count the tokens from now on. Raises MemoryError, with nothing changed, when the pages do not suffice."""
+        sequences count the tokens from now on; undo() takes that back. Raises MemoryError when the pages do not suffice.
+        Nothing is changed when it raises."""
         if len(seqs) != len(counts) or not len(seqs):
             raise ValueError(f"plan: {len(seqs)} sequences, {len(counts)} counts")
         if len(set(seqs)) != len(seqs):
@@ -192,7 +198,22 @@ class PagedCache:
             raise ValueError(f"plan: counts {list(counts)} (at least one token each)")
         ss, counts = [self._of(q) for q in seqs], [int(c) for c in counts]
         self._grow(list(zip(ss, counts)))
-        return self._step(ss, counts, list(seqs))
+        try:
+            return self._step(ss, counts, list(seqs))
+        except BaseException:
+            self._shrink(list(zip(ss, counts)))
+            raise
+
+    def undo(self, step):
+        """Take back a plan() whose rows did not get through every layer, the last one of its sequences: they lose its tokens,
+        and the pages that it took are free again. (remove()'s note on queued work holds.) A sequence whose GDN states have
+        taken rows of the step cannot go back and is lost: every call on it but remove() raises RuntimeError."""
+        ss = [self._of(q) for q in step.seqs]
+        if [s.tokens for s in ss] != step.ends:
+            raise ValueError("undo: not the last plan of its sequences")
+        self._shrink([(s, n) for q, s, n in zip(step.seqs, ss, step.counts) if q not in step.moved])
+        for q, s in zip(step.seqs, ss):
+            s.lost = q in step.moved
 
     def _grow(self, wants):
         need = [-(-(s.tokens + n) // self.page) - len(s.pages) for s, n in wants]
@@ -201,6 +222,13 @@ class PagedCache:
         for (s, n), m in zip(wants, need):
             s.pages += [self._free.pop() for _ in range(m)]
             s.tokens += n
+
+    def _shrink(self, wants):               # _grow taken back
+        for s, n in reversed(wants):
+            s.tokens -= n
+            keep = -(-s.tokens // self.page)
+            self._free += reversed(s.pages[keep:])
+            del s.pages[keep:]
 
     def _step(self, ss, counts, seqs=None):
         dev = self.model.device
@@ -216,7 +244,8 @@ class PagedCache:
         else:
             slots, pos = ops.paged_slots(table, lens, cu, sum(counts), next(iter(self.pools.values())))
             cs = self.model.rope_table(pos)
-        return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(s.tokens for s in ss))
+        ends = [s.tokens for s in ss]
+        return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(ends), ends)
 
     def read(self, seq):
         """The sequence's cache as FillModel.new_cache lays it out (bf16 buffers of its own; of 4-bit pages what they hold)."""
