@@ -248,7 +248,8 @@ class PagedCache:
         return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(ends), ends)
 
     def read(self, seq):
-        """The sequence's cache as FillModel.new_cache lays it out (bf16 buffers of its own; of 4-bit pages what they hold)."""
+        """The sequence's cache as FillModel.new_cache lays it out (bf16 buffers of its own; of 4-bit pages what they hold). The
+        rows of a plan() must have run through the layers."""
         s = self._of(seq)
         out = self.model.new_cache()
         step = self._step([s], [s.tokens]) if s.tokens else None
@@ -264,5 +265,7 @@ class PagedCache:
                 self.model.commit(c, n)
             else:
                 st = self.states(seq, i)
+                if st["conv"] is None or st["rec"] is None:
+                    raise RuntimeError(f"read: the planned tokens of sequence {seq!r} have not run through layer {i}")
                 out[i].update(conv=st["conv"].clone(), rec=st["rec"].clone(), len=s.tokens)
         return out

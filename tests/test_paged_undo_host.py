@@ -72,6 +72,14 @@ def test_lost_sequences():
         c.remove(a)
 
 
+def test_read_before_the_layers_ran():
+    c = _cache()
+    a = c.add()
+    c.plan([a], [3])
+    with pytest.raises(RuntimeError, match="not run"):
+        c.read(a)
+
+
 @pytest.mark.parametrize("moved", [(), (1,)])
 @pytest.mark.parametrize("where", ["layer", "logits"])
 def test_forward_paged_takes_its_step_back(where, moved):
