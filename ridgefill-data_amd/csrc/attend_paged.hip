@@ -689,7 +689,7 @@ __device__ __forceinline__ void edge_step(Tile<D, MX>& tl, const Queries<D, MX> 
     for (int j = 0; j < 4; ++j)
       if (hidden || k0 + 8 * g + 4 * kb + j > pos) sc[kb][j] = -INFINITY;
   const float tmax = lane_max(sc);
-  if (__any(tmax > st.m + RESCALE_LOG2 / c)) raise<D>(st, tmax, c, g);
+  if (__any(tmax > st.m + headroom(c))) raise<D>(st, tmax, c, g);
   const bf16x8 pf = probabilities(sc, st.m, c, st.l);
   if constexpr (MX) read_v<D>(tl.v, slot, n, g);
   // (4 bits: the scales 253 and 254 take some codes past bf16, 255 makes NaN of all)
@@ -916,7 +916,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
             scores<D, true>(kt, qf, sc[x], n);
             tmax = fmaxf(tmax, lane_max(sc[x]));
           }
-          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) {
+          if (__any(tmax > st.m + headroom(a.c))) {
             if (!fresh) break;
             fresh = false;
             st.m = row_max(tmax);
@@ -999,7 +999,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
           for (int x = 0; x < NT; ++x) scores<D, false>(tl[x].k, qf, sc[x], n);
           tmax = lane_max(sc[0]);
           if constexpr (NT > 1) tmax = fmaxf(tmax, lane_max(sc[NT - 1]));
-          if (__any(tmax > st.m + RESCALE_LOG2 / a.c)) {
+          if (__any(tmax > st.m + headroom(a.c))) {
             if (!fresh) break;
             fresh = false;
             st.m = row_max(tmax);
@@ -1210,7 +1210,7 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
       if (gone || 32 * kb + 8 * (j >> 2) + (j & 3) > rel) sc[kb][j] = -INFINITY;
     }
   const float tmax = top_score<AD>(sc);
-  if (__any(tmax > mref + RESCALE_LOG2 / c)) raise_tile<AD>(o, mref, lsum, tmax, c);
+  if (__any(tmax > mref + headroom(c))) raise_tile<AD>(o, mref, lsum, tmax, c);
   uint32_t pk[8 * KB];
   tile_probabilities<AD>(sc, pk, mref, lsum, c);
   bool odd = false;

@@ -69,6 +69,9 @@ struct Layout {
 // only on the tiles that raise it.
 constexpr float RESCALE_LOG2 = 8.0f;
 
+// That headroom in raw scores (c = scale log2(e)), a float still where c is tiny: from a maximum of -infinity any score rises.
+__device__ __forceinline__ float headroom(float c) { return fminf(RESCALE_LOG2 / c, 3e38f); }
+
 // Per-lane LDS byte offsets of the fragments within a stage, the same for every tile. K fragment (key
 // half kb, d step s): row 32 kb + n, chunk 2 s + hh, at k(s) + kb * 32 KCPR 16 (row 32 kb + n has the
 // swizzle of row n). V^T fragment (d block b, 16-key step stp): lane l = 16 g + t takes, in each of two
@@ -161,7 +164,7 @@ __device__ __forceinline__ void tile_step(const char* __restrict__ st, const cha
   float lo, hi;
   lane_pair(tmax, lo, hi);
   tmax = fmaxf(lo, hi);
-  if (tmax > mref + RESCALE_LOG2 / c) {                 // raise the reference (always on the first visible key)
+  if (tmax > mref + headroom(c)) {                 // raise the reference (always on the first visible key)
     const float alpha = __builtin_amdgcn_exp2f((mref - tmax) * c);    // 0 while mref is -inf
     mref = tmax;
 #pragma unroll
