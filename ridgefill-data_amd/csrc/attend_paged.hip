@@ -137,7 +137,8 @@ __device__ int split_length(const PagedArgs& a, float work, float blocks, int tm
   }
   const float lo = fmaxf(static_cast<float>(a.wmin), ceilf(work / (once ? fit : 3.f * fit)));
   const float hi = fmaxf(static_cast<float>(tmax), lo);
-  const float W = ceilf(lo * __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(hi / lo) * (static_cast<float>(lane) / 63.f)));
+  const float step = __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(hi / lo) * (static_cast<float>(lane) / 63.f));
+  const float W = lane == 63 ? hi : ceilf(lo * step);        // (hi itself: past 4 million tiles the rounded power may fall short of it)
   const float inv = 1.f / W;
   float units = 0.f;
   for (int b = 0; b < a.n_seq; ++b)
