@@ -364,21 +364,21 @@ __device__ __forceinline__ void read_v(VTile<D, true>& vt, const char* slot, int
 }
 
 // Loads from memory into LDS (64 lanes side by side from lds on), without destination registers: the kernel's own waits
-// order them. (As builtins the compiler makes every LDS read wait for all of them. M0 has no other use in this kernel.)
+// order them. (As builtins the compiler makes every LDS read wait for all of them.)
 __device__ __forceinline__ void to_lds16(uint32_t lds, const char* base, uint32_t off) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);
   const uint64_t s = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)))) << 32 |
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b)));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-               "v"(off), "s"(s) : "memory");
+               "v"(off), "s"(s) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds16(uint32_t lds, const char* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-               "v"(at) : "memory");
+               "v"(at) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds4(uint32_t lds, const void* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-               "v"(at) : "memory");
+               "v"(at) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
