@@ -17,7 +17,9 @@
 //       8 bits or less would round the probabilities by 2^-4 and more; they keep bf16's 2^-8.)
 // The waves' parts are merged through LDS in wave order. Measured, merge included: 32 sequences of 500 to 8111 keys, 8 heads of
 // 128, bf16, 79 us for the 377 MB they hold (4.8 TB/s); 48 of 1500 to 24001 in 4 bits 91 us for 405 MB; one of 122880 keys in 4
-// bits, 2 heads of 256, 30 us for 67 MB: of that 7 are the merge and 10 the launch, the first tiles' way and the end.
+// bits, 2 heads of 256, 30 us for 67 MB: of that 9 are the merge and 10 the launch, the first tiles' way and the end.
+// The bf16 kernels' addresses take more scalar registers than there are: 115, 210 and 406 of them at head_dim 64, 128 and 256 lie
+// in lanes of vector registers (4 bits: 45 to 51); no vector register spills.
 #include <stdint.h>
 
 #include <algorithm>
@@ -120,13 +122,14 @@ __device__ __forceinline__ int wave_max(int v) {                                
   return __builtin_amdgcn_readlane(wave_scan(v, 0, [](int x, int y) { return max(x, y); }), 63);
 }
 
-// k_paged_many: the key tiles of a split. Where the row blocks leave a quarter of the GPU idle (once), splits are as short as one
-// round of blocks allows (fit: its units a head): a few more than fill it wait for a second round. Otherwise the length of the
-// least estimated time: all tiles and what each unit costs besides over the round's blocks, and a third of a split for the end
-// (or one round's longest split): 1499-row chunks of three prompts 521 us at three rounds, 599 at 1.6; a unit's cost as 6, 10 or
-// 16 tiles instead of 3 changed nothing that stood out. Up to 64 sequences the lanes try 64 lengths each; more of them take a
-// length that surely fits. Every block does the same arithmetic on the same sizes: no launch has to plan before this one, and a
-// captured graph follows its lens.
+// k_paged_many: the key tiles of a split. Where the row blocks leave a quarter of the GPU idle (once), splits are as short as
+// one round of blocks allows (fit: its units a head): a few more than fill it wait for a second round. Otherwise the length of
+// the least estimated time: all tiles and what each unit costs besides over the round's blocks, and a third of a split for the
+// end (or one round's longest split): 1499-row chunks of three prompts 521 us at three rounds, 599 at 1.6; a unit's cost as 6,
+// 10 or 16 tiles instead of 3 changed nothing that stood out. Without the end's third three chunks of 1499 rows in 4 bits took
+// 905 us for 802 and three of 700 in bf16 250 for 240, but five of 500 over 5000 keys 154 for 187; with a whole split all as
+// with a third. Up to 64 sequences the lanes try 64 lengths each; more of them take a length that surely fits. Every block does
+// the same arithmetic on the same sizes: no launch has to plan before this one, and a captured graph follows its lens.
 constexpr float UNIT_TILES = 3.f;
 __device__ int split_length(const PagedArgs& a, float work, float blocks, int tmax, int nrb0, int tiles0, int lane) {
   const float fit = static_cast<float>(a.fit);
@@ -1245,7 +1248,8 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
 }
 
 // Its waves (32 rows each): 8, two a SIMD. head_dim 256: 4, with the 512 registers that O^T (128), the queries (64), two tiles'
-// scores and the edge tiles' code want (8 waves of 256 spilled 360 registers, and 350 us of 13 sequences of 256 rows were 157).
+// scores and the edge tiles' code want, and 59 more that spill (236 bytes a lane of scratch; 8 waves of 256 spilled 360 registers,
+// and 13 sequences of 256 rows took 350 us instead of 157).
 constexpr int many_waves(int d) { return d == 256 ? 4 : 8; }
 constexpr int many_rows(int d) { return 32 * many_waves(d); }
 
@@ -1580,7 +1584,10 @@ Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_
   p.kt = p.many ? (d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
   p.blocks = std::min<int64_t>(T * rep, T * rep / p.rows() + n_seq);
   const int round = p.many ? 256 : 256 * few_blocks(d, mx);
-  // (no splits either where the tiles would not count in 31 bits)
+  // No splits up to 2048 keys (or where the tiles would not count in 31 bits). One number for all: at most 1000 keys, split against
+  // not, 8 sequences of 8 heads of 128 20 / 16 us, one of 2 heads of 64 15 / 11; 2000 keys 8 of 2 heads of 64 18 / 16, of 8 heads of
+  // 128 21 / 25, of 2 heads of 256 24 / 46, in 4 bits 18 / 17 and 26 / 27, a chunk of 200 rows 32 / 62; 4000 keys 26 / 43, 4 bits
+  // 19 / 28, a chunk 40 / 111. By the number of blocks as well it could begin earlier for chunks and head_dim 256.
   const bool split = max_keys > 16 * NW * KT && static_cast<double>(p.blocks) * static_cast<double>(max_keys / p.kt + 1) < 1e9;
   p.fit = split ? std::max(1, round / hkv) : 0;
   p.once = p.blocks * 4 <= static_cast<int64_t>(p.fit) * 3;
@@ -1644,6 +1651,8 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(max_keys),
                     scale * 1.4426950408889634f, out, ldo, static_cast<float*>(workspace),
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
+                    // key tiles a split at least (a quarter or half of it, this, four times it): one sequence of 4000 keys 16 / 17 /
+                    // 33 us, of 6000 in 4 bits 15 / 14 / 20; chunks of 200 rows over 4000 keys 38 / 38 / 46, 2 of 64 over 3000 33 / 36 / 47
                     p.many ? 4 : 2 * NW};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few

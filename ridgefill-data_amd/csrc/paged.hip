@@ -120,10 +120,11 @@ __device__ __forceinline__ float inverse_rms(const float (&f)[8], float eps) {
   return static_cast<float>(m < 1e300 ? y * fma(-0.5 * m * y, y, 1.5) : y);       // (an infinity's root is 0)
 }
 
-// D / 8 lanes a head vector, 8 values a lane; blockIdx.y is the head of [queries | keys | values] (four heads of the queries, whose
-// gains and rotation are then loaded once: 6200 rows of 32 of them 35 -> 29 us, 4.6 TB/s), blockIdx.x a run of rows: the rows of one head lie side by side in a block, so that the codes of a page's tokens, side by side in memory, are
-// written together. Heads that stay bf16: a lane takes 4 values and their rotation partners. Keys that become codes: 8 values
-// side by side, for a block's scale comes from 4 lanes, and their partners once more (d / 2 apart or less, in L1).
+// D / 8 lanes a head vector, 8 values a lane; blockIdx.x is a run of rows, blockIdx.y the head of [queries | keys | values]:
+// the rows of one head lie side by side in a block, so that the codes of a page's tokens, side by side in memory, are written
+// together. Queries: four heads a block, whose gains and rotation are then loaded once (6200 rows of 32 of them 35 -> 29 us,
+// 4.6 TB/s). Heads that stay bf16: a lane takes 4 values and their rotation partners. Keys that become codes: 8 values side by
+// side, for a block's scale comes from 4 lanes, and their partners once more (d / 2 apart or less, in L1).
 constexpr int HG = 4;
 template <int D, bool MX>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {

@@ -559,7 +559,10 @@ class FillModel:
         """Exact layer i for the new rows h [rows, H] bf16 of several sequences over a paged cache (rfill.paged.PagedCache;
         step: its plan() of these rows), as layer() of each sequence alone: queries, gate, K and V of all rows from one
         product, K and V normed and rotated into the pages, attention over them, then o_proj, the residual and the MLP. GDN
-        layers continue each sequence's states. Returns (layer output [rows, H] bf16, its row sum-of-squares partials)."""
+        layers continue each sequence's states. The workspaces are the model's, as for its other layers: calls on one model
+        run on one stream, or one after the other, and a captured step is made of the operators (ops.paged_append,
+        ops.attend_paged) with a workspace of its own. Returns (layer output [rows, H] bf16, its row sum-of-squares
+        partials)."""
         if h.shape[0] != step.rows:
             raise ValueError(f"layer_paged: {h.shape[0]} rows, the step has {step.rows}")
         if ssq is None:
