@@ -128,3 +128,20 @@ def test_rows_beyond_bfloat16(dev, d):                                     # noq
         got = got.cpu().double()
         assert torch.equal(got.isnan(), want.isnan()) and bool((want == float("inf")).any())
         assert torch.equal(got.nan_to_num(7.0, float("inf"), float("-inf")), want.nan_to_num(7.0, float("inf"), float("-inf")))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_of_the_smallest_scales(dev, d):                              # noqa: F811
+    """Blocks of bytes 0 to 8, 2^-127 to 2^-119: their codes' values down to 2^-128 are bfloat16 numbers, and read as such."""
+    from rfill import ops
+    from rfill.paged import Pages
+    hkv, page, n_pages = 2, 16, 2
+    pools = OP.Pools(n_pages, hkv, page, d, True)
+    g = torch.Generator().manual_seed(d)
+    for t in (pools.k, pools.v):
+        t.copy_(torch.randint(0, 256, t.shape, generator=g, dtype=torch.uint8))
+    for t in (pools.ks, pools.vs):
+        t.copy_(torch.randint(0, 9, t.shape, generator=g, dtype=torch.uint8))
+    raw = Pages(*(t.to(dev) for t in (pools.k, pools.v, pools.ks, pools.vs)))
+    for got, want in zip(ops.paged_read(raw, torch.arange(n_pages * page, device=dev)), values(pools)):
+        assert torch.equal(got.cpu().double(), want.transpose(1, 2).reshape(n_pages * page, hkv, d))
