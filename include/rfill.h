@@ -654,6 +654,66 @@ int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_
 int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows,
                                     int64_t max_keys, size_t* bytes);
 
+/* ---- answering by drafts: trees of drafted tokens over the paged cache. No counterpart in the reference. A sequence's new
+ * rows are the nodes of a tree (or several), a parent before its children; they are appended in that order like any new
+ * rows, attended by rf_attend_tree, verified by rf_verify_drafts, and rf_paged_keep moves the accepted ones together. ---- */
+
+/* rf_paged_slots for such rows: parents int32 [T] has each row's parent by its place among its sequence's rows (-1, or one
+ * that does not come before it: none). Slots are those of rf_paged_slots (rows lie in their order), positions count the
+ * tokens above a row: lens[b] - rows + its depth. seen [T, words] (row stride ld_seen, 8-byte aligned): bit j % 64 of word
+ * j / 64 is set if the row sees row j of its sequence: itself and those above it (words that are too few for a sequence
+ * lose the bits past them); zeros for rows of no sequence. */
+int rf_paged_tree(const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu,
+                  const int32_t* parents, int n_seq, int64_t n_pages, int page, int64_t T, int64_t words, int64_t* slots,
+                  int64_t* pos, uint64_t* seen, int64_t ld_seen, hipStream_t stream);
+
+/* rf_attend_paged for such rows: row i of a sequence with n new ones sees the keys before position lens[b] - n, and of the
+ * new ones those j <= i whose bit is set in its words of seen (as rf_paged_tree writes them, or any others; 64 words at
+ * least max_rows). All else, the workspace among it, is rf_attend_paged's. */
+int rf_attend_tree(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages, const int32_t* table,
+                   int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu, const uint64_t* seen,
+                   int64_t ld_seen, int64_t words, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out,
+                   int64_t ldo, void* workspace, size_t ws_bytes, hipStream_t stream);
+
+#define RF_F32 0
+#define RF_BF16 1
+
+/* Which drafted tokens the target accepts, and the token after them, from given random numbers. Sequence b's rows
+ * [cu[b], cu[b + 1]) of the T are a tree: its row 0 the root (a token that is decided), parents as rf_paged_tree, tokens
+ * int64 [T]. logits [T, vocab] (row stride ld, fp32 or bf16 by logits_kind, any alignment of a value): a row's are the target's for
+ * the token after it. With p = softmax(logits / temperature[b]) (fp32 [n_seq]) the walk starts at row 0; a row's children are
+ * tested in order, child i with u[i] (fp32 [T], in [0, 1)), the first that is accepted is the path's next row:
+ *   without draft: accepted if u[i] < p'(token), p' = p without the tokens rejected at this row, renormalised;
+ *   with draft [T, vocab] (fp32 or bf16, row stride ld_draft): draft[row] has the shares from which the row's children were
+ *     drawn; accepted if u[i] draft(token) < p'(token), p' = p, after each rejection max(p' - draft, 0), renormalised.
+ * When none is accepted, and at a row without children, the next token is the first at which the running sum of p' exceeds
+ * r[b] (fp32 [n_seq]) of its total; the largest logit's where nothing is left of p'. temperature[b] <= 0 or NaN, and
+ * temperature NULL for all (u, r and draft are then not read): the next token is the row's largest logit, the first of equal
+ * ones, and a child is accepted if it is that token. A NaN logit counts as -infinity, a NaN or negative share as 0; tokens
+ * outside [0, vocab) are rejected. A row without any logit above -infinity has no next token: -1.
+ * path [n_seq, depth] int32 (row stride ld_path): the accepted rows by their place in the sequence, from the root on, -1 behind
+ * them (a path has depth rows at most; the last one's children are then not tested); count [n_seq] int32; next [n_seq] int64.
+ * A sequence without rows gets count 0 and next -1. Weights and sums are in 64 bits. cu, tokens and parents are read on
+ * the device; max_rows <= 1024 bounds a sequence's rows (it is taken to have as many), vocab <= 2^20. The workspace (16-byte
+ * aligned, of rf_verify_drafts_workspace_bytes) need not be kept or cleared; calls that may run at once need one each. */
+int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld, int64_t vocab, int64_t T, const int64_t* tokens,
+                     const int32_t* parents, const int32_t* cu, int n_seq, const float* u, const float* r,
+                     const float* temperature, const void* draft, int draft_kind, int64_t ld_draft, int64_t max_rows,
+                     int64_t depth, int32_t* path, int64_t ld_path, int32_t* count, int64_t* next, void* workspace,
+                     size_t ws_bytes, hipStream_t stream);
+
+/* Bytes of rf_verify_drafts' workspace (draft: whether it gets one). Host only. */
+int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_t max_rows, int draft, size_t* bytes);
+
+/* K and V of the accepted rows moved together, in n_layers layers (pages: host array of their rf_pages, alike in kind, heads,
+ * head_dim and page): of sequence b's n new rows (its last tokens of lens[b]) row path[b][j] becomes row j, for j < count[b]
+ * (int32, device; at most path_width and n are taken). A path rises; an entry that does not, or that is no row, ends it.
+ * Codes and scales move as they are. Rows behind the moved ones keep what they hold, and lens is the caller's to change. A
+ * row on a page that is none does not move. */
+int rf_paged_keep(const rf_pages* const* pages, int n_layers, const int32_t* table, int64_t ld_table, int64_t table_width,
+                  const int32_t* lens, const int32_t* cu, int n_seq, const int32_t* path, int64_t ld_path, int64_t path_width,
+                  const int32_t* count, hipStream_t stream);
+
 /* ---- map formats ---- */
 
 /* int8 map rows with per-row group scales -> bf16 maps: out[i][j] = bf16(codes[i][j] * scale[i][j / group]),

@@ -56,6 +56,9 @@ struct PagedArgs {
   bool once;                               // k_paged_many: as many units as that at most
   int64_t units;                           // units a head that the launch has blocks and the workspace partials for
   int kt, wmin;                            // keys a tile, key tiles a split at least
+  const uint64_t* seen;                    // trees: of each row of q, bits of the new rows of its sequence that it sees
+  int64_t ld_seen;
+  int words;
 };
 
 struct Seq {
@@ -85,6 +88,23 @@ struct RowBlock {
     rows = min(a.rpb, s.rows * a.rep - r0);
   }
 };
+
+// Trees: of the 64 keys from the sequence's new row `off` on (before 0: its earlier tokens, which every row sees) those that
+// new row i sees, by its words; none past itself.
+__device__ __forceinline__ uint64_t tree_bits(const uint64_t* row, int words, int i, int off) {
+  auto word = [&](int w) { return w < words ? row[w] : 0ull; };
+  if (off > i) return 0;
+  if (off <= -64) return ~0ull;
+  uint64_t b;
+  if (off < 0) {
+    b = word(0) << -off | ((1ull << -off) - 1);
+  } else {
+    const int w = off >> 6, x = off & 63;
+    b = word(w) >> x;
+    if (x) b |= word(w + 1) << (64 - x);
+  }
+  return i - off >= 63 ? b : b & ((2ull << (i - off)) - 1);
+}
 
 __device__ __forceinline__ int tiles_of(int keys, int kt) { return max(1, (keys + kt - 1) / kt); }
 
@@ -678,20 +698,26 @@ __device__ __forceinline__ void product(const VTile<D, MX>& vt, const bf16x8 &pf
 // all finite, what no row sees of it and what is not finite enters the product as zero, and the latter leaves its marks in the
 // rows that see it. slot: the tile in LDS (4 bits). (Zeros in any case: 8 sequences of up to 2000 keys in 4 bits 20 us for 18, 48
 // of up to 24001 94 for 91.)
-template <int D, bool MX>
+// Trees: base is the position of the sequence's first new row, seen the words of the block's first query (and head).
+template <int D, bool MX, bool TREE>
 __device__ __forceinline__ void edge_step(Tile<D, MX>& tl, const Queries<D, MX> &qf, int pos,
-                                          Rows<D>& st, float c, int p0, int plast, const RowBlock& rows, int rep, int lane,
-                                          uint32_t* marks, [[maybe_unused]] const char* slot) {
+                                          Rows<D>& st, const PagedArgs& a, int p0, int plast, const RowBlock& rows, int lane,
+                                          uint32_t* marks, [[maybe_unused]] const char* slot,
+                                          [[maybe_unused]] const uint64_t* seen, [[maybe_unused]] int base) {
   constexpr int NB = D / 16;
-  const int n = lane & 15, g = lane >> 4, k0 = tl.k0;
+  const int n = lane & 15, g = lane >> 4, k0 = tl.k0, rep = a.rep;
+  const float c = a.c;
   f32x4 sc[2];
   scores<D, MX>(tl.k, qf, sc, n);
   const bool hidden = (tl.bad >> (g >> 1)) & 1u;             // the lane's 8 keys lie on a page that is none
+  [[maybe_unused]] uint32_t bits = 0;                        // those of its keys that its row sees
+  if constexpr (TREE)                                        // (pos -1: no row; positions before 0 see nothing)
+    bits = pos < 0 ? 0u : static_cast<uint32_t>(tree_bits(seen + (pos - p0) * a.ld_seen, a.words, pos - base, k0 + 8 * g - base));
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (hidden || k0 + 8 * g + 4 * kb + j > pos) sc[kb][j] = -INFINITY;
+      if (hidden || (TREE ? !((bits >> (4 * kb + j)) & 1u) : k0 + 8 * g + 4 * kb + j > pos)) sc[kb][j] = -INFINITY;
   const float tmax = lane_max(sc);
   if (__any(tmax > st.m + headroom(c))) raise<D>(st, tmax, c, g);
   const bf16x8 pf = probabilities(sc, st.m, c, st.l);
@@ -713,6 +739,10 @@ __device__ __forceinline__ void edge_step(Tile<D, MX>& tl, const Queries<D, MX> 
   auto mark = [&](int e, int g, int from, uint32_t m) {
     const int first = max(0, (k0 + 8 * g + e - p0) * rep - rows.off);
     for (int r = first; r < rows.rows; ++r) {
+      if constexpr (TREE) {
+        const int i = (rows.off + r) / rep;                  // its query among the block's
+        if (!(tree_bits(seen + i * a.ld_seen, a.words, p0 - base + i, k0 + 8 * g + e - base) & 1u)) continue;
+      }
       const int at = r * D + from;
       atomicOr(marks + at / 16, m << (2 * (at % 16)));
     }
@@ -764,7 +794,7 @@ struct FewLds {
   static constexpr int BYTES = MARKS + 4 * D + 16;
 };
 
-template <int D, bool MX>
+template <int D, bool MX, bool TREE>
 __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(PagedArgs a) {
   constexpr int NB = D / 16;
   using F = FewLds<D, MX>;
@@ -797,7 +827,8 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
     const int64_t part = static_cast<int64_t>(2 * x0 + (once ? 0 : 1)) * a.hkv + head;    // (only the first and last pieces are parts)
     at += a.fit ? itn - it0 : 1;
     const RowBlock r(a, u.s, u.rb);
-    const int p0 = u.s.keys - u.s.rows + r.q0;                 // position of its first query (may lie before 0)
+    const int base = u.s.keys - u.s.rows, p0 = base + r.q0;    // position of its first query (may lie before 0)
+    [[maybe_unused]] const uint64_t* seen = TREE ? a.seen + (u.s.first + r.q0) * a.ld_seen : nullptr;
     const int plast = p0 + (r.off + r.rows - 1) / a.rep;       // keys 0 .. plast are read
     const int it1 = min(itn, plast < 0 ? 0 : plast / KT + 1);
 
@@ -840,7 +871,8 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
     // Whole tiles first, then the tiles that some row sees in part; from the first page that is none on all of them are taken as
     // such. A maximum that has to rise leaves the inner loop: with the rescale inside it the compiler moves all of O at every tile.
     // (Not the first of a piece, which 13 sequences at head_dim 256, two tiles a wave, took 2 us longer for.)
-    const int whole = p0 >= KT - 1 ? min(mine, ((p0 + 1) / KT - it0 - w + NW - 1) / NW) : 0;
+    const int sure = TREE ? base : p0 + 1;                     // keys that every row sees
+    const int whole = sure >= KT ? min(mine, (sure / KT - it0 - w + NW - 1) / NW) : 0;
     int i = 0;
     bool none = false, fresh = true;                           // fresh: O is zero, nothing to rescale
     if constexpr (MX) {
@@ -951,7 +983,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
         read_k<D>(tl.k, slot, n, g);
         tl.k0 = (it0 + w + NW * i) * KT;
         tl.bad = (bads >> (2 * (i % G::R))) & 3u;
-        edge_step<D, true>(tl, qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks, slot);
+        edge_step<D, true, TREE>(tl, qf, pos, st, a, p0, plast, r, lane, marks, slot, seen, base);
         wait_lds_reads();
         if (i + G::R < mine) {
           issue_k(i + G::R);
@@ -1023,7 +1055,7 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
         if (!none && i + NT <= whole) raise<D>(st, tmax, a.c, g);
       }
       for (; i < mine; ++i) {
-        edge_step<D, false>(tl[0], qf, pos, st, a.c, p0, plast, r, a.rep, lane, marks, nullptr);
+        edge_step<D, false, TREE>(tl[0], qf, pos, st, a, p0, plast, r, lane, marks, nullptr, seen, base);
         if constexpr (NT > 1) {                                // the next one is here, the one after it on its way
           tl[0] = tl[1];
           if (i + 2 < mine) {
@@ -1199,19 +1231,22 @@ __device__ __forceinline__ void tile_probabilities(const f32x16 (&sc)[Cfg<AD>::K
 // tile_step for a tile of which some row does not see some key, without the next tile's scores: bad has a bit a 16-key half
 // on a page that is none. Of V, what is not finite enters the product as zero; a row that sees such a value takes it
 // from LDS afterwards (0 x infinity must not reach the rows that do not).
-template <int AD>
+// Trees: bits are those of the tile's keys that the lane's row sees.
+template <int AD, bool TREE>
 __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&sc)[Cfg<AD>::KB], f32x16 (&o)[AD / 32],
                                           float& mref, float& lsum, int k0, uint32_t bad, int mypos, int hh, float c,
-                                          const FragOffsets<AD>& fo) {
+                                          const FragOffsets<AD>& fo, [[maybe_unused]] uint64_t bits) {
   using L = Layout<AD>;
   constexpr int NB = AD / 32, KB = Cfg<AD>::KB, KTL = Cfg<AD>::KT;
   const int rel = min(max(mypos - k0, -1), KTL) - 4 * hh;
+  [[maybe_unused]] const uint64_t mine = bits >> (4 * hh);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const bool gone = (bad >> (2 * kb + (j >> 3))) & 1u;   // keys 32 kb + 8 (j / 4) + ..
-      if (gone || 32 * kb + 8 * (j >> 2) + (j & 3) > rel) sc[kb][j] = -INFINITY;
+      const int key = 32 * kb + 8 * (j >> 2) + (j & 3);      // (of the lane's half: 4 hh more)
+      if (gone || (TREE ? !((mine >> key) & 1u) : key > rel)) sc[kb][j] = -INFINITY;
     }
   const float tmax = top_score<AD>(sc);
   if (__any(tmax > mref + headroom(c))) raise_tile<AD>(o, mref, lsum, tmax, c);
@@ -1233,7 +1268,7 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
   }
   if (!__any(odd)) return;
   for (int kk = 0; kk < KTL; ++kk) {
-    if (((bad >> (kk >> 4)) & 1u) || k0 + kk > mypos) continue;
+    if (((bad >> (kk >> 4)) & 1u) || (TREE ? !((bits >> kk) & 1u) : k0 + kk > mypos)) continue;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1253,7 +1288,7 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
 constexpr int many_waves(int d) { return d == 256 ? 4 : 8; }
 constexpr int many_rows(int d) { return 32 * many_waves(d); }
 
-template <int AD, bool MX>
+template <int AD, bool MX, bool TREE>
 __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs a) {
   using L = Layout<AD>;
   constexpr int NS = AD / 16, NB = AD / 32, KTL = Cfg<AD>::KT, QROWS = many_rows(AD), KB = Cfg<AD>::KB;
@@ -1268,7 +1303,7 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
   if (u.b < 0) return;                                       // (uniform over the block: before any barrier)
   const RowBlock rb(a, u.s, u.rb);
   const int q0 = rb.q0, rows = rb.rows;
-  const int p0 = u.s.keys - u.s.rows + q0, plast = p0 + (rb.off + rows - 1) / a.rep;
+  const int base = u.s.keys - u.s.rows, p0 = base + q0, plast = p0 + (rb.off + rows - 1) / a.rep;
   const int ntiles = plast < 0 ? 0 : plast / KTL + 1;
   const int it0 = u.sp * u.W, it1 = min(ntiles, it0 + u.W);
 
@@ -1314,8 +1349,8 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
     return static_cast<uint32_t>((win == window ? bad : bad_before) >> x) & ((1u << HPT) - 1u);
   };
   const int mask = (1 << a.pg.shift) - 1;
-  char* base = reinterpret_cast<char*>(lds);
-  auto stage = [&](int it) { return base + ((it - it0) % NSTAGE) * L::STAGE_U4 * 16; };
+  char* stages = reinterpret_cast<char*>(lds);
+  auto stage = [&](int it) { return stages + ((it - it0) % NSTAGE) * L::STAGE_U4 * 16; };
   auto id_of = [&](int it, int half) { return __builtin_amdgcn_readlane(ids, ((it - it0) % WIN) * HPT + half); };
 
   // bf16: instruction i of wave w fills 64 consecutive 16-byte slots, rows row0 .. of one half; the lane's slot gives the row
@@ -1393,7 +1428,8 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
     for (int it = it0; it < it1; ++it) turn(it);
     return;
   }
-  const int full = p0 >= KTL - 1 ? min(it1, (p0 + 1) / KTL) : it0;
+  const int sure = TREE ? base : p0 + 1;                     // keys that every row sees
+  const int full = sure >= KTL ? min(it1, sure / KTL) : it0;
   int it = it0;
   for (; it + 1 < full; it += 2) {
     if (bad_of(it) | bad_of(it + 1)) break;
@@ -1405,7 +1441,9 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
   for (; it < it1; ++it) {
     turn(it);
     if (it * KTL > wave_last) continue;                      // this and every later tile lie past the wave's rows
-    edge_tile<AD>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), mypos, hh, c, fo);
+    uint64_t bits = 0;
+    if constexpr (TREE) bits = tree_bits(a.seen + static_cast<int64_t>(u.s.first + q0 + qi) * a.ld_seen, a.words, q0 + qi, it * KTL - base);
+    edge_tile<AD, TREE>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), mypos, hh, c, fo, bits);
     tile_scores<AD>(stage(it + 1), qf, sc, fo);
   }
   wait_vm_lgkm0<0>();
@@ -1621,15 +1659,18 @@ extern "C" int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d
   return RF_OK;
 }
 
-extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages,
-                               const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens,
-                               const int32_t* cu, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out,
-                               int64_t ldo, void* workspace, size_t ws_bytes, hipStream_t stream) {
-  const char* fn = "rf_attend_paged";
+namespace rf {
+namespace {
+
+template <bool TREE>
+int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages, const int32_t* table,
+           int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu, const uint64_t* seen, int64_t ld_seen,
+           int64_t words, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out, int64_t ldo,
+           void* workspace, size_t ws_bytes, hipStream_t stream) {
   PagesDev pg;
   if (int rc = check_pages(fn, pages, &pg)) return rc;
   const int d = pages->d, hkv = pages->hkv;
-  if (!q || !table || !lens || !cu || !out) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (!q || !table || !lens || !cu || !out || (TREE && !seen)) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
   if (int rc = attend_sizes(fn, T, hq, hkv, d, pages->kind, n_seq, max_rows, max_keys)) return rc;
   if (ldq < static_cast<int64_t>(hq) * d || ldo < static_cast<int64_t>(hq) * d || ldq % 8 || ldo % 4 || table_width < 0 ||
       table_width > (1 << 26) || ld_table < table_width)
@@ -1639,6 +1680,9 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
     return fail(RF_EINVAL_SHAPE, "%s: alignment", fn);
   if (!(scale > 0.f) || !(scale < 1e30f))
     return fail(RF_EINVAL_ARG, "%s: scale %g (must be positive)", fn, static_cast<double>(scale));
+  if (TREE && (words < 1 || words > (1 << 18) || ld_seen < words || 64 * words < std::min(max_rows, T) || (reinterpret_cast<uintptr_t>(seen) & 7u)))
+    return fail(RF_EINVAL_SHAPE, "%s: %lld words of bits a row (row stride %lld) for up to %lld rows a sequence", fn, (long long)words,
+                (long long)ld_seen, (long long)max_rows);
   if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
   Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys);
   if (std::max(p.units, p.blocks) * hkv > INT32_MAX)
@@ -1653,7 +1697,7 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
                     // key tiles a split at least (a quarter or half of it, this, four times it): one sequence of 4000 keys 16 / 17 /
                     // 33 us, of 6000 in 4 bits 15 / 14 / 20; chunks of 200 rows over 4000 keys 38 / 38 / 46, 2 of 64 over 3000 33 / 36 / 47
-                    p.many ? 4 : 2 * NW};
+                    p.many ? 4 : 2 * NW, seen, ld_seen, static_cast<int>(words)};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
   const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, p.rows());
@@ -1663,10 +1707,10 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
 #define RF_ATTEND(D)                                                                                     \
   do {                                                                                                   \
     if (p.many && mx) {                                                                                  \
-      if constexpr (D != 256) hipLaunchKernelGGL((k_paged_many<D, true>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
-    } else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
-    else if (mx) hipLaunchKernelGGL((k_paged_few<D, true>), grid, dim3(64 * NW), 0, stream, a);          \
-    else hipLaunchKernelGGL((k_paged_few<D, false>), grid, dim3(64 * NW), 0, stream, a);                 \
+      if constexpr (D != 256) hipLaunchKernelGGL((k_paged_many<D, true, TREE>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    } else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false, TREE>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    else if (mx) hipLaunchKernelGGL((k_paged_few<D, true, TREE>), grid, dim3(64 * NW), 0, stream, a);          \
+    else hipLaunchKernelGGL((k_paged_few<D, false, TREE>), grid, dim3(64 * NW), 0, stream, a);                 \
     if (p.fit) {                                                                                         \
       if (int rc = check_launch(fn)) return rc;                                                          \
       if (p.many) hipLaunchKernelGGL((k_paged_merge<D, false>), grid2, merge, 0, stream, a);   \
@@ -1678,4 +1722,24 @@ extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq
   else RF_ATTEND(256);
 #undef RF_ATTEND
   return check_launch(fn);
+}
+
+}  // namespace
+}  // namespace rf
+
+extern "C" int rf_attend_paged(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages,
+                               const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens,
+                               const int32_t* cu, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out,
+                               int64_t ldo, void* workspace, size_t ws_bytes, hipStream_t stream) {
+  return attend<false>("rf_attend_paged", q, ldq, T, hq, pages, table, ld_table, table_width, lens, cu, nullptr, 0, 0, n_seq,
+                       max_rows, max_keys, scale, out, ldo, workspace, ws_bytes, stream);
+}
+
+extern "C" int rf_attend_tree(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages,
+                              const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens,
+                              const int32_t* cu, const uint64_t* seen, int64_t ld_seen, int64_t words, int n_seq,
+                              int64_t max_rows, int64_t max_keys, float scale, uint16_t* out, int64_t ldo, void* workspace,
+                              size_t ws_bytes, hipStream_t stream) {
+  return attend<true>("rf_attend_tree", q, ldq, T, hq, pages, table, ld_table, table_width, lens, cu, seen, ld_seen, words, n_seq,
+                      max_rows, max_keys, scale, out, ldo, workspace, ws_bytes, stream);
 }

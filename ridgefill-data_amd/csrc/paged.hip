@@ -12,30 +12,186 @@ namespace {
 
 // Sequence of row t: the last b with cu[b] <= t (empty sequences share a start, the last of them wins, which holds row t
 // if any does). cu need not rise for the search to stay inside [0, n_seq).
-__global__ __launch_bounds__(256) void k_paged_slots(const int32_t* __restrict__ table, int64_t ld_table, int64_t width,
-                                                     const int32_t* __restrict__ lens, const int32_t* __restrict__ cu,
-                                                     int n_seq, int64_t n_pages, int shift, int64_t T,
-                                                     int64_t* __restrict__ slots, int64_t* __restrict__ pos) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (t >= T) return;
+__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int n_seq, int64_t t) {
   int lo = 0, hi = n_seq;                                    // cu[lo] <= t (or lo = 0), hi past it
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (cu[mid] <= t) lo = mid;
     else hi = mid;
   }
+  return lo;
+}
+
+// The slot of a sequence's position p by its row of the table; -1: none.
+__device__ __forceinline__ int64_t slot_of(const int32_t* __restrict__ row, int64_t width, int64_t n_pages, int shift, int64_t p) {
+  const int64_t at = p >> shift;
+  if (p < 0 || at >= width) return -1;
+  const int64_t pg = row[at];
+  return pg >= 0 && pg < n_pages ? (pg << shift) + (p & ((1 << shift) - 1)) : -1;
+}
+
+__global__ __launch_bounds__(256) void k_paged_slots(const int32_t* __restrict__ table, int64_t ld_table, int64_t width,
+                                                     const int32_t* __restrict__ lens, const int32_t* __restrict__ cu,
+                                                     int n_seq, int64_t n_pages, int shift, int64_t T,
+                                                     int64_t* __restrict__ slots, int64_t* __restrict__ pos) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (t >= T) return;
+  const int b = sequence_of(cu, n_seq, t);
   int64_t slot = -1, p = 0;
-  if (n_seq > 0 && t >= cu[lo] && t < cu[lo + 1]) {
-    p = static_cast<int64_t>(lens[lo]) - cu[lo + 1] + t;
-    const int64_t at = p >> shift;
-    if (p >= 0 && at < width) {
-      const int64_t pg = table[lo * ld_table + at];
-      if (pg >= 0 && pg < n_pages) slot = (pg << shift) + (p & ((1 << shift) - 1));
-    }
+  if (n_seq > 0 && t >= cu[b] && t < cu[b + 1]) {
+    p = static_cast<int64_t>(lens[b]) - cu[b + 1] + t;
+    slot = slot_of(table + b * ld_table, width, n_pages, shift, p);
     if (p < 0) p = 0;
   }
   slots[t] = slot;
   pos[t] = p;
+}
+
+// Of new rows that are the nodes of trees: slots as above, positions by depth, and the bits of the rows each one sees (itself
+// and those above it). A thread walks up from its row; the block's rows and what comes before them in their sequences have
+// their parents in LDS (a step up is then some 60 cycles, not a load from L2).
+constexpr int TREE_PARENTS = 4096;
+__global__ __launch_bounds__(256) void k_paged_tree(const int32_t* __restrict__ table, int64_t ld_table, int64_t width,
+                                                    const int32_t* __restrict__ lens, const int32_t* __restrict__ cu,
+                                                    const int32_t* __restrict__ parents, int n_seq, int64_t n_pages, int shift,
+                                                    int64_t T, int words, int64_t* __restrict__ slots, int64_t* __restrict__ pos,
+                                                    uint64_t* __restrict__ seen, int64_t ld_seen) {
+  __shared__ int32_t held[TREE_PARENTS];
+  __shared__ int64_t from;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * 256, t = t0 + threadIdx.x, end = min(T, t0 + 256);
+  const int b = n_seq > 0 ? sequence_of(cu, n_seq, min(t, T - 1)) : 0;
+  if (threadIdx.x == 0) from = n_seq > 0 ? min(max<int64_t>(cu[b], 0), t0) : t0;
+  __syncthreads();
+  const int64_t lo = max(from, end - TREE_PARENTS);
+  for (int64_t i = lo + threadIdx.x; i < end; i += 256) held[i - lo] = parents[i];
+  __syncthreads();
+  if (t >= T) return;
+  uint64_t* row = seen + t * ld_seen;
+  int64_t slot = -1, p = 0;
+  int w = words;                                             // words from here on are written
+  if (n_seq > 0 && t >= cu[b] && t < cu[b + 1] && cu[b] >= 0) {
+    const int64_t c0 = cu[b], base = static_cast<int64_t>(lens[b]) - (cu[b + 1] - c0);
+    slot = slot_of(table + b * ld_table, width, n_pages, shift, base + t - c0);
+    int j = static_cast<int>(t - c0), depth = 0, at = j >> 6;
+    uint64_t bits = 1ull << (j & 63);
+    while (true) {
+      const int64_t g = c0 + j;
+      const int up = g >= lo ? held[g - lo] : parents[g];
+      if (up < 0 || up >= j) break;                          // (a parent comes before its row; anything else is none)
+      ++depth;
+      j = up;
+      if (j >> 6 != at) {
+        for (; w > at + 1; --w) row[w - 1] = 0;
+        if (w == at + 1) row[--w] = bits;
+        at = j >> 6;
+        bits = 0;
+      }
+      bits |= 1ull << (j & 63);
+    }
+    for (; w > at + 1; --w) row[w - 1] = 0;
+    if (w == at + 1) row[--w] = bits;
+    p = max<int64_t>(base + depth, 0);
+  }
+  for (; w > 0; --w) row[w - 1] = 0;
+  slots[t] = slot;
+  pos[t] = p;
+}
+
+// The accepted rows of each sequence's tree moved together: row path[j] to row j, in all layers. A thread takes one piece of one
+// head's rows of one layer through the path in order, eight loads before their stores: the path rises, so no row is read after
+// the thread has overwritten it, and no other thread touches the piece. Bound by launch and two dependent loads (24 sequences,
+// 32 layers of 8 heads of 128: 4 MB).
+constexpr int KEEP_LAYERS = 32;
+struct KeepArgs {
+  PagesDev pg[KEEP_LAYERS];
+  const int32_t* table;
+  int64_t ld_table, width;
+  const int32_t* lens;
+  const int32_t* cu;
+  const int32_t* path;
+  int64_t ld_path;
+  int path_width;
+  const int32_t* count;
+  int items, parts;                        // pieces of a layer's rows, blocks that they take
+};
+
+constexpr int KEEP_RUN = 256;              // entries of a path at once
+struct KeepRun {
+  int32_t sp[KEEP_RUN], dp[KEEP_RUN];      // pages (-1: nothing to move)
+  int16_t so[KEEP_RUN], to[KEEP_RUN];      // tokens of them
+};
+
+template <class W, class F>
+__device__ __forceinline__ void move_pieces(const KeepRun& run, int n, char* pool, int64_t stride, F&& at) {
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < n; j0 += U) {
+    W w[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = min(j0 + i, n - 1);
+      if (j0 + i < n && run.sp[j] >= 0) w[i] = *reinterpret_cast<const W*>(pool + run.sp[j] * stride + at(run.so[j]));
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = min(j0 + i, n - 1);
+      if (j0 + i < n && run.sp[j] >= 0) *reinterpret_cast<W*>(pool + run.dp[j] * stride + at(run.to[j])) = w[i];
+    }
+  }
+}
+
+template <int D, bool MX>
+__global__ __launch_bounds__(256) void k_paged_keep(KeepArgs a) {
+  __shared__ KeepRun run;
+  __shared__ int stop;
+  const int b = blockIdx.x / a.parts, item = (blockIdx.x - b * a.parts) * 256 + threadIdx.x, t = threadIdx.x;
+  const PagesDev& pg = a.pg[blockIdx.y];
+  const int rows = max(0, a.cu[b + 1] - a.cu[b]), n = max(0, min(min(a.count[b], a.path_width), rows));
+  const int64_t base = static_cast<int64_t>(a.lens[b]) - rows;
+  const int32_t* path = a.path + b * a.ld_path;
+  const int32_t* table = a.table + b * a.ld_table;
+  constexpr int HEAD = MX ? D / 32 + 16 + D / 16 : D / 4;    // pieces of a head's row, of K and V
+  const int h = item / HEAD, x = item - h * HEAD;
+  for (int j0 = 0; j0 < n; j0 += KEEP_RUN) {
+    __syncthreads();
+    if (t == 0) stop = n - j0;
+    __syncthreads();
+    const int j = j0 + t;
+    if (j < n) {
+      const int p = path[j];
+      if (p <= (j ? path[j - 1] : -1) || p >= rows) atomicMin(&stop, t);       // (a whole number: in any order)
+      int64_t s = -1, d = -1;
+      if (p != j && p >= 0 && p < rows) {
+        s = slot_of(table, a.width, pg.n_pages, pg.shift, base + p);
+        d = slot_of(table, a.width, pg.n_pages, pg.shift, base + j);
+      }
+      const bool go = s >= 0 && d >= 0;
+      const int mask = (1 << pg.shift) - 1;
+      run.sp[t] = go ? static_cast<int32_t>(s >> pg.shift) : -1;
+      run.dp[t] = go ? static_cast<int32_t>(d >> pg.shift) : -1;
+      run.so[t] = static_cast<int16_t>(s & mask);
+      run.to[t] = static_cast<int16_t>(d & mask);
+    }
+    __syncthreads();
+    const int m = min(stop, KEEP_RUN);
+    if (item < a.items) {
+      const int64_t head = static_cast<int64_t>(h) * pg.head_bytes, scales = static_cast<int64_t>(h) * pg.head_scales;
+      if constexpr (!MX) {
+        const int y = x % (D / 8);
+        move_pieces<uint4>(run, m, (x < D / 8 ? pg.k : pg.v) + head + y * 16, pg.page_stride, [&](int tok) { return tok * (D * 2); });
+      } else if (x < D / 32) {
+        move_pieces<uint4>(run, m, pg.k + head + x * 16, pg.page_stride, [&](int tok) { return tok * (D / 2); });
+      } else if (x < D / 32 + 16) {
+        using W = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>>;
+        constexpr int RB = D / 32;
+        move_pieces<W>(run, m, pg.v + head + (x - RB) * (8 * RB), pg.page_stride, [&](int tok) { return (tok >> 3) * (4 * D) + (tok & 7) * RB; });
+      } else {
+        const int y = x - D / 32 - 16, z = y % (D / 32);
+        move_pieces<uint8_t>(run, m, reinterpret_cast<char*>(y < D / 32 ? pg.ks : pg.vs) + scales + z * 8, pg.scale_stride,
+                             [&](int tok) { return (tok >> 3) * (D / 4) + (tok & 7); });
+      }
+    }
+    if (stop < min(n - j0, KEEP_RUN)) return;                // (uniform: an entry that does not rise ends the path)
+  }
 }
 
 struct AppendArgs {
@@ -388,4 +544,73 @@ extern "C" int rf_paged_read(const rf_pages* pages, const int64_t* slots, int64_
   else { RF_READ(256); }
 #undef RF_READ
   return check_launch(fn);
+}
+
+extern "C" int rf_paged_tree(const int32_t* table, int64_t ld_table, int64_t table_width, const int32_t* lens,
+                             const int32_t* cu, const int32_t* parents, int n_seq, int64_t n_pages, int page, int64_t T,
+                             int64_t words, int64_t* slots, int64_t* pos, uint64_t* seen, int64_t ld_seen, hipStream_t stream) {
+  const char* fn = "rf_paged_tree";
+  if (!table || !lens || !cu || !parents || !slots || !pos || !seen) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (T < 0 || T > INT32_MAX || n_seq < 0 || table_width < 0 || ld_table < table_width || n_pages < 0 || page < 16 ||
+      page > 1024 || (page & (page - 1)) || words < 1 || words > (1 << 18) || ld_seen < words ||
+      (reinterpret_cast<uintptr_t>(seen) & 7u))
+    return fail(RF_EINVAL_SHAPE, "%s: %lld rows, %d sequences, table %lld wide (row stride %lld), %lld pages of %d tokens (a "
+                "power of two from 16 to 1024), %lld words a row (row stride %lld)", fn, (long long)T, n_seq,
+                (long long)table_width, (long long)ld_table, (long long)n_pages, page, (long long)words, (long long)ld_seen);
+  if (T == 0) return RF_OK;
+  hipLaunchKernelGGL(k_paged_tree, dim3(static_cast<unsigned>((T + 255) / 256)), dim3(256), 0, stream, table, ld_table,
+                     table_width, lens, cu, parents, n_seq, n_pages, log2_of(page), T, static_cast<int>(words), slots, pos, seen,
+                     ld_seen);
+  return check_launch(fn);
+}
+
+extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const int32_t* table, int64_t ld_table,
+                             int64_t table_width, const int32_t* lens, const int32_t* cu, int n_seq, const int32_t* path,
+                             int64_t ld_path, int64_t path_width, const int32_t* count, hipStream_t stream) {
+  const char* fn = "rf_paged_keep";
+  if (!pages || !table || !lens || !cu || !path || !count) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (n_layers < 1 || n_layers > 4096 || n_seq < 0 || n_seq > (1 << 20) || table_width < 0 || ld_table < table_width ||
+      path_width < 0 || path_width > (1 << 24) || ld_path < path_width)
+    return fail(RF_EINVAL_SHAPE, "%s: %d layers, %d sequences, table %lld wide (row stride %lld), paths of %lld rows (row stride "
+                "%lld)", fn, n_layers, n_seq, (long long)table_width, (long long)ld_table, (long long)path_width, (long long)ld_path);
+  const rf_pages* first = pages[0];
+  for (int i = 0; i < n_layers; ++i) {                       // (every layer is checked before any is changed)
+    PagesDev pg;
+    if (int rc = check_pages(fn, pages[i], &pg)) return rc;
+    if (pages[i]->kind != first->kind || pages[i]->hkv != first->hkv || pages[i]->d != first->d || pages[i]->page != first->page)
+      return fail(RF_EINVAL_SHAPE, "%s: layer %d's pages (kind %d, %d heads of %d, %d tokens) differ from the first's", fn, i,
+                  pages[i]->kind, pages[i]->hkv, pages[i]->d, pages[i]->page);
+  }
+  if (n_seq == 0 || path_width == 0) return RF_OK;
+  const int d = first->d;
+  const bool mx = first->kind == RF_PAGES_MX4;
+  KeepArgs a;
+  a.table = table;
+  a.ld_table = ld_table;
+  a.width = table_width;
+  a.lens = lens;
+  a.cu = cu;
+  a.path = path;
+  a.ld_path = ld_path;
+  a.path_width = static_cast<int>(path_width);
+  a.count = count;
+  a.items = first->hkv * (mx ? d / 32 + 16 + d / 16 : d / 4);
+  a.parts = (a.items + 255) / 256;
+  if (static_cast<int64_t>(n_seq) * a.parts > INT32_MAX)
+    return fail(RF_EINVAL_SHAPE, "%s: %d sequences of %d heads", fn, n_seq, first->hkv);
+  for (int at = 0; at < n_layers; at += KEEP_LAYERS) {
+    const int n = std::min(KEEP_LAYERS, n_layers - at);
+    for (int i = 0; i < n; ++i)
+      if (int rc = check_pages(fn, pages[at + i], &a.pg[i])) return rc;
+    const dim3 grid(static_cast<unsigned>(n_seq * a.parts), static_cast<unsigned>(n));
+#define RF_KEEP(D)                                                                       \
+  if (mx) hipLaunchKernelGGL((k_paged_keep<D, true>), grid, dim3(256), 0, stream, a);    \
+  else hipLaunchKernelGGL((k_paged_keep<D, false>), grid, dim3(256), 0, stream, a)
+    if (d == 64) { RF_KEEP(64); }
+    else if (d == 128) { RF_KEEP(128); }
+    else { RF_KEEP(256); }
+#undef RF_KEEP
+    if (int rc = check_launch(fn)) return rc;
+  }
+  return RF_OK;
 }

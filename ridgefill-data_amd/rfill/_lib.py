@@ -110,6 +110,13 @@ SIGNATURES = {
     "rf_paged_read": [_P, _P, _I64, _P, _I64, _P, _I64, _P],
     "rf_attend_paged": [_P, _I64, _I64, _I32, _P, _P, _I64, _I64, _P, _P, _I32, _I64, _I64, _F32, _P, _I64, _P, _SZ, _P],
     "rf_attend_paged_workspace_bytes": [_I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _PSZ],
+    "rf_paged_tree": [_P, _I64, _I64, _P, _P, _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _P],
+    "rf_attend_tree": [_P, _I64, _I64, _I32, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I32, _I64, _I64, _F32, _P, _I64, _P, _SZ,
+                       _P],
+    "rf_verify_drafts": [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
+                         _SZ, _P],
+    "rf_verify_drafts_workspace_bytes": [_I64, _I64, _I32, _I64, _I32, _PSZ],
+    "rf_paged_keep": [_PP, _I32, _P, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P],
     "rf_window_mass_workspace_bytes": [_I32, _I32, _I32, _I32, _I64, _PSZ],
     "rf_window_mass": [_P, _I64, _I32, _I64, _I32, _I32, _P, _I32, _I64, _I64, _F32, _P, _P, _SZ, _P],
 }

@@ -1129,27 +1129,162 @@ def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=N
     (more of either is not looked at). Returns [rows, hq d] bf16; a row that sees no key gets zeros, a row of no sequence is
     left as it was. workspace: uint8 device memory for splits of the keys ("auto": allocated here; None: no split; calls that
     may run at once need one each)."""
+    return _attend("attend_paged", q, pages, table, lens, cu, None, hq, scale, max_rows, max_keys, out, workspace)
+
+
+def attend_tree(q, pages, table, lens, cu, seen, hq, scale, max_rows, max_keys, out=None, workspace="auto"):
+    """attend_paged for new rows that are the nodes of trees: a row sees its sequence's earlier tokens, and of the new rows up
+    to itself those whose bit is set in seen [rows, words] (int64, as paged_tree gives it; 64 words >= max_rows)."""
+    _need(seen, "seen", torch.int64, 2)
+    if seen.shape[0] != q.shape[0] or seen.shape[1] * 64 < min(max_rows, q.shape[0]) or not seen.shape[1]:
+        raise ValueError(f"attend_tree: seen {tuple(seen.shape)} for {q.shape[0]} rows, up to {max_rows} a sequence")
+    return _attend("attend_tree", q, pages, table, lens, cu, seen, hq, scale, max_rows, max_keys, out, workspace)
+
+
+def _attend(fn, q, pages, table, lens, cu, seen, hq, scale, max_rows, max_keys, out, workspace):
     _need(q, "q", torch.bfloat16, 2)
     n = _sequences(table, lens, cu)
     rows, d = q.shape[0], pages.d
     if q.shape[1] < hq * d:
-        raise ValueError(f"attend_paged: q {tuple(q.shape)} for {hq} heads of {d}")
+        raise ValueError(f"{fn}: q {tuple(q.shape)} for {hq} heads of {d}")
     if out is None:
         out = torch.empty(rows, hq * d, dtype=torch.bfloat16, device=q.device)
     else:
         _need(out, "out", torch.bfloat16, 2)
         if out.shape[0] != rows or out.shape[1] < hq * d:
-            raise ValueError(f"attend_paged: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
+            raise ValueError(f"{fn}: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
     need = attend_paged_workspace_bytes(rows, hq, pages.hkv, d, pages.kind, n, max_rows, max_keys)
     if isinstance(workspace, str):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     if workspace is not None:
         _need(workspace, "workspace", torch.uint8, 1)
-    _same_device(pages, q, table, lens, cu, out, workspace)
+    _same_device(pages, q, table, lens, cu, seen, out, workspace)
     if rows == 0 or n == 0:
         return out
-    _call_on(q, "rf_attend_paged", _ptr(q), _rows_apart(q, hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),
-             _rows_apart(table, table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), n, max_rows, max_keys, float(scale),
+    bits = () if seen is None else (_ptr(seen), _rows_apart(seen, seen.shape[1]), seen.shape[1])
+    _call_on(q, "rf_" + fn, _ptr(q), _rows_apart(q, hq * d), rows, hq, pages.handle, _ptr(table) or _ptr(lens),
+             _rows_apart(table, table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), *bits, n, max_rows, max_keys, float(scale),
              _ptr(out), _rows_apart(out, hq * d), _ptr(workspace), 0 if workspace is None else workspace.numel(),
              _stream(q))
     return out
+
+
+# ------------------------------------------------------------------------------------------ answering by drafts
+
+def paged_tree(table, lens, cu, parents, rows, pages, max_rows):
+    """paged_slots for new rows that are the nodes of trees: parents int32 [rows], each row's parent by its place among its
+    sequence's rows (a parent comes before its children; -1: none). Returns slots, positions (the tokens before the new ones
+    and the rows above) and seen, int64 [rows, ceil(max_rows / 64)]: the bits of the rows that each one sees, itself and
+    those above it."""
+    n = _sequences(table, lens, cu)
+    _need(parents, "parents", torch.int32, 1)
+    if parents.shape[0] != rows:
+        raise ValueError(f"paged_tree: {parents.shape[0]} parents of {rows} rows")
+    if max_rows < 0:
+        raise ValueError(f"paged_tree: up to {max_rows} rows a sequence")
+    _same_device(pages, table, lens, cu, parents)
+    words = max(1, -(-max_rows // 64))
+    slots = torch.empty(rows, dtype=torch.int64, device=table.device)
+    pos, seen = torch.empty_like(slots), torch.empty(rows, words, dtype=torch.int64, device=table.device)
+    if rows:
+        _call_on(table, "rf_paged_tree", _ptr(table) or _ptr(cu), _rows_apart(table, table.shape[1]), table.shape[1],
+                 _ptr(lens) or _ptr(cu), _ptr(cu), _ptr(parents), n, pages.n_pages, pages.page, rows, words, _ptr(slots),
+                 _ptr(pos), _ptr(seen), words, _stream(cu))
+    return slots, pos, seen
+
+
+_KINDS = {torch.float32: 0, torch.bfloat16: 1}          # RF_F32, RF_BF16
+
+
+@_size_rule
+def verify_drafts_workspace_bytes(rows, vocab, n_seq, max_rows, draft):
+    """Device bytes of verify_drafts' workspace."""
+    b = ctypes.c_size_t(0)
+    _lib.call("rf_verify_drafts_workspace_bytes", rows, vocab, n_seq, max_rows, int(draft), ctypes.byref(b))
+    return b.value
+
+
+def verify_drafts(logits, tokens, parents, cu, u, r, temperature, max_rows, depth=None, draft=None, workspace="auto"):
+    """Which drafted tokens of several sequences the target accepts, and the token after them. Sequence b's rows
+    [cu[b], cu[b + 1]) (cu int32 [n + 1]) are a tree, row 0 its root; tokens int64 [rows], parents int32 [rows] (paged_tree).
+    logits [rows, vocab] fp32 or bf16: the target's for the token after each row. The path starts at the root; a row's
+    children are tested in order, child i with the random number u[i] (fp32 [rows], in [0, 1)), and the first accepted one
+    is the path's next row. With p = softmax(logits / temperature[b]) (fp32 [n]):
+      without draft, a child's token is accepted if u < p'(token), p' = p without the tokens rejected there, renormalised;
+      with draft [rows, vocab] (fp32 or bf16; draft[row]: the shares that the row's children were drawn from), if
+        u draft(token) < p'(token), p' = p, after each rejection max(p' - draft, 0), renormalised.
+    When none is accepted the next token is the first at which the running sum of p' exceeds r[b] (fp32 [n]) of its total.
+    temperature[b] <= 0 (None: all of them; u and r may be None): the largest logit's token, accepted if it is a child's.
+    max_rows: host bound on a sequence's rows (up to 1024); depth: on a path's (max_rows). Returns path int32 [n, depth] (rows
+    by their place in the sequence, -1 behind the last), count int32 [n] and next int64 [n] (-1: no logit above -infinity, or
+    no rows). workspace: uint8 device memory ("auto": allocated here; calls that may run at once need one each)."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _KINDS:
+        raise ValueError(f"verify_drafts: logits {getattr(logits, 'dtype', type(logits))}, expected float32 or bfloat16")
+    _need(logits, "logits", logits.dtype, 2)
+    rows, vocab = logits.shape
+    _need(tokens, "tokens", torch.int64, 1)
+    _need(parents, "parents", torch.int32, 1)
+    _need(cu, "cu", torch.int32, 1)
+    n = cu.shape[0] - 1
+    if n < 0 or tokens.shape[0] != rows or parents.shape[0] != rows:
+        raise ValueError(f"verify_drafts: {rows} rows of logits, {tokens.shape[0]} tokens, {parents.shape[0]} parents, "
+                         f"{cu.shape[0]} offsets")
+    if temperature is None:
+        u = r = draft = None
+    else:
+        for name, t, m in (("temperature", temperature, n), ("u", u, rows), ("r", r, n)):
+            _need(t, name, torch.float32, 1)
+            if t.shape[0] != m:
+                raise ValueError(f"verify_drafts: {name} {tuple(t.shape)}, expected [{m}]")
+    if draft is not None:
+        if not isinstance(draft, torch.Tensor) or draft.dtype not in _KINDS:
+            raise ValueError(f"verify_drafts: draft {getattr(draft, 'dtype', type(draft))}, expected float32 or bfloat16")
+        _need(draft, "draft", draft.dtype, 2)
+        if draft.shape != logits.shape:
+            raise ValueError(f"verify_drafts: draft {tuple(draft.shape)}, expected {tuple(logits.shape)}")
+    depth = max(1, max_rows) if depth is None else depth
+    if depth < 1:
+        raise ValueError(f"verify_drafts: paths of {depth} rows")
+    dev = logits.get_device()
+    for name, t in (("tokens", tokens), ("parents", parents), ("cu", cu), ("u", u), ("r", r), ("temperature", temperature),
+                    ("draft", draft)):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"verify_drafts: {name} is on {t.device}, logits on {logits.device}")
+    need = verify_drafts_workspace_bytes(rows, vocab, n, max_rows, draft is not None)
+    if isinstance(workspace, str):
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    _need(workspace, "workspace", torch.uint8, 1)
+    if workspace.get_device() != dev or workspace.numel() < need:
+        raise ValueError(f"verify_drafts: workspace of {workspace.numel()} bytes on {workspace.device}, {need} needed")
+    path = torch.empty(n, depth, dtype=torch.int32, device=logits.device)
+    count, nxt = torch.empty(n, dtype=torch.int32, device=logits.device), torch.empty(n, dtype=torch.int64, device=logits.device)
+    if n:
+        _call_on(logits, "rf_verify_drafts", _ptr(logits), _KINDS[logits.dtype], _rows_apart(logits, vocab), vocab, rows,
+                 _ptr(tokens), _ptr(parents), _ptr(cu), n, _ptr(u), _ptr(r), _ptr(temperature), _ptr(draft),
+                 0 if draft is None else _KINDS[draft.dtype], 0 if draft is None else _rows_apart(draft, vocab), max_rows, depth,
+                 _ptr(path), depth, _ptr(count), _ptr(nxt), _ptr(workspace) or None, workspace.numel(), _stream(logits))
+    return path, count, nxt
+
+
+def paged_keep(pools, table, lens, cu, path, count):
+    """Move the accepted rows of each sequence's tree together, in all layers' pages (pools: a list of rfill.paged.Pages,
+    alike but for their memory): of its new rows [cu[b], cu[b + 1]), the last of its lens[b] tokens in the pages table[b]
+    lists, row path[b, j] becomes row j, for j < count[b] (path int32 [n, depth], count int32 [n], as verify_drafts gives
+    them, on the device). An entry that does not rise, or is no row, ends a path. K and V keep their bits."""
+    if not pools:
+        raise ValueError("paged_keep: no layers")
+    n = _sequences(table, lens, cu)
+    _need(path, "path", torch.int32, 2)
+    _need(count, "count", torch.int32, 1)
+    if path.shape[0] != n or count.shape[0] != n:
+        raise ValueError(f"paged_keep: path {tuple(path.shape)}, count {tuple(count.shape)} of {n} sequences")
+    first = pools[0]
+    for p in pools:
+        if (p.kind, p.hkv, p.d, p.page) != (first.kind, first.hkv, first.d, first.page):
+            raise ValueError("paged_keep: the layers' pages differ in kind, heads, head_dim or tokens a page")
+        _same_device(p, table, lens, cu, path, count)
+    if n == 0 or path.shape[1] == 0:
+        return
+    _call_on(table, "rf_paged_keep", (ctypes.c_void_p * len(pools))(*(p.handle for p in pools)), len(pools),
+             _ptr(table) or _ptr(cu), _rows_apart(table, table.shape[1]), table.shape[1], _ptr(lens), _ptr(cu), n, _ptr(path),
+             _rows_apart(path, path.shape[1]), path.shape[1], _ptr(count), _stream(table))
