@@ -694,7 +694,7 @@ int rf_attend_tree(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_p
  * path [n_seq, depth] int32 (row stride ld_path): the accepted rows by their place in the sequence, from the root on, -1 behind
  * them (a path has depth rows at most; the last one's children are then not tested); count [n_seq] int32; next [n_seq] int64.
  * A sequence without rows gets count 0 and next -1. Weights and sums are in 64 bits. cu, tokens and parents are read on
- * the device; max_rows <= 1024 bounds a sequence's rows (it is taken to have as many), vocab <= 2^20. The workspace (16-byte
+ * the device; max_rows <= 1024 bounds a sequence's rows (it is taken to have as many), vocab <= 2^19. The workspace (16-byte
  * aligned, of rf_verify_drafts_workspace_bytes) need not be kept or cleared; calls that may run at once need one each. */
 int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld, int64_t vocab, int64_t T, const int64_t* tokens,
                      const int32_t* parents, const int32_t* cu, int n_seq, const float* u, const float* r,
@@ -702,8 +702,8 @@ int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld, int64_t vo
                      int64_t depth, int32_t* path, int64_t ld_path, int32_t* count, int64_t* next, void* workspace,
                      size_t ws_bytes, hipStream_t stream);
 
-/* Bytes of rf_verify_drafts' workspace (draft: whether it gets one). Host only. */
-int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_t max_rows, int draft, size_t* bytes);
+/* Bytes of rf_verify_drafts' workspace. Host only. */
+int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_t max_rows, size_t* bytes);
 
 /* K and V of the accepted rows moved together, in n_layers layers (pages: host array of their rf_pages, alike in kind, heads,
  * head_dim and page): of sequence b's n new rows (its last tokens of lens[b]) row path[b][j] becomes row j, for j < count[b]

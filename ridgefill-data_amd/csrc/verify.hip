@@ -9,34 +9,39 @@
 //       takes one pass over a row and no memory; a child's token is accepted if u q Z_k < max(p - c_k q, 0).
 //   the next token: the first at which the running sum of what is left exceeds r times its total.
 // The answers are whole numbers and a draw may lie next to a border (there are as many as tokens), so weights and sums are in
-// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones, and 17 instructions a logit stay below what HBM
-// takes to bring four bytes of it.
+// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones.
 //
-// Which rows a path meets is known row by row only, and a launch a row costs more than reading the others: the first launch
-// takes every row's largest logit and weight sums by chunks (HBM's rate is its bound), the last walks (a block a sequence; its
-// rows' numbers are gathered at once into LDS) and finds the next token in one chunk. With draft probabilities a launch between
-// them has the sums of the first row in which a token is rejected, on as many blocks as the row has chunks; later rejections
-// the walking block sums by itself.
+// Three launches. k_verify_rows: every row with children gets its largest logit and weight sum by chunks (which rows a path meets
+// is known row by row only, and a launch a row costs more than reading the others; a row without children is read only where a
+// path ends). k_verify_sums: the blocks of a sequence, one a chunk, gather its rows' numbers into LDS, take the walk, each the
+// same, up to the first sums that it needs (what a rejection leaves, or the last row's weights), and sum their own chunk.
+// k_verify_draw: a block a sequence draws, or, where a draft's token was rejected before its last sibling, walks on alone.
+// (The last two as one, its last block going on: the fences before and behind the count of blocks that are done take 50 ns a
+// block, one after the other: 60 us for 32 sequences over 32 chunks.)
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "rf_common.h"
 
 namespace rf {
 namespace {
 
-constexpr int CHUNK = 4096;                // logits a block of the passes over rows
-constexpr int MAX_CHUNKS = 256;
+constexpr int CHUNK = 4096;                // logits a part
+constexpr int MAX_CHUNKS = 128;
 constexpr int MAX_ROWS = 1024;             // of a sequence
-constexpr int NT = 256;                    // threads of the passes
-constexpr int NW = 1024;                   // of the walk
+constexpr int NT = 256;                    // threads of k_verify_rows
+constexpr int NW = 512;                    // of k_verify_sums
+constexpr int ND = 1024;                   // of k_verify_draw
 
 struct Part {                              // of a chunk of a row: its largest logit, where it first is (-1: nowhere), and the
   float top;                               // sum of the weights relative to it (0 for greedy rows)
   int best;
   double sum;
 };
+
+struct Stop;
 
 struct VerifyArgs {
   const char* logits;
@@ -57,7 +62,9 @@ struct VerifyArgs {
   int32_t* count;
   int64_t* next;
   Part* parts;                             // [T, chunks]
-  double* rest;                            // [n_seq, chunks]
+  Part* ends;                              // [n_seq, chunks * RUNS]: of the row whose sums a walk wants first, by runs
+  Stop* stops;                             // [n_seq]
+  int32_t* gone;                           // [n_seq, rows]
 };
 
 // N values from element e on, of which n are there (the others: 0, not read). Rows begin at any element.
@@ -93,284 +100,219 @@ __device__ __forceinline__ float load1(const E* p) {
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }        // NaN: never taken
 __device__ __forceinline__ float share(float q) { return q > 0.f ? q : 0.f; }             // (of a draft; NaN: none)
 
-// 2^t for t <= 0 (below -1075: 0; NaN likewise), to 3e-12: n = t to the nearest whole, 2^(t - n) = 1 + f g(f) with g
-// interpolated at the 8 Chebyshev nodes of [-1/2, 1/2] (2^0 is 1 exactly).
-__device__ __forceinline__ double exp2_64(double t) {
-  t = __builtin_fmax(t, -1100.0);
-  const double n = __builtin_rint(t), f = t - n;
-  double g = 0x1.63b2d796dd1efp-20;
-  g = __builtin_fma(g, f, 0x1.00c0e4e1528e6p-16);
-  g = __builtin_fma(g, f, 0x1.4308c7183d8ecp-13);
-  g = __builtin_fma(g, f, 0x1.5d877598350eap-10);
-  g = __builtin_fma(g, f, 0x1.3b2ab70ad2565p-7);
-  g = __builtin_fma(g, f, 0x1.c6b08da70cce3p-5);
-  g = __builtin_fma(g, f, 0x1.ebfbdff82a734p-3);
-  g = __builtin_fma(g, f, 0x1.62e42fef9cc69p-1);
-  return __builtin_amdgcn_ldexp(__builtin_fma(g, f, 1.0), static_cast<int>(n));
-}
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
 
-// A row's weights relative to its largest logit: log2(e) / T, or (odd) an infinite logit or temperature, where the largest
-// logits or all that are not -infinity share alike.
-struct Scale {
-  double c;
-  float top;
-  bool odd;
-  __device__ Scale(double c, float top) : c(c), top(top), odd(!(top < INFINITY) || !(c > 0)) {}
-  __device__ __forceinline__ double even(float x) const { return exp2_64((static_cast<double>(x) - top) * c); }
-  __device__ __forceinline__ double weight(float x) const {
-    if (odd) return top < INFINITY ? (x > -INFINITY ? 1.0 : 0.0) : (x == top ? 1.0 : 0.0);
-    return x > -INFINITY ? even(x) : 0.0;                    // (a row of nothing: top is -infinity too)
+// 2^t for -1022 <= t <= 0, to 3e-12: n = t to the nearest whole by adding 1.5 2^52 (n is then in the low word), 2^(t - n) =
+// 1 + f g(f) with g interpolated at the 8 Chebyshev nodes of [-1/2, 1/2] (2^0 is 1 exactly), and n added to the exponent. The
+// coefficients are kept in scalar registers: as literals each is two moves beside its product.
+struct Exp2 {
+  double g[8];
+  __device__ Exp2() : g{0x1.62e42fef9cc69p-1, 0x1.ebfbdff82a734p-3, 0x1.c6b08da70cce3p-5, 0x1.3b2ab70ad2565p-7,
+                        0x1.5d877598350eap-10, 0x1.4308c7183d8ecp-13, 0x1.00c0e4e1528e6p-16, 0x1.63b2d796dd1efp-20} {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("" : "+s"(g[i]));
+  }
+  __device__ __forceinline__ double operator()(double t) const {
+    constexpr double WHOLE = 6755399441055744.0;
+    const double n = t + WHOLE, f = t - (n - WHOLE);
+    double p = g[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = __builtin_fma(p, f, g[i]);
+    p = __builtin_fma(p, f, 1.0);
+    words2 w = __builtin_bit_cast(words2, p);                // (low, high)
+    w.y += __builtin_bit_cast(words2, n).x << 20;
+    return __builtin_bit_cast(double, w);
   }
 };
+
+// The weight of a logit x <= top relative to top: 2^((x - top) c), c = log2(e) / T; nothing below 2^-1022, for -infinity and
+// NaN. An infinite top is shared by the logits like it (any c), c = 0 by all above -infinity.
+__device__ __forceinline__ double weight(const Exp2& e, float x, float top, double c) {
+  const double t = x == top ? 0.0 : __builtin_fmax((static_cast<double>(x) - static_cast<double>(top)) * c, -1022.0);
+  const double w = e(t);
+  return t > -1022.0 && x > -INFINITY ? w : 0.0;
+}
 
 __device__ __forceinline__ double slope(float t) { return 1.4426950408889634 / static_cast<double>(t); }
 
 __device__ __forceinline__ double shfl_xor64(double v, int m) { return __shfl_xor(v, m, 64); }
 
-// The sequence that row t may lie in (as rf_paged_slots): the last b with cu[b] <= t.
+// The sequence that row t may lie in (as rf_paged_slots): the last b with cu[b] <= t. A wave looks at 64 offsets at once.
 __device__ __forceinline__ int sequence_of(const int32_t* cu, int n_seq, int64_t t) {
-  int lo = 0, hi = n_seq;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n_seq;                                    // cu[lo] <= t (or lo = 0), hi past it
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t below = __ballot(at < hi && (lane == 0 || cu[min(at, n_seq)] <= t));
+    const int k = 63 - __clzll(static_cast<long long>(below));
+    hi = min(hi, lo + (k + 1) * step);
+    lo += k * step;
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// A block a (row, chunk): 256 threads x 16 logits, all loaded before the first is used.
-template <class E>
-__global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a) {
-  constexpr int N = 16 / sizeof(E), I = CHUNK / NT / N;      // values a load, loads
-  const int64_t row = blockIdx.x / a.chunks;
-  const int x = static_cast<int>(blockIdx.x - row * a.chunks), t = threadIdx.x, lane = t & 63;
-  __shared__ float tops[NT / 64];
-  __shared__ int bests[NT / 64];
-  __shared__ double sums[NT / 64];
-  const int b = sequence_of(a.cu, a.n_seq, row);
-  if (row < a.cu[b] || row >= a.cu[b + 1]) return;           // a row of no sequence (uniform)
-  const E* src = reinterpret_cast<const E*>(a.logits) + row * a.ld;
-  float f[I][N];
-  float top = -INFINITY;
+// Largest of a block's THREADS values; every thread gets it. (lds: a value a wave; the barrier before its next use is the caller's)
+template <int THREADS>
+__device__ __forceinline__ float block_top(float v, float* lds) {
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int e = x * CHUNK + (i * NT + t) * N;
-    load<E, N>(f[i], src + e, a.V - e);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      f[i][k] = e + k < a.V ? logit(f[i][k]) : -INFINITY;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int k = 0; k < N; ++k) top = fmaxf(top, f[i][k]);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  if (lane == 0) tops[t >> 6] = top;
+  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  int best = INT32_MAX;
+  v = lds[0];
 #pragma unroll
-  for (int i = I - 1; i >= 0; --i)
+  for (int x = 1; x < THREADS / 64; ++x) v = fmaxf(v, lds[x]);
+  return v;
+}
+
+// A wave's 1024 logits from element e0 on, 16 a lane in loads of 16 bytes; past the vocabulary -infinity.
+template <class E>
+struct Step {
+  static constexpr int N = 16 / sizeof(E), I = 16 / N, SIZE = 1024;
+  float f[16];
+  __device__ __forceinline__ static int at(int e0, int k) { return e0 + (k / N) * 64 * N + static_cast<int>(threadIdx.x & 63) * N + k % N; }
+  __device__ __forceinline__ void fetch(const E* row, int e0, int V) {
+    if (e0 + SIZE <= V) {                                    // (uniform)
 #pragma unroll
-    for (int k = N - 1; k >= 0; --k)
-      if (f[i][k] == top) best = x * CHUNK + (i * NT + t) * N + k;
-  const float temp = a.temperature ? a.temperature[b] : 0.f;
-  double sum = 0;
-  if (temp > 0.f && top > -INFINITY) {                       // (uniform)
-    const Scale s(slope(temp), top);
-    if (s.odd) {
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int k = 0; k < N; ++k) sum += s.weight(f[i][k]);
+      for (int i = 0; i < I; ++i) load<E, N>(reinterpret_cast<float(&)[N]>(f[i * N]), row + at(e0, i * N), N);
     } else {
 #pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int k = 0; k < N; ++k) sum += s.even(f[i][k]);
+      for (int k = 0; k < 16; ++k) f[k] = at(e0, k) < V ? load1(row + at(e0, k)) : -INFINITY;
     }
   }
+};
+
+// A wave a share of a row's chunks: `shares` of them a row. Sums are relative to the first step's largest logit as long as the
+// others stay near it, so a step has no more to do than its maximum and its weights.
+// EXACT (with a draft: p - c q, and with it every border of what is left, moves with the row's sum): weights in 64 bits, 16
+// instructions a logit (none of them at a quarter of the rate), as 2^(x c - ref c) of logits not below ref - 1000 / c (those, NaN
+// and -infinity count 2^-1000). Without a draft a row's sum decides only whether u Z < w, and the draw sums its row again: there
+// weights are in 32 bits, 16 of them a sum in 32 bits and those in 64; the sum is off by some 1e-7 of itself, a test by a chance
+// of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, @@ in 32; their bytes take 22.)
+// Where reference and slope allow neither, weight by weight.
+template <class E, bool EXACT>
+__global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a, int shares) {
+  const int lane = threadIdx.x & 63;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (NT / 64) + (threadIdx.x >> 6);
+  const int64_t row = __builtin_amdgcn_readfirstlane(static_cast<int>(task / shares));
+  const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(task - row * shares));
+  if (row >= a.T) return;
+  const int b = sequence_of(a.cu, a.n_seq, row);
+  const int64_t c0 = a.cu[b], c1 = min<int64_t>(a.cu[b + 1], a.T);
+  if (row < c0 || row >= c1) return;                         // a row of no sequence
+  const float temp = a.temperature ? a.temperature[b] : 0.f;
+  const bool drawn = temp > 0.f;
+  if (a.temperature) {                                       // has it children? (without temperatures nothing reads a path's end again)
+    bool any = false;
+    for (int64_t i = row + 1; i < c1 && !any; i += 64) any = __any(i + lane < c1 && a.parents[min(i + lane, c1 - 1)] == row - c0);
+    if (!any) return;
+  }
+  const E* src = reinterpret_cast<const E*>(a.logits) + row * a.ld;
+  const Exp2 e2;
+  const double c = drawn ? slope(temp) : 0.0;
+  const float reach = EXACT ? static_cast<float>(1000.0 / c) : 0.f, c32 = static_cast<float>(c);
+  Part* parts = a.parts + row * a.chunks;
+  constexpr int STEPS = CHUNK / 1024;
+  const int chunks = (a.chunks - share + shares - 1) / shares, steps = chunks * STEPS;       // its chunks: share, share + shares ..
+  auto begin = [&](int i) { return (share + i / STEPS * shares) * CHUNK + i % STEPS * 1024; };
+  Step<E> now, coming;
+  now.fetch(src, begin(0), a.V);
+  float top = -INFINITY, ref = -INFINITY, lo = 0.f;          // of the chunk: the lane's largest logit, the reference
+  double sum = 0, k = 0;
+  bool fast = false;
+  int best = INT32_MAX;
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    if (i + 1 < steps) coming.fetch(src, begin(i + 1), a.V);
+    float own = now.f[0];
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    best = min(best, __shfl_xor(best, m, 64));
-    sum += shfl_xor64(sum, m);
-  }
-  if (lane == 0) {
-    bests[t >> 6] = best;
-    sums[t >> 6] = sum;
-  }
-  __syncthreads();
-  if (t == 0) {
-    best = min(min(bests[0], bests[1]), min(bests[2], bests[3]));
-    a.parts[blockIdx.x] = Part{top, top > -INFINITY ? best : -1, (sums[0] + sums[1]) + (sums[2] + sums[3])};
+    for (int x = 1; x < 16; ++x) own = fmaxf(own, now.f[x]);   // (NaN is left out by the maximum)
+    if (own > top) {
+      top = own;
+#pragma unroll
+      for (int x = 15; x >= 0; --x)
+        if (now.f[x] == own) best = now.at(begin(i), x);
+    }
+    if (drawn) {
+      if (!__all(fast ? (static_cast<double>(top) - ref) * c < (EXACT ? 500 : 64) : top == -INFINITY)) {
+        float high = top;                                    // the chunk's reference, or a new one
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) high = fmaxf(high, __shfl_xor(high, m, 64));
+        if (high > ref) {
+          sum = ref > -INFINITY ? sum * weight(e2, ref, high, c) : 0.0;
+          ref = high;
+          if constexpr (EXACT) {
+            lo = ref - reach;
+            k = -ref * c;
+            const double far = (static_cast<double>(ref) - lo) * c;
+            fast = far > 100 && far < 1020 && k > -1024 && k < 1024;
+          } else {
+            fast = ref < INFINITY && ref > -1e30f && c > 1e-25 && c < 1e25;            // (-3e38 is then nothing)
+          }
+        }
+      }
+      if (__builtin_expect(fast, 1)) {                       // (uniform; the median of three is its smallest where one is NaN)
+        std::conditional_t<EXACT, double, float> s[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          if constexpr (EXACT) s[x & 3] += e2(__builtin_fma(static_cast<double>(__builtin_amdgcn_fmed3f(now.f[x], lo, INFINITY)), c, k));
+          else s[x & 3] += __builtin_amdgcn_exp2f((__builtin_amdgcn_fmed3f(now.f[x], -3e38f, INFINITY) - ref) * c32);
+        }
+        sum += (s[0] + s[1]) + (s[2] + s[3]);
+      } else if (ref > -INFINITY) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sum += weight(e2, now.f[x], ref, c);
+      }
+    }
+    if (i % STEPS == STEPS - 1) {                            // the chunk's part
+      float high = top;
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) high = fmaxf(high, __shfl_xor(high, m, 64));
+      int first = top == high ? best : INT32_MAX;
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) {
+        first = min(first, __shfl_xor(first, m, 64));
+        sum += shfl_xor64(sum, m);
+      }
+      if (lane == 0)
+        parts[share + i / STEPS * shares] = Part{high, high > -INFINITY ? first : -1, drawn && high > -INFINITY ? sum * weight(e2, ref, high, c) : 0.0};
+      top = ref = -INFINITY;
+      sum = 0;
+      fast = false;
+      best = INT32_MAX;
+    }
+    now = coming;
   }
 }
 
-// What a block knows of its sequence's rows, in LDS.
+// What a block knows of its sequence's rows, in LDS. Of rows without children in a sequence that is not greedy: no sums.
 struct Rows {
   double* sum;                             // of the weights
+  double* w;                               // its token's weight in its parent's row
   float* top;
   int* best;
   int* parent;
   int* token;                              // -1: none of the vocabulary's
-  float* x;                                // its logit in its parent's row
   float* q;                                // its share of its parent's row of the draft
   float* u;
   __device__ Rows(char* lds, int rows) {
     sum = reinterpret_cast<double*>(lds);
-    top = reinterpret_cast<float*>(sum + rows);
+    w = sum + rows;
+    top = reinterpret_cast<float*>(w + rows);
     best = reinterpret_cast<int*>(top + rows);
     parent = best + rows;
     token = parent + rows;
-    x = reinterpret_cast<float*>(token + rows);
-    q = x + rows;
+    q = reinterpret_cast<float*>(token + rows);
     u = q + rows;
   }
 };
-constexpr int ROW_BYTES = 36;
+constexpr int ROW_BYTES = 40;
 
-// Where a sequence's path has come to.
-struct State {
-  int node, count;
-  double c, Z;                             // what is left of the node's distribution (Z in weights without a draft)
-  bool cut;                                // a draft's token was rejected here
-};
-
-struct Block {                             // a block of `threads` threads on sequence b
+struct Block {                             // a block's sequence
   int b, n;                                // its rows
   int64_t first;
   double slope;
   bool greedy;
 };
-
-template <class E, class Q>
-__device__ void gather(const VerifyArgs& a, const Block& s, const Rows& l, int threads) {
-  const int t = threadIdx.x;
-  const E* logits = reinterpret_cast<const E*>(a.logits);
-  for (int i = t; i < s.n; i += threads) {
-    const int p = i ? a.parents[s.first + i] : -1;
-    const int64_t tok = a.tokens[s.first + i];
-    const int par = p >= 0 && p < i ? p : -1, id = tok >= 0 && tok < a.V ? static_cast<int>(tok) : -1;
-    l.parent[i] = par;
-    l.token[i] = id;
-    l.u[i] = a.u ? a.u[s.first + i] : 0.f;
-    const bool in = par >= 0 && id >= 0;
-    l.x[i] = in ? logit(load1(logits + (s.first + par) * a.ld + id)) : -INFINITY;
-    l.q[i] = in && a.draft ? share(load1(reinterpret_cast<const Q*>(a.draft) + (s.first + par) * a.ld_draft + id)) : 0.f;
-  }
-  // a row's chunks by 16 lanes
-  const int j = t & 15;
-  for (int i0 = 0; i0 < s.n; i0 += threads / 16) {
-    const int i = i0 + t / 16;
-    const Part* parts = a.parts + (s.first + min(i, s.n - 1)) * a.chunks;
-    float top = -INFINITY;
-    int best = INT32_MAX;
-    for (int x = j; x < a.chunks; x += 16) {
-      const float m = parts[x].top;
-      if (m > top) {
-        top = m;
-        best = parts[x].best;
-      }
-    }
-    float all = top;
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) all = fmaxf(all, __shfl_xor(all, m, 64));
-    if (top != all) best = INT32_MAX;
-    double sum = 0;
-    if (!s.greedy && all > -INFINITY) {
-      const Scale sc(s.slope, all);
-      for (int x = j; x < a.chunks; x += 16) sum += parts[x].sum * sc.weight(parts[x].top);
-    }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-      best = min(best, __shfl_xor(best, m, 64));
-      sum += shfl_xor64(sum, m);
-    }
-    if (j == 0 && i < s.n) {
-      l.top[i] = all;
-      l.best[i] = all > -INFINITY ? best : -1;
-      l.sum[i] = sum;
-    }
-  }
-  __syncthreads();
-}
-
-// The walk: every wave takes it with the same numbers. rest(node, c) gives sum max(p - c q, 0) of a row, or NaN for "stop here".
-template <class F>
-__device__ State walk(const VerifyArgs& a, const Block& s, const Rows& l, bool write, F&& rest) {
-  const int lane = threadIdx.x & 63;
-  const bool drawn = a.draft != nullptr && !s.greedy;
-  State st{0, 1, 0.0, drawn ? 1.0 : l.sum[0], false};
-  if (write) a.path[s.b * a.ld_path] = 0;
-  int i = 1;
-  while (st.count < a.depth) {
-    // the next row below the node
-    int at = -1;
-    for (int i0 = i; i0 < s.n; i0 += 64) {
-      const uint64_t hit = __ballot(i0 + lane < s.n && l.parent[min(i0 + lane, s.n - 1)] == st.node);
-      if (hit) {
-        at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-        break;
-      }
-    }
-    if (at < 0) break;
-    at = __builtin_amdgcn_readfirstlane(at);
-    i = at + 1;
-    const int tok = l.token[at];
-    bool yes;
-    if (s.greedy) {
-      yes = tok >= 0 && tok == l.best[st.node];
-    } else {
-      const Scale sc(s.slope, l.top[st.node]);
-      const double w = sc.weight(l.x[at]), u = l.u[at];
-      if (!drawn) {
-        bool gone = tok < 0;                                 // rejected before, or no token at all
-        for (int k0 = st.node + 1; k0 < at; k0 += 64) {
-          const int k = min(k0 + lane, at - 1);
-          gone |= __any(k0 + lane < at && l.parent[k] == st.node && l.token[k] == tok);
-        }
-        const double own = gone ? 0.0 : w;
-        yes = u * st.Z < own;
-        if (!yes) st.Z = __builtin_fmax(st.Z - own, 0.0);
-      } else {
-        const double q = l.q[at], total = l.sum[st.node];
-        const double p = total > 0 ? __builtin_fmax(w / total - st.c * q, 0.0) : 0.0;
-        yes = tok >= 0 && u * q * st.Z < p;
-        if (!yes) {
-          st.c += st.Z;
-          st.cut = true;
-          const double z = rest(st.node, st.c);
-          if (!(z == z)) return st;
-          st.Z = z;
-        }
-      }
-    }
-    if (yes) {
-      st.node = at;
-      st.c = 0.0;
-      st.Z = drawn ? 1.0 : l.sum[at];
-      st.cut = false;
-      if (write) a.path[s.b * a.ld_path + st.count] = at;
-      ++st.count;
-    }
-  }
-  return st;
-}
-
-// sum max(p - c q, 0) of up to N logits and shares.
-template <int N>
-__device__ __forceinline__ double rest_of(const float (&x)[N], const float (&q)[N], const Scale& sc, double inv, double c, int n) {
-  double s = 0;
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (k < n) s += __builtin_fmax(sc.weight(logit(x[k])) * inv - c * share(q[k]), 0.0);
-  return s;
-}
-
-// 1 / S once a row: as p of the walk's tests but for its last bit. (fp64; 0 for a row of nothing)
-__device__ __forceinline__ double inverse(double s) { return s > 0 ? 1.0 / s : 0.0; }
 
 __device__ __forceinline__ Block block_of(const VerifyArgs& a, int b) {
   const int64_t c0 = max(a.cu[b], 0), c1 = min<int64_t>(a.cu[b + 1], a.T);
@@ -384,247 +326,446 @@ __device__ __forceinline__ Block block_of(const VerifyArgs& a, int b) {
   return s;
 }
 
-// The sums of the first row in which a drawn token is rejected: a block a (sequence, chunk).
-template <class E, class Q>
-__global__ __launch_bounds__(NT) void k_verify_rest(VerifyArgs a) {
-  extern __shared__ double lds[];
-  __shared__ double sums[NT / 64];
-  const int b = blockIdx.x / a.chunks, x = blockIdx.x - b * a.chunks, t = threadIdx.x;
-  const Block s = block_of(a, b);
-  if (s.n == 0 || s.greedy) return;                          // (uniform)
-  const Rows l(reinterpret_cast<char*>(lds), a.rows);
-  gather<E, Q>(a, s, l, NT);
-  const State st = walk(a, s, l, false, [](int, double) { return static_cast<double>(NAN); });
-  if (!st.cut) return;
-  const Scale sc(s.slope, l.top[st.node]);
-  const double inv = inverse(l.sum[st.node]);
-  const E* src = reinterpret_cast<const E*>(a.logits) + (s.first + st.node) * a.ld;
-  const Q* from = reinterpret_cast<const Q*>(a.draft) + (s.first + st.node) * a.ld_draft;
-  constexpr int N = 4, I = CHUNK / NT / N;
-  float f[I][N], q[I][N];
+template <class E, class Q, int THREADS>
+__device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, const Rows& l, const Exp2& e2) {
+  const int t = threadIdx.x, j = t & 15;
+  const E* logits = reinterpret_cast<const E*>(a.logits) + s.first * a.ld;
+  // a row's chunks by 16 lanes (their first loads go before those of the rows, which wait for one another)
+#pragma unroll 1
+  for (int i0 = 0; i0 < s.n; i0 += THREADS / 16) {
+    const int i = i0 + t / 16;
+    const Part* parts = a.parts + (s.first + min(i, s.n - 1)) * a.chunks;
+    const Part p0 = parts[min(j, a.chunks - 1)], p1 = parts[min(j + 16, a.chunks - 1)];
+    if (i0 == 0) {
+#pragma unroll 1
+      for (int r = t; r < s.n; r += THREADS) {
+        const int p = r ? a.parents[s.first + r] : -1;
+        const int64_t tok = a.tokens[s.first + r];
+        const int par = p >= 0 && p < r ? p : -1, id = tok >= 0 && tok < a.V ? static_cast<int>(tok) : -1;
+        l.parent[r] = par;
+        l.token[r] = id;
+        l.u[r] = a.u ? a.u[s.first + r] : 0.f;
+        const bool in = par >= 0 && id >= 0;
+        l.w[r] = in && !s.greedy ? logit(load1(logits + par * a.ld + id)) : -INFINITY;       // (its logit first)
+        l.q[r] = in && a.draft ? share(load1(reinterpret_cast<const Q*>(a.draft) + (s.first + par) * a.ld_draft + id)) : 0.f;
+      }
+    }
+    float top = j < a.chunks ? p0.top : -INFINITY;
+    int best = top > -INFINITY ? p0.best : INT32_MAX;
+    auto larger = [&](const Part& p) {
+      if (p.top > top) {
+        top = p.top;
+        best = p.best;
+      }
+    };
+    if (j + 16 < a.chunks) larger(p1);
+#pragma unroll 1
+    for (int x = j + 32; x < a.chunks; x += 16) larger(parts[x]);
+    float all = top;
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int e = x * CHUNK + (i * NT + t) * N;
-    load<E, N>(f[i], src + e, a.V - e);
-    load<Q, N>(q[i], from + e, a.V - e);
+    for (int m = 1; m < 16; m <<= 1) all = fmaxf(all, __shfl_xor(all, m, 64));
+    if (top != all) best = INT32_MAX;
+    double sum = 0;
+    if (!s.greedy && all > -INFINITY) {
+      Part p = p0;
+#pragma unroll 1
+      for (int x = j; x < a.chunks; x += 16) {
+        if (x >= 32) p = parts[x];
+        if (p.top > -INFINITY) sum += p.sum * weight(e2, p.top, all, s.slope);               // (rows without sums: left out)
+        p = p1;
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+      best = min(best, __shfl_xor(best, m, 64));
+      sum += shfl_xor64(sum, m);
+    }
+    if (j == 0 && i < s.n) {
+      l.top[i] = all;
+      l.best[i] = all > -INFINITY ? best : -1;
+      l.sum[i] = sum;
+    }
   }
-  double sum = 0;
-#pragma unroll
-  for (int i = 0; i < I; ++i) sum += rest_of<N>(f[i], q[i], sc, inv, st.c, a.V - (x * CHUNK + (i * NT + t) * N));
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) sum += shfl_xor64(sum, m);
-  if ((t & 63) == 0) sums[t >> 6] = sum;
   __syncthreads();
-  if (t == 0) a.rest[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if (!s.greedy) {
+#pragma unroll 1
+    for (int r = t; r < s.n; r += THREADS)
+      l.w[r] = l.parent[r] >= 0 && l.token[r] >= 0 ? weight(e2, static_cast<float>(l.w[r]), l.top[l.parent[r]], s.slope) : 0.0;
+    __syncthreads();
+  }
 }
 
-// A row's weights, or what is left of it, by elements.
+// Where a sequence's path has come to.
+struct State {
+  int node, count, next;                   // next: the row from which on the node's children are still to be tested
+  double c, Z;                             // what is left of the node's distribution (Z in weights without a draft)
+  bool cut;                                // a draft's token was rejected here
+};
+
+// ... when its first sums are wanted, for k_verify_draw.
+struct Stop {
+  State st;
+  double sum;                              // of the node's weights (cut)
+  float top;
+  int more, n_gone;                        // whether the walk goes on, the tokens rejected at its last row (without a draft)
+};
+
+// The walk from st on, by every wave with the same numbers. True: a drawn token was rejected, and Z = sum max(p - c q, 0) of the
+// node is wanted; false: the path has ended.
+__device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const Rows& l, State& st) {
+  const int lane = threadIdx.x & 63;
+  const bool drawn = a.draft != nullptr && !s.greedy;
+  while (st.count < a.depth) {
+    int at = -1;                                             // the next row below the node
+    for (int i0 = st.next; i0 < s.n; i0 += 64) {
+      const uint64_t hit = __ballot(i0 + lane < s.n && l.parent[min(i0 + lane, s.n - 1)] == st.node);
+      if (hit) {
+        at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        break;
+      }
+    }
+    if (at < 0) return false;
+    at = __builtin_amdgcn_readfirstlane(at);
+    st.next = at + 1;
+    const int tok = l.token[at];
+    bool yes;
+    if (s.greedy) {
+      yes = tok >= 0 && tok == l.best[st.node];
+    } else if (!drawn) {
+      if (st.Z < 0) st.Z = l.sum[st.node];                   // (the node's first child)
+      bool gone = tok < 0;                                   // rejected before, or no token at all
+      for (int k0 = st.node + 1; k0 < at; k0 += 64) {
+        const int k = min(k0 + lane, at - 1);
+        gone |= __any(k0 + lane < at && l.parent[k] == st.node && l.token[k] == tok);
+      }
+      const double own = gone ? 0.0 : l.w[at];
+      yes = l.u[at] * st.Z < own;
+      if (!yes) st.Z = __builtin_fmax(st.Z - own, 0.0);
+    } else {
+      const double q = l.q[at], total = l.sum[st.node];
+      const double p = total > 0 ? __builtin_fmax(l.w[at] / total - st.c * q, 0.0) : 0.0;
+      yes = tok >= 0 && l.u[at] * q * st.Z < p;
+      if (!yes) {
+        st.c += st.Z;
+        st.cut = true;
+        return true;
+      }
+    }
+    if (yes) {
+      st.node = at;
+      st.c = 0.0;
+      st.Z = drawn ? 1.0 : -1.0;
+      st.cut = false;
+      ++st.count;
+    }
+  }
+  return false;
+}
+
+// 1 / S once a row: as p of the walk's tests but for its last bit. (0 for a row of nothing)
+__device__ __forceinline__ double inverse(double s) { return s > 0 ? 1.0 / s : 0.0; }
+
+// What is left of a row: its weights without the tokens in `gone`, or max(p - c q, 0).
 template <class E, class Q>
 struct Left {
   const E* src;
-  const Q* from;                           // null: weights without the tokens in `gone`
-  Scale sc;
-  double inv, c;
+  const Q* from;                           // null: weights
+  double slope, inv, c;
   const int* gone;
   int n_gone;
-  __device__ __forceinline__ void weights(double (&w)[4], int e, int V) const {
-    float f[4], q[4];
-    load<E, 4>(f, src + e, V - e);
-    if (from) load<Q, 4>(q, from + e, V - e);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = e + k < V ? sc.weight(logit(f[k])) : 0.0;
-      if (from) w[k] = __builtin_fmax(w[k] * inv - c * (e + k < V ? share(q[k]) : 0.f), 0.0);
-    }
-    for (int g = 0; g < n_gone; ++g) {
-      const int at = gone[g] - e;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (at == k) w[k] = 0.0;
-    }
-  }
 };
 
-// All chunks' sums by one block of NW threads, a wave a chunk; returns their total (every thread).
-__device__ __forceinline__ double total_of(const double* cs, int chunks) {
-  double z = 0;
-  for (int x = threadIdx.x & 63; x < chunks; x += 64) z += cs[x];
+// A lane's four elements e .. e + 3: logits (NaN, what is gone and what lies past the vocabulary as -infinity) and shares.
+template <class E, class Q>
+__device__ __forceinline__ void fetch4(const Left<E, Q>& left, float (&f)[4], float (&q)[4], int e, int V) {
+  load<E, 4>(f, left.src + min(e, V), V - e);
+  if (left.from) load<Q, 4>(q, left.from + min(e, V), V - e);
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) z += shfl_xor64(z, m);
-  return z;
+  for (int k = 0; k < 4; ++k) f[k] = e + k < V ? logit(f[k]) : -INFINITY;
+#pragma unroll 1
+  for (int g = 0; g < left.n_gone; ++g) {
+    const int at = left.gone[g] - e;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = at == k ? -INFINITY : f[k];
+  }
 }
 
 template <class E, class Q>
-__device__ double sum_chunks(const Left<E, Q>& left, double* cs, int chunks, int V) {
+__device__ __forceinline__ double left4(const Left<E, Q>& left, const Exp2& e2, double (&w)[4], const float (&f)[4],
+                                        const float (&q)[4], float top) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    w[k] = weight(e2, f[k], top, left.slope);
+    if (left.from) w[k] = __builtin_fmax(w[k] * left.inv - left.c * share(q[k]), 0.0);
+  }
+  return (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+// A wave's run of RUN elements, four a lane of its first half and four of its second: its sum and its largest logit (of what is
+// left by a draft: relative to the row's).
+constexpr int RUN = 512, RUNS = CHUNK / RUN;
+static_assert(RUNS == NW / 64, "a wave a run of a chunk");
+template <class E, class Q>
+__device__ __forceinline__ Part sum_run(const Left<E, Q>& left, const Exp2& e2, int run, int V, float top) {
   const int lane = threadIdx.x & 63;
-  __syncthreads();                                           // the last sums were read
-  for (int x = threadIdx.x >> 6; x < chunks; x += NW / 64) {
-    double s = 0;
-    const int end = min(V, (x + 1) * CHUNK);
-#pragma unroll 4
-    for (int e = x * CHUNK + 4 * lane; e < end; e += 256) {
-      double w[4];
-      left.weights(w, e, V);
-      s += (w[0] + w[1]) + (w[2] + w[3]);
-    }
+  float f[2][4], q[2][4] = {};
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) s += shfl_xor64(s, m);
-    if (lane == 0) cs[x] = s;
+  for (int k = 0; k < 2; ++k) fetch4(left, f[k], q[k], run * RUN + 256 * k + 4 * lane, V);
+  if (!left.from) {
+    top = fmaxf(fmaxf(fmaxf(f[0][0], f[0][1]), fmaxf(f[0][2], f[0][3])), fmaxf(fmaxf(f[1][0], f[1][1]), fmaxf(f[1][2], f[1][3])));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
   }
-  __syncthreads();
-  return total_of(cs, chunks);
+  double sum = 0, w[4];
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    sum += left4(left, e2, w, f[0], q[0], top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[0][i] = f[1][i], q[0][i] = q[1][i];
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) sum += shfl_xor64(sum, m);
+  return Part{top, 0, sum};
 }
 
-// The first token at which the running sum exceeds r times the total, from the chunks' sums; -1: there is none to take.
+// The path of a sequence from its last row up, and its length.
+__device__ __forceinline__ void write_path(const VerifyArgs& a, int b, const int* parent, const State& st) {
+  int32_t* path = a.path + b * a.ld_path;
+#pragma unroll 1
+  for (int j = st.count + threadIdx.x; j < a.depth; j += blockDim.x) path[j] = -1;
+  if (threadIdx.x) return;
+  int at = st.node;
+#pragma unroll 1
+  for (int j = st.count - 1; j >= 0; --j) {
+    path[j] = at;
+    at = parent[at];
+  }
+  a.count[b] = st.count;
+}
+
 template <class E, class Q>
-__device__ int draw(const Left<E, Q>& left, const double* cs, int chunks, int V, double r, double* scan, int* found) {
-  const int t = threadIdx.x, lane = t & 63;
-  const double total = total_of(cs, chunks);
-  if (!(total > 0)) return -1;                               // (uniform)
-  const double want = r * total;
-  // the chunk: lane l has chunks 4 l .. 4 l + 3
-  double c4[4], own = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    c4[k] = 4 * lane + k < chunks ? cs[4 * lane + k] : 0.0;
-    own += c4[k];
+__device__ __forceinline__ Left<E, Q> left_of(const VerifyArgs& a, const Block& s, const State& st, double sum, const int* gone, int n_gone) {
+  return Left<E, Q>{reinterpret_cast<const E*>(a.logits) + (s.first + st.node) * a.ld,
+                    st.cut ? reinterpret_cast<const Q*>(a.draft) + (s.first + st.node) * a.ld_draft : nullptr, s.slope,
+                    st.cut ? inverse(sum) : 1.0, st.c, gone, n_gone};
+}
+
+// `blocks` blocks a sequence; without temperatures one, which has the answers.
+template <class E, class Q>
+__global__ __launch_bounds__(NW) void k_verify_sums(VerifyArgs a, int blocks) {
+  extern __shared__ double lds[];
+  __shared__ int n_gone;
+  const int b = blockIdx.x / blocks, x = blockIdx.x - b * blocks, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const Block s = block_of(a, b);
+  if ((s.n == 0 || !a.temperature) && x) return;             // (uniform)
+  const Rows l(reinterpret_cast<char*>(lds), a.rows);
+  State st{0, 0, 1, 0.0, a.draft != nullptr ? 1.0 : -1.0, false};
+  if (s.n == 0) {
+    write_path(a, b, l.parent, st);
+    if (t == 0) a.next[b] = -1;
+    return;
   }
-  double run = own;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double y = __shfl_up(run, m, 64);
-    if (lane >= m) run += y;
+  st.count = 1;
+  const Exp2 e2;
+  gather<E, Q, NW>(a, s, l, e2);
+  const bool more = walk(a, s, l, st);
+  if (x == 0) write_path(a, b, l.parent, st);
+  if (!a.temperature) {
+    if (t == 0) a.next[b] = l.best[st.node];
+    return;
   }
-  double before = run - own;
-  int at = -1, last = -1;
-  double base = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (at < 0 && c4[k] > 0 && before + c4[k] > want) {
-      at = 4 * lane + k;
-      base = before;
+  // the tokens rejected at the last row, each once, in the rows' order; they take the place of the rows' u
+  int* gone = reinterpret_cast<int*>(l.u);
+  int dropped = 0;
+  if (a.draft == nullptr && !s.greedy) {
+    __syncthreads();
+    if (wave == 0) {
+      int m = 0;
+#pragma unroll 1
+      for (int k0 = st.node + 1; st.count < a.depth && k0 < s.n; k0 += 64) {
+        const int k = min(k0 + lane, s.n - 1), tok = l.token[k];
+        bool here = k0 + lane < s.n && l.parent[k] == st.node && tok >= 0;
+#pragma unroll 1
+        for (int y = st.node + 1; here && y < k; ++y) here = !(l.parent[y] == st.node && l.token[y] == tok);
+        const uint64_t mask = __ballot(here);
+        if (here) gone[m + __popcll(mask & ((1ull << lane) - 1))] = tok;
+        m += __popcll(mask);
+      }
+      if (lane == 0) n_gone = m;
     }
-    if (c4[k] > 0) last = 4 * lane + k;
-    before += c4[k];
+    __syncthreads();
+    dropped = n_gone;
   }
-  const uint64_t hit = __ballot(at >= 0), some = __ballot(last >= 0);
-  int chunk;
-  if (hit) {
-    const int from = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-    chunk = __shfl(at, from, 64);
-    base = __shfl(base, from, 64);
-  } else {                                                   // r of 1 or more, or a rounding: the last token there is
-    chunk = __shfl(last, 63 - __clzll(static_cast<long long>(some)), 64);
-    base = -INFINITY;
+  const Left<E, Q> left = left_of<E, Q>(a, s, st, l.sum[st.node], gone, dropped);
+#pragma unroll 1
+  for (int run = x * RUNS + wave; run * RUN < a.V; run += blocks * RUNS) {
+    const Part p = sum_run(left, e2, run, a.V, l.top[st.node]);
+    if (lane == 0) a.ends[static_cast<int64_t>(b) * a.chunks * RUNS + run] = p;
   }
-  // its elements: thread t has 4 side by side
-  const int e = chunk * CHUNK + 4 * t;
-  double w[4];
-  left.weights(w, min(e, V), V);
-  own = (w[0] + w[1]) + (w[2] + w[3]);
-  run = own;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double y = __shfl_up(run, m, 64);
-    if (lane >= m) run += y;
-  }
-  __syncthreads();                                           // (scan, found of an earlier call)
-  if (lane == 63) scan[t >> 6] = run;
-  if (t == 0) found[0] = INT32_MAX, found[1] = -1;
-  __syncthreads();
-  double upto = base;
-  for (int x = 0; x < t >> 6; ++x) upto += scan[x];
-  upto += run - own;
-  int first = INT32_MAX, end = -1;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    upto += w[k];
-    if (w[k] > 0) {
-      if (first == INT32_MAX && upto > want) first = e + k;
-      end = e + k;
-    }
-  }
-  if (first != INT32_MAX) atomicMin(&found[0], first);       // (whole numbers: in any order)
-  if (end >= 0) atomicMax(&found[1], end);
-  __syncthreads();
-  return found[0] != INT32_MAX ? found[0] : found[1];
+  if (x) return;
+  if (t == 0) a.stops[b] = Stop{st, l.sum[st.node], l.top[st.node], more, dropped};
+#pragma unroll 1
+  for (int g = t; g < dropped; g += NW) a.gone[static_cast<int64_t>(b) * a.rows + g] = gone[g];
 }
 
 // A block a sequence.
 template <class E, class Q>
-__global__ __launch_bounds__(NW) void k_verify_walk(VerifyArgs a) {
+__global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
   extern __shared__ double lds[];
-  __shared__ double cs[MAX_CHUNKS], scan[NW / 64];
-  __shared__ int found[2], n_gone;
-  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  __shared__ float tops[ND / 64];
+  __shared__ int found;
+  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, runs = (a.V + RUN - 1) / RUN;
+  const Part* ends = a.ends + static_cast<int64_t>(b) * a.chunks * RUNS;
+  const Part mine = ends[min(t, runs - 1)];
+  const Stop stop = a.stops[b];
   const Block s = block_of(a, b);
-  if (s.n == 0) {                                            // (uniform)
-    for (int j = t; j < a.depth; j += NW) a.path[b * a.ld_path + j] = -1;
-    if (t == 0) {
-      a.count[b] = 0;
-      a.next[b] = -1;
+  if (s.n == 0) return;                                      // (uniform)
+  const Rows l(reinterpret_cast<char*>(lds), a.rows);
+  double* cs = reinterpret_cast<double*>(reinterpret_cast<char*>(lds) + static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES);    // the runs' sums
+  float* ct = reinterpret_cast<float*>(cs + runs);           // ... and largest logits
+  const Exp2 e2;
+  State st = stop.st;
+  bool more = stop.more;
+  const int* gone = a.gone + static_cast<int64_t>(b) * a.rows;
+  Left<E, Q> left = left_of<E, Q>(a, s, st, stop.sum, gone, stop.n_gone);
+  float top = stop.top;                                      // what the sums are relative to
+#pragma unroll 1
+  for (int y = t; y < runs; y += ND) {
+    const Part p = y < ND ? mine : ends[y];
+    ct[y] = p.top;
+    cs[y] = p.sum;
+  }
+  if (more) gather<E, Q, ND>(a, s, l, e2);
+  while (true) {
+    if (!st.cut) {                                           // (runs' sums are relative to their own)
+      float own = -INFINITY;
+#pragma unroll 1
+      for (int y = t; y < runs; y += ND) own = fmaxf(own, ct[y]);
+      top = block_top<ND>(own, tops);
+      if (s.greedy) break;
+#pragma unroll 1
+      for (int y = t; y < runs; y += ND) cs[y] = ct[y] > -INFINITY ? cs[y] * weight(e2, ct[y], top, s.slope) : 0.0;
     }
+    __syncthreads();
+    if (!more) break;
+    double z = 0;                                            // (every wave the same)
+#pragma unroll 1
+    for (int y = lane; y < runs; y += 64) z += cs[y];
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) z += shfl_xor64(z, m);
+    st.Z = z;
+    more = walk(a, s, l, st);
+    if (!more && st.cut) break;                              // no child was accepted: cs is what is left
+    __syncthreads();                                         // else further sums, of another rejection or the last row
+    top = l.top[st.node];
+    left = left_of<E, Q>(a, s, st, l.sum[st.node], gone, 0);
+#pragma unroll 1
+    for (int run = wave; run < runs; run += ND / 64) {
+      const Part p = sum_run(left, e2, run, a.V, top);
+      if (lane == 0) {
+        ct[run] = p.top;
+        cs[run] = p.sum;
+      }
+    }
+    __syncthreads();
+  }
+  if (stop.more) write_path(a, b, l.parent, st);
+  if (s.greedy) {                                            // the first of the row's largest logits, in the first run that has it
+    __syncthreads();
+    if (t == 0) found = INT32_MAX;
+    __syncthreads();
+#pragma unroll 1
+    for (int y = t; y < runs; y += ND)
+      if (ct[y] == top) atomicMin(&found, y);                // (whole numbers: in any order)
+    __syncthreads();
+    const int e = found * RUN + t;
+    __syncthreads();
+    if (t == 0) found = INT32_MAX;
+    __syncthreads();
+    if (top > -INFINITY && t < RUN && e < a.V && load1(left.src + e) == top) atomicMin(&found, e);
+    __syncthreads();
+    if (t == 0) a.next[b] = found == INT32_MAX ? -1 : found;
     return;
   }
-  const Rows l(reinterpret_cast<char*>(lds), a.rows);
-  gather<E, Q>(a, s, l, NW);
-  const E* logits = reinterpret_cast<const E*>(a.logits) + s.first * a.ld;
-  const Q* draft = reinterpret_cast<const Q*>(a.draft) + s.first * a.ld_draft;
-  bool ready = a.draft != nullptr;                           // k_verify_rest has the first rejection's sums
-  const State st = walk(a, s, l, t == 0, [&](int node, double c) {
-    if (ready) {
-      ready = false;
-      for (int x = t; x < a.chunks; x += NW) cs[x] = a.rest[static_cast<int64_t>(b) * a.chunks + x];
-      __syncthreads();
-      return total_of(cs, a.chunks);
-    }
-    return sum_chunks(Left<E, Q>{logits + node * a.ld, draft + node * a.ld_draft, Scale(s.slope, l.top[node]), inverse(l.sum[node]), c,
-                                 nullptr, 0}, cs, a.chunks, a.V);
-  });
-  for (int j = st.count + t; j < a.depth; j += NW) a.path[b * a.ld_path + j] = -1;
-  int next = l.best[st.node];
-  if (!s.greedy && next >= 0) {
-    Left<E, Q> left{logits + st.node * a.ld, st.cut ? draft + st.node * a.ld_draft : nullptr, Scale(s.slope, l.top[st.node]),
-                    inverse(l.sum[st.node]), st.c, nullptr, 0};
-    if (!st.cut) {
-      // the tokens rejected here, each once, in the rows' order; they take the place of the rows' u
-      __syncthreads();
-      int* gone = reinterpret_cast<int*>(l.u);
-      if (t < 64) {
-        int m = 0;
-        for (int k0 = st.node + 1; a.draft == nullptr && st.count < a.depth && k0 < s.n; k0 += 64) {
-          const int k = min(k0 + lane, s.n - 1), tok = l.token[k];
-          bool here = k0 + lane < s.n && l.parent[k] == st.node && tok >= 0;
-          for (int y = st.node + 1; here && y < k; ++y) here = !(l.parent[y] == st.node && l.token[y] == tok);
-          const uint64_t mask = __ballot(here);
-          if (here) gone[m + __popcll(mask & ((1ull << lane) - 1))] = tok;
-          m += __popcll(mask);
+  // the draw, by one wave: the run, then the token in it, at which the running sum first exceeds r times the total
+  if (wave == 0) {
+    int next = -1;
+    const int per = (runs + 63) / 64, y0 = min(lane * per, runs), y1 = min(y0 + per, runs);
+    double own = 0;
+#pragma unroll 1
+    for (int y = y0; y < y1; ++y) own += cs[y];
+    auto scan_of = [&](double v) {                           // inclusive sums over the lanes
+#pragma unroll 1
+      for (int m = 1; m < 64; m <<= 1) {
+        const double y = __shfl_up(v, m, 64);
+        if (lane >= m) v += y;
+      }
+      return v;
+    };
+    const double upto = scan_of(own), total = __shfl(upto, 63, 64), want = a.r[b] * total;
+    double before = upto - own, base = 0;
+    int run = -1, end = -1;
+#pragma unroll 1
+    for (int y = y0; y < y1; ++y) {
+      if (cs[y] > 0) {
+        end = y;
+        if (run < 0 && before + cs[y] > want) {
+          run = y;
+          base = before;
         }
-        if (lane == 0) n_gone = m;
       }
-      __syncthreads();
-      left.gone = gone;
-      left.n_gone = n_gone;
-      const Part* parts = a.parts + (s.first + st.node) * a.chunks;
-      for (int x = t; x < a.chunks; x += NW) {
-        double z = parts[x].sum * left.sc.weight(parts[x].top);
-        for (int g = 0; g < left.n_gone; ++g)
-          if (gone[g] / CHUNK == x) z -= left.sc.weight(logit(load1(left.src + gone[g])));
-        cs[x] = __builtin_fmax(z, 0.0);
+      before += cs[y];
+    }
+    const uint64_t hit = __ballot(run >= 0), some = __ballot(end >= 0);
+    if (some) {
+      if (hit) {
+        const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        run = __shfl(run, at, 64);
+        base = __shfl(base, at, 64);
+      } else {                                               // r of 1 or more, or a rounding: the last token there is
+        run = __shfl(end, 63 - __clzll(static_cast<long long>(some)), 64);
+        base = -INFINITY;
       }
-      __syncthreads();
+      int tail = -1;
+#pragma unroll 1
+      for (int k = 0; k < 2 && next < 0; ++k) {
+        const int e = run * RUN + 256 * k + 4 * lane;
+        float f[4], q[4] = {};
+        double w[4];
+        fetch4(left, f, q, e, a.V);
+        const double four = left4(left, e2, w, f, q, top), sums = scan_of(four);
+        double at = base + (sums - four);
+        int first = -1, some_last = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          at += w[i];
+          if (w[i] > 0) {
+            some_last = e + i;
+            if (first < 0 && at > want) first = e + i;
+          }
+        }
+        const uint64_t here = __ballot(first >= 0), any = __ballot(some_last >= 0);
+        if (here) next = __shfl(first, __ffsll(static_cast<unsigned long long>(here)) - 1, 64);
+        if (any) tail = __shfl(some_last, 63 - __clzll(static_cast<long long>(any)), 64);
+        base += __shfl(sums, 63, 64);
+      }
+      if (next < 0) next = tail;
     }
-    int at = draw(left, cs, a.chunks, a.V, a.r ? a.r[b] : 0.f, scan, found);
-    if (at < 0 && left.n_gone) {                             // (a chunk's difference that was only rounding)
-      sum_chunks(left, cs, a.chunks, a.V);
-      at = draw(left, cs, a.chunks, a.V, a.r ? a.r[b] : 0.f, scan, found);
-    }
-    if (at >= 0) next = at;
+    if (lane == 0) found = next >= 0 ? next : INT32_MAX;
   }
-  if (t == 0) {
-    a.count[b] = st.count;
-    a.next[b] = next;
+  __syncthreads();
+  if (found == INT32_MAX) {                                  // nothing is left: the row's largest logit
+    float own = -INFINITY;
+#pragma unroll 1
+    for (int e = t; e < a.V; e += ND) own = fmaxf(own, load1(left.src + e));
+    own = block_top<ND>(own, tops);
+    if (own > -INFINITY)
+#pragma unroll 1
+      for (int e = t; e < a.V; e += ND)
+        if (load1(left.src + e) == own) atomicMin(&found, e);        // (whole numbers: in any order)
+    __syncthreads();
   }
+  if (t == 0) a.next[b] = found == INT32_MAX ? -1 : found;
 }
 
 int sizes(const char* fn, int64_t T, int64_t V, int n_seq, int64_t max_rows, int* chunks) {
@@ -638,21 +779,25 @@ int sizes(const char* fn, int64_t T, int64_t V, int n_seq, int64_t max_rows, int
   return RF_OK;
 }
 
-size_t bytes_of(int64_t T, int n_seq, int chunks, bool draft) {
-  return static_cast<size_t>(T) * chunks * sizeof(Part) + (draft ? static_cast<size_t>(n_seq) * chunks * sizeof(double) : 0);
-}
+// The workspace: parts, ends, stops, gone.
+struct Space {
+  size_t ends, stops, gone, bytes;
+  Space(int64_t T, int n_seq, int chunks, int64_t max_rows)
+      : ends(static_cast<size_t>(T) * chunks * sizeof(Part)), stops(ends + static_cast<size_t>(n_seq) * chunks * RUNS * sizeof(Part)),
+        gone(stops + static_cast<size_t>(n_seq) * sizeof(Stop)), bytes(gone + static_cast<size_t>(n_seq) * std::min(max_rows, T) * 4) {}
+};
 
 }  // namespace
 }  // namespace rf
 
 using namespace rf;
 
-extern "C" int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_t max_rows, int draft, size_t* bytes) {
+extern "C" int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_t max_rows, size_t* bytes) {
   const char* fn = "rf_verify_drafts_workspace_bytes";
   int chunks;
   if (!bytes) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
   if (int rc = sizes(fn, T, vocab, n_seq, max_rows, &chunks)) return rc;
-  *bytes = n_seq ? bytes_of(T, n_seq, chunks, draft != 0) : 0;
+  *bytes = T && n_seq ? Space(T, n_seq, chunks, max_rows).bytes : 0;
   return RF_OK;
 }
 
@@ -675,26 +820,34 @@ extern "C" int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld,
   const int size = logits_kind == RF_F32 ? 4 : 2, dsize = draft_kind == RF_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size || (draft && reinterpret_cast<uintptr_t>(draft) % dsize) || !aligned16(workspace))
     return fail(RF_EINVAL_SHAPE, "%s: alignment", fn);
-  if (T && ws_bytes < bytes_of(T, n_seq, chunks, draft != nullptr))
-    return fail(RF_EINVAL_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, bytes_of(T, n_seq, chunks, draft != nullptr));
-  const bool drawn = draft && temperature && T;
+  const Space space(T, n_seq, chunks, max_rows);
+  if (T && ws_bytes < space.bytes)
+    return fail(RF_EINVAL_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, space.bytes);
+  const bool drawn = temperature && T;
+  char* ws = static_cast<char*>(workspace);
   const VerifyArgs a{static_cast<const char*>(logits), ld, T, static_cast<int>(vocab), chunks, tokens, parents, cu, n_seq, u, r,
-                     temperature, drawn ? static_cast<const char*>(draft) : nullptr, ld_draft,
-                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(depth), path, ld_path, count,
-                     next, static_cast<Part*>(workspace),
-                     reinterpret_cast<double*>(static_cast<char*>(workspace) + static_cast<size_t>(T) * chunks * sizeof(Part))};
-  const size_t shared = static_cast<size_t>(std::max(1, a.rows)) * ROW_BYTES;
+                     T ? temperature : nullptr, drawn ? static_cast<const char*>(draft) : nullptr, ld_draft,
+                     static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(depth), path, ld_path, count, next,
+                     reinterpret_cast<Part*>(ws), reinterpret_cast<Part*>(ws + space.ends), reinterpret_cast<Stop*>(ws + space.stops),
+                     reinterpret_cast<int32_t*>(ws + space.gone)};
+  const size_t rows = static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES, sums = static_cast<size_t>((vocab + RUN - 1) / RUN) * 12;
+  // k_verify_sums: a block a chunk, fewer where that is more than a round of blocks (two a CU): 32 sequences over 32 chunks
+  // @@ us with a block a chunk, @@ with 16 blocks each
+  const int shares = T ? static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, 8192 / T))) : 1;    // waves a row
+  const dim3 grid(static_cast<unsigned>((T * shares + NT / 64 - 1) / (NT / 64)));
+  const int blocks = drawn ? std::min(chunks, std::max(1, 512 / n_seq)) : 1;
 #define RF_VERIFY(E, Q)                                                                                                       \
   do {                                                                                                                        \
-    if (T) hipLaunchKernelGGL((k_verify_rows<E>), dim3(static_cast<unsigned>(T * chunks)), dim3(NT), 0, stream, a);           \
-    if (drawn) hipLaunchKernelGGL((k_verify_rest<E, Q>), dim3(static_cast<unsigned>(n_seq * chunks)), dim3(NT), shared, stream, a); \
-    hipLaunchKernelGGL((k_verify_walk<E, Q>), dim3(static_cast<unsigned>(n_seq)), dim3(NW), shared, stream, a);               \
+    if (T && a.draft) hipLaunchKernelGGL((k_verify_rows<E, true>), grid, dim3(NT), 0, stream, a, shares);                     \
+    else if (T) hipLaunchKernelGGL((k_verify_rows<E, false>), grid, dim3(NT), 0, stream, a, shares);                          \
+    hipLaunchKernelGGL((k_verify_sums<E, Q>), dim3(static_cast<unsigned>(n_seq * blocks)), dim3(NW), rows + 16, stream, a, blocks); \
+    if (drawn) hipLaunchKernelGGL((k_verify_draw<E, Q>), dim3(static_cast<unsigned>(n_seq)), dim3(ND), rows + sums, stream, a); \
   } while (0)
   if (logits_kind == RF_F32) {
-    if (!drawn || draft_kind == RF_F32) RF_VERIFY(float, float);
+    if (!a.draft || draft_kind == RF_F32) RF_VERIFY(float, float);
     else RF_VERIFY(float, uint16_t);
   } else {
-    if (!drawn || draft_kind == RF_F32) RF_VERIFY(uint16_t, float);
+    if (a.draft && draft_kind == RF_F32) RF_VERIFY(uint16_t, float);
     else RF_VERIFY(uint16_t, uint16_t);
   }
 #undef RF_VERIFY

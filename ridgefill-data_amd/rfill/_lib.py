@@ -115,7 +115,7 @@ SIGNATURES = {
                        _P],
     "rf_verify_drafts": [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
                          _SZ, _P],
-    "rf_verify_drafts_workspace_bytes": [_I64, _I64, _I32, _I64, _I32, _PSZ],
+    "rf_verify_drafts_workspace_bytes": [_I64, _I64, _I32, _I64, _PSZ],
     "rf_paged_keep": [_PP, _I32, _P, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P],
     "rf_window_mass_workspace_bytes": [_I32, _I32, _I32, _I32, _I64, _PSZ],
     "rf_window_mass": [_P, _I64, _I32, _I64, _I32, _I32, _P, _I32, _I64, _I64, _F32, _P, _P, _SZ, _P],

@@ -1197,10 +1197,10 @@ _KINDS = {torch.float32: 0, torch.bfloat16: 1}          # RF_F32, RF_BF16
 
 
 @_size_rule
-def verify_drafts_workspace_bytes(rows, vocab, n_seq, max_rows, draft):
+def verify_drafts_workspace_bytes(rows, vocab, n_seq, max_rows):
     """Device bytes of verify_drafts' workspace."""
     b = ctypes.c_size_t(0)
-    _lib.call("rf_verify_drafts_workspace_bytes", rows, vocab, n_seq, max_rows, int(draft), ctypes.byref(b))
+    _lib.call("rf_verify_drafts_workspace_bytes", rows, vocab, n_seq, max_rows, ctypes.byref(b))
     return b.value
 
 
@@ -1250,7 +1250,7 @@ def verify_drafts(logits, tokens, parents, cu, u, r, temperature, max_rows, dept
                     ("draft", draft)):
         if t is not None and t.get_device() != dev:
             raise ValueError(f"verify_drafts: {name} is on {t.device}, logits on {logits.device}")
-    need = verify_drafts_workspace_bytes(rows, vocab, n, max_rows, draft is not None)
+    need = verify_drafts_workspace_bytes(rows, vocab, n, max_rows)
     if isinstance(workspace, str):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
     _need(workspace, "workspace", torch.uint8, 1)
