@@ -28,14 +28,14 @@
 namespace rf {
 namespace {
 
-constexpr int CHUNK = 4096;                // logits a part
+constexpr int CHUNK = 4096;                // logits a share of a row has at least, and a block of k_verify_sums at once
 constexpr int MAX_CHUNKS = 128;
 constexpr int MAX_ROWS = 1024;             // of a sequence
 constexpr int NT = 256;                    // threads of k_verify_rows
 constexpr int NW = 512;                    // of k_verify_sums
 constexpr int ND = 1024;                   // of k_verify_draw
 
-struct Part {                              // of a chunk of a row: its largest logit, where it first is (-1: nowhere), and the
+struct Part {                              // of some of a row's logits: the largest logit, where it first is (-1: nowhere), and the
   float top;                               // sum of the weights relative to it (0 for greedy rows)
   int best;
   double sum;
@@ -46,7 +46,7 @@ struct Stop;
 struct VerifyArgs {
   const char* logits;
   int64_t ld, T;
-  int V, chunks;
+  int V, chunks, shares;                   // chunks of a row; the waves that read one in k_verify_rows
   const int64_t* tokens;
   const int32_t* parents;
   const int32_t* cu;
@@ -61,7 +61,7 @@ struct VerifyArgs {
   int64_t ld_path;
   int32_t* count;
   int64_t* next;
-  Part* parts;                             // [T, chunks]
+  Part* parts;                             // [T, shares]
   Part* ends;                              // [n_seq, chunks * RUNS]: of the row whose sums a walk wants first, by runs
   Stop* stops;                             // [n_seq]
   int32_t* gone;                           // [n_seq, rows]
@@ -181,7 +181,7 @@ struct Step {
   }
 };
 
-// A wave a share of a row's chunks: `shares` of them a row. Sums are relative to the first step's largest logit as long as the
+// A wave a share of a row: chunks share, share + shares .. Sums are relative to the first step's largest logit as long as the
 // others stay near it, so a step has no more to do than its maximum and its weights.
 // EXACT (with a draft: p - c q, and with it every border of what is left, moves with the row's sum): weights in 64 bits, 16
 // instructions a logit (none of them at a quarter of the rate), as 2^(x c - ref c) of logits not below ref - 1000 / c (those, NaN
@@ -190,9 +190,10 @@ struct Step {
 // of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, @@ in 32; their bytes take 22.)
 // Where reference and slope allow neither, weight by weight.
 template <class E, bool EXACT>
-__global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a, int shares) {
+__global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t task = static_cast<int64_t>(blockIdx.x) * (NT / 64) + (threadIdx.x >> 6);
+  const int shares = a.shares;
   const int64_t row = __builtin_amdgcn_readfirstlane(static_cast<int>(task / shares));
   const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(task - row * shares));
   if (row >= a.T) return;
@@ -210,13 +211,12 @@ __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a, int shares) {
   const Exp2 e2;
   const double c = drawn ? slope(temp) : 0.0;
   const float reach = EXACT ? static_cast<float>(1000.0 / c) : 0.f, c32 = static_cast<float>(c);
-  Part* parts = a.parts + row * a.chunks;
   constexpr int STEPS = CHUNK / 1024;
-  const int chunks = (a.chunks - share + shares - 1) / shares, steps = chunks * STEPS;       // its chunks: share, share + shares ..
+  const int chunks = (a.chunks - share + shares - 1) / shares, steps = chunks * STEPS;
   auto begin = [&](int i) { return (share + i / STEPS * shares) * CHUNK + i % STEPS * 1024; };
   Step<E> now, coming;
   now.fetch(src, begin(0), a.V);
-  float top = -INFINITY, ref = -INFINITY, lo = 0.f;          // of the chunk: the lane's largest logit, the reference
+  float top = -INFINITY, ref = -INFINITY, lo = 0.f;          // the lane's largest logit, the sums' reference
   double sum = 0, k = 0;
   bool fast = false;
   int best = INT32_MAX;
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a, int shares) {
     }
     if (drawn) {
       if (!__all(fast ? (static_cast<double>(top) - ref) * c < (EXACT ? 500 : 64) : top == -INFINITY)) {
-        float high = top;                                    // the chunk's reference, or a new one
+        float high = top;                                    // the first reference, or a new one
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) high = fmaxf(high, __shfl_xor(high, m, 64));
         if (high > ref) {
@@ -263,25 +263,19 @@ __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a, int shares) {
         for (int x = 0; x < 16; ++x) sum += weight(e2, now.f[x], ref, c);
       }
     }
-    if (i % STEPS == STEPS - 1) {                            // the chunk's part
-      float high = top;
-#pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) high = fmaxf(high, __shfl_xor(high, m, 64));
-      int first = top == high ? best : INT32_MAX;
-#pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) {
-        first = min(first, __shfl_xor(first, m, 64));
-        sum += shfl_xor64(sum, m);
-      }
-      if (lane == 0)
-        parts[share + i / STEPS * shares] = Part{high, high > -INFINITY ? first : -1, drawn && high > -INFINITY ? sum * weight(e2, ref, high, c) : 0.0};
-      top = ref = -INFINITY;
-      sum = 0;
-      fast = false;
-      best = INT32_MAX;
-    }
     now = coming;
   }
+  float high = top;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) high = fmaxf(high, __shfl_xor(high, m, 64));
+  int first = top == high ? best : INT32_MAX;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    first = min(first, __shfl_xor(first, m, 64));
+    sum += shfl_xor64(sum, m);
+  }
+  if (lane == 0)
+    a.parts[row * shares + share] = Part{high, high > -INFINITY ? first : -1, drawn && high > -INFINITY ? sum * weight(e2, ref, high, c) : 0.0};
 }
 
 // What a block knows of its sequence's rows, in LDS. Of rows without children in a sequence that is not greedy: no sums.
@@ -330,12 +324,12 @@ template <class E, class Q, int THREADS>
 __device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, const Rows& l, const Exp2& e2) {
   const int t = threadIdx.x, j = t & 15;
   const E* logits = reinterpret_cast<const E*>(a.logits) + s.first * a.ld;
-  // a row's chunks by 16 lanes (their first loads go before those of the rows, which wait for one another)
+  // a row's parts by 16 lanes (their first loads go before those of the rows, which wait for one another)
 #pragma unroll 1
   for (int i0 = 0; i0 < s.n; i0 += THREADS / 16) {
     const int i = i0 + t / 16;
-    const Part* parts = a.parts + (s.first + min(i, s.n - 1)) * a.chunks;
-    const Part p0 = parts[min(j, a.chunks - 1)], p1 = parts[min(j + 16, a.chunks - 1)];
+    const Part* parts = a.parts + (s.first + min(i, s.n - 1)) * a.shares;
+    const Part p0 = parts[min(j, a.shares - 1)], p1 = parts[min(j + 16, a.shares - 1)];
     if (i0 == 0) {
 #pragma unroll 1
       for (int r = t; r < s.n; r += THREADS) {
@@ -350,17 +344,17 @@ __device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, cons
         l.q[r] = in && a.draft ? share(load1(reinterpret_cast<const Q*>(a.draft) + (s.first + par) * a.ld_draft + id)) : 0.f;
       }
     }
-    float top = j < a.chunks ? p0.top : -INFINITY;
+    float top = j < a.shares ? p0.top : -INFINITY;
     int best = top > -INFINITY ? p0.best : INT32_MAX;
     auto larger = [&](const Part& p) {
-      if (p.top > top) {
+      if (p.top > top || (p.top == top && p.best < best)) {
         top = p.top;
         best = p.best;
       }
     };
-    if (j + 16 < a.chunks) larger(p1);
+    if (j + 16 < a.shares) larger(p1);
 #pragma unroll 1
-    for (int x = j + 32; x < a.chunks; x += 16) larger(parts[x]);
+    for (int x = j + 32; x < a.shares; x += 16) larger(parts[x]);
     float all = top;
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) all = fmaxf(all, __shfl_xor(all, m, 64));
@@ -369,7 +363,7 @@ __device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, cons
     if (!s.greedy && all > -INFINITY) {
       Part p = p0;
 #pragma unroll 1
-      for (int x = j; x < a.chunks; x += 16) {
+      for (int x = j; x < a.shares; x += 16) {
         if (x >= 32) p = parts[x];
         if (p.top > -INFINITY) sum += p.sum * weight(e2, p.top, all, s.slope);               // (rows without sums: left out)
         p = p1;
@@ -411,21 +405,22 @@ struct Stop {
 };
 
 // The walk from st on, by every wave with the same numbers. True: a drawn token was rejected, and Z = sum max(p - c q, 0) of the
-// node is wanted; false: the path has ended.
+// node is wanted for the next child; false: the path has ended (cut: with a rejected token, and c is new).
 __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const Rows& l, State& st) {
   const int lane = threadIdx.x & 63;
   const bool drawn = a.draft != nullptr && !s.greedy;
-  while (st.count < a.depth) {
-    int at = -1;                                             // the next row below the node
-    for (int i0 = st.next; i0 < s.n; i0 += 64) {
+  auto child = [&](int from) {                               // the next row below the node; -1: none
+#pragma unroll 1
+    for (int i0 = from; i0 < s.n; i0 += 64) {
       const uint64_t hit = __ballot(i0 + lane < s.n && l.parent[min(i0 + lane, s.n - 1)] == st.node);
-      if (hit) {
-        at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-        break;
-      }
+      if (hit) return i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
     }
+    return -1;
+  };
+#pragma unroll 1
+  while (st.count < a.depth) {
+    const int at = __builtin_amdgcn_readfirstlane(child(st.next));
     if (at < 0) return false;
-    at = __builtin_amdgcn_readfirstlane(at);
     st.next = at + 1;
     const int tok = l.token[at];
     bool yes;
@@ -448,7 +443,7 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const 
       if (!yes) {
         st.c += st.Z;
         st.cut = true;
-        return true;
+        return child(st.next) >= 0;
       }
     }
     if (yes) {
@@ -655,8 +650,7 @@ __global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
     for (int m = 32; m >= 1; m >>= 1) z += shfl_xor64(z, m);
     st.Z = z;
     more = walk(a, s, l, st);
-    if (!more && st.cut) break;                              // no child was accepted: cs is what is left
-    __syncthreads();                                         // else further sums, of another rejection or the last row
+    __syncthreads();                                         // then further sums, of another rejection or the last row
     top = l.top[st.node];
     left = left_of<E, Q>(a, s, st, l.sum[st.node], gone, 0);
 #pragma unroll 1
@@ -774,17 +768,21 @@ int sizes(const char* fn, int64_t T, int64_t V, int n_seq, int64_t max_rows, int
   if (max_rows < 0 || max_rows > MAX_ROWS)
     return fail(RF_EUNSUPPORTED, "%s: %lld rows a sequence (up to %d)", fn, (long long)max_rows, MAX_ROWS);
   *chunks = static_cast<int>((V + CHUNK - 1) / CHUNK);
-  if (T < 0 || n_seq < 0 || n_seq > (1 << 20) || T > (INT32_MAX / *chunks) || static_cast<int64_t>(n_seq) * *chunks > INT32_MAX)
+  if (T < 0 || n_seq < 0 || n_seq > (1 << 20) || T > (1 << 30) || static_cast<int64_t>(n_seq) * *chunks > INT32_MAX)
     return fail(RF_EINVAL_SHAPE, "%s: %lld rows of %d sequences over a vocabulary of %lld", fn, (long long)T, n_seq, (long long)V);
   return RF_OK;
 }
+
+// Waves a row in k_verify_rows: 8192 in all (a CU holds 28), a chunk each at least.
+int shares_of(int64_t T, int chunks) { return static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, 8192 / std::max<int64_t>(T, 1)))); }
 
 // The workspace: parts, ends, stops, gone.
 struct Space {
   size_t ends, stops, gone, bytes;
   Space(int64_t T, int n_seq, int chunks, int64_t max_rows)
-      : ends(static_cast<size_t>(T) * chunks * sizeof(Part)), stops(ends + static_cast<size_t>(n_seq) * chunks * RUNS * sizeof(Part)),
-        gone(stops + static_cast<size_t>(n_seq) * sizeof(Stop)), bytes(gone + static_cast<size_t>(n_seq) * std::min(max_rows, T) * 4) {}
+      : ends(static_cast<size_t>(T) * shares_of(T, chunks) * sizeof(Part)),
+        stops(ends + static_cast<size_t>(n_seq) * chunks * RUNS * sizeof(Part)), gone(stops + static_cast<size_t>(n_seq) * sizeof(Stop)),
+        bytes(gone + static_cast<size_t>(n_seq) * std::min(max_rows, T) * 4) {}
 };
 
 }  // namespace
@@ -825,7 +823,7 @@ extern "C" int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld,
     return fail(RF_EINVAL_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, space.bytes);
   const bool drawn = temperature && T;
   char* ws = static_cast<char*>(workspace);
-  const VerifyArgs a{static_cast<const char*>(logits), ld, T, static_cast<int>(vocab), chunks, tokens, parents, cu, n_seq, u, r,
+  const VerifyArgs a{static_cast<const char*>(logits), ld, T, static_cast<int>(vocab), chunks, shares_of(T, chunks), tokens, parents, cu, n_seq, u, r,
                      T ? temperature : nullptr, drawn ? static_cast<const char*>(draft) : nullptr, ld_draft,
                      static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(depth), path, ld_path, count, next,
                      reinterpret_cast<Part*>(ws), reinterpret_cast<Part*>(ws + space.ends), reinterpret_cast<Stop*>(ws + space.stops),
@@ -833,13 +831,12 @@ extern "C" int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld,
   const size_t rows = static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES, sums = static_cast<size_t>((vocab + RUN - 1) / RUN) * 12;
   // k_verify_sums: a block a chunk, fewer where that is more than a round of blocks (two a CU): 32 sequences over 32 chunks
   // @@ us with a block a chunk, @@ with 16 blocks each
-  const int shares = T ? static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, 8192 / T))) : 1;    // waves a row
-  const dim3 grid(static_cast<unsigned>((T * shares + NT / 64 - 1) / (NT / 64)));
+  const dim3 grid(static_cast<unsigned>((T * a.shares + NT / 64 - 1) / (NT / 64)));
   const int blocks = drawn ? std::min(chunks, std::max(1, 512 / n_seq)) : 1;
 #define RF_VERIFY(E, Q)                                                                                                       \
   do {                                                                                                                        \
-    if (T && a.draft) hipLaunchKernelGGL((k_verify_rows<E, true>), grid, dim3(NT), 0, stream, a, shares);                     \
-    else if (T) hipLaunchKernelGGL((k_verify_rows<E, false>), grid, dim3(NT), 0, stream, a, shares);                          \
+    if (T && a.draft) hipLaunchKernelGGL((k_verify_rows<E, true>), grid, dim3(NT), 0, stream, a);                             \
+    else if (T) hipLaunchKernelGGL((k_verify_rows<E, false>), grid, dim3(NT), 0, stream, a);                                  \
     hipLaunchKernelGGL((k_verify_sums<E, Q>), dim3(static_cast<unsigned>(n_seq * blocks)), dim3(NW), rows + 16, stream, a, blocks); \
     if (drawn) hipLaunchKernelGGL((k_verify_draw<E, Q>), dim3(static_cast<unsigned>(n_seq)), dim3(ND), rows + sums, stream, a); \
   } while (0)

@@ -63,15 +63,17 @@ def test_keep():
 
 
 def test_workspace_sizes_and_refusals():
-    """Host-only size rule: 16 bytes a (row, 4096 logits), 128 a (sequence, 4096 logits), 64 a sequence and four a row of each."""
+    """Host-only size rule: 16 bytes a row and share of it (a share a 4096 logits, 8192 in all but at least one a row), 128 a
+    (sequence, 4096 logits), 64 a sequence and four a row of each."""
     from rfill import _lib, ops
     size = ops.verify_drafts_workspace_bytes
     assert size(10, 4096, 2, 8) == 10 * 16 + 2 * (128 + 64 + 4 * 8) and size(10, 4097, 5, 80) == 20 * 16 + 5 * (256 + 64 + 4 * 10)
+    assert size(5000, 40960, 1, 8) == 5000 * 16 + 1280 + 64 + 32 and size(9000, 40960, 1, 8) == 9000 * 16 + 1280 + 64 + 32
     assert size(0, 100, 3, 8) == 0 and size(5, 100, 0, 8) == 0
     for rows, vocab, n, most in ((1, (1 << 19) + 1, 1, 1), (1, 0, 1, 1), (1, 100, 1, 1025)):
         with pytest.raises(_lib.UnsupportedArchitecture):
             size(rows, vocab, n, most)
     with pytest.raises(ValueError):
-        size(1 << 30, 1 << 19, 1, 1)
+        size((1 << 30) + 1, 1 << 19, 1, 1)
     with pytest.raises(ValueError):
         size(1, 100, -1, 1)
