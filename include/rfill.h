@@ -669,11 +669,15 @@ int rf_paged_tree(const int32_t* table, int64_t ld_table, int64_t table_width, c
 
 /* rf_attend_paged for such rows: row i of a sequence with n new ones sees the keys before position lens[b] - n, and of the
  * new ones those j <= i whose bit is set in its words of seen (as rf_paged_tree writes them, or any others; 64 words at
- * least max_rows). All else, the workspace among it, is rf_attend_paged's. */
+ * least max_rows). All else is rf_attend_paged's; the workspace is of rf_attend_tree_workspace_bytes. */
 int rf_attend_tree(const uint16_t* q, int64_t ldq, int64_t T, int hq, const rf_pages* pages, const int32_t* table,
                    int64_t ld_table, int64_t table_width, const int32_t* lens, const int32_t* cu, const uint64_t* seen,
                    int64_t ld_seen, int64_t words, int n_seq, int64_t max_rows, int64_t max_keys, float scale, uint16_t* out,
                    int64_t ldo, void* workspace, size_t ws_bytes, hipStream_t stream);
+
+/* Bytes of rf_attend_tree's workspace for these sizes (0: the keys are not split). Host only. */
+int rf_attend_tree_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows,
+                                   int64_t max_keys, size_t* bytes);
 
 #define RF_F32 0
 #define RF_BF16 1

@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attend_tile.h"
 #include "paged.h"
@@ -1170,9 +1171,8 @@ __device__ __forceinline__ uint4 eight_values(uint32_t w, float s) {
 }
 
 // ... as bf16 into a stage.
-template <int AD>
+template <int AD, class L>
 __device__ __forceinline__ void store_codes(const ManyCodes<AD, true>& c, char* st, int w, int lane) {
-  using L = Layout<AD>;
   const int row = 8 * w + lane / 8, part = lane % 8;
   uint4* s4 = reinterpret_cast<uint4*>(st);
   const float ks = scale_of<0>(c.ks), vs = scale_of<0>(c.vs);
@@ -1189,11 +1189,11 @@ __device__ __forceinline__ void store_codes(const ManyCodes<AD, true>& c, char* 
 }
 
 // The largest of a row's scores of a tile.
-template <int AD>
-__device__ __forceinline__ float top_score(const f32x16 (&sc)[Cfg<AD>::KB]) {
+template <int KB>
+__device__ __forceinline__ float top_score(const f32x16 (&sc)[KB]) {
   float tmax = -INFINITY, lo, hi;
 #pragma unroll
-  for (int kb = 0; kb < Cfg<AD>::KB; ++kb)
+  for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int j = 0; j < 16; ++j) tmax = fmaxf(tmax, sc[kb][j]);
   lane_pair(tmax, lo, hi);
@@ -1213,13 +1213,12 @@ __device__ __forceinline__ void raise_tile(f32x16 (&o)[AD / 32], float& mref, fl
 }
 
 // The probabilities of a tile, in pairs as the product takes them; their sum goes to lsum.
-template <int AD>
-__device__ __forceinline__ void tile_probabilities(const f32x16 (&sc)[Cfg<AD>::KB], uint32_t (&pk)[8 * Cfg<AD>::KB], float mref,
-                                                   float& lsum, float c) {
+template <int KB>
+__device__ __forceinline__ void tile_probabilities(const f32x16 (&sc)[KB], uint32_t (&pk)[8 * KB], float mref, float& lsum, float c) {
   const float mc = mref == -INFINITY ? 0.f : mref * c;
   float psum = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8 * Cfg<AD>::KB; ++e) {
+  for (int e = 0; e < 8 * KB; ++e) {
     const float q0 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8)], c, -mc));
     const float q1 = __builtin_amdgcn_exp2f(fmaf(sc[e / 8][2 * (e % 8) + 1], c, -mc));
     psum += q0 + q1;
@@ -1232,12 +1231,11 @@ __device__ __forceinline__ void tile_probabilities(const f32x16 (&sc)[Cfg<AD>::K
 // on a page that is none. Of V, what is not finite enters the product as zero; a row that sees such a value takes it
 // from LDS afterwards (0 x infinity must not reach the rows that do not).
 // Trees: bits are those of the tile's keys that the lane's row sees.
-template <int AD, bool TREE>
-__device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&sc)[Cfg<AD>::KB], f32x16 (&o)[AD / 32],
+template <int AD, bool TREE, class L, int KB>
+__device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&sc)[KB], f32x16 (&o)[AD / 32],
                                           float& mref, float& lsum, int k0, uint32_t bad, int mypos, int hh, float c,
                                           const FragOffsets<AD>& fo, [[maybe_unused]] uint64_t bits) {
-  using L = Layout<AD>;
-  constexpr int NB = AD / 32, KB = Cfg<AD>::KB, KTL = Cfg<AD>::KT;
+  constexpr int NB = AD / 32, KTL = 32 * KB;
   const int rel = min(max(mypos - k0, -1), KTL) - 4 * hh;
   [[maybe_unused]] const uint64_t mine = bits >> (4 * hh);
 #pragma unroll
@@ -1248,10 +1246,10 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
       const int key = 32 * kb + 8 * (j >> 2) + (j & 3);      // (of the lane's half: 4 hh more)
       if (gone || (TREE ? !((mine >> key) & 1u) : key > rel)) sc[kb][j] = -INFINITY;
     }
-  const float tmax = top_score<AD>(sc);
+  const float tmax = top_score<KB>(sc);
   if (__any(tmax > mref + headroom(c))) raise_tile<AD>(o, mref, lsum, tmax, c);
   uint32_t pk[8 * KB];
-  tile_probabilities<AD>(sc, pk, mref, lsum, c);
+  tile_probabilities<KB>(sc, pk, mref, lsum, c);
   bool odd = false;
 #pragma unroll
   for (int stp = 0; stp < KTL / 16; ++stp) {
@@ -1286,13 +1284,19 @@ __device__ __forceinline__ void edge_tile(const char* __restrict__ st, f32x16 (&
 // scores and the edge tiles' code want, and 59 more that spill (236 bytes a lane of scratch; 8 waves of 256 spilled 360 registers,
 // and 13 sequences of 256 rows took 350 us instead of 157).
 constexpr int many_waves(int d) { return d == 256 ? 4 : 8; }
-constexpr int many_rows(int d) { return 32 * many_waves(d); }
+// SMALL: trees of up to 128 rows in bf16 (head_dim 64, 128). Two blocks a CU, each of 4 waves on tiles of 32 keys: of a block of 256 rows
+// half of the waves have none, the others are alone on their SIMD, and what a block does before its first tile nobody hides (24
+// sequences of up to 16 new tokens and 8111 keys, bf16: 85 us, so 65, of which their bytes take 57). Not in 4 bits: beside the
+// codes two waves a SIMD have too few registers (spilling 524 us where blocks of 8 waves take 318, with the codes through a ring in
+// LDS and no spills 359).
+constexpr int many_waves(int d, bool small) { return small ? 4 : many_waves(d); }
+constexpr int many_rows(int d, bool small) { return 32 * many_waves(d, small); }
 
-template <int AD, bool MX, bool TREE>
-__global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs a) {
-  using L = Layout<AD>;
-  constexpr int NS = AD / 16, NB = AD / 32, KTL = Cfg<AD>::KT, QROWS = many_rows(AD), KB = Cfg<AD>::KB;
-  constexpr int NWM = many_waves(AD), SHARES = Cfg<AD>::NW / NWM;      // shares of a tile's loads a wave takes
+template <int AD, bool MX, bool TREE, bool SMALL>
+__global__ __launch_bounds__(64 * many_waves(AD, SMALL), SMALL ? 2 : 1) void k_paged_many(PagedArgs a) {
+  using L = std::conditional_t<SMALL, Layout<AD, 32, 4>, Layout<AD>>;
+  constexpr int NS = AD / 16, NB = AD / 32, KTL = L::KT, QROWS = many_rows(AD, SMALL), KB = KTL / 32;
+  constexpr int NWM = many_waves(AD, SMALL), SHARES = L::NW / NWM;     // shares of a tile's loads a wave takes
   constexpr int KLOADS = L::KLOADS * SHARES, LOADS = L::LOADS * SHARES;
   constexpr int HPT = KTL / 16, WIN = 64 / HPT;              // 16-key halves a tile, tiles a window of table entries
   __shared__ uint4 lds[NSTAGE * L::STAGE_U4];
@@ -1311,6 +1315,7 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
   const int r = min(32 * w + n, rows - 1), qi = (rb.off + r) / a.rep, hd = head * a.rep + rb.off + r - qi * a.rep;
   const bool live = 32 * w + n < rows;
   const int mypos = p0 + qi;
+  [[maybe_unused]] const int r0 = q0 * a.rep + rb.off;       // the block's first row among the sequence's
   const int wave_last = 32 * w < rows ? p0 + (rb.off + min(32 * w + 31, rows - 1)) / a.rep : -1;
   bf16x8 qf[NS];
   {
@@ -1388,7 +1393,7 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
     for (int x = 0; x < 16; ++x) o[b][x] = 0.f;
   float m = -INFINITY, lsum = 0.f;
   const float c = a.c;
-  const FragOffsets<AD> fo(lane);
+  const FragOffsets<AD> fo(lane, L::K_U4);
   f32x16 sc[KB], sn[KB];
   // Turn it, then softmax and product of tile it, with the scores of tile it + 1 in the same block. bf16: tile it + 3 is
   // loaded into the stage of tile it - 1, whose last reads ended before this iteration's barrier. 4 bits: the codes of tile
@@ -1397,7 +1402,7 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
     for (int i = 0; i < 2; ++i)
       if (it0 + i < it1) {
         fetch(it0 + i);
-        store_codes<AD>(codes, stage(it0 + i), w, lane);
+        store_codes<AD, L>(codes, stage(it0 + i), w, lane);
       }
     if (it0 + 2 < it1) fetch(it0 + 2);
     __syncthreads();
@@ -1409,11 +1414,11 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
     else wait_vm_lgkm0<0>();
     __builtin_amdgcn_s_barrier();
   }
-  if (it0 < it1) tile_scores<AD>(stage(it0), qf, sc, fo);
+  if (it0 < it1) tile_scores<AD, KB>(stage(it0), qf, sc, fo);
   auto turn = [&](int it) {
     if constexpr (MX) {
       __syncthreads();
-      if (it + 2 < it1) store_codes<AD>(codes, stage(it + 2), w, lane);
+      if (it + 2 < it1) store_codes<AD, L>(codes, stage(it + 2), w, lane);
       if (it + 3 < it1) fetch(it + 3);
     } else {
       if (it + 2 < it1) wait_vm_lgkm0<LOADS>();           // tile it + 1 landed, tile it + 2 may fly
@@ -1434,17 +1439,27 @@ __global__ __launch_bounds__(64 * many_waves(AD), 1) void k_paged_many(PagedArgs
   for (; it + 1 < full; it += 2) {
     if (bad_of(it) | bad_of(it + 1)) break;
     turn(it);
-    tile_step<AD>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
+    tile_step<AD, KB>(stage(it), stage(it + 1), qf, sc, sn, o, m, lsum, it * KTL, false, mypos, hh, c, fo);
     turn(it + 1);
-    tile_step<AD>(stage(it + 1), stage(it + 2), qf, sn, sc, o, m, lsum, it * KTL + KTL, false, mypos, hh, c, fo);
+    tile_step<AD, KB>(stage(it + 1), stage(it + 2), qf, sn, sc, o, m, lsum, it * KTL + KTL, false, mypos, hh, c, fo);
   }
   for (; it < it1; ++it) {
     turn(it);
     if (it * KTL > wave_last) continue;                      // this and every later tile lie past the wave's rows
-    uint64_t bits = 0;
-    if constexpr (TREE) bits = tree_bits(a.seen + static_cast<int64_t>(u.s.first + q0 + qi) * a.ld_seen, a.words, q0 + qi, it * KTL - base);
-    edge_tile<AD, TREE>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), mypos, hh, c, fo, bits);
-    tile_scores<AD>(stage(it + 1), qf, sc, fo);
+    if constexpr (SMALL) {
+      int here = lane;                                       // (nothing that follows from it is kept through the loop above)
+      asm volatile("" : "+v"(here));
+      const FragOffsets<AD> fe(here, L::K_U4);
+      const int row_of = r0 + min(32 * w + (here & 31), rows - 1), i = row_of / a.rep;   // (of the sequence's rows)
+      const uint64_t bits = tree_bits(a.seen + static_cast<int64_t>(u.s.first + i) * a.ld_seen, a.words, i, it * KTL - base);
+      edge_tile<AD, TREE, L, KB>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), base + i, here >> 5, c, fe, bits);
+      tile_scores<AD, KB>(stage(it + 1), qf, sc, fe);
+    } else {
+      uint64_t bits = 0;
+      if constexpr (TREE) bits = tree_bits(a.seen + static_cast<int64_t>(u.s.first + q0 + qi) * a.ld_seen, a.words, q0 + qi, it * KTL - base);
+      edge_tile<AD, TREE, L, KB>(stage(it), sc, o, m, lsum, it * KTL, bad_of(it), mypos, hh, c, fo, bits);
+      tile_scores<AD, KB>(stage(it + 1), qf, sc, fo);
+    }
   }
   wait_vm_lgkm0<0>();
 
@@ -1596,12 +1611,12 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a) {
 }
 
 struct Plan {
-  bool many, once;
+  bool many, small, once;
   int fit, kt;
   int64_t blocks, units;                   // (sequence, row block)s at most, and with their splits
   size_t bytes;
   int d;
-  int rows() const { return many ? many_rows(d) : 16; }
+  int rows() const { return many ? many_rows(d, small) : 16; }
 };
 
 // The most rows a sequence that k_paged_few takes in blocks of 16. 13 sequences of 2000 to 8000 keys, few against many (us):
@@ -1609,19 +1624,25 @@ struct Plan {
 // 105 / 110, 256 185 / 157. 4 bits, d 128, 64 rows 45 / 65, 128 71 / 67, 256 121 / 92; d 64, 64 rows 23 / 23, 128 26 / 25;
 // d 256, 256 rows 81 / 146, 512 138 / 239: there k_paged_many is not built (its products take bf16, those of k_paged_few the
 // keys' codes at four times the rate, and a wave's 256 columns leave no registers to convert the codes beside them).
-constexpr int64_t few_rows(int d, bool mx) { return d == 256 ? (mx ? INT64_MAX : 128) : mx ? 96 : 16; }
+// Trees, ragged: most have fewer rows than the largest. In 4 bits, largest of 64 / 104 / 128 / 192 rows, 40 of up to 24000 keys,
+// d 128 239 / 470, 391 / 476, 392 / 486, 635 / 534; 13 of 8000 40 / 64, 65 / 76, 67 / 76, 93 / 92; d 64 (2 rows a token) 64 and
+// 128 rows 53 / 105, 90 / 110, 192 of 9000 keys 56 / 59, 256 73 / 66. bf16 against small blocks: d 128, 20 rows 13 of 8000 56 /
+// 54, 24 101 / 107, 32 rows 73 / 55 and 116 / 108, 64 91 / 57 and 194 / 116; d 64, 16 rows 25 / 25, 48 32 / 27.
+constexpr int64_t few_rows(int d, bool mx, bool tree) { return d == 256 ? (mx ? INT64_MAX : 128) : !mx ? 16 : tree ? 128 : 96; }
 
 // The launch for these sizes: k_paged_few or k_paged_many. Row blocks: sum of ceil(rows rep / rpb) <= T rep / rpb + n_seq.
 // k_paged_few: `fit` runs a head, two parts each; k_paged_many: with splits of W tiles at most work / W units more
 // (split_length: one round of blocks, or W >= work / 3 fit).
-Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys) {
+Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_rows, int64_t max_keys, bool tree) {
   Plan p{};
   p.d = d;
   const int rep = hq / hkv;
-  p.many = std::min<int64_t>(max_rows, T) * rep > few_rows(d, mx);
-  p.kt = p.many ? (d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
+  const int64_t rows = std::min<int64_t>(max_rows, T) * rep;
+  p.many = rows > few_rows(d, mx, tree);
+  p.small = p.many && tree && !mx && d != 256 && rows <= many_rows(d, true);
+  p.kt = p.many ? (p.small ? 32 : d == 256 ? Cfg<256>::KT : Cfg<128>::KT) : KT;
   p.blocks = std::min<int64_t>(T * rep, T * rep / p.rows() + n_seq);
-  const int round = p.many ? 256 : 256 * few_blocks(d, mx);
+  const int round = p.small ? 512 : p.many ? 256 : 256 * few_blocks(d, mx);
   // No splits up to 2048 keys (or where the tiles would not count in 31 bits). One number for all: at most 1000 keys, split against
   // not, 8 sequences of 8 heads of 128 20 / 16 us, one of 2 heads of 64 15 / 11; 2000 keys 8 of 2 heads of 64 18 / 16, of 8 heads of
   // 128 21 / 25, of 2 heads of 256 24 / 46, in 4 bits 18 / 17 and 26 / 27, a chunk of 200 rows 32 / 62; 4000 keys 26 / 43, 4 bits
@@ -1655,7 +1676,16 @@ extern "C" int rf_attend_paged_workspace_bytes(int64_t T, int hq, int hkv, int d
   const char* fn = "rf_attend_paged_workspace_bytes";
   if (!bytes) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
   if (int rc = attend_sizes(fn, T, hq, hkv, d, kind, n_seq, max_rows, max_keys)) return rc;
-  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, kind == RF_PAGES_MX4, n_seq, max_rows, max_keys).bytes : 0;
+  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, kind == RF_PAGES_MX4, n_seq, max_rows, max_keys, false).bytes : 0;
+  return RF_OK;
+}
+
+extern "C" int rf_attend_tree_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, int n_seq, int64_t max_rows,
+                                              int64_t max_keys, size_t* bytes) {
+  const char* fn = "rf_attend_tree_workspace_bytes";
+  if (!bytes) return fail(RF_EINVAL_ARG, "%s: null pointer", fn);
+  if (int rc = attend_sizes(fn, T, hq, hkv, d, kind, n_seq, max_rows, max_keys)) return rc;
+  *bytes = T && n_seq && max_rows ? plan_of(T, hq, hkv, d, kind == RF_PAGES_MX4, n_seq, max_rows, max_keys, true).bytes : 0;
   return RF_OK;
 }
 
@@ -1684,7 +1714,7 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
     return fail(RF_EINVAL_SHAPE, "%s: %lld words of bits a row (row stride %lld) for up to %lld rows a sequence", fn, (long long)words,
                 (long long)ld_seen, (long long)max_rows);
   if (T == 0 || n_seq == 0 || max_rows == 0) return RF_OK;
-  Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys);
+  Plan p = plan_of(T, hq, hkv, d, pages->kind == RF_PAGES_MX4, n_seq, max_rows, max_keys, TREE);
   if (std::max(p.units, p.blocks) * hkv > INT32_MAX)
     return fail(RF_EINVAL_SHAPE, "%s: %lld blocks of query rows over %d K / V heads", fn, (long long)p.blocks, hkv);
   if (p.fit && (!workspace || ws_bytes < p.bytes)) {
@@ -1697,7 +1727,7 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
                     // key tiles a split at least (a quarter or half of it, this, four times it): one sequence of 4000 keys 16 / 17 /
                     // 33 us, of 6000 in 4 bits 15 / 14 / 20; chunks of 200 rows over 4000 keys 38 / 38 / 46, 2 of 64 over 3000 33 / 36 / 47
-                    p.many ? 4 : 2 * NW, seen, ld_seen, static_cast<int>(words)};
+                    p.small ? 8 : p.many ? 4 : 2 * NW, seen, ld_seen, static_cast<int>(words)};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
   const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, p.rows());
@@ -1706,11 +1736,14 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
   const bool mx = pages->kind == RF_PAGES_MX4;
 #define RF_ATTEND(D)                                                                                     \
   do {                                                                                                   \
-    if (p.many && mx) {                                                                                  \
-      if constexpr (D != 256) hipLaunchKernelGGL((k_paged_many<D, true, TREE>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
-    } else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false, TREE>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
-    else if (mx) hipLaunchKernelGGL((k_paged_few<D, true, TREE>), grid, dim3(64 * NW), 0, stream, a);          \
-    else hipLaunchKernelGGL((k_paged_few<D, false, TREE>), grid, dim3(64 * NW), 0, stream, a);                 \
+    if (p.small) {                                                                                       \
+      if constexpr (TREE && D != 256)                                                                    \
+        hipLaunchKernelGGL((k_paged_many<D, false, true, true>), grid, dim3(64 * many_waves(D, true)), 0, stream, a); \
+    } else if (p.many && mx) {                                                                           \
+      if constexpr (D != 256) hipLaunchKernelGGL((k_paged_many<D, true, TREE, false>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    } else if (p.many) hipLaunchKernelGGL((k_paged_many<D, false, TREE, false>), grid, dim3(64 * many_waves(D)), 0, stream, a); \
+    else if (mx) hipLaunchKernelGGL((k_paged_few<D, true, TREE>), grid, dim3(64 * NW), 0, stream, a);    \
+    else hipLaunchKernelGGL((k_paged_few<D, false, TREE>), grid, dim3(64 * NW), 0, stream, a);           \
     if (p.fit) {                                                                                         \
       if (int rc = check_launch(fn)) return rc;                                                          \
       if (p.many) hipLaunchKernelGGL((k_paged_merge<D, false>), grid2, merge, 0, stream, a);   \

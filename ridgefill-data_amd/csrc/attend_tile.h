@@ -45,9 +45,9 @@ __device__ __forceinline__ void wait_vm_lgkm0() {
 // hit distinct banks. V row r's chunk c sits at K_U4 + r * KCPR + (c ^ (4 vsw(r))): a transpose read takes
 // 8 bytes in each of 4 consecutive rows over 4 chunks per row per 32 lanes, and the swizzle moves the four
 // rows onto four different 64-byte bank ranges.
-template <int AD>
+template <int AD, int KEYS = Cfg<AD>::KT, int WAVES = Cfg<AD>::NW>
 struct Layout {
-  static constexpr int KT = Cfg<AD>::KT, NW = Cfg<AD>::NW;
+  static constexpr int KT = KEYS, NW = WAVES;
   static constexpr int KCPR = AD / 8;
   static constexpr int K_U4 = KT * KCPR;
   static constexpr int V_U4 = KT * KCPR;
@@ -85,12 +85,12 @@ __device__ __forceinline__ float headroom(float c) { return fminf(RESCALE_LOG2 /
 template <int AD>
 struct FragOffsets {
   uint32_t kz, vz;
-  __device__ FragOffsets(int lane) {
+  __device__ FragOffsets(int lane, int k_u4 = Layout<AD>::K_U4) {          // (the tile's keys, in 16-byte chunks)
     using L = Layout<AD>;
     const int n = lane & 31, hh = lane >> 5, g = lane >> 4, t = lane & 15;
     kz = static_cast<uint32_t>(n * L::KCPR * 16) | static_cast<uint32_t>(16 * (hh ^ (n & (L::KCPR - 1))));
     const int r0 = 4 * (g >> 1) + (t >> 2), cl = 2 * (g & 1) + ((t & 3) >> 1);
-    vz = static_cast<uint32_t>((L::K_U4 + r0 * L::KCPR + cl) * 16 + 8 * (t & 1)) |
+    vz = static_cast<uint32_t>((k_u4 + r0 * L::KCPR + cl) * 16 + 8 * (t & 1)) |
          static_cast<uint32_t>(64 * L::vsw(r0));
   }
   __device__ uint32_t k(int s) const { return kz ^ static_cast<uint32_t>(32 * s); }
@@ -117,11 +117,11 @@ __device__ __forceinline__ void lane_pair(float v, float& lo, float& hi) {
 // score of key 32 kb + 8 (j / 4) + 4 hh + j % 4 of the tile for query n. (The stage pointers are
 // __restrict__: the LDS reads then carry alias information, and the compiler does not make them wait for
 // the direct loads in flight into the other stages; the kernel's own waits order them.)
-template <int AD>
+template <int AD, int KB = Cfg<AD>::KB>
 __device__ __forceinline__ void tile_scores(const char* __restrict__ st, const bf16x8 (&qf)[AD / 16],
-                                            f32x16 (&sc)[Cfg<AD>::KB], const FragOffsets<AD>& fo) {
+                                            f32x16 (&sc)[KB], const FragOffsets<AD>& fo) {
   using L = Layout<AD>;
-  constexpr int NS = AD / 16, KB = Cfg<AD>::KB;
+  constexpr int NS = AD / 16;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -138,14 +138,14 @@ __device__ __forceinline__ void tile_scores(const char* __restrict__ st, const b
 // maximum mref (raw-score units, -inf until a key is visible) lazily, then in one block the base-2
 // probabilities exp2(fma(s, c, -mref c)) of sc (c = scale * log2(e) > 0) beside the MFMAs of the next
 // tile's scores sn (from stage sn_st), and O^T += V^T P^T from this tile's stage st.
-template <int AD>
+template <int AD, int KB = Cfg<AD>::KB>
 __device__ __forceinline__ void tile_step(const char* __restrict__ st, const char* __restrict__ sn_st,
-                                          const bf16x8 (&qf)[AD / 16], f32x16 (&sc)[Cfg<AD>::KB],
-                                          f32x16 (&sn)[Cfg<AD>::KB], f32x16 (&o)[AD / 32], float& mref, float& lsum,
+                                          const bf16x8 (&qf)[AD / 16], f32x16 (&sc)[KB],
+                                          f32x16 (&sn)[KB], f32x16 (&o)[AD / 32], float& mref, float& lsum,
                                           int k0, bool edge, int mypos, int hh, float c,
                                           const FragOffsets<AD>& fo) {
   using L = Layout<AD>;
-  constexpr int NB = AD / 32, NS = AD / 16, KB = Cfg<AD>::KB, KT = Cfg<AD>::KT;
+  constexpr int NB = AD / 32, NS = AD / 16, KT = 32 * KB;
   constexpr int NP = 8 * KB;                            // probability pairs per lane
   if (edge) {
     // key 32 kb + 8 (j / 4) + 4 hh + j % 4 of the tile is past the query when its offset exceeds rel

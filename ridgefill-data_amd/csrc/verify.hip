@@ -187,7 +187,7 @@ struct Step {
 // instructions a logit (none of them at a quarter of the rate), as 2^(x c - ref c) of logits not below ref - 1000 / c (those, NaN
 // and -infinity count 2^-1000). Without a draft a row's sum decides only whether u Z < w, and the draw sums its row again: there
 // weights are in 32 bits, 16 of them a sum in 32 bits and those in 64; the sum is off by some 1e-7 of itself, a test by a chance
-// of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, @@ in 32; their bytes take 22.)
+// of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, 35 in 32; their bytes take 22.)
 // Where reference and slope allow neither, weight by weight.
 template <class E, bool EXACT>
 __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a) {
@@ -830,7 +830,7 @@ extern "C" int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld,
                      reinterpret_cast<int32_t*>(ws + space.gone)};
   const size_t rows = static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES, sums = static_cast<size_t>((vocab + RUN - 1) / RUN) * 12;
   // k_verify_sums: a block a chunk, fewer where that is more than a round of blocks (two a CU): 32 sequences over 32 chunks
-  // @@ us with a block a chunk, @@ with 16 blocks each
+  // 19 us with a block a chunk, 15 with 16 blocks each
   const dim3 grid(static_cast<unsigned>((T * a.shares + NT / 64 - 1) / (NT / 64)));
   const int blocks = drawn ? std::min(chunks, std::max(1, 512 / n_seq)) : 1;
 #define RF_VERIFY(E, Q)                                                                                                       \

@@ -113,6 +113,7 @@ SIGNATURES = {
     "rf_paged_tree": [_P, _I64, _I64, _P, _P, _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _P],
     "rf_attend_tree": [_P, _I64, _I64, _I32, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I32, _I64, _I64, _F32, _P, _I64, _P, _SZ,
                        _P],
+    "rf_attend_tree_workspace_bytes": [_I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _PSZ],
     "rf_verify_drafts": [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
                          _SZ, _P],
     "rf_verify_drafts_workspace_bytes": [_I64, _I64, _I32, _I64, _PSZ],

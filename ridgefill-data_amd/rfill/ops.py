@@ -1122,6 +1122,14 @@ def attend_paged_workspace_bytes(rows, hq, hkv, d, kind, n_seq, max_rows, max_ke
     return b.value
 
 
+@_size_rule
+def attend_tree_workspace_bytes(rows, hq, hkv, d, kind, n_seq, max_rows, max_keys):
+    """Device bytes attend_tree uses to split the keys of a sequence over more blocks (0: no split)."""
+    b = ctypes.c_size_t(0)
+    _lib.call("rf_attend_tree_workspace_bytes", rows, hq, hkv, d, kind, n_seq, max_rows, max_keys, ctypes.byref(b))
+    return b.value
+
+
 def attend_paged(q, pages, table, lens, cu, hq, scale, max_rows, max_keys, out=None, workspace="auto"):
     """Causal attention of the new rows q [rows, hq d] of several sequences over their pages (rfill.paged.Pages): sequence
     b's rows [cu[b], cu[b + 1]) are its last tokens of lens[b], in the pages table[b] lists in order (table int32 [n, width],
@@ -1153,7 +1161,8 @@ def _attend(fn, q, pages, table, lens, cu, seen, hq, scale, max_rows, max_keys, 
         _need(out, "out", torch.bfloat16, 2)
         if out.shape[0] != rows or out.shape[1] < hq * d:
             raise ValueError(f"{fn}: out {tuple(out.shape)}, expected [{rows}, {hq * d}]")
-    need = attend_paged_workspace_bytes(rows, hq, pages.hkv, d, pages.kind, n, max_rows, max_keys)
+    size = attend_paged_workspace_bytes if seen is None else attend_tree_workspace_bytes
+    need = size(rows, hq, pages.hkv, d, pages.kind, n, max_rows, max_keys)
     if isinstance(workspace, str):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     if workspace is not None:

@@ -550,7 +550,7 @@ def test_together_captured_and_on_another_stream(dev):                          
                     q=torch.zeros(T, V, device=dev))
         tb = table.to(dev)
         ws = torch.zeros(ops.verify_drafts_workspace_bytes(T, V, 3, most), dtype=torch.uint8, device=dev)
-        aws = torch.zeros(max(16, ops.attend_paged_workspace_bytes(T, hq, hkv, d, pages[0].kind, 3, most, 130)), dtype=torch.uint8, device=dev)
+        aws = torch.zeros(max(16, ops.attend_tree_workspace_bytes(T, hq, hkv, d, pages[0].kind, 3, most, 130)), dtype=torch.uint8, device=dev)
 
         def step():
             h = hold
