@@ -11,6 +11,8 @@ arithmetic in librfill's HIP kernels.
   layer_paged(i, h, step, cache), forward_paged(cache, seqs, ids)
                                 exact layers and forward of new tokens of several sequences over a
                                 paged cache (rfill.paged.PagedCache)
+  verify_paged(cache, seqs, ids, parents, ...)
+                                the same for drafted tokens: those that this model accepts stay
 
 Cache layout (code/kva/model.py:139-159): attention layers hold kbuf / vbuf [Hkv, cap, d] bf16 with
 cap = rows + KV_RESERVE, 'n' and the views k / v = buf[:, :n]; appended row j lands in slot n + j.
@@ -558,11 +560,11 @@ class FillModel:
     def layer_paged(self, i, h, step, cache, ssq=None):
         """Exact layer i for the new rows h [rows, H] bf16 of several sequences over a paged cache (rfill.paged.PagedCache;
         step: its plan() of these rows), as layer() of each sequence alone: queries, gate, K and V of all rows from one
-        product, K and V normed and rotated into the pages, attention over them, then o_proj, the residual and the MLP. GDN
-        layers continue each sequence's states. The workspaces are the model's, as for its other layers: calls on one model
-        run on one stream, or one after the other, and a captured step is made of the operators (ops.paged_append,
-        ops.attend_paged) with a workspace of its own. Returns (layer output [rows, H] bf16, its row sum-of-squares
-        partials)."""
+        product, K and V normed and rotated into the pages, attention over them (of trees' rows to those above them), then
+        o_proj, the residual and the MLP. GDN layers continue each sequence's states. The workspaces are the model's, as for
+        its other layers: calls on one model run on one stream, or one after the other, and a captured step is made of the
+        operators (ops.paged_append, ops.attend_paged, ops.attend_tree) with a workspace of its own. Returns (layer output
+        [rows, H] bf16, its row sum-of-squares partials)."""
         if h.shape[0] != step.rows:
             raise ValueError(f"layer_paged: {h.shape[0]} rows, the step has {step.rows}")
         if ssq is None:
@@ -579,14 +581,19 @@ class FillModel:
         k, v = (x[:, N - j * hkv * d:N - (j - 1) * hkv * d].unflatten(1, (hkv, d)) for j in (2, 1))
         ops.paged_append(k, v, step.slots, pages, cs=step.cs, q=q, out=q, qnorm=w.get("q_norm"), knorm=w.get("k_norm"),
                          norm_kind=self.knorm_kind, eps=self.eps)
-        o = ops.attend_paged(q, pages, step.table, step.lens, step.cu, hq, self.scale, step.max_rows, step.max_keys,
-                             workspace=self._paged_workspace(R, pages, step, h.device))
+        ws = self._paged_workspace(R, pages, step, h.device)
+        if step.seen is None:
+            o = ops.attend_paged(q, pages, step.table, step.lens, step.cu, hq, self.scale, step.max_rows, step.max_keys,
+                                 workspace=ws)
+        else:
+            o = ops.attend_tree(q, pages, step.table, step.lens, step.cu, step.seen, hq, self.scale, step.max_rows,
+                                step.max_keys, workspace=ws)
         return self._out_mlp(w, h, self._gate(w, h, ssq, o, g))
 
     def _paged_workspace(self, rows, pages, step, device):
-        """attend_paged's workspace, shared by every layer (stream-ordered reuse)."""
-        need = ops.attend_paged_workspace_bytes(rows, self.n_heads, self.n_kv, self.head_dim, pages.kind, len(step.counts),
-                                                step.max_rows, step.max_keys)
+        """attend_paged's or attend_tree's workspace, shared by every layer (stream-ordered reuse)."""
+        size = ops.attend_paged_workspace_bytes if step.seen is None else ops.attend_tree_workspace_bytes
+        need = size(rows, self.n_heads, self.n_kv, self.head_dim, pages.kind, len(step.counts), step.max_rows, step.max_keys)
         ws = getattr(self, "_paged_ws", None)
         if need and (ws is None or ws.numel() < need or ws.device != device):
             self._paged_ws = ws = None                  # (the old one back before the larger one is taken)
@@ -631,6 +638,51 @@ class FillModel:
         except BaseException:
             cache.undo(step)
             raise
+
+    def verify_paged(self, cache, seqs, ids, parents=None, temperature=None, u=None, r=None, draft=None):
+        """Drafted tokens of several sequences of a paged cache, all in one exact forward: ids[b], the token that sequence
+        seqs[b] decided last (not in the cache yet), then the drafted ones. They follow one another, or are trees:
+        parents[b][i], the place in ids[b] of the token that ids[b][i] follows (an earlier one; -1 for the first, 0 at least
+        for the others). Those that this model accepts stay in the cache behind the first, the others leave it.
+        temperature: a number, or one a sequence; None or 0 takes the likeliest token. u (fp32 [tokens of all]), r (fp32
+        [len(seqs)]) on the device, in [0, 1): the random numbers (None: torch's). draft [tokens of all, V]: row i holds the
+        shares that the children of token i were drawn from (None: they were chosen, not drawn; ops.verify_drafts).
+        Returns, for each sequence, the list of accepted drafted ids and the id after them (-1: no logit above -infinity),
+        which begins the next call's ids. If it raises, the sequences are as they were."""
+        ids = [torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in ids]
+        if len(cache.layers) != self.n_layers or cache.model is not self:
+            raise ValueError("verify_paged: a cache of this model, with every layer packed")
+        cache._all_attention("dropping tokens")
+        counts = [x.numel() for x in ids]
+        if parents is None:
+            above = [list(range(-1, n - 1)) for n in counts]
+        else:
+            above = parents = [[int(p) for p in x] for x in parents]
+            if any(p < 0 for x in parents for p in x[1:]):
+                raise ValueError("verify_paged: the drafted tokens follow the first or one another")
+        n, rows, dev = len(seqs), sum(counts), self.device
+        if temperature is not None:
+            t = torch.as_tensor(temperature, dtype=torch.float32).reshape(-1)
+            if t.numel() not in (1, n):
+                raise ValueError(f"verify_paged: {t.numel()} temperatures of {n} sequences")
+            temperature = t.expand(n).contiguous().to(dev)
+            u = torch.rand(rows, device=dev) if u is None else u
+            r = torch.rand(n, device=dev) if r is None else r
+        h, ssq = self.embed(torch.cat(ids) if ids else torch.empty(0, dtype=torch.int64))
+        step = cache.plan(seqs, counts, parents)
+        try:
+            tokens = torch.cat(ids).to(dev)
+            above = torch.tensor([p for x in above for p in x], dtype=torch.int32, device=dev)
+            for i in range(self.n_layers):
+                h, ssq = self.layer_paged(i, h, step, cache, ssq=ssq)
+            path, count, after = ops.verify_drafts(self._head_rows(h, ssq), tokens, above, step.cu, u, r, temperature,
+                                                   step.max_rows, draft=draft)
+            after = after.tolist()
+            kept = cache.accept(step, path, count)
+        except BaseException:
+            cache.undo(step)
+            raise
+        return [[int(x[i]) for i in row[1:]] for x, row in zip(ids, kept)], after
 
     def embed(self, ids):
         """Embedding rows of token ids [T] (code/kva/model.py:108-109): a bit-exact row gather from the bf16
@@ -684,6 +736,10 @@ class FillModel:
     def logits(self, h, ssq=None):
         """F.linear(final_norm(h), lm_head).float() (code/kva/model.py:110-111): [rows, V] fp32 from bf16
         rows. The final norm's gain is folded into the packed lm_head (zero rows up to a multiple of 256)."""
+        return self._head_rows(h, ssq).float()
+
+    def _head_rows(self, h, ssq):
+        """The logits as the product rounds them, bf16."""
         if getattr(self, "_lm", None) is None:
             src, pre = self._src, self._pre
             dev = lambda k: src[k].to(self.device, torch.bfloat16).contiguous()   # noqa: E731
@@ -697,7 +753,7 @@ class FillModel:
         if ssq is None:
             ssq = ops.row_ssq(h)
         return ops.norm_linear(h, ssq, self.eps, head,
-                               workspace=self.gemm_workspace(h.shape[0], head.shape[0], h.shape[1], h.device))[:, :V].float()
+                               workspace=self.gemm_workspace(h.shape[0], head.shape[0], h.shape[1], h.device))[:, :V]
 
     def fill_kv(self, i, k, v, pos, cache, cs=None):
         """Cache-only fill from pre-RoPE K and V [P, Hkv, d] (the reads() layout)."""

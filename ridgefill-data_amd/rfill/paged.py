@@ -4,7 +4,8 @@ Pages: the pools of one layer as the kernels read them (ops.paged_append, paged_
 bits (17 / 32 byte a value: E2M1 codes with a power-of-two scale for each 32 values; include/rfill.h has the layout).
 PagedCache: the pages of every attention layer of a FillModel and the states of its GDN layers, for sequences that come
 (empty, or with a cache that finish() or forward_exact() filled), grow (plan(), then FillModel.layer_paged of each layer;
-FillModel.forward_paged does both) and go.
+FillModel.forward_paged does both) and go. Tokens that a cheaper model drafted, in a row or as trees, grow a sequence at once
+and are then cut to those that were accepted (plan(parents=), accept(); FillModel.verify_paged does it all).
 """
 import ctypes
 from dataclasses import dataclass, field
@@ -85,7 +86,8 @@ class Pages:
 class Step:
     """New tokens of several sequences (PagedCache.plan): sequence b's rows are [cu[b], cu[b + 1]) and become its last
     tokens. On the device: table (its pages), lens (its tokens with them), cu, and of each row the slot, the position and
-    the RoPE table row. moved: the sequences whose GDN states have taken rows of it."""
+    the RoPE table row. moved: the sequences whose GDN states have taken rows of it. Trees: seen, the bits of the new rows that
+    each row sees (ops.paged_tree), the positions by depth, and on the host parents, a list for each sequence."""
     seqs: list
     counts: list
     table: torch.Tensor
@@ -98,6 +100,8 @@ class Step:
     max_keys: int
     ends: list = None                       # tokens of each sequence with the new ones
     moved: set = field(default_factory=set)
+    seen: torch.Tensor = None
+    parents: list = None
 
     @property
     def rows(self):
@@ -186,10 +190,13 @@ class PagedCache:
         del self._seqs[seq]
         self._free += reversed(s.pages)
 
-    def plan(self, seqs, counts):
+    def plan(self, seqs, counts, parents=None):
         """Room for counts[b] new tokens of each sequence seqs[b]: the Step that layer_paged of every layer takes. The
         sequences count the tokens from now on; undo() takes that back. Raises MemoryError when the pages do not suffice.
-        Nothing is changed when it raises."""
+        Nothing is changed when it raises.
+        parents: the new tokens are nodes of trees, parents[b][i] the place among the sequence's new ones of the token that
+        token i follows (an earlier one; -1: it follows the tokens before the new ones). A token sees those above it, and its
+        position is its depth's. GDN layers take their rows in order: UnsupportedArchitecture."""
         if len(seqs) != len(counts) or not len(seqs):
             raise ValueError(f"plan: {len(seqs)} sequences, {len(counts)} counts")
         if len(set(seqs)) != len(seqs):
@@ -197,9 +204,18 @@ class PagedCache:
         if any(int(c) < 1 for c in counts):
             raise ValueError(f"plan: counts {list(counts)} (at least one token each)")
         ss, counts = [self._of(q) for q in seqs], [int(c) for c in counts]
+        trees = ()
+        if parents is not None:
+            self._all_attention("trees of new tokens")
+            parents = [[int(p) for p in x] for x in parents]
+            if [len(x) for x in parents] != counts:
+                raise ValueError(f"plan: parents of {[len(x) for x in parents]} tokens, counts {counts}")
+            if any(not -1 <= p < i for x in parents for i, p in enumerate(x)):
+                raise ValueError("plan: a token's parent is an earlier one of its sequence's new tokens, or -1")
+            trees = (parents,)
         self._grow(list(zip(ss, counts)))
         try:
-            return self._step(ss, counts, list(seqs))
+            return self._step(ss, counts, list(seqs), *trees)
         except BaseException:
             self._shrink(list(zip(ss, counts)))
             raise
@@ -214,6 +230,38 @@ class PagedCache:
         self._shrink([(s, n) for q, s, n in zip(step.seqs, ss, step.counts) if q not in step.moved])
         for q, s in zip(step.seqs, ss):
             s.lost = q in step.moved
+
+    def accept(self, step, path, count):
+        """Keep of each sequence's new tokens those on a path: of a plan() whose rows are through every layer, the last one of
+        its sequences, token path[b, j] becomes the j-th new one for j < count[b], in every layer's pages (path int32 [n,
+        depth], count int32 [n] on the device, as ops.verify_drafts gives them). The sequences lose the others, and pages
+        without tokens are free again (remove()'s note on queued work holds). A path goes from a token without a parent down,
+        a child each; of a plan() without parents it is the first tokens. Returns the paths as lists. Nothing is changed when
+        it raises."""
+        self._all_attention("dropping tokens")
+        ss = [self._of(q) for q in step.seqs]
+        if [s.tokens for s in ss] != step.ends:
+            raise ValueError("accept: not the last plan of its sequences")
+        ops._need(path, "path", torch.int32, 2)
+        ops._need(count, "count", torch.int32, 1)
+        if path.shape[0] != len(ss) or count.shape[0] != len(ss):
+            raise ValueError(f"accept: path {tuple(path.shape)}, count {tuple(count.shape)} of {len(ss)} sequences")
+        kept = []
+        for n, b, row in zip(step.counts, range(len(ss)), torch.cat((count[:, None], path), 1).tolist()):
+            m, row = row[0], row[1:]
+            above = range(-1, n - 1) if step.parents is None else step.parents[b]
+            if not 0 <= m <= min(n, len(row)) or any(not 0 <= i < n or above[i] != (row[j - 1] if j else -1)
+                                                     for j, i in enumerate(row[:m])):
+                raise ValueError(f"accept: {m} tokens {row[:max(0, m)]} of {n} new ones are no path")
+            kept.append(row[:m])
+        if self.pools and any(i != j for row in kept for j, i in enumerate(row)):
+            ops.paged_keep(list(self.pools.values()), step.table, step.lens, step.cu, path, count)
+        self._shrink([(s, n - len(row)) for s, n, row in zip(ss, step.counts, kept)])
+        return kept
+
+    def _all_attention(self, what):
+        if any(self.model.layer_types[i] != "attn" for i in self.layers):
+            raise _lib.UnsupportedArchitecture(f"{what}: GDN layers take their rows in order, and none back")
 
     def _grow(self, wants):
         need = [-(-(s.tokens + n) // self.page) - len(s.pages) for s, n in wants]
@@ -230,7 +278,7 @@ class PagedCache:
             self._free += reversed(s.pages[keep:])
             del s.pages[keep:]
 
-    def _step(self, ss, counts, seqs=None):
+    def _step(self, ss, counts, seqs=None, parents=None):
         dev = self.model.device
         width = max(1, max(len(s.pages) for s in ss))
         cu = [0]
@@ -239,13 +287,17 @@ class PagedCache:
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
         table = i32([s.pages + [-1] * (width - len(s.pages)) for s in ss])
         lens, cu = i32([s.tokens for s in ss]), i32(cu)
-        if not self.pools:                  # GDN layers alone: no slots
-            slots = pos = cs = None
-        else:
-            slots, pos = ops.paged_slots(table, lens, cu, sum(counts), next(iter(self.pools.values())))
+        slots = pos = cs = seen = None
+        if self.pools:                      # (GDN layers alone: no slots)
+            pool = next(iter(self.pools.values()))
+            if parents is None:
+                slots, pos = ops.paged_slots(table, lens, cu, sum(counts), pool)
+            else:
+                slots, pos, seen = ops.paged_tree(table, lens, cu, i32([p for x in parents for p in x]), sum(counts), pool,
+                                                  max(counts))
             cs = self.model.rope_table(pos)
         ends = [s.tokens for s in ss]
-        return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(ends), ends)
+        return Step(seqs, counts, table, lens, cu, slots, pos, cs, max(counts), max(ends), ends, seen=seen, parents=parents)
 
     def read(self, seq):
         """The sequence's cache as FillModel.new_cache lays it out (bf16 buffers of its own; of 4-bit pages what they hold). The
