@@ -112,7 +112,7 @@ struct KeepArgs {
   int64_t ld_path;
   int path_width;
   const int32_t* count;
-  int items, parts;                        // pieces of a layer's rows, blocks that they take
+  int hkv, items, parts;                   // pieces of a layer's rows, blocks that they take
 };
 
 constexpr int KEEP_RUN = 256;              // entries of a path at once
@@ -139,6 +139,10 @@ __device__ __forceinline__ void move_pieces(const KeepRun& run, int n, char* poo
   }
 }
 
+// 4 bits: the pieces of the keys' codes, of the values' and of the scales begin a wave each (with a head's in a row every wave went
+// through all three: 13 sequences of up to 64 rows, 2 layers 12 us, so 7).
+__host__ __device__ constexpr int waves_of(int pieces) { return (pieces + 63) & ~63; }
+
 template <int D, bool MX>
 __global__ __launch_bounds__(256) void k_paged_keep(KeepArgs a) {
   __shared__ KeepRun run;
@@ -149,8 +153,6 @@ __global__ __launch_bounds__(256) void k_paged_keep(KeepArgs a) {
   const int64_t base = static_cast<int64_t>(a.lens[b]) - rows;
   const int32_t* path = a.path + b * a.ld_path;
   const int32_t* table = a.table + b * a.ld_table;
-  constexpr int HEAD = MX ? D / 32 + 16 + D / 16 : D / 4;    // pieces of a head's row, of K and V
-  const int h = item / HEAD, x = item - h * HEAD;
   for (int j0 = 0; j0 < n; j0 += KEEP_RUN) {
     __syncthreads();
     if (t == 0) stop = n - j0;
@@ -173,21 +175,30 @@ __global__ __launch_bounds__(256) void k_paged_keep(KeepArgs a) {
     }
     __syncthreads();
     const int m = min(stop, KEEP_RUN);
-    if (item < a.items) {
-      const int64_t head = static_cast<int64_t>(h) * pg.head_bytes, scales = static_cast<int64_t>(h) * pg.head_scales;
-      if constexpr (!MX) {
-        const int y = x % (D / 8);
-        move_pieces<uint4>(run, m, (x < D / 8 ? pg.k : pg.v) + head + y * 16, pg.page_stride, [&](int tok) { return tok * (D * 2); });
-      } else if (x < D / 32) {
-        move_pieces<uint4>(run, m, pg.k + head + x * 16, pg.page_stride, [&](int tok) { return tok * (D / 2); });
-      } else if (x < D / 32 + 16) {
-        using W = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>>;
-        constexpr int RB = D / 32;
-        move_pieces<W>(run, m, pg.v + head + (x - RB) * (8 * RB), pg.page_stride, [&](int tok) { return (tok >> 3) * (4 * D) + (tok & 7) * RB; });
+    if constexpr (!MX) {
+      const int h = item / (D / 4), x = item % (D / 4), y = x % (D / 8);
+      if (item < a.items)
+        move_pieces<uint4>(run, m, (x < D / 8 ? pg.k : pg.v) + static_cast<int64_t>(h) * pg.head_bytes + y * 16, pg.page_stride,
+                           [&](int tok) { return tok * (D * 2); });
+    } else {
+      using W = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>>;
+      constexpr int G = D / 32;
+      const int nk = waves_of(a.hkv * G), nv = waves_of(a.hkv * 16), x = item < nk ? item : item < nk + nv ? item - nk : item - nk - nv;
+      if (item < nk) {
+        const int h = x / G, y = x % G;
+        if (h < a.hkv)
+          move_pieces<uint4>(run, m, pg.k + static_cast<int64_t>(h) * pg.head_bytes + y * 16, pg.page_stride,
+                             [&](int tok) { return tok * (D / 2); });
+      } else if (item < nk + nv) {
+        const int h = x / 16, y = x % 16;
+        if (h < a.hkv)
+          move_pieces<W>(run, m, pg.v + static_cast<int64_t>(h) * pg.head_bytes + y * (8 * G), pg.page_stride,
+                         [&](int tok) { return (tok >> 3) * (4 * D) + (tok & 7) * G; });
       } else {
-        const int y = x - D / 32 - 16, z = y % (D / 32);
-        move_pieces<uint8_t>(run, m, reinterpret_cast<char*>(y < D / 32 ? pg.ks : pg.vs) + scales + z * 8, pg.scale_stride,
-                             [&](int tok) { return (tok >> 3) * (D / 4) + (tok & 7); });
+        const int h = x / (2 * G), y = x % (2 * G), z = y % G;
+        if (h < a.hkv)
+          move_pieces<uint8_t>(run, m, reinterpret_cast<char*>(y < G ? pg.ks : pg.vs) + static_cast<int64_t>(h) * pg.head_scales + z * 8,
+                               pg.scale_stride, [&](int tok) { return (tok >> 3) * (D / 4) + (tok & 7); });
       }
     }
     if (stop < min(n - j0, KEEP_RUN)) return;                // (uniform: an entry that does not rise ends the path)
@@ -580,6 +591,8 @@ extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const i
     if (pages[i]->kind != first->kind || pages[i]->hkv != first->hkv || pages[i]->d != first->d || pages[i]->page != first->page)
       return fail(RF_EINVAL_SHAPE, "%s: layer %d's pages (kind %d, %d heads of %d, %d tokens) differ from the first's", fn, i,
                   pages[i]->kind, pages[i]->hkv, pages[i]->d, pages[i]->page);
+    for (int j = 0; j < i; ++j)                              // (moved by two blocks at once)
+      if (pages[j]->k == pages[i]->k) return fail(RF_EINVAL_ARG, "%s: layers %d and %d have the same pages", fn, j, i);
   }
   if (n_seq == 0 || path_width == 0) return RF_OK;
   const int d = first->d;
@@ -594,7 +607,8 @@ extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const i
   a.ld_path = ld_path;
   a.path_width = static_cast<int>(path_width);
   a.count = count;
-  a.items = first->hkv * (mx ? d / 32 + 16 + d / 16 : d / 4);
+  a.hkv = first->hkv;
+  a.items = mx ? waves_of(first->hkv * (d / 32)) + waves_of(first->hkv * 16) + waves_of(first->hkv * (d / 16)) : first->hkv * (d / 4);
   a.parts = (a.items + 255) / 256;
   if (static_cast<int64_t>(n_seq) * a.parts > INT32_MAX)
     return fail(RF_EINVAL_SHAPE, "%s: %d sequences of %d heads", fn, n_seq, first->hkv);

@@ -1289,9 +1289,9 @@ def paged_keep(pools, table, lens, cu, path, count):
         raise ValueError(f"paged_keep: path {tuple(path.shape)}, count {tuple(count.shape)} of {n} sequences")
     first = pools[0]
     for p in pools:
-        if (p.kind, p.hkv, p.d, p.page) != (first.kind, first.hkv, first.d, first.page):
-            raise ValueError("paged_keep: the layers' pages differ in kind, heads, head_dim or tokens a page")
-        _same_device(p, table, lens, cu, path, count)
+        if p.form != first.form:
+            raise ValueError("paged_keep: the layers' pages differ in kind, heads, head_dim, tokens a page or device")
+    _same_device(first, table, lens, cu, path, count)
     if n == 0 or path.shape[1] == 0:
         return
     _call_on(table, "rf_paged_keep", (ctypes.c_void_p * len(pools))(*(p.handle for p in pools)), len(pools),

@@ -59,6 +59,7 @@ class Pages:
         if strides[0] != strides[1] or strides[2:3] != strides[3:]:
             raise ValueError(f"Pages: strides between pages {strides} bytes differ")
         self.k, self.v, self.ks, self.vs = k, v, ks, vs
+        self.form = (self.kind, self.hkv, self.d, self.page, dev)
         self._struct = _lib.RfPages(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else None,
                                     vs.data_ptr() if vs is not None else None, self.n_pages, strides[0],
                                     strides[2] if ks is not None else 0, self.kind, self.hkv, self.d, self.page)

@@ -84,3 +84,18 @@ def test_accept(monkeypatch):
     with pytest.raises(ValueError):
         c.accept(row, _i32([[0, 2]]), _i32([2]))               # a row of tokens, of which one was left out
     assert c.accept(row, _i32([[0]]), _i32([0])) == [[]] and c.tokens(a) == 20 and c.free_pages == 12 - 4
+
+
+def test_keep_refuses_the_same_pages_twice():
+    """In the library, before any launch: two blocks would move the same rows at once."""
+    import ctypes
+    from rfill import _lib
+    from test_paged_host import _pages
+    pages = [_pages(), _pages(k=5 << 20), _pages()]
+    for which, n in ((pages, 0), (pages[:2], 1)):
+        handles = (ctypes.c_void_p * len(which))(*(ctypes.addressof(p) for p in which))
+        if n:                                                  # others: accepted, and of no sequences nothing is launched
+            _lib.call("rf_paged_keep", handles, len(which), 1 << 20, 4, 4, 1 << 20, 1 << 20, 0, 1 << 20, 3, 3, 1 << 20, None)
+            continue
+        with pytest.raises(ValueError, match="same pages"):
+            _lib.call("rf_paged_keep", handles, len(which), 1 << 20, 4, 4, 1 << 20, 1 << 20, 0, 1 << 20, 3, 3, 1 << 20, None)
