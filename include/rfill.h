@@ -697,7 +697,8 @@ int rf_attend_tree_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, 
  * outside [0, vocab) are rejected. A row without any logit above -infinity has no next token: -1.
  * path [n_seq, depth] int32 (row stride ld_path): the accepted rows by their place in the sequence, from the root on, -1 behind
  * them (a path has depth rows at most; the last one's children are then not tested); count [n_seq] int32; next [n_seq] int64.
- * A sequence without rows gets count 0 and next -1. Weights and sums are in 64 bits. cu, tokens and parents are read on
+ * A sequence without rows gets count 0 and next -1. Weights and sums are in 64 bits, but for the sums of whole rows that tests
+ * without draft use (32-bit weights: such a test goes the other way with a chance of about 1e-6). cu, tokens and parents are read on
  * the device; max_rows <= 1024 bounds a sequence's rows (it is taken to have as many), vocab <= 2^19. The workspace (16-byte
  * aligned, of rf_verify_drafts_workspace_bytes) need not be kept or cleared; calls that may run at once need one each. */
 int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld, int64_t vocab, int64_t T, const int64_t* tokens,
@@ -713,7 +714,7 @@ int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_
  * head_dim and page): of sequence b's n new rows (its last tokens of lens[b]) row path[b][j] becomes row j, for j < count[b]
  * (int32, device; at most path_width and n are taken). A path rises; an entry that does not, or that is no row, ends it.
  * Codes and scales move as they are. Rows behind the moved ones keep what they hold, and lens is the caller's to change. A
- * row on a page that is none does not move. */
+ * row on a page that is none does not move. Two layers with the same pages are refused. */
 int rf_paged_keep(const rf_pages* const* pages, int n_layers, const int32_t* table, int64_t ld_table, int64_t table_width,
                   const int32_t* lens, const int32_t* cu, int n_seq, const int32_t* path, int64_t ld_path, int64_t path_width,
                   const int32_t* count, hipStream_t stream);

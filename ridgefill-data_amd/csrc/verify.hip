@@ -9,7 +9,8 @@
 //       takes one pass over a row and no memory; a child's token is accepted if u q Z_k < max(p - c_k q, 0).
 //   the next token: the first at which the running sum of what is left exceeds r times its total.
 // The answers are whole numbers and a draw may lie next to a border (there are as many as tokens), so weights and sums are in
-// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones.
+// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones. (But for whole rows' sums without a draft:
+// k_verify_rows.)
 //
 // Three launches. k_verify_rows: every row with children gets its largest logit and weight sum by chunks (which rows a path meets
 // is known row by row only, and a launch a row costs more than reading the others; a row without children is read only where a
@@ -186,8 +187,9 @@ struct Step {
 // EXACT (with a draft: p - c q, and with it every border of what is left, moves with the row's sum): weights in 64 bits, 16
 // instructions a logit (none of them at a quarter of the rate), as 2^(x c - ref c) of logits not below ref - 1000 / c (those, NaN
 // and -infinity count 2^-1000). Without a draft a row's sum decides only whether u Z < w, and the draw sums its row again: there
-// weights are in 32 bits, 16 of them a sum in 32 bits and those in 64; the sum is off by some 1e-7 of itself, a test by a chance
-// of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, 35 in 32; their bytes take 22.)
+// weights are in 32 bits, 16 of them a sum in 32 bits and those in 64: a weight 2^-t is off by about t 2^-24 of itself, the sum by
+// some 1e-7 to 1e-6, a test by a chance of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, 35
+// in 32; their bytes take 22.)
 // Where reference and slope allow neither, weight by weight.
 template <class E, bool EXACT>
 __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a) {
