@@ -57,6 +57,8 @@ struct PagedArgs {
   bool once;                               // k_paged_many: as many units as that at most
   int64_t units;                           // units a head that the launch has blocks and the workspace partials for
   int kt, wmin;                            // keys a tile, key tiles a split at least
+  float unit_tiles;                        // what a unit costs besides its tiles, in tiles (apart: 3, 24, 150 make 2 % of difference)
+  bool apart;                              // k_paged_few: units of splits, not runs
   const uint64_t* seen;                    // trees: of each row of q, bits of the new rows of its sequence that it sees
   int64_t ld_seen;
   int words;
@@ -151,7 +153,6 @@ __device__ __forceinline__ int wave_max(int v) {                                
 // 905 us for 802 and three of 700 in bf16 250 for 240, but five of 500 over 5000 keys 154 for 187; with a whole split all as
 // with a third. Up to 64 sequences the lanes try 64 lengths each; more of them take a length that surely fits. Every block does
 // the same arithmetic on the same sizes: no launch has to plan before this one, and a captured graph follows its lens.
-constexpr float UNIT_TILES = 3.f;
 __device__ int split_length(const PagedArgs& a, float work, float blocks, int tmax, int nrb0, int tiles0, int lane) {
   const float fit = static_cast<float>(a.fit);
   const bool once = a.once;
@@ -169,7 +170,7 @@ __device__ int split_length(const PagedArgs& a, float work, float blocks, int tm
     units += static_cast<float>(__builtin_amdgcn_readlane(nrb0, b)) *
              ceilf(static_cast<float>(__builtin_amdgcn_readlane(tiles0, b)) * inv);
   const float longest = fminf(W, static_cast<float>(tmax));
-  float cost = units <= fit ? fmaxf(longest, work / fit) : (work + UNIT_TILES * units) / fit + 0.35f * longest;
+  float cost = units <= fit ? fmaxf(longest, work / fit) : (work + a.unit_tiles * units) / fit + 0.35f * longest;
   // (lane 63's length is every tile: one unit a row block, which always fits)
   if (once && units > fit + 0.5f && lane != 63) cost = 3e38f;
   // the least cost, the shorter length among equals (the bits of positive floats are in order)
@@ -795,6 +796,26 @@ struct FewLds {
   static constexpr int BYTES = MARKS + 4 * D + 16;
 };
 
+// Trees of more rows than a block in 4 bits (apart): the row blocks of a sequence's split read the same tiles, so they run beside one
+// another on one XCD (blocks go round the eight of them), whose L2 gives a tile to all but the first: splits of one length for all
+// (find_unit), not runs. head_dim 256, groups of 8: 9 sequences of up to 13 new tokens and 30011 keys fetch 114 MB for 383 and take
+// 60 us for 75, 13 and 8000 40 / 50, 2 of 64 and 30000 115 / 158; 128, groups of 4: 40 of 26 and 24001 449 MB for 1517 and 264 us
+// for 269 (the vector pipe is busy half of the time), 2 of 26 and 30000 52 / 62. 64 stays with runs: 40 of 64 and 9000 57 / 48.
+// Blocks -> (head, unit), eight units in a row an XCD; the number of units is a multiple of 64.
+__device__ __forceinline__ void near_blocks(int block, int hkv, int units, int& head, int& unit) {
+  const int x = block & 7, k = block >> 3;
+  if (hkv % 8 == 0) {
+    head = x + 8 * (k / units);
+    unit = k % units;
+  } else if (8 % hkv == 0) {
+    head = x % hkv;
+    unit = (k / 8) * (64 / hkv) + (x / hkv) * 8 + k % 8;
+  } else {
+    head = block % hkv;
+    unit = block / hkv;
+  }
+}
+
 template <int D, bool MX, bool TREE>
 __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(PagedArgs a) {
   constexpr int NB = D / 16;
@@ -804,16 +825,21 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), n = lane & 15, g = lane >> 4;
   // (heads slowest: the blocks of an XCD then read all heads' parts of the pages. With heads fastest and 8 of them each XCD
   // reads one head's, which all lie at the same offset of a page, and in 4 bits, 4 KB of 32, 4 % slower)
-  const int blocks = gridDim.x / a.hkv, head = blockIdx.x / blocks, mask = (1 << a.pg.shift) - 1;
+  const int blocks = gridDim.x / a.hkv, mask = (1 << a.pg.shift) - 1;
+  int head = blockIdx.x / blocks, x0 = blockIdx.x - head * blocks;
+  constexpr bool APART = TREE && MX && D != 64;
+  if constexpr (APART) {
+    if (a.apart) near_blocks(blockIdx.x, a.hkv, blocks, head, x0);
+  }
   uint32_t* marks = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(lds4) + F::MARKS);
   for (int x = t; x <= D; x += 64 * NW) marks[x] = 0u;
   __syncthreads();
   Seq s0{0, 0, 0};
   if (lane < a.n_seq) s0 = seq_of(a, lane);
   // the block's run of tiles [at, end), or (unsplit) its row block
-  const int x0 = blockIdx.x - head * blocks;
   int at = 0, end = 1, run = 0;
-  if (a.fit) {
+  const bool runs = a.fit && !(APART && a.apart);
+  if (runs) {
     int total;
     run = run_length(a, s0, lane, total);
     at = x0 * run;
@@ -821,12 +847,22 @@ __global__ __launch_bounds__(64 * NW, (few_blocks(D, MX))) void k_paged_few(Page
     if (blockIdx.x == 0 && t == 0) *a.length = run;          // for the merge
   }
   for (bool once = true; at < end; once = false) {           // (uniform over the block)
-    const Piece u = a.fit ? piece_at(a, s0, at, false, lane) : piece_at(a, s0, x0, true, lane);
+    Piece u;
+    int itn;
+    int64_t part = static_cast<int64_t>(2 * x0 + (once ? 0 : 1)) * a.hkv + head;    // (only a run's first and last pieces are parts)
+    if (APART && a.fit && !runs) {
+      const Unit v = find_unit(a, x0, false);
+      u = Piece{v.b, v.rb, v.sp * v.W, v.b < 0 ? 0 : tiles_of(v.s.keys, KT), 0, v.s};
+      itn = min(u.nt, u.t0 + v.W);
+      part = static_cast<int64_t>(x0) * a.hkv + head;
+    } else {
+      u = runs ? piece_at(a, s0, at, false, lane) : piece_at(a, s0, x0, true, lane);
+      itn = runs ? min(u.nt, u.t0 + end - at) : u.nt;
+    }
     if (u.b < 0) return;
-    const int it0 = u.t0, itn = a.fit ? min(u.nt, it0 + end - at) : u.nt;
+    const int it0 = u.t0;
     const bool whole_block = it0 == 0 && itn == u.nt;
-    const int64_t part = static_cast<int64_t>(2 * x0 + (once ? 0 : 1)) * a.hkv + head;    // (only the first and last pieces are parts)
-    at += a.fit ? itn - it0 : 1;
+    at += runs ? itn - it0 : 1;
     const RowBlock r(a, u.s, u.rb);
     const int base = u.s.keys - u.s.rows, p0 = base + r.q0;    // position of its first query (may lie before 0)
     [[maybe_unused]] const uint64_t* seen = TREE ? a.seen + (u.s.first + r.q0) * a.ld_seen : nullptr;
@@ -1611,7 +1647,7 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedArgs a) {
 }
 
 struct Plan {
-  bool many, small, once;
+  bool many, small, once, apart;
   int fit, kt;
   int64_t blocks, units;                   // (sequence, row block)s at most, and with their splits
   size_t bytes;
@@ -1650,8 +1686,11 @@ Plan plan_of(int64_t T, int hq, int hkv, int d, bool mx, int n_seq, int64_t max_
   const bool split = max_keys > 16 * NW * KT && static_cast<double>(p.blocks) * static_cast<double>(max_keys / p.kt + 1) < 1e9;
   p.fit = split ? std::max(1, round / hkv) : 0;
   p.once = p.blocks * 4 <= static_cast<int64_t>(p.fit) * 3;
-  p.units = !p.fit ? p.blocks : !p.many || p.once ? p.fit : 3 * p.fit + 1 + p.blocks;
-  p.bytes = p.fit ? static_cast<size_t>(p.many ? p.units : 2 * p.units) * hkv * (p.rows() * (d + 2)) * 4 + 16 : 0;
+  p.apart = tree && mx && d != 64 && p.fit && !p.many && rows > 16;
+  const bool units = p.many || p.apart;
+  p.units = !p.fit ? p.blocks : !units || p.once ? p.fit : 3 * p.fit + 1 + p.blocks;
+  if (p.apart) p.units = (p.units + 63) & ~static_cast<int64_t>(63);
+  p.bytes = p.fit ? static_cast<size_t>(units ? p.units : 2 * p.units) * hkv * (p.rows() * (d + 2)) * 4 + 16 : 0;
   return p;
 }
 
@@ -1719,6 +1758,7 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
     return fail(RF_EINVAL_SHAPE, "%s: %lld blocks of query rows over %d K / V heads", fn, (long long)p.blocks, hkv);
   if (p.fit && (!workspace || ws_bytes < p.bytes)) {
     p.fit = 0;
+    p.apart = false;
     p.units = p.blocks;
   }
   const PagedArgs a{q, ldq, T, pg, table, ld_table, static_cast<int>(table_width), lens, cu, n_seq, hq, hkv, hq / hkv, p.rows(),
@@ -1727,7 +1767,7 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
                     // key tiles a split at least (a quarter or half of it, this, four times it): one sequence of 4000 keys 16 / 17 /
                     // 33 us, of 6000 in 4 bits 15 / 14 / 20; chunks of 200 rows over 4000 keys 38 / 38 / 46, 2 of 64 over 3000 33 / 36 / 47
-                    p.small ? 8 : p.many ? 4 : 2 * NW, seen, ld_seen, static_cast<int>(words)};
+                    p.small ? 8 : p.many ? 4 : 2 * NW, p.apart ? 24.f : 3.f, p.apart, seen, ld_seen, static_cast<int>(words)};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
   const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, p.rows());
@@ -1746,7 +1786,7 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
     else hipLaunchKernelGGL((k_paged_few<D, false, TREE>), grid, dim3(64 * NW), 0, stream, a);           \
     if (p.fit) {                                                                                         \
       if (int rc = check_launch(fn)) return rc;                                                          \
-      if (p.many) hipLaunchKernelGGL((k_paged_merge<D, false>), grid2, merge, 0, stream, a);   \
+      if (p.many || p.apart) hipLaunchKernelGGL((k_paged_merge<D, false>), grid2, merge, 0, stream, a);   \
       else hipLaunchKernelGGL((k_paged_merge<D, true>), grid2, merge, 0, stream, a);           \
     }                                                                                                    \
   } while (0)
