@@ -144,6 +144,20 @@ def test_attend_long(dev, d, mx):                                               
         check(run(dev, pools, table, q, see, lens, hq, d ** -0.5, workspace=None), want, size, "whole")
 
 
+@pytest.mark.parametrize("hkv,rep", [(1, 4), (3, 2), (4, 4), (8, 4), (16, 2)])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attend_row_blocks_beside_one_another(dev, d, hkv, rep):                           # noqa: F811
+    """4-bit pages and several row blocks a sequence: any number of heads over the XCDs, few and many sequences, split and not."""
+    for counts, lens in (([9, 20, 1, 30], [4000, 2500, 70, 300]), ([1 + i % 17 for i in range(70)], [20 + i for i in range(70)])):
+        see = sees([tree(n, n) for n in counts])
+        pools, table, n_pages, q = batch(hkv * rep, hkv, d, 64, True, counts, lens, hkv)
+        want, size = oracle(pools, table, n_pages, q, see, lens, hkv * rep, d ** -0.5)
+        for kw in (dict(), dict(max_keys=1 << 20), dict(max_keys=1 << 20, max_rows=32)):
+            got = run(dev, pools, table, q, see, lens, hkv * rep, d ** -0.5, **kw)
+            check(got, want, size, (hkv, kw))
+            assert torch.equal(got, run(dev, pools, table, q, see, lens, hkv * rep, d ** -0.5, **kw))
+
+
 @pytest.mark.parametrize("mx", [False, True])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attend_any_bits(dev, d, mx):                                                      # noqa: F811
