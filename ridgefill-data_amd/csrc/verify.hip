@@ -9,14 +9,15 @@
 //       takes one pass over a row and no memory; a child's token is accepted if u q Z_k < max(p - c_k q, 0).
 //   the next token: the first at which the running sum of what is left exceeds r times its total.
 // The answers are whole numbers and a draw may lie next to a border (there are as many as tokens), so weights and sums are in
-// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones. (But for whole rows' sums without a draft:
-// k_verify_rows.)
+// 64 bits: the vector pipe's 64-bit products run at the rate of 32-bit ones. Without a draft the walk begins with sums of whole rows
+// from 32-bit weights (k_verify_rows) and takes a test that they leave open again with a 64-bit sum of what is left (walk).
 //
 // Three launches. k_verify_rows: every row with children gets its largest logit and weight sum by chunks (which rows a path meets
 // is known row by row only, and a launch a row costs more than reading the others; a row without children is read only where a
 // path ends). k_verify_sums: the blocks of a sequence, one a chunk, gather its rows' numbers into LDS, take the walk, each the
 // same, up to the first sums that it needs (what a rejection leaves, or the last row's weights), and sum their own chunk.
-// k_verify_draw: a block a sequence draws, or, where a draft's token was rejected before its last sibling, walks on alone.
+// k_verify_draw: a block a sequence draws, or, where a draft's token was rejected before its last sibling or a test was left open,
+// walks on alone.
 // (The last two as one, its last block going on: the fences before and behind the count of blocks that are done take 50 ns a
 // block, one after the other: 60 us for 32 sequences over 32 chunks.)
 #include <stdint.h>
@@ -182,14 +183,18 @@ struct Step {
   }
 };
 
+// How far, of themselves, sums without a draft may be off: those of k_verify_rows, and 64-bit ones (weights 3e-12, scaled twice).
+constexpr double ROW_ERROR = 1e-5, SUM_ERROR = 2e-11;
+
 // A wave a share of a row: chunks share, share + shares .. Sums are relative to the first step's largest logit as long as the
 // others stay near it, so a step has no more to do than its maximum and its weights.
 // EXACT (with a draft: p - c q, and with it every border of what is left, moves with the row's sum): weights in 64 bits, 16
 // instructions a logit (none of them at a quarter of the rate), as 2^(x c - ref c) of logits not below ref - 1000 / c (those, NaN
 // and -infinity count 2^-1000). Without a draft a row's sum decides only whether u Z < w, and the draw sums its row again: there
-// weights are in 32 bits, 16 of them a sum in 32 bits and those in 64: a weight 2^-t is off by about t 2^-24 of itself, the sum by
-// some 1e-7 to 1e-6, a test by a chance of as much. (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, 35
-// in 32; their bytes take 22.)
+// weights are in 32 bits, 16 of them a sum in 32 bits and those in 64. A weight 2^t is off by three roundings of its exponent (the
+// difference, c, the product), t 3 2^-24 ln 2 of itself, by 2^-23 of v_exp_f32 and 5 2^-24 of the sum; no t is above 64 (the reference
+// is raised), and weights below 2^-64 are nothing beside the reference's 1: a sum is within 8.4e-6 of itself, ROW_ERROR with room.
+// (527 rows of 151936 in bf16, of which 374 have children: 52 us in 64 bits, 35 in 32; their bytes take 22.)
 // Where reference and slope allow neither, weight by weight.
 template <class E, bool EXACT>
 __global__ __launch_bounds__(NT) void k_verify_rows(VerifyArgs a) {
@@ -395,7 +400,9 @@ __device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, cons
 struct State {
   int node, count, next;                   // next: the row from which on the node's children are still to be tested
   double c, Z;                             // what is left of the node's distribution (Z in weights without a draft)
+  double off;                              // without a draft: by how much Z may be wrong
   bool cut;                                // a draft's token was rejected here
+  bool fresh;                              // without a draft: Z was summed for the next test
 };
 
 // ... when its first sums are wanted, for k_verify_draw.
@@ -406,8 +413,10 @@ struct Stop {
   int more, n_gone;                        // whether the walk goes on, the tokens rejected at its last row (without a draft)
 };
 
-// The walk from st on, by every wave with the same numbers. True: a drawn token was rejected, and Z = sum max(p - c q, 0) of the
-// node is wanted for the next child; false: the path has ended (cut: with a rejected token, and c is new).
+// The walk from st on, by every wave with the same numbers. True: Z of the node is wanted for the next child, of a drawn token's
+// rejection sum max(p - c q, 0), without a draft the weights left, because u Z lies nearer to w than Z is known (the row's sum is off
+// by up to ROW_ERROR, and what a rejection leaves by as much as the whole: where little is left of a row, nearly every test); false:
+// the path has ended (cut: with a rejected token, and c is new).
 __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const Rows& l, State& st) {
   const int lane = threadIdx.x & 63;
   const bool drawn = a.draft != nullptr && !s.greedy;
@@ -429,14 +438,22 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const 
     if (s.greedy) {
       yes = tok >= 0 && tok == l.best[st.node];
     } else if (!drawn) {
-      if (st.Z < 0) st.Z = l.sum[st.node];                   // (the node's first child)
+      if (st.Z < 0) {                                        // (the node's first child)
+        st.Z = l.sum[st.node];
+        st.off = ROW_ERROR * st.Z;
+      }
       bool gone = tok < 0;                                   // rejected before, or no token at all
       for (int k0 = st.node + 1; k0 < at; k0 += 64) {
         const int k = min(k0 + lane, at - 1);
         gone |= __any(k0 + lane < at && l.parent[k] == st.node && l.token[k] == tok);
       }
-      const double own = gone ? 0.0 : l.w[at];
-      yes = l.u[at] * st.Z < own;
+      const double own = gone ? 0.0 : l.w[at], mark = l.u[at] * st.Z;
+      if (own > 0 && !st.fresh && __builtin_fabs(mark - own) <= l.u[at] * st.off + SUM_ERROR * own) {
+        st.next = at;
+        return true;
+      }
+      st.fresh = false;
+      yes = mark < own;
       if (!yes) st.Z = __builtin_fmax(st.Z - own, 0.0);
     } else {
       const double q = l.q[at], total = l.sum[st.node];
@@ -471,6 +488,24 @@ struct Left {
   const int* gone;
   int n_gone;
 };
+
+// The tokens rejected at the node without a draft, each once, in the rows' order, by one wave: of the children before the next one to be
+// tested. Returns how many.
+__device__ __forceinline__ int rejected(const Block& s, const Rows& l, const State& st, int* gone) {
+  const int lane = threadIdx.x & 63, end = min(st.next, s.n);
+  int m = 0;
+#pragma unroll 1
+  for (int k0 = st.node + 1; k0 < end; k0 += 64) {
+    const int k = min(k0 + lane, end - 1), tok = l.token[k];
+    bool here = k0 + lane < end && l.parent[k] == st.node && tok >= 0;
+#pragma unroll 1
+    for (int y = st.node + 1; here && y < k; ++y) here = !(l.parent[y] == st.node && l.token[y] == tok);
+    const uint64_t mask = __ballot(here);
+    if (here) gone[m + __popcll(mask & ((1ull << lane) - 1))] = tok;
+    m += __popcll(mask);
+  }
+  return m;
+}
 
 // A lane's four elements e .. e + 3: logits (NaN, what is gone and what lies past the vocabulary as -infinity) and shares.
 template <class E, class Q>
@@ -556,7 +591,7 @@ __global__ __launch_bounds__(NW) void k_verify_sums(VerifyArgs a, int blocks) {
   const Block s = block_of(a, b);
   if ((s.n == 0 || !a.temperature) && x) return;             // (uniform)
   const Rows l(reinterpret_cast<char*>(lds), a.rows);
-  State st{0, 0, 1, 0.0, a.draft != nullptr ? 1.0 : -1.0, false};
+  State st{0, 0, 1, 0.0, a.draft != nullptr ? 1.0 : -1.0, 0.0, false, false};
   if (s.n == 0) {
     write_path(a, b, l.parent, st);
     if (t == 0) a.next[b] = -1;
@@ -577,17 +612,7 @@ __global__ __launch_bounds__(NW) void k_verify_sums(VerifyArgs a, int blocks) {
   if (a.draft == nullptr && !s.greedy) {
     __syncthreads();
     if (wave == 0) {
-      int m = 0;
-#pragma unroll 1
-      for (int k0 = st.node + 1; st.count < a.depth && k0 < s.n; k0 += 64) {
-        const int k = min(k0 + lane, s.n - 1), tok = l.token[k];
-        bool here = k0 + lane < s.n && l.parent[k] == st.node && tok >= 0;
-#pragma unroll 1
-        for (int y = st.node + 1; here && y < k; ++y) here = !(l.parent[y] == st.node && l.token[y] == tok);
-        const uint64_t mask = __ballot(here);
-        if (here) gone[m + __popcll(mask & ((1ull << lane) - 1))] = tok;
-        m += __popcll(mask);
-      }
+      const int m = rejected(s, l, st, gone);
       if (lane == 0) n_gone = m;
     }
     __syncthreads();
@@ -610,7 +635,7 @@ template <class E, class Q>
 __global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
   extern __shared__ double lds[];
   __shared__ float tops[ND / 64];
-  __shared__ int found;
+  __shared__ int found, n_gone;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, runs = (a.V + RUN - 1) / RUN;
   const Part* ends = a.ends + static_cast<int64_t>(b) * a.chunks * RUNS;
   const Part mine = ends[min(t, runs - 1)];
@@ -620,10 +645,12 @@ __global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
   const Rows l(reinterpret_cast<char*>(lds), a.rows);
   double* cs = reinterpret_cast<double*>(reinterpret_cast<char*>(lds) + static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES);    // the runs' sums
   float* ct = reinterpret_cast<float*>(cs + runs);           // ... and largest logits
+  int* gone = reinterpret_cast<int*>(ct + runs);
   const Exp2 e2;
   State st = stop.st;
   bool more = stop.more;
-  const int* gone = a.gone + static_cast<int64_t>(b) * a.rows;
+#pragma unroll 1
+  for (int g = t; g < stop.n_gone; g += ND) gone[g] = a.gone[static_cast<int64_t>(b) * a.rows + g];
   Left<E, Q> left = left_of<E, Q>(a, s, st, stop.sum, gone, stop.n_gone);
   float top = stop.top;                                      // what the sums are relative to
 #pragma unroll 1
@@ -650,11 +677,26 @@ __global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
     for (int y = lane; y < runs; y += 64) z += cs[y];
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) z += shfl_xor64(z, m);
-    st.Z = z;
+    if (st.cut) {
+      st.Z = z;
+    } else {                                                 // (as the children's weights, relative to the row's largest logit)
+      st.Z = z * weight(e2, top, l.top[st.node], s.slope);
+      st.off = SUM_ERROR * st.Z;
+      st.fresh = true;
+    }
     more = walk(a, s, l, st);
-    __syncthreads();                                         // then further sums, of another rejection or the last row
+    __syncthreads();                                         // then further sums, of another test or the last row
+    int dropped = 0;
+    if (a.draft == nullptr) {
+      if (wave == 0) {
+        const int m = rejected(s, l, st, gone);
+        if (lane == 0) n_gone = m;
+      }
+      __syncthreads();
+      dropped = n_gone;
+    }
     top = l.top[st.node];
-    left = left_of<E, Q>(a, s, st, l.sum[st.node], gone, 0);
+    left = left_of<E, Q>(a, s, st, l.sum[st.node], gone, dropped);
 #pragma unroll 1
     for (int run = wave; run < runs; run += ND / 64) {
       const Part p = sum_run(left, e2, run, a.V, top);
@@ -830,7 +872,7 @@ extern "C" int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld,
                      static_cast<int>(std::min<int64_t>(max_rows, T)), static_cast<int>(depth), path, ld_path, count, next,
                      reinterpret_cast<Part*>(ws), reinterpret_cast<Part*>(ws + space.ends), reinterpret_cast<Stop*>(ws + space.stops),
                      reinterpret_cast<int32_t*>(ws + space.gone)};
-  const size_t rows = static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES, sums = static_cast<size_t>((vocab + RUN - 1) / RUN) * 12;
+  const size_t rows = static_cast<size_t>((a.rows + 1) & ~1) * ROW_BYTES, sums = static_cast<size_t>((vocab + RUN - 1) / RUN) * 12 + static_cast<size_t>(a.rows) * 4;
   // k_verify_sums: a block a chunk, fewer where that is more than a round of blocks (two a CU): 32 sequences over 32 chunks
   // 19 us with a block a chunk, 15 with 16 blocks each
   const dim3 grid(static_cast<unsigned>((T * a.shares + NT / 64 - 1) / (NT / 64)));
