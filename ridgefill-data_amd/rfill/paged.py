@@ -88,7 +88,8 @@ class Step:
     """New tokens of several sequences (PagedCache.plan): sequence b's rows are [cu[b], cu[b + 1]) and become its last
     tokens. On the device: table (its pages), lens (its tokens with them), cu, and of each row the slot, the position and
     the RoPE table row. moved: the sequences whose GDN states have taken rows of it. Trees: seen, the bits of the new rows that
-    each row sees (ops.paged_tree), the positions by depth, and on the host parents, a list for each sequence."""
+    each row sees (ops.paged_tree), the positions by depth, and on the host parents, a list for each sequence. mark: what its
+    sequences hold as long as it is their last plan; before: what they held until then."""
     seqs: list
     counts: list
     table: torch.Tensor
@@ -103,6 +104,8 @@ class Step:
     moved: set = field(default_factory=set)
     seen: torch.Tensor = None
     parents: list = None
+    mark: object = None
+    before: list = None
 
     @property
     def rows(self):
@@ -115,6 +118,7 @@ class _Sequence:
         self.pages = []
         self.states = {}                    # GDN layers: conv, rec (own tensors, updated in place)
         self.lost = False                   # a step failed after its GDN states had moved (undo)
+        self.mark = None                    # Step.mark of the last plan, of which tokens may go back (None: of none)
 
 
 class PagedCache:
@@ -216,33 +220,41 @@ class PagedCache:
             trees = (parents,)
         self._grow(list(zip(ss, counts)))
         try:
-            return self._step(ss, counts, list(seqs), *trees)
+            step = self._step(ss, counts, list(seqs), *trees)
         except BaseException:
             self._shrink(list(zip(ss, counts)))
             raise
+        step.mark, step.before = object(), [s.mark for s in ss]
+        for s in ss:
+            s.mark = step.mark
+        return step
+
+    def _last(self, step, what):
+        """The step's sequences, if it is the last plan of each and none of its tokens have gone back or were kept yet. (Their
+        counts would not tell: another plan may have brought them to the same ones, on other pages.)"""
+        ss = [self._of(q) for q in step.seqs]
+        if step.mark is None or any(s.mark is not step.mark for s in ss):
+            raise ValueError(f"{what}: not the last plan of its sequences")
+        return ss
 
     def undo(self, step):
         """Take back a plan() whose rows did not get through every layer, the last one of its sequences: they lose its tokens,
         and the pages that it took are free again. (remove()'s note on queued work holds.) A sequence whose GDN states have
         taken rows of the step cannot go back and is lost: every call on it but remove() raises RuntimeError."""
-        ss = [self._of(q) for q in step.seqs]
-        if [s.tokens for s in ss] != step.ends:
-            raise ValueError("undo: not the last plan of its sequences")
+        ss = self._last(step, "undo")
         self._shrink([(s, n) for q, s, n in zip(step.seqs, ss, step.counts) if q not in step.moved])
-        for q, s in zip(step.seqs, ss):
-            s.lost = q in step.moved
+        for q, s, mark in zip(step.seqs, ss, step.before):
+            s.lost, s.mark = q in step.moved, mark
 
     def accept(self, step, path, count):
         """Keep of each sequence's new tokens those on a path: of a plan() whose rows are through every layer, the last one of
         its sequences, token path[b, j] becomes the j-th new one for j < count[b], in every layer's pages (path int32 [n,
         depth], count int32 [n] on the device, as ops.verify_drafts gives them). The sequences lose the others, and pages
         without tokens are free again (remove()'s note on queued work holds). A path goes from a token without a parent down,
-        a child each; of a plan() without parents it is the first tokens. Returns the paths as lists. Nothing is changed when
-        it raises."""
+        a child each; of a plan() without parents it is the first tokens. Returns the paths as lists; a step is accepted once.
+        Nothing is changed when it raises."""
         self._all_attention("dropping tokens")
-        ss = [self._of(q) for q in step.seqs]
-        if [s.tokens for s in ss] != step.ends:
-            raise ValueError("accept: not the last plan of its sequences")
+        ss = self._last(step, "accept")
         ops._need(path, "path", torch.int32, 2)
         ops._need(count, "count", torch.int32, 1)
         if path.shape[0] != len(ss) or count.shape[0] != len(ss):
@@ -258,6 +270,8 @@ class PagedCache:
         if self.pools and any(i != j for row in kept for j, i in enumerate(row)):
             ops.paged_keep(list(self.pools.values()), step.table, step.lens, step.cu, path, count)
         self._shrink([(s, n - len(row)) for s, n, row in zip(ss, step.counts, kept)])
+        for s, row, mark in zip(ss, kept, step.before):
+            s.mark = None if row else mark
         return kept
 
     def _all_attention(self, what):
