@@ -714,7 +714,7 @@ int rf_verify_drafts_workspace_bytes(int64_t T, int64_t vocab, int n_seq, int64_
  * head_dim and page): of sequence b's n new rows (its last tokens of lens[b]) row path[b][j] becomes row j, for j < count[b]
  * (int32, device; at most path_width and n are taken). A path rises; an entry that does not, or that is no row, ends it.
  * Codes and scales move as they are. Rows behind the moved ones keep what they hold, and lens is the caller's to change. A
- * row on a page that is none does not move. Two layers with the same pages are refused. */
+ * row on a page that is none does not move. Layers with the same pages, or pools that share memory, are refused. */
 int rf_paged_keep(const rf_pages* const* pages, int n_layers, const int32_t* table, int64_t ld_table, int64_t table_width,
                   const int32_t* lens, const int32_t* cu, int n_seq, const int32_t* path, int64_t ld_path, int64_t path_width,
                   const int32_t* count, hipStream_t stream);

@@ -3,6 +3,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "paged.h"
@@ -575,6 +577,43 @@ extern "C" int rf_paged_tree(const int32_t* table, int64_t ld_table, int64_t tab
   return check_launch(fn);
 }
 
+namespace rf {
+namespace {
+
+// One of a layer's pools: n pages of `size` bytes, `stride` apart.
+struct Pool {
+  int64_t lo, stride, size, n;
+  int layer;
+  int64_t hi() const { return lo + (n - 1) * stride + size; }
+};
+
+struct At {                                // where a pool begins
+  int64_t lo;
+  int pool;
+};
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether a page of one has bytes of a page of the other (each lies within its stride).
+bool overlap(const Pool& a, const Pool& b) {
+  if (a.lo >= b.hi() || b.lo >= a.hi()) return false;
+  if (a.n > b.n) return overlap(b, a);
+  const int64_t delta = b.lo - a.lo;
+  if (a.stride == b.stride) {                                // pages p, q overlap: delta - a.size < d stride < delta + b.size, d = p - q
+    for (int64_t d = floor_div(delta + b.size - 1, a.stride); d * a.stride > delta - a.size; --d)
+      if (d > -b.n && d < a.n) return true;
+    return false;
+  }
+  for (int64_t p = 0; p < a.n; ++p) {                        // the first page of b that ends behind page p's beginning
+    const int64_t at = p * a.stride - delta, q = std::max<int64_t>(0, floor_div(at - b.size, b.stride) + 1);
+    if (q < b.n && q * b.stride < at + a.size) return true;
+  }
+  return false;
+}
+
+}  // namespace
+}  // namespace rf
+
 extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const int32_t* table, int64_t ld_table,
                              int64_t table_width, const int32_t* lens, const int32_t* cu, int n_seq, const int32_t* path,
                              int64_t ld_path, int64_t path_width, const int32_t* count, hipStream_t stream) {
@@ -585,6 +624,10 @@ extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const i
     return fail(RF_EINVAL_SHAPE, "%s: %d layers, %d sequences, table %lld wide (row stride %lld), paths of %lld rows (row stride "
                 "%lld)", fn, n_layers, n_seq, (long long)table_width, (long long)ld_table, (long long)path_width, (long long)ld_path);
   const rf_pages* first = pages[0];
+  std::unique_ptr<Pool[]> pools(new (std::nothrow) Pool[static_cast<size_t>(n_layers) * 4]);
+  std::unique_ptr<At[]> order(new (std::nothrow) At[static_cast<size_t>(n_layers) * 4]);
+  if (!pools || !order) return fail(RF_EINVAL_ARG, "%s: no host memory for %d layers", fn, n_layers);
+  int n_pools = 0;
   for (int i = 0; i < n_layers; ++i) {                       // (every layer is checked before any is changed)
     PagesDev pg;
     if (int rc = check_pages(fn, pages[i], &pg)) return rc;
@@ -593,10 +636,31 @@ extern "C" int rf_paged_keep(const rf_pages* const* pages, int n_layers, const i
                   pages[i]->kind, pages[i]->hkv, pages[i]->d, pages[i]->page);
     for (int j = 0; j < i; ++j)                              // (moved by two blocks at once)
       if (pages[j]->k == pages[i]->k) return fail(RF_EINVAL_ARG, "%s: layers %d and %d have the same pages", fn, j, i);
+    auto add = [&](const void* at, int64_t stride, int64_t head) {
+      pools[n_pools] = Pool{reinterpret_cast<int64_t>(at), stride, first->hkv * head, pg.n_pages, i};
+      order[n_pools] = At{pools[n_pools].lo, n_pools};
+      ++n_pools;
+    };
+    add(pg.k, pg.page_stride, pg.head_bytes);
+    add(pg.v, pg.page_stride, pg.head_bytes);
+    if (pages[i]->kind == RF_PAGES_MX4) {
+      add(pg.ks, pg.scale_stride, pg.head_scales);
+      add(pg.vs, pg.scale_stride, pg.head_scales);
+    }
   }
   if (n_seq == 0 || path_width == 0) return RF_OK;
   const int d = first->d;
   const bool mx = first->kind == RF_PAGES_MX4;
+  // no byte is two layers', or two pools': the pools by address, each against those that begin before it ends
+  std::sort(order.get(), order.get() + n_pools, [](const At& x, const At& y) { return x.lo < y.lo; });
+  for (int i = 0; i < n_pools; ++i) {
+    const Pool& p = pools[order[i].pool];
+    for (int j = i + 1; j < n_pools && order[j].lo < p.hi(); ++j) {
+      const Pool& o = pools[order[j].pool];
+      if (overlap(p, o))
+        return fail(RF_EINVAL_ARG, "%s: the pages of layers %d and %d overlap", fn, std::min(p.layer, o.layer), std::max(p.layer, o.layer));
+    }
+  }
   KeepArgs a;
   a.table = table;
   a.ld_table = ld_table;
