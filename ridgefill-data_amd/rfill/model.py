@@ -647,6 +647,7 @@ class FillModel:
         temperature: a number, or one a sequence; None or 0 takes the likeliest token. u (fp32 [tokens of all]), r (fp32
         [len(seqs)]) on the device, in [0, 1): the random numbers (None: torch's). draft [tokens of all, V]: row i holds the
         shares that the children of token i were drawn from (None: they were chosen, not drawn; ops.verify_drafts).
+        A sequence has at most 1024 tokens of one call.
         Returns, for each sequence, the list of accepted drafted ids and the id after them (-1: no logit above -infinity),
         which begins the next call's ids. If it raises, the sequences are as they were."""
         ids = [torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in ids]
@@ -669,6 +670,8 @@ class FillModel:
             u = torch.rand(rows, device=dev) if u is None else u
             r = torch.rand(n, device=dev) if r is None else r
         h, ssq = self.embed(torch.cat(ids) if ids else torch.empty(0, dtype=torch.int64))
+        drawn = (None,) * 4 if temperature is None else (u, r, temperature, draft)
+        ops._check_drafts(rows, self._vocab(), n, h.get_device(), max(counts, default=0), *drawn)
         step = cache.plan(seqs, counts, parents)
         try:
             tokens = torch.cat(ids).to(dev)
@@ -738,12 +741,20 @@ class FillModel:
         rows. The final norm's gain is folded into the packed lm_head (zero rows up to a multiple of 256)."""
         return self._head_rows(h, ssq).float()
 
+    def _head_weight(self):
+        """lm_head [V, H] as it was given, or the embedding that stands for it."""
+        return self._src["lm_head.weight" if "lm_head.weight" in self._src else self._pre + "embed_tokens.weight"]
+
+    def _vocab(self):
+        lm = getattr(self, "_lm", None)
+        return self._head_weight().shape[0] if lm is None else lm[1]
+
     def _head_rows(self, h, ssq):
         """The logits as the product rounds them, bf16."""
         if getattr(self, "_lm", None) is None:
             src, pre = self._src, self._pre
             dev = lambda k: src[k].to(self.device, torch.bfloat16).contiguous()   # noqa: E731
-            head = dev("lm_head.weight") if "lm_head.weight" in src else dev(pre + "embed_tokens.weight")
+            head = self._head_weight().to(self.device, torch.bfloat16).contiguous()
             V = head.shape[0]
             pad = (-V) % 256
             if pad:

@@ -1213,6 +1213,25 @@ def verify_drafts_workspace_bytes(rows, vocab, n_seq, max_rows):
     return b.value
 
 
+def _check_drafts(rows, vocab, n, dev, max_rows, u, r, temperature, draft):
+    """What verify_drafts checks before there are logits (of `rows` rows, on device number dev). Returns its workspace's bytes."""
+    if temperature is not None:
+        for name, t, m in (("temperature", temperature, n), ("u", u, rows), ("r", r, n)):
+            _need(t, name, torch.float32, 1)
+            if t.shape[0] != m:
+                raise ValueError(f"verify_drafts: {name} {tuple(t.shape)}, expected [{m}]")
+    if draft is not None:
+        if not isinstance(draft, torch.Tensor) or draft.dtype not in _KINDS:
+            raise ValueError(f"verify_drafts: draft {getattr(draft, 'dtype', type(draft))}, expected float32 or bfloat16")
+        _need(draft, "draft", draft.dtype, 2)
+        if draft.shape != (rows, vocab) or _rows_apart(draft, vocab) < vocab:
+            raise ValueError(f"verify_drafts: draft {tuple(draft.shape)} (row stride {draft.stride(0)}), expected {(rows, vocab)}")
+    for name, t in (("u", u), ("r", r), ("temperature", temperature), ("draft", draft)):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"verify_drafts: {name} is on {t.device}, the logits on GPU {dev}")
+    return verify_drafts_workspace_bytes(rows, vocab, n, max_rows)
+
+
 def verify_drafts(logits, tokens, parents, cu, u, r, temperature, max_rows, depth=None, draft=None, workspace="auto"):
     """Which drafted tokens of several sequences the target accepts, and the token after them. Sequence b's rows
     [cu[b], cu[b + 1]) (cu int32 [n + 1]) are a tree, row 0 its root; tokens int64 [rows], parents int32 [rows] (paged_tree).
@@ -1240,26 +1259,14 @@ def verify_drafts(logits, tokens, parents, cu, u, r, temperature, max_rows, dept
                          f"{cu.shape[0]} offsets")
     if temperature is None:
         u = r = draft = None
-    else:
-        for name, t, m in (("temperature", temperature, n), ("u", u, rows), ("r", r, n)):
-            _need(t, name, torch.float32, 1)
-            if t.shape[0] != m:
-                raise ValueError(f"verify_drafts: {name} {tuple(t.shape)}, expected [{m}]")
-    if draft is not None:
-        if not isinstance(draft, torch.Tensor) or draft.dtype not in _KINDS:
-            raise ValueError(f"verify_drafts: draft {getattr(draft, 'dtype', type(draft))}, expected float32 or bfloat16")
-        _need(draft, "draft", draft.dtype, 2)
-        if draft.shape != logits.shape:
-            raise ValueError(f"verify_drafts: draft {tuple(draft.shape)}, expected {tuple(logits.shape)}")
     depth = max(1, max_rows) if depth is None else depth
     if depth < 1:
         raise ValueError(f"verify_drafts: paths of {depth} rows")
     dev = logits.get_device()
-    for name, t in (("tokens", tokens), ("parents", parents), ("cu", cu), ("u", u), ("r", r), ("temperature", temperature),
-                    ("draft", draft)):
-        if t is not None and t.get_device() != dev:
+    for name, t in (("tokens", tokens), ("parents", parents), ("cu", cu)):
+        if t.get_device() != dev:
             raise ValueError(f"verify_drafts: {name} is on {t.device}, logits on {logits.device}")
-    need = verify_drafts_workspace_bytes(rows, vocab, n, max_rows)
+    need = _check_drafts(rows, vocab, n, dev, max_rows, u, r, temperature, draft)
     if isinstance(workspace, str):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
     _need(workspace, "workspace", torch.uint8, 1)
