@@ -667,8 +667,8 @@ class FillModel:
             if t.numel() not in (1, n):
                 raise ValueError(f"verify_paged: {t.numel()} temperatures of {n} sequences")
             temperature = t.expand(n).contiguous().to(dev)
-            u = torch.rand(rows, device=dev) if u is None else u
-            r = torch.rand(n, device=dev) if r is None else r
+            u = torch.rand(rows, dtype=torch.float32, device=dev) if u is None else u
+            r = torch.rand(n, dtype=torch.float32, device=dev) if r is None else r
         h, ssq = self.embed(torch.cat(ids) if ids else torch.empty(0, dtype=torch.int64))
         drawn = (None,) * 4 if temperature is None else (u, r, temperature, draft)
         ops._check_drafts(rows, self._vocab(), n, h.get_device(), max(counts, default=0), *drawn)
