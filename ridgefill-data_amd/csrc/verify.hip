@@ -399,8 +399,7 @@ __device__ __forceinline__ void gather(const VerifyArgs& a, const Block& s, cons
 // Where a sequence's path has come to.
 struct State {
   int node, count, next;                   // next: the row from which on the node's children are still to be tested
-  double c, Z;                             // what is left of the node's distribution (Z in weights without a draft)
-  double off;                              // without a draft: by how much Z may be wrong
+  double c, Z;                             // what is left of the node's distribution (without a draft Z in weights, off by up to c)
   bool cut;                                // a draft's token was rejected here
   bool fresh;                              // without a draft: Z was summed for the next test
 };
@@ -440,7 +439,7 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const 
     } else if (!drawn) {
       if (st.Z < 0) {                                        // (the node's first child)
         st.Z = l.sum[st.node];
-        st.off = ROW_ERROR * st.Z;
+        st.c = ROW_ERROR * st.Z;
       }
       bool gone = tok < 0;                                   // rejected before, or no token at all
       for (int k0 = st.node + 1; k0 < at; k0 += 64) {
@@ -448,7 +447,7 @@ __device__ __forceinline__ bool walk(const VerifyArgs& a, const Block& s, const 
         gone |= __any(k0 + lane < at && l.parent[k] == st.node && l.token[k] == tok);
       }
       const double own = gone ? 0.0 : l.w[at], mark = l.u[at] * st.Z;
-      if (own > 0 && !st.fresh && __builtin_fabs(mark - own) <= l.u[at] * st.off + SUM_ERROR * own) {
+      if (own > 0 && !st.fresh && __builtin_fabs(mark - own) <= l.u[at] * st.c + SUM_ERROR * own) {
         st.next = at;
         return true;
       }
@@ -591,7 +590,7 @@ __global__ __launch_bounds__(NW) void k_verify_sums(VerifyArgs a, int blocks) {
   const Block s = block_of(a, b);
   if ((s.n == 0 || !a.temperature) && x) return;             // (uniform)
   const Rows l(reinterpret_cast<char*>(lds), a.rows);
-  State st{0, 0, 1, 0.0, a.draft != nullptr ? 1.0 : -1.0, 0.0, false, false};
+  State st{0, 0, 1, 0.0, a.draft != nullptr ? 1.0 : -1.0, false, false};
   if (s.n == 0) {
     write_path(a, b, l.parent, st);
     if (t == 0) a.next[b] = -1;
@@ -681,7 +680,7 @@ __global__ __launch_bounds__(ND) void k_verify_draw(VerifyArgs a) {
       st.Z = z;
     } else {                                                 // (as the children's weights, relative to the row's largest logit)
       st.Z = z * weight(e2, top, l.top[st.node], s.slope);
-      st.off = SUM_ERROR * st.Z;
+      st.c = SUM_ERROR * st.Z;
       st.fresh = true;
     }
     more = walk(a, s, l, st);
