@@ -699,8 +699,9 @@ int rf_attend_tree_workspace_bytes(int64_t T, int hq, int hkv, int d, int kind, 
  * them (a path has depth rows at most; the last one's children are then not tested); count [n_seq] int32; next [n_seq] int64.
  * A sequence without rows gets count 0 and next -1. Weights are within 3e-12 of themselves, sums in 64 bits (without draft tests begin
  * with sums of whole rows from 32-bit weights; one that lies within their bound, 1e-5, of its border is taken again with a 64-bit sum
- * of what is left). cu, tokens and parents are read on the device; max_rows <= 1024 bounds a sequence's rows (it is taken to have as many), vocab <= 2^19. The workspace (16-byte
- * aligned, of rf_verify_drafts_workspace_bytes) need not be kept or cleared; calls that may run at once need one each. */
+ * of what is left). cu, tokens and parents are read on the device; max_rows <= 1024 bounds a sequence's rows (it is taken to
+ * have as many), vocab <= 2^19. The workspace (16-byte aligned, of rf_verify_drafts_workspace_bytes) need not be kept or
+ * cleared; calls that may run at once need one each. */
 int rf_verify_drafts(const void* logits, int logits_kind, int64_t ld, int64_t vocab, int64_t T, const int64_t* tokens,
                      const int32_t* parents, const int32_t* cu, int n_seq, const float* u, const float* r,
                      const float* temperature, const void* draft, int draft_kind, int64_t ld_draft, int64_t max_rows,

@@ -57,7 +57,7 @@ struct PagedArgs {
   bool once;                               // k_paged_many: as many units as that at most
   int64_t units;                           // units a head that the launch has blocks and the workspace partials for
   int kt, wmin;                            // keys a tile, key tiles a split at least
-  float unit_tiles;                        // what a unit costs besides its tiles, in tiles (apart: 3, 24, 150 make 2 % of difference)
+  float unit_tiles;                        // what a unit costs besides its tiles, in tiles
   bool apart;                              // k_paged_few: units of splits, not runs
   const uint64_t* seen;                    // trees: of each row of q, bits of the new rows of its sequence that it sees
   int64_t ld_seen;
@@ -798,9 +798,10 @@ struct FewLds {
 
 // Trees of more rows than a block in 4 bits (apart): the row blocks of a sequence's split read the same tiles, so they run beside one
 // another on one XCD (blocks go round the eight of them), whose L2 gives a tile to all but the first: splits of one length for all
-// (find_unit), not runs. head_dim 256, groups of 8: 9 sequences of up to 13 new tokens and 30011 keys fetch 114 MB for 383 and take
-// 60 us for 75, 13 and 8000 40 / 50, 2 of 64 and 30000 115 / 158; 128, groups of 4: 40 of 26 and 24001 449 MB for 1517 and 264 us
-// for 269 (the vector pipe is busy half of the time), 2 of 26 and 30000 52 / 62. 64 stays with runs: 40 of 64 and 9000 57 / 48.
+// (find_unit), not runs. Microseconds a call, side by side / runs, in turn on one box: head_dim 256, groups of 8: 9 sequences of up to
+// 13 new tokens and 30011 keys 59 / 77 (114 MB fetched for 383), 13 and 8000 36 / 45, 2 of 64 and 30000 117 / 119; 128, groups of 4: 40
+// of 26 and 24001 243 / 266 (444 MB for 1517; the vector pipe is busy half of the time), 2 of 26 and 30000 63 / 71, 2 of 64 and 30000
+// 80 / 80, but 13 of 26 and 8000 76 / 71. 64 stays with runs: 40 of 64 and 9000 57 / 48.
 // Blocks -> (head, unit), eight units in a row an XCD; the number of units is a multiple of 64.
 __device__ __forceinline__ void near_blocks(int block, int hkv, int units, int& head, int& unit) {
   const int x = block & 7, k = block >> 3;
@@ -1767,7 +1768,10 @@ int attend(const char* fn, const uint16_t* q, int64_t ldq, int64_t T, int hq, co
                     p.fit ? reinterpret_cast<int*>(static_cast<char*>(workspace) + p.bytes) - 4 : nullptr, p.fit, p.once, p.units, p.kt,
                     // key tiles a split at least (a quarter or half of it, this, four times it): one sequence of 4000 keys 16 / 17 /
                     // 33 us, of 6000 in 4 bits 15 / 14 / 20; chunks of 200 rows over 4000 keys 38 / 38 / 46, 2 of 64 over 3000 33 / 36 / 47
-                    p.small ? 8 : p.many ? 4 : 2 * NW, p.apart ? 24.f : 3.f, p.apart, seen, ld_seen, static_cast<int>(words)};
+                    p.small ? 8 : p.many ? 4 : 2 * NW,
+                    // what a unit costs, side by side 3 / 24 / 150: 40 trees of up to 26 new tokens and 24001 keys, head_dim 128 246 / 243
+                    // / 284 us, 13 of 26 and 8000 76 / 76 / 71; 2 of 64 and 30000 and those of head_dim 256 the same
+                    p.apart ? 24.f : 3.f, p.apart, seen, ld_seen, static_cast<int>(words)};
   const dim3 grid(static_cast<unsigned>(p.units * hkv));
   // the merge: a block a row block and head, or a share of its rows; wide blocks where they are few
   const int64_t pairs = p.blocks * hkv, rows = std::min<int64_t>(static_cast<int64_t>(a.max_rows) * a.rep, p.rows());
